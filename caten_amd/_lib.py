@@ -106,6 +106,15 @@ PROTOTYPES = {
     "cthip_kv_page_rows": (_i, []),
     "cthip_kv_append_paged": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i]),
     "cthip_sdpa_cached_paged": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _i]),
+    "cthip_kv_page_bytes_q4": (_i64, [_i, _i]),
+    "cthip_kv_plan_paged": (_i, [_vp, _vp, _vp, _vp, _i, _vp, _vp, _vp, _vp, _vp, _i, _vp, _vp, _i]),
+    "cthip_kv_append_paged_q4": (_i, [_vp, _vp, _vp, _vp, _i64, _i64, _vp, _i, _i, _i, _i]),
+    "cthip_kv_rows_paged_q4": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i]),
+    "cthip_sdpa_paged_q4_workspace": (_i64, [_i]),
+    "cthip_sdpa_paged_q4": (_i, [_vp, _vp, _i64, _vp, _vp, _i, _vp, _i, _vp, _vp, _i, _i, _i, _i, _i, _vp]),
+    "cthip_beam_select_workspace": (_i64, [_i, _i]),
+    "cthip_beam_select": (_i, [_vp, _vp, _vp, _vp, _vp, _i64, _vp, _vp, _i, _i, _i, _i, _vp]),
+    "cthip_beam_reorder_paged_q4": (_i, [_vp, _vp, _vp, _vp, _i, _i, _vp, _i, _vp, _vp, _i, _i, _i, _i, _vp, _i, _vp, _vp]),
     "cthip_decoder_create": (_i, [_vpp, C.POINTER(DecoderConfig)]),
     "cthip_decoder_destroy": (_i, [_vp]),
     "cthip_decoder_load": (_i, [_vp, C.c_char_p, _i, _vp, _i64, _i64]),

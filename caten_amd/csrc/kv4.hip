@@ -1,0 +1,370 @@
+// Batched serving over a paged KV cache in 4 bits: block tables and slot maps from the sequences' lengths, rows into the
+// cache and back, and the reordering of a beam search's sequences.  The reference keeps one dense fp32 cache per model
+// (external/llm/layers.lisp:19-33) and one sequence; a server holds many sequences of different lengths, so here all of them
+// take pages from one pool, and everything a step needs to know about who owns what is worked out on the device: a step's
+// launches can be captured once and replayed.  Layout of a page: kv4.h.
+#include "kv4.h"
+
+namespace cthip {
+
+// ---- block tables and slot maps ----
+// starts = exclusive sum of the new rows, pages wanted = ceil((len + new) / 64) - ceil(len / 64), and their exclusive sum says
+// which entries of the free stack a sequence gets.  Every workgroup works the two sums out for itself (n <= 4096 in LDS, at most
+// four sequences a thread) and then finds the sequence of each of its rows by bisection: one launch, nothing to wait for
+// between workgroups.  The row that opens a page enters it into the table.
+constexpr int kPlanThreads = 1024, kPlanRows = 8192;  // rows of a workgroup: a decode step of any size is one workgroup
+
+__device__ __forceinline__ int64_t block_scan(int64_t v, int64_t *part, int64_t &total) {  // exclusive, over kPlanThreads threads
+  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+  int64_t s = v;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int64_t u = __shfl_up(s, o, 64);
+    if (lane >= o) s += u;
+  }
+  if (lane == 63) part[wv] = s;
+  __syncthreads();
+  int64_t before = 0;
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < kPlanThreads / 64; w++) {
+    if (w < wv) before += part[w];
+    total += part[w];
+  }
+  __syncthreads();
+  return before + s - v;
+}
+
+__global__ __launch_bounds__(kPlanThreads) void k_kv_plan(int *__restrict__ slots, int *__restrict__ positions, int *__restrict__ starts, int *tables,
+                                                          int table_stride, int *lens_out, int *n_free_out, int *refused, const int *lens,
+                                                          const int *__restrict__ new_lens, int n, const int *__restrict__ free_pages,
+                                                          const int *n_free, int max_rows, bool rows_too, bool lens_too) {
+  __shared__ int s_start[kKv4MaxSeqs + 1];  // first row; rows past max_rows are all the same to a reader: they saturate
+  __shared__ int s_len[kKv4MaxSeqs];        // rows in the cache, -1 = refused
+  __shared__ int s_page[kKv4MaxSeqs];       // pages handed out in front of it
+  __shared__ int64_t part[kPlanThreads / 64];
+  __shared__ int s_refused, s_used;
+  const int tid = threadIdx.x;
+  const int64_t cap = (int64_t)table_stride * kKvPageRows, have_free = n_free[0];
+  if (tid == 0) s_refused = 0, s_used = 0;
+  __syncthreads();
+  int64_t row0 = 0, page0 = 0;
+  int bad = 0;
+  for (int i0 = 0; i0 < n; i0 += kPlanThreads) {
+    const int i = i0 + tid;
+    const int64_t len = i < n ? lens[i] : 0, add = i < n ? new_lens[i] : 0;
+    int64_t rows, pages;
+    const int64_t start = row0 + block_scan(add > 0 ? add : 0, part, rows);
+    bool ok = len >= 0 && add >= 0 && len + add <= cap && start + add <= max_rows;
+    const int64_t need = ok ? (len + add + kKvPageRows - 1) / kKvPageRows - (len + kKvPageRows - 1) / kKvPageRows : 0;
+    const int64_t before = page0 + block_scan(need, part, pages);
+    ok = ok && (need == 0 || before + need <= have_free);
+    if (i < n) {
+      s_start[i] = (int)min(start, (int64_t)INT_MAX);
+      s_len[i] = ok ? (int)len : -1;
+      s_page[i] = (int)min(before, (int64_t)INT_MAX);
+      if (!ok) bad++;
+      else if (need) atomicMax(&s_used, (int)(before + need));  // sequences are refused from one on: the last one with pages has the sum of them all
+    }
+    row0 += rows;
+    page0 += pages;
+  }
+  if (bad) atomicAdd(&s_refused, bad);
+  if (tid == 0) s_start[n] = (int)min(row0, (int64_t)INT_MAX);
+  __syncthreads();  // every length has been read: lens_out may be the same array where this is the only workgroup
+  if (blockIdx.x == 0 && lens_too) {
+    for (int i = tid; i < n; i += kPlanThreads) {
+      if (s_len[i] >= 0) lens_out[i] = s_len[i] + s_start[i + 1] - s_start[i];
+      else if (lens_out != lens) lens_out[i] = lens[i];
+    }
+    if (tid == 0) {
+      n_free_out[0] = (int)have_free - s_used;
+      refused[0] = s_refused;
+    }
+  }
+  if (!rows_too) return;
+  if (blockIdx.x == 0)
+    for (int i = tid; i <= n; i += kPlanThreads) starts[i] = s_start[i];
+  const int rows = s_start[n];
+  const int r1 = min((int64_t)max_rows, (int64_t)(blockIdx.x + 1) * kPlanRows);
+  for (int r = blockIdx.x * kPlanRows + tid; r < r1; r += kPlanThreads) {
+    int slot = -1, at = -1;
+    if (r < rows) {
+      int lo = 0, hi = n;  // s_start[lo] <= r < s_start[hi]
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (s_start[mid] <= r) lo = mid;
+        else hi = mid;
+      }
+      const int len = s_len[lo];
+      if (len >= 0) {
+        at = len + r - s_start[lo];
+        const int page = at / kKvPageRows, have = (len + kKvPageRows - 1) / kKvPageRows;
+        int id;
+        if (page < have) {
+          id = tables[(int64_t)lo * table_stride + page];
+        } else {
+          id = free_pages[(int)have_free - 1 - (s_page[lo] + page - have)];
+          if (at % kKvPageRows == 0) tables[(int64_t)lo * table_stride + page] = id;
+        }
+        if (id >= 0 && id <= INT_MAX / kKvPageRows - 1) slot = id * kKvPageRows + at % kKvPageRows;
+      }
+    }
+    slots[r] = slot;
+    if (positions) positions[r] = at;
+  }
+}
+
+// ---- rows into the cache ----
+// Four lanes hold a block of 32 channels, eight each.  d = m / -8 as fp16, m the value of largest magnitude (the positive one
+// of two), kept finite; q = floor(x / d + 8.5) within 0 .. 15, d being the scale as it is STORED.  The quotient is taken by a
+// reciprocal and then held against the borders (q - 8.5) d and (q - 7.5) d, which are exact in fp32 (5 bits times 11): the
+// number is the one of real arithmetic whatever the reciprocal's rounding.  A block with an infinity or a NaN has a NaN scale.
+__device__ __forceinline__ float quad_max(float v) {
+  v = fmaxf(v, dpp_f<0xB1>(v));
+  return fmaxf(v, dpp_f<0x4E>(v));
+}
+
+__device__ __forceinline__ uint32_t kv4_quantise8(const float *x, unsigned short &scale) {  // the eight two's complement nibbles, channel 0 lowest
+  float hi = x[0], lo = x[0], odd = 0.0f;
+#pragma unroll
+  for (int e = 0; e < 8; e++) {
+    hi = fmaxf(hi, x[e]);
+    lo = fminf(lo, x[e]);
+    if (!(fabsf(x[e]) < INFINITY)) odd = 1.0f;
+  }
+  hi = quad_max(hi);
+  lo = -quad_max(-lo);
+  odd = quad_max(odd);
+  const float m = hi >= -lo ? hi : lo;
+  const _Float16 d16 = (_Float16)fminf(fmaxf(m * -0.125f, -65504.0f), 65504.0f);
+  const float d = (float)d16, ds = fabsf(d);
+  scale = odd != 0.0f ? (unsigned short)0x7E00 : __builtin_bit_cast(unsigned short, d16);
+  if (odd != 0.0f || ds == 0.0f) return 0u;
+  const float inv = 1.0f / ds;
+  uint32_t w = 0;
+#pragma unroll
+  for (int e = 0; e < 8; e++) {
+    const float xs = d < 0.0f ? -x[e] : x[e];
+    float t = fminf(fmaxf(floorf(fmaf(xs, inv, 8.5f)), 0.0f), 15.0f);
+    if (t > 0.0f && xs < (t - 8.5f) * ds) t -= 1.0f;
+    else if (t < 15.0f && xs >= (t - 7.5f) * ds) t += 1.0f;
+    w |= ((uint32_t)(int)t ^ 8u) << (4 * e);
+  }
+  return w;
+}
+
+// one row per blockIdx.x, keys (blockIdx.z = 0) or values; a thread per eight channels
+__global__ __launch_bounds__(256) void k_kv4_append(unsigned char *__restrict__ kp, unsigned char *__restrict__ vp, const float *__restrict__ kr,
+                                                    const float *__restrict__ vr, int64_t k_stride, int64_t v_stride,
+                                                    const int *__restrict__ slots, int n_pages, int kv, int dh) {
+  const int e8 = blockIdx.y * 256 + threadIdx.x;  // eighth of the row
+  if (e8 >= kv * dh / 8) return;                   // (kv * dh / 8 is a multiple of 4: whole quads leave)
+  const int slot = slots[blockIdx.x];
+  if (slot < 0 || slot >= n_pages * kKvPageRows) return;
+  const bool values = blockIdx.z != 0;
+  const float *src = (values ? vr + blockIdx.x * v_stride : kr + blockIdx.x * k_stride) + 8 * e8;
+  float x[8];
+  *(f4_any *)x = *(const f4_any *)src;
+  *(f4_any *)(x + 4) = *(const f4_any *)(src + 4);
+  unsigned short d;
+  const uint32_t w = kv4_quantise8(x, d);
+  const int row = slot % kKvPageRows, h = 8 * e8 / dh, c8 = e8 - h * (dh / 8), b = c8 >> 2, g = c8 & 3;
+  unsigned char *head = (values ? vp : kp) + ((int64_t)(slot / kKvPageRows) * kv + h) * kv4_head_bytes(dh);
+  if (g == 0) *(unsigned short *)(head + kv4_scale_offset(row, b, dh)) = d;
+  if (!values) {
+    // bytes j: channel j low, channel 4 + j high
+    const uint32_t lo = (w & 0xF) | (w & 0xF0) << 4 | (w & 0xF00) << 8 | (w & 0xF000) << 12;
+    const uint32_t hi = w >> 16, up = (hi & 0xF) | (hi & 0xF0) << 4 | (hi & 0xF00) << 8 | (hi & 0xF000) << 12;
+    *(uint32_t *)(head + kv4_key_offset(row, g, b, dh)) = lo | up << 4;
+  } else {
+    // lanes 0 and 1 of the quad hold channels 0 .. 15 of the block, 2 and 3 their partners; each lane stores four bytes
+    const uint32_t other = __builtin_bit_cast(uint32_t, dpp_f<0x4E>(__builtin_bit_cast(float, w)));
+    const uint32_t low = g < 2 ? w : other, high = g < 2 ? other : w;
+    const int j0 = g < 2 ? 0 : 4, c = 8 * (g & 1) + j0;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      const int sh = 4 * (j0 + j);
+      head[kv4_value_offset(row, b, c + j)] = (unsigned char)(((low >> sh) & 15u) | ((high >> sh) & 15u) << 4);
+    }
+  }
+}
+
+// ---- rows of the cache back as fp32, by their slots ----
+__global__ __launch_bounds__(256) void k_kv4_rows(float *__restrict__ ko, float *__restrict__ vo, const unsigned char *__restrict__ kp,
+                                                  const unsigned char *__restrict__ vp, const int *__restrict__ slots, int n_pages, int kv, int dh) {
+  const int e8 = blockIdx.y * 256 + threadIdx.x;
+  if (e8 >= kv * dh / 8) return;
+  const int slot = slots[blockIdx.x];
+  if (slot < 0 || slot >= n_pages * kKvPageRows) return;
+  const bool values = blockIdx.z != 0;
+  float *out = values ? vo : ko;
+  if (!out) return;
+  const int row = slot % kKvPageRows, h = 8 * e8 / dh, c8 = e8 - h * (dh / 8), b = c8 >> 2, g = c8 & 3;
+  const unsigned char *head = (values ? vp : kp) + ((int64_t)(slot / kKvPageRows) * kv + h) * kv4_head_bytes(dh);
+  const float d = half_bits_to_float(*(const unsigned short *)(head + kv4_scale_offset(row, b, dh)));
+  float x[8];
+  if (!values) {
+    const uint32_t w = *(const uint32_t *)(head + kv4_key_offset(row, g, b, dh));
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      x[j] = d * (float)((int)(w << (28 - 8 * j)) >> 28);
+      x[4 + j] = d * (float)((int)(w << (24 - 8 * j)) >> 28);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      const int v = head[kv4_value_offset(row, b, 8 * (g & 1) + j)];
+      x[j] = d * (float)((int)((uint32_t)v << (g < 2 ? 28 : 24)) >> 28);
+    }
+  }
+  float *dst = out + (int64_t)blockIdx.x * kv * dh + 8 * e8;
+  *(f4_any *)dst = *(const f4_any *)x;
+  *(f4_any *)(dst + 4) = *(const f4_any *)(x + 4);
+}
+
+// ---- reordering of beams ----
+// Pages that are full are the same for all beams of a request and stay shared; the partly filled last page is each beam's
+// own.  A parent's page goes to its first child as it is; every further child needs a copy, and there are as many pages of
+// beams without a child: the further children take them in order.  A page that is copied from is kept by somebody and is not
+// copied to, so the copies need no order among themselves, and a call repeated on the same tables writes the same bytes.
+struct ReorderArgs {
+  int *tables_out, *history_out;
+  unsigned char *k_pages, *v_pages;
+  const int *tables, *lens, *parents, *history, *tokens, *step;
+  int table_stride, n_layers, n_pages, beams, cols, page_bytes;
+};
+constexpr int kMaxBeams = 32;
+
+// blockIdx.y = beam; blockIdx.x = 0: its row of the table and its history, otherwise the pages of layer (x - 1) / 2
+__global__ __launch_bounds__(256) void k_beam_reorder(ReorderArgs a) {
+  const int n0 = blockIdx.y / a.beams * a.beams, j = blockIdx.y - n0, tid = threadIdx.x;
+  const int len = a.lens[blockIdx.y / a.beams];
+  int mine = j, rank = 0;  // rank: children in front of this one that need a copy
+  bool further = false;
+  unsigned alive = 0;
+  for (int i = 0; i < a.beams; i++) {
+    int p = a.parents[n0 + i];
+    if (p < 0 || p >= a.beams) p = i;
+    const bool again = (alive >> p) & 1u;
+    alive |= 1u << p;
+    if (i < j && again) rank++;
+    if (i == j) mine = p, further = again;
+  }
+  const int last = len > 0 ? len / kKvPageRows : 0;
+  const bool tail = len > 0 && len % kKvPageRows != 0 && last < a.table_stride;
+  int owner = mine;  // whose last page this beam gets
+  if (further)
+    for (int i = 0, k = 0; i < a.beams; i++)
+      if (!((alive >> i) & 1u) && k++ == rank) {
+        owner = i;
+        break;
+      }
+  const int *from = a.tables + (int64_t)(n0 + mine) * a.table_stride;
+  if (blockIdx.x == 0) {
+    const int *own = a.tables + (int64_t)blockIdx.y * a.table_stride, *tail_of = a.tables + (int64_t)(n0 + owner) * a.table_stride;
+    int *to = a.tables_out + (int64_t)blockIdx.y * a.table_stride;
+    for (int c = tid; c < a.table_stride; c += 256) to[c] = c < last ? from[c] : c == last && tail ? tail_of[c] : own[c];
+    if (a.history_out) {
+      const int at = a.step[0];
+      const int *old = a.history + (int64_t)(n0 + mine) * a.cols;
+      int *h = a.history_out + (int64_t)blockIdx.y * a.cols;
+      for (int c = tid; c < a.cols; c += 256) h[c] = c == at ? a.tokens[blockIdx.y] : old[c];
+    }
+    return;
+  }
+  if (!further || !tail) return;
+  const int src = from[last], dst = a.tables[(int64_t)(n0 + owner) * a.table_stride + last];
+  if (src < 0 || src >= a.n_pages || dst < 0 || dst >= a.n_pages) return;
+  const int x = blockIdx.x - 1;
+  unsigned char *pool = (x & 1 ? a.v_pages : a.k_pages) + (int64_t)(x >> 1) * a.n_pages * a.page_bytes;
+  const uint4 *s = (const uint4 *)(pool + (int64_t)src * a.page_bytes);
+  uint4 *d = (uint4 *)(pool + (int64_t)dst * a.page_bytes);
+  for (int e = tid; e < a.page_bytes / 16; e += 256) d[e] = s[e];
+}
+
+}  // namespace cthip
+
+using namespace cthip;
+
+static bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
+
+extern "C" {
+
+int64_t cthip_kv_page_bytes_q4(int kv_heads, int head_dim) {
+  if (!kv4_shape_ok(kv_heads, head_dim)) return fail(CTHIP_E_BAD_ARG, "cthip_kv_page_bytes_q4: %d heads of %d (head sizes 32, 64, 128)", kv_heads, head_dim);
+  return (int64_t)kv_heads * kv4_head_bytes(head_dim);
+}
+
+int cthip_kv_plan_paged(int *slots, int *positions, int *starts, int *tables, int table_stride, int *lens_out, int *n_free_out, int *refused,
+                        const int *lens, const int *new_lens, int n_seqs, const int *free_pages, const int *n_free, int max_rows) {
+  CTHIP_REQUIRE_INIT();
+  CTHIP_ARG(n_seqs >= 0 && max_rows >= 0 && max_rows <= (1 << 30) && table_stride > 0 && table_stride <= INT_MAX / kKvPageRows);
+  if (n_seqs > kKv4MaxSeqs) return fail(CTHIP_E_UNSUPPORTED, "cthip_kv_plan_paged: %d sequences in one call (at most %d)", n_seqs, kKv4MaxSeqs);
+  CTHIP_ARG(starts && lens_out && n_free_out && refused && n_free && (max_rows == 0 || slots));
+  CTHIP_ARG(n_seqs == 0 || (tables && lens && new_lens && free_pages));
+  const int blocks = max_rows > 0 ? (max_rows + kPlanRows - 1) / kPlanRows : 1;
+  // several workgroups read the lengths while one of them would overwrite them: a launch of its own behind them then
+  const bool apart = blocks > 1 && (lens_out == lens || n_free_out == n_free);
+  hipLaunchKernelGGL(k_kv_plan, dim3((unsigned)blocks), dim3(kPlanThreads), 0, state().stream, slots, positions, starts, tables, table_stride, lens_out, n_free_out, refused,
+                     lens, new_lens, n_seqs, free_pages, n_free, max_rows, true, !apart);
+  CTHIP_LAUNCH_CHECK();
+  if (apart) {
+    hipLaunchKernelGGL(k_kv_plan, dim3(1), dim3(kPlanThreads), 0, state().stream, slots, positions, starts, tables, table_stride, lens_out, n_free_out, refused, lens,
+                       new_lens, n_seqs, free_pages, n_free, max_rows, false, true);
+    CTHIP_LAUNCH_CHECK();
+  }
+  return 0;
+}
+
+int cthip_kv_append_paged_q4(void *k_pages, void *v_pages, const float *k_rows, const float *v_rows, int64_t k_stride, int64_t v_stride, const int *slots,
+                             int n_rows, int n_pages, int kv_heads, int head_dim) {
+  CTHIP_REQUIRE_INIT();
+  CTHIP_ARG(n_rows >= 0 && n_pages >= 0 && n_pages <= INT_MAX / kKvPageRows);
+  if (!kv4_shape_ok(kv_heads, head_dim)) return fail(CTHIP_E_UNSUPPORTED, "cthip_kv_append_paged_q4: %d heads of %d (head sizes 32, 64, 128)", kv_heads, head_dim);
+  if (n_rows == 0 || n_pages == 0) return 0;
+  CTHIP_ARG(k_pages && v_pages && k_rows && v_rows && slots);
+  CTHIP_ARG(aligned16(k_pages) && aligned16(v_pages) && k_stride >= (int64_t)kv_heads * head_dim && v_stride >= (int64_t)kv_heads * head_dim);
+  const int eighths = kv_heads * head_dim / 8;
+  hipLaunchKernelGGL(k_kv4_append, dim3((unsigned)n_rows, (unsigned)((eighths + 255) / 256), 2), dim3(256), 0, state().stream, (unsigned char *)k_pages,
+                     (unsigned char *)v_pages, k_rows, v_rows, k_stride, v_stride, slots, n_pages, kv_heads, head_dim);
+  CTHIP_LAUNCH_CHECK();
+  return 0;
+}
+
+int cthip_kv_rows_paged_q4(float *k_rows, float *v_rows, const void *k_pages, const void *v_pages, const int *slots, int n_rows, int n_pages, int kv_heads,
+                           int head_dim) {
+  CTHIP_REQUIRE_INIT();
+  CTHIP_ARG(n_rows >= 0 && n_pages >= 0 && n_pages <= INT_MAX / kKvPageRows);
+  if (!kv4_shape_ok(kv_heads, head_dim)) return fail(CTHIP_E_UNSUPPORTED, "cthip_kv_rows_paged_q4: %d heads of %d (head sizes 32, 64, 128)", kv_heads, head_dim);
+  if (n_rows == 0 || n_pages == 0 || (!k_rows && !v_rows)) return 0;
+  CTHIP_ARG(slots && (!k_rows || k_pages) && (!v_rows || v_pages) && aligned16(k_pages) && aligned16(v_pages));
+  const int eighths = kv_heads * head_dim / 8;
+  hipLaunchKernelGGL(k_kv4_rows, dim3((unsigned)n_rows, (unsigned)((eighths + 255) / 256), 2), dim3(256), 0, state().stream, k_rows, v_rows,
+                     (const unsigned char *)k_pages, (const unsigned char *)v_pages, slots, n_pages, kv_heads, head_dim);
+  CTHIP_LAUNCH_CHECK();
+  return 0;
+}
+
+int cthip_beam_reorder_paged_q4(int *tables_out, int *history_out, void *k_pages, void *v_pages, int n_layers, int n_pages, const int *tables, int table_stride,
+                                const int *lens, const int *parents, int n_batch, int n_beams, int kv_heads, int head_dim, const int *history, int cols,
+                                const int *tokens, const int *step) {
+  CTHIP_REQUIRE_INIT();
+  CTHIP_ARG(n_batch >= 0 && n_beams >= 1 && n_layers >= 0 && n_pages >= 0 && n_pages <= INT_MAX / kKvPageRows && table_stride > 0 && cols >= 0);
+  if (n_beams > kMaxBeams) return fail(CTHIP_E_UNSUPPORTED, "cthip_beam_reorder_paged_q4: %d beams (at most %d)", n_beams, kMaxBeams);
+  if (!kv4_shape_ok(kv_heads, head_dim)) return fail(CTHIP_E_UNSUPPORTED, "cthip_beam_reorder_paged_q4: %d heads of %d (head sizes 32, 64, 128)", kv_heads, head_dim);
+  if (n_layers > (1 << 20) || (int64_t)n_batch * n_beams > 65535)
+    return fail(CTHIP_E_UNSUPPORTED, "cthip_beam_reorder_paged_q4: %d layers, %d x %d beams (at most 1048576 layers, 65535 beams)", n_layers, n_batch, n_beams);
+  if (n_batch == 0) return 0;
+  CTHIP_ARG(tables_out && tables && tables_out != tables && lens && parents);
+  CTHIP_ARG(n_layers == 0 || n_pages == 0 || (k_pages && v_pages && aligned16(k_pages) && aligned16(v_pages)));
+  CTHIP_ARG(!history_out || (history && history_out != history && tokens && step));
+  const ReorderArgs a = {tables_out, cols ? history_out : nullptr, (unsigned char *)k_pages, (unsigned char *)v_pages, tables, lens, parents, history, tokens, step,
+                         table_stride, n_layers, n_pages, n_beams, cols, kv_heads * kv4_head_bytes(head_dim)};
+  const unsigned copies = n_pages ? 2u * (unsigned)n_layers : 0u;
+  hipLaunchKernelGGL(k_beam_reorder, dim3(1 + copies, (unsigned)(n_batch * n_beams)), dim3(256), 0, state().stream, a);
+  CTHIP_LAUNCH_CHECK();
+  return 0;
+}
+
+}  // extern "C"

@@ -252,3 +252,113 @@ def sdpa_cached(q, k_cache, v_cache, start_pos: int):
     out = DeviceArray(q.shape, np.float32)
     _lib.check(_lib.load().cthip_sdpa_cached(out.ptr, dq.ptr, dk.ptr, dv.ptr, S, start_pos, H, Hkv, Dh))
     return out.numpy()
+
+
+def kv_plan(lens, new_lens, tables, free_pages, max_rows: int, n_free: Optional[int] = None) -> dict:
+    """Block tables and slot maps of a step of a batch (cthip_kv_plan_paged): `lens` rows held and `new_lens` new ones per
+    sequence, `tables` (n, stride) page ids, `free_pages` a stack of which the last `n_free` entries are taken first."""
+    lens, new_lens, tables, free_pages = (np.ascontiguousarray(a, np.int32) for a in (lens, new_lens, tables, free_pages))
+    n = lens.size
+    if new_lens.size != n or tables.ndim != 2 or tables.shape[0] != n:
+        raise ValueError(f"kv_plan: {n} lengths, {new_lens.size} new lengths and a table of shape {tables.shape}")
+    n_free = free_pages.size if n_free is None else int(n_free)
+    if not 0 <= n_free <= free_pages.size:
+        raise ValueError(f"kv_plan: {n_free} free pages of a stack of {free_pages.size}")
+    d_lens, d_new, d_tables, d_free, d_n = (DeviceArray.from_numpy(a) for a in (lens, new_lens, tables, free_pages, np.array([n_free], np.int32)))
+    slots, positions, starts, refused = (DeviceArray((m,), np.int32) for m in (max_rows, max_rows, n + 1, 1))
+    _lib.check(_lib.load().cthip_kv_plan_paged(slots.ptr, positions.ptr, starts.ptr, d_tables.ptr, tables.shape[1], d_lens.ptr, d_n.ptr, refused.ptr, d_lens.ptr,
+                                               d_new.ptr, n, d_free.ptr, d_n.ptr, max_rows))
+    return dict(slots=slots.numpy(), positions=positions.numpy(), starts=starts.numpy(), tables=d_tables.numpy(), lens=d_lens.numpy(), n_free=int(d_n.numpy()[0]),
+                refused=int(refused.numpy()[0]))
+
+
+class PagedCacheQ4:
+    """The keys and values of a batch of sequences in 4 bits, in pages of 64 rows (one layer, or `layers` of them)."""
+
+    def __init__(self, n_pages: int, kv_heads: int, head_dim: int, layers: int = 1):
+        self.n_pages, self.kv_heads, self.head_dim, self.layers = n_pages, kv_heads, head_dim, layers
+        lib = _lib.init()
+        self.page_bytes = int(lib.cthip_kv_page_bytes_q4(kv_heads, head_dim))
+        if self.page_bytes < 0:
+            _lib.check(self.page_bytes)
+        self.k, self.v = (DeviceArray((layers, n_pages, self.page_bytes), np.uint8) for _ in range(2))
+        self.workspace = DeviceArray((int(lib.cthip_sdpa_paged_q4_workspace(head_dim)),), np.uint8)
+
+    def _pools(self, layer):
+        if not 0 <= layer < self.layers:
+            raise ValueError(f"PagedCacheQ4: layer {layer} of {self.layers}")
+        at = layer * self.n_pages * self.page_bytes
+        return self.k.ptr + at, self.v.ptr + at
+
+    def append(self, k, v, slots, layer: int = 0) -> None:
+        """Rows (n, kv_heads, head_dim) into the cache rows `slots`."""
+        width = self.kv_heads * self.head_dim
+        k, v = (np.ascontiguousarray(a, np.float32).reshape(-1, width) for a in (k, v))
+        slots = np.ascontiguousarray(slots, np.int32).ravel()
+        if k.shape != v.shape or slots.size != k.shape[0]:
+            raise ValueError(f"PagedCacheQ4.append: keys {k.shape}, values {v.shape}, {slots.size} slots")
+        dk, dv, ds = (DeviceArray.from_numpy(a) for a in (k, v, slots))
+        kp, vp = self._pools(layer)
+        _lib.check(_lib.load().cthip_kv_append_paged_q4(kp, vp, dk.ptr, dv.ptr, width, width, ds.ptr, slots.size, self.n_pages, self.kv_heads, self.head_dim))
+
+    def rows(self, slots, layer: int = 0):
+        """The keys and values of cache rows, (n, kv_heads, head_dim) each; rows outside the pool are zero."""
+        slots = np.ascontiguousarray(slots, np.int32).ravel()
+        ds = DeviceArray.from_numpy(slots)
+        k, v = (DeviceArray((slots.size, self.kv_heads, self.head_dim), np.float32) for _ in range(2))
+        kp, vp = self._pools(layer)
+        _lib.check(_lib.load().cthip_kv_rows_paged_q4(k.ptr, v.ptr, kp, vp, ds.ptr, slots.size, self.n_pages, self.kv_heads, self.head_dim))
+        return k.numpy(), v.numpy()
+
+    def attend(self, q, tables, lens, starts, layer: int = 0) -> np.ndarray:
+        """q (rows, heads, head_dim): rows starts[i] .. starts[i + 1] are the last ones of sequence i, which holds lens[i] keys."""
+        q = np.ascontiguousarray(q, np.float32)
+        n_rows, heads, dh = q.shape
+        if dh != self.head_dim:
+            raise ValueError(f"PagedCacheQ4.attend: heads of {dh}, the cache's have {self.head_dim}")
+        tables, lens, starts = (np.ascontiguousarray(a, np.int32) for a in (tables, lens, starts))
+        if tables.ndim != 2 or tables.shape[0] != lens.size or starts.size != lens.size + 1:
+            raise ValueError(f"PagedCacheQ4.attend: a table of shape {tables.shape}, {lens.size} lengths, {starts.size} starts")
+        dq, dt, dl, ds = (DeviceArray.from_numpy(a) for a in (q, tables, lens, starts))
+        out = DeviceArray(q.shape, np.float32)
+        kp, vp = self._pools(layer)
+        _lib.check(_lib.load().cthip_sdpa_paged_q4(out.ptr, dq.ptr, heads * dh, kp, vp, self.n_pages, dt.ptr, tables.shape[1], dl.ptr, ds.ptr, lens.size, n_rows, heads,
+                                                   self.kv_heads, dh, self.workspace.ptr))
+        return out.numpy()
+
+    def reorder(self, tables, lens, parents, history=None, tokens=None, step: int = 0):
+        """A beam search's reordering (cthip_beam_reorder_paged_q4) in all layers: `parents` (requests, beams), `lens` per
+        request, `tables` (requests * beams, stride).  Returns the new tables, and the new history where one is given."""
+        tables, lens, parents = (np.ascontiguousarray(a, np.int32) for a in (tables, lens, parents))
+        if parents.ndim != 2 or lens.size != parents.shape[0] or tables.ndim != 2 or tables.shape[0] != parents.size:
+            raise ValueError(f"PagedCacheQ4.reorder: parents {parents.shape}, {lens.size} lengths, a table of shape {tables.shape}")
+        dt, dl, dp = (DeviceArray.from_numpy(a) for a in (tables, lens, parents))
+        out = DeviceArray(tables.shape, np.int32)
+        dh = do = dtok = dstep = None
+        cols = 0
+        if history is not None:
+            history, tokens = np.ascontiguousarray(history, np.int32), np.ascontiguousarray(tokens, np.int32)
+            if history.ndim != 2 or history.shape[0] != parents.size or tokens.size != parents.size:
+                raise ValueError(f"PagedCacheQ4.reorder: a history of shape {history.shape} and {tokens.size} tokens for {parents.size} beams")
+            cols = history.shape[1]
+            dh, dtok, dstep, do = DeviceArray.from_numpy(history), DeviceArray.from_numpy(tokens), DeviceArray.from_numpy(np.array([step], np.int32)), DeviceArray(history.shape, np.int32)
+        _lib.check(_lib.load().cthip_beam_reorder_paged_q4(out.ptr, _p(do), self.k.ptr, self.v.ptr, self.layers, self.n_pages, dt.ptr, tables.shape[1], dl.ptr, dp.ptr, parents.shape[0],
+                                                           parents.shape[1], self.kv_heads, self.head_dim, _p(dh), cols, _p(dtok), _p(dstep)))
+        return out.numpy() if history is None else (out.numpy(), do.numpy())
+
+
+def beam_select(logits, scores, finished=None, eos: int = -1) -> dict:
+    """The best continuations of each request's beams (cthip_beam_select): logits (requests, beams, vocab), scores (requests, beams)."""
+    logits, scores = np.ascontiguousarray(logits, np.float32), np.ascontiguousarray(scores, np.float32)
+    if logits.ndim != 3 or logits.shape[:2] != scores.shape:
+        raise ValueError(f"beam_select: logits {logits.shape}, scores {scores.shape}")
+    n, k, vocab = logits.shape
+    size = int(_lib.init().cthip_beam_select_workspace(n, k))
+    if size < 0:
+        _lib.check(size)
+    dl, dsc, ws = DeviceArray.from_numpy(logits), DeviceArray.from_numpy(scores), DeviceArray((size,), np.uint8)
+    df = _dev(finished, np.int32)
+    tokens, parents, done = (DeviceArray((n, k), np.int32) for _ in range(3))
+    best = DeviceArray((n, k), np.float32)
+    _lib.check(_lib.load().cthip_beam_select(tokens.ptr, parents.ptr, best.ptr, done.ptr, dl.ptr, vocab, dsc.ptr, _p(df), n, k, vocab, eos, ws.ptr))
+    return dict(tokens=tokens.numpy(), parents=parents.numpy(), scores=best.numpy(), finished=done.numpy())

@@ -365,6 +365,69 @@ int cthip_kv_append_paged(void *const *k_pages, void *const *v_pages, const floa
 int cthip_sdpa_cached_paged(float *out, const float *q, const void *const *k_pages, const void *const *v_pages, int T, int H, int Hkv,
                             int Dh);
 
+/* ---- many sequences over one pool of pages, rows in 4 bits; beam search ----
+ * The reference decodes one sequence over a dense fp32 cache (layers.lisp:19-33, apps/gpt2/gpt2.lisp:97-113).  A step of a
+ * batch is cthip_kv_plan_paged, then per layer cthip_kv_append_paged_q4 and cthip_sdpa_paged_q4, then cthip_argmax or
+ * cthip_beam_select and cthip_beam_reorder_paged_q4; lengths, tables and page ids stay on the device, so a step can be
+ * captured into a graph and replayed.  All arrays are device memory, indices int32, arrays of different arguments
+ * do not overlap unless an entry says so.
+ * Pages: cthip_kv_page_rows() rows of every key / value head; a pool is (n_pages, cthip_kv_page_bytes_q4) bytes for the keys
+ * and the same for the values, 16-byte aligned.  A row's block of 32 channels is an fp16 scale and 32 numbers -8 .. 7 (4.5
+ * bits per channel); the layout inside a page is described in caten_amd/csrc/kv4.h.  head_dim 32, 64 or 128. */
+int64_t cthip_kv_page_bytes_q4(int kv_heads, int head_dim); /* of one page of keys, or of values; negative on error */
+/* Block tables and slot maps.  Sequence i holds lens[i] rows and gets new_lens[i] more (0: it sits this step out).
+ *   starts (n_seqs + 1)     first of the step's rows of each sequence, then their number
+ *   tables (n_seqs, table_stride)  page ids of each sequence; entries of pages opened by this call are written
+ *   slots, positions (max_rows)    of each of the step's rows: page id * rows of a page + row in the page, and its position in
+ *                           its sequence; -1 behind the last row.  positions may be NULL
+ *   lens_out, n_free_out    lens + new_lens, and what is left of the free pages; may be lens / n_free themselves
+ * free_pages is a stack of n_free[0] page ids: pages are taken from its end, in the order of the sequences, and the array
+ * itself is not changed.  A sequence is refused whole -- length kept, slots and positions -1, no pages -- where a count is
+ * negative, its table row or max_rows is too short, or too few pages are left; once pages have run out, every later
+ * sequence that needs one is refused too.  refused[0] is their number: such a sequence's rows must not be attended.  At most 4096 sequences. */
+int cthip_kv_plan_paged(int *slots, int *positions, int *starts, int *tables, int table_stride, int *lens_out, int *n_free_out, int *refused,
+                        const int *lens, const int *new_lens, int n_seqs, const int *free_pages, const int *n_free, int max_rows);
+/* Key and value rows (n_rows, kv_heads * head_dim), k_stride / v_stride floats apart (they may be slices of a fused product),
+ * into the cache rows their slots name; a slot outside the pool (-1) is skipped, two rows with one slot are undefined.  Per block
+ * of 32: m = the value of largest magnitude (the positive one of two), d = fp16(m / -8) held within +-65504, number =
+ * clamp(floor(x / d + 8.5), 0, 15) - 8, decided exactly; a block with an infinity or a NaN reads back as NaN.
+ * cthip_kv_rows_paged_q4 is the way back: (n_rows, kv_heads * head_dim) fp32, contiguous; rows whose slot is outside
+ * the pool are left as they were; either of k_rows / v_rows may be NULL. */
+int cthip_kv_append_paged_q4(void *k_pages, void *v_pages, const float *k_rows, const float *v_rows, int64_t k_stride, int64_t v_stride, const int *slots,
+                             int n_rows, int n_pages, int kv_heads, int head_dim);
+int cthip_kv_rows_paged_q4(float *k_rows, float *v_rows, const void *k_pages, const void *v_pages, const int *slots, int n_rows, int n_pages, int kv_heads,
+                           int head_dim);
+/* Attention (layers.lisp:3-5) of a ragged batch over the cache.  Rows starts[i] .. starts[i + 1] - 1 of q are the last rows of
+ * sequence i, which holds lens[i] keys (those rows' own among them): each sees the keys up to its own position.  One row a
+ * sequence is a decode step, more are a prompt or a piece of one.  q rows are (H, Dh), q_stride floats apart; out (n_rows, H,
+ * Dh) contiguous, not q.  A row that sees no key is zero; rows behind starts[n_seqs] are left as they were; a table entry outside the pool is
+ * a page without keys.  fp32 sums; q and the probabilities enter the integer products with 22 bits.
+ * workspace: cthip_sdpa_paged_q4_workspace(Dh) = 4 * (2048 + 2048 * 16 * (Dh + 2)) bytes, 16-byte aligned, zeroed once
+ * (cthip_alloc does); every call leaves it ready for the next.  Calls that may overlap (graphs replayed on other streams) need one each. */
+int64_t cthip_sdpa_paged_q4_workspace(int Dh);
+int cthip_sdpa_paged_q4(float *out, const float *q, int64_t q_stride, const void *k_pages, const void *v_pages, int n_pages, const int *tables, int table_stride,
+                        const int *lens, const int *starts, int n_seqs, int n_rows, int H, int Hkv, int Dh, void *workspace);
+/* The n_beams best continuations of each request: candidates (beam, token) score scores[beam] + log softmax(logits[beam])[token];
+ * a finished beam (finished may be NULL) has one, its eos with its score as it is.  Highest score first; ties go to the lower
+ * beam, then to the higher logit, then to the lower token.  NaN logits and scores count as minus infinity, and a
+ * candidate of minus infinity is taken only where nothing else is left.  logits rows (n_batch * n_beams, vocab), logits_stride
+ * floats apart; scores, finished and the outputs (n_batch, n_beams); parents count within the request; finished_out (may be
+ * NULL) = the parent's, or token == eos; eos -1 = none.  n_beams 1 .. 32, vocab >= n_beams.  Not in place.
+ * workspace: cthip_beam_select_workspace(...) = 256 + 4 n_batch + 32 n_batch n_beams (24 + 8 n_beams) bytes, as above. */
+int64_t cthip_beam_select_workspace(int n_batch, int n_beams);
+int cthip_beam_select(int *tokens, int *parents, float *scores_out, int *finished_out, const float *logits, int64_t logits_stride, const float *scores,
+                      const int *finished, int n_batch, int n_beams, int vocab, int eos, void *workspace);
+/* What the beams hold follows them: beam j of request i becomes a child of parents[i][j] (a parent outside 0 .. n_beams - 1
+ * counts as j itself).  The beams of a request hold lens[i] rows each and share their full pages; a partly filled last page
+ * is each beam's own.  Row j of tables_out is the parent's row of tables up to the last page; the last page is the parent's own
+ * for its first child, and for further ones the page of a beam without children, into which the parent's is copied in
+ * all n_layers pools ((n_layers, n_pages, page bytes) each); behind it row j of tables.  history_out (n_batch * n_beams, cols; may be NULL):
+ * the parent's row of history with tokens[j] in column step[0].  tables_out and history_out are not in place.  At most 32 beams,
+ * 65535 beams of all requests. */
+int cthip_beam_reorder_paged_q4(int *tables_out, int *history_out, void *k_pages, void *v_pages, int n_layers, int n_pages, const int *tables, int table_stride,
+                                const int *lens, const int *parents, int n_batch, int n_beams, int kv_heads, int head_dim, const int *history, int cols,
+                                const int *tokens, const int *step);
+
 /* ================================================================== */
 /* Decoder session: Transformer (external/llm/layers.lisp:73-90) and   */
 /* the gpt2-generate loop (apps/gpt2/gpt2.lisp:97-113)                 */
