@@ -1,8 +1,10 @@
 // Attention of a ragged batch of query rows over the 4-bit paged cache (layout: kv4.h).  The reference attends one sequence over
 // a dense fp32 cache (external/llm/layers.lisp:3-5,19-33).
+#include <algorithm>
 #include <type_traits>
 
 #include "kv4.h"
+#include "planes.h"
 
 namespace cthip {
 
@@ -13,7 +15,8 @@ struct Kv4Attn {
   const int *tables, *lens, *starts;
   int64_t q_stride;
   int n_pages, table_stride, n_seqs, n_rows, H, Hkv;
-  int unit;        // pages are counted in units of 2^unit where they are shared out
+  int group;       // query heads of a key / value head
+  int piece_log2;  // pages are shared out in pieces of this many
   int *tickets;    // workspace: a counter per job that is shared, zero between calls
   float *parts;    // and the shares' records: 16 rows of unnormalised outputs, their maxima, their sums
 };
@@ -23,12 +26,12 @@ typedef _Float16 half4 __attribute__((ext_vector_type(4)));
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef float f2_any __attribute__((ext_vector_type(2), aligned(4)));  // an 8-byte access at 4-byte alignment
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
-constexpr int kTileRows = 16;        // rows (query row, query head of the group) of a tile
-constexpr int kTargetGroups = 1024;  // workgroups that the pages are shared out to
-constexpr int kSplitSlots = 2048;    // records of shares in the workspace
-constexpr int kMaxShares = 64;
+constexpr int kTileRows = 16;       // rows (query row, query head of the group) of a tile
+constexpr int kSplitSlots = 2048;   // records of shares in the workspace, two a workgroup
+constexpr int kMaxShares = 64;      // of one tile: their records are added up by one workgroup
 
 // sum over the lanes up to this one
 __device__ __forceinline__ int wave_scan_int(int v) {
@@ -41,74 +44,82 @@ __device__ __forceinline__ int wave_scan_int(int v) {
   return v;
 }
 
-// Which part of the batch a workgroup takes.  A job is a tile of rows of one key / value head of one sequence; a job with many
-// pages is shared by several workgroups.  The lengths are on the device only, so every wavefront works the division out for
-// itself: pages of all jobs / kTargetGroups = pages of a share, and the running sum of jobs x shares says whose share this is.
-struct Share {
-  int seq, head, tile;
-  int len, rows, row0;    // of the sequence: keys, rows of this step and the first of them
-  int first, pages, per;  // this share's first page, the job's pages, the pages of a share
-  int share, shares;      // of the job
-  int slot;               // of the job's first record
+// Which part of the batch a workgroup takes.  A job is a tile of rows of one key / value head of one sequence.  Its cost is
+// its pages in pieces of `piece` (four, one a wavefront, or more where numbers would not fit 32 bits) and one piece for what a job costs
+// besides; the jobs' costs laid end to end are cut into as many equal parts as workgroups run at once, so that a long sequence is
+// shared by many workgroups and many short ones go to one.  The lengths are on the device only: every wavefront works
+// the division out for itself, 64 sequences at a time.
+struct Batch {
+  int first = 0, before = 0;  // of the 64 sequences in the lanes: the first, and the cost in front of it
+  int len, row0, rows, tiles, cost, upto;  // this lane's; cost: of one job; upto: of all up to the end of this sequence
+  // A wavefront keeps them in LDS while it works on a job: they are needed again for the next one only.
+  __device__ __forceinline__ void put(int (*to)[64]) const {
+    const int l = threadIdx.x & 63;
+    to[0][l] = len, to[1][l] = row0, to[2][l] = rows, to[3][l] = tiles, to[4][l] = cost, to[5][l] = upto;
+  }
+  __device__ __forceinline__ void get(const int (*from)[64]) {
+    const int l = threadIdx.x & 63;
+    len = from[0][l], row0 = from[1][l], rows = from[2][l], tiles = from[3][l], cost = from[4][l], upto = from[5][l];
+  }
 };
-__device__ __forceinline__ bool find_share(const Kv4Attn &a, int id, Share &w) {
-  const int lane = threadIdx.x & 63, G = a.H / a.Hkv;
-  const int64_t most = (int64_t)a.table_stride * kKvPageRows;
-  auto look = [&](int i, int &len, int &row0, int &rows, int &tiles, int &pages) {
-    len = 0, row0 = 0, rows = 0;
-    if (i < a.n_seqs) {
-      len = a.lens[i], row0 = a.starts[i];
-      const int end = min(a.starts[i + 1], a.n_rows);
-      rows = row0 >= 0 && end > row0 ? end - row0 : 0;
-    }
-    tiles = (rows * G + kTileRows - 1) / kTileRows;
-    pages = a.n_pages > 0 && len > 0 ? (int)((min((int64_t)len, most) + kKvPageRows - 1) / kKvPageRows) : 0;
-  };
-  int len, row0, rows, tiles, pages;
-  int64_t total = 0;
-  int longest = 0;
-  for (int i0 = 0; i0 < a.n_seqs; i0 += 64) {
-    look(i0 + lane, len, row0, rows, tiles, pages);
-    // (in units of 2^unit pages, rounded up, so that 64 sequences' sum fits: the launcher chooses)
-    const int sum = wave_scan_int(tiles * a.Hkv * ((pages >> a.unit) + 1));
-    total += __builtin_amdgcn_readlane(sum, 63);
-    int p = tiles ? pages : 0;
-    for (int o = 32; o > 0; o >>= 1) p = max(p, __shfl_xor(p, o, 64));
-    longest = max(longest, p);
+__device__ __forceinline__ void look(const Kv4Attn &a, Batch &s) {
+  const int i = s.first + (int)(threadIdx.x & 63);
+  s.len = 0, s.row0 = 0, s.rows = 0;
+  if (i < a.n_seqs) {
+    s.len = a.lens[i], s.row0 = a.starts[i];
+    const int end = min(a.starts[i + 1], a.n_rows);
+    s.rows = s.row0 >= 0 && end > s.row0 ? end - s.row0 : 0;
   }
-  int64_t per = ((total + kTargetGroups - 1) / kTargetGroups) << a.unit;
-  per = max(per, (int64_t)(longest + kMaxShares - 1) / kMaxShares);
-  w.per = (int)min((per + 3) / 4 * 4, (int64_t)1 << 30);  // four wavefronts take pages in turn
-  int before = 0, slots = 0;
-  for (int i0 = 0; i0 < a.n_seqs; i0 += 64) {
-    if (a.n_seqs > 64) look(i0 + lane, len, row0, rows, tiles, pages);
-    const int shares = max(1, (pages + w.per - 1) / w.per), jobs = tiles * a.Hkv;
-    const int sum = wave_scan_int(jobs * shares), sums = wave_scan_int(shares > 1 ? jobs * shares : 0);
-    const unsigned long long past = __ballot(before + sum > id);
-    if (past) {
-      const int l = (int)__builtin_ctzll(past);
-      const int mine = __builtin_amdgcn_readlane(sum, l) - __builtin_amdgcn_readlane(jobs * shares, l);
-      const int at = id - before - mine;
-      w.shares = __builtin_amdgcn_readlane(shares, l);
-      // (starts that overlap can sum to anything: such rows are nobody's)
-      if ((unsigned)at >= (unsigned)__builtin_amdgcn_readlane(jobs * shares, l)) return false;
-      const int job = at / w.shares, nt = __builtin_amdgcn_readlane(tiles, l);
-      w.share = at - job * w.shares;
-      w.head = job / nt;
-      w.tile = job - w.head * nt;
-      w.seq = i0 + l;
-      w.len = __builtin_amdgcn_readlane(len, l);
-      w.rows = __builtin_amdgcn_readlane(rows, l);
-      w.row0 = __builtin_amdgcn_readlane(row0, l);
-      w.pages = __builtin_amdgcn_readlane(pages, l);
-      w.slot = slots + __builtin_amdgcn_readlane(sums, l) - __builtin_amdgcn_readlane(shares > 1 ? jobs * shares : 0, l) + job * w.shares;
-      return w.shares == 1 || (unsigned)w.slot <= (unsigned)(kSplitSlots - w.shares);
-    }
-    before += __builtin_amdgcn_readlane(sum, 63);
-    slots += __builtin_amdgcn_readlane(sums, 63);
-  }
-  return false;
+  s.tiles = (s.rows * a.group + kTileRows - 1) / kTileRows;
+  const int pages = a.n_pages > 0 && s.len > 0 ? (int)min(((unsigned)s.len + kKvPageRows - 1) / kKvPageRows, (unsigned)a.table_stride) : 0;
+  s.cost = (pages + (1 << a.piece_log2) - 1 >> a.piece_log2) + 1;
+  s.upto = s.before + wave_scan_int(s.tiles * a.Hkv * s.cost);
 }
+struct Job {
+  int seq, head, tile;
+  int len, rows, row0;  // of the sequence: keys, rows of this step and the first of them
+  int at, cost;         // its place on the line of all costs
+};
+// the job at a place on the line, which lies in front of its end
+__device__ __forceinline__ bool find_job(const Kv4Attn &a, int &first, int &before, int (*kept)[64], int place, Job &j) {
+  Batch s;
+  s.first = first, s.before = before;
+  s.get(kept);
+  unsigned long long past;
+  while (!(past = __ballot(s.upto > place))) {
+    if (s.first + 64 >= a.n_seqs) return false;
+    s.before = __builtin_amdgcn_readlane(s.upto, 63);
+    s.first += 64;
+    look(a, s);
+    s.put(kept);
+  }
+  first = s.first, before = s.before;
+  const int l = (int)__builtin_ctzll(past);
+  const int tiles = __builtin_amdgcn_readlane(s.tiles, l), all = tiles * a.Hkv;
+  j.cost = __builtin_amdgcn_readlane(s.cost, l);
+  const int start = __builtin_amdgcn_readlane(s.upto, l) - all * j.cost, job = (place - start) / j.cost;
+  // (starts that overlap can sum to anything: such rows are nobody's)
+  if (place < start || job >= all) return false;
+  j.at = start + job * j.cost;
+  j.seq = s.first + l;
+  j.head = job / tiles;
+  // tiles from both ends in turn: in a prompt's own pages late rows see more than early ones, and a workgroup gets some of each
+  const int t = job - j.head * tiles;
+  j.tile = t & 1 ? tiles - 1 - (t >> 1) : t >> 1;
+  j.len = __builtin_amdgcn_readlane(s.len, l);
+  j.rows = __builtin_amdgcn_readlane(s.rows, l);
+  j.row0 = __builtin_amdgcn_readlane(s.row0, l);
+  return true;
+}
+
+// The pages come straight into LDS, two of them on their way beside the one that is worked on: a wavefront's ring of two, each the
+// keys and the values of a head as they lie in memory.
+template <int DH>
+struct Kv4Lds {
+  static constexpr int HEAD = 36 * DH, SLOT = 2 * HEAD, WAVE = 2 * SLOT, STATS = 4 * WAVE, SEQS = STATS + 14 * kTileRows * 4, BYTES = SEQS + 4 * 6 * 64 * 4;
+  static constexpr int REQUESTS = DH / 32 + (DH / 32 + 1) / 2;  // of a head's part of a page: 16 bytes a lane, then 4
+  static_assert(WAVE >= kTileRows * (DH + 4) * 4 && 4 * WAVE >= 8 * kMaxShares * kTileRows, "results and shares in the pages' place");
+};
 
 // One page for one wavefront and 16 rows.  S^T = K Q^T and O^T = V^T P^T: the row is the lane's number modulo 16 throughout (scores,
 // maxima, sums and outputs), lane group g = lane / 16 holds keys 16 s + 4 g + i of the page and channels 4 g + i of a result tile.
@@ -119,17 +130,44 @@ __device__ __forceinline__ bool find_share(const Kv4Attn &a, int id, Share &w) {
 //           scale seen so far to 2^13: products down to 2^-27 of p = 1 at that scale keep their 22 bits, smaller ones lie on a grid
 //           of 2^-38 of it.  It goes into the exponent of p, so that sums and outputs carry it alike.
 template <int DH>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k_kv4_attn(Kv4Attn a) {
-  constexpr int NB = DH / 32, PITCH = DH + 4;
-  __shared__ float s_o[4][kTileRows][PITCH];
-  __shared__ float s_m[4][kTileRows], s_l[4][kTileRows], s_w[4][kTileRows];
-  __shared__ float s_sum[kTileRows];
-  __shared__ __attribute__((aligned(16))) unsigned char s_scale[4][2][kKvPageRows * NB * 2];
-  __shared__ int s_ticket;
-  Share w;
-  if (!find_share(a, blockIdx.x, w)) return;
-  const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 15, g = lane >> 4;
-  const int G = a.H / a.Hkv;
+__global__ __launch_bounds__(256, DH == 128 ? 2 : DH == 64 ? 3 : 4) void k_kv4_attn(Kv4Attn a) {
+  using L = Kv4Lds<DH>;
+  constexpr int NB = DH / 32;
+  extern __shared__ __align__(16) unsigned char smem[];
+  float (*s_m)[kTileRows] = (float (*)[kTileRows])(smem + L::STATS), (*s_l)[kTileRows] = s_m + 4, (*s_w)[kTileRows] = s_m + 8, *s_sum = s_m[12];
+  int *s_ticket = (int *)s_m[13];
+  int (*s_seqs)[6][64] = (int (*)[6][64])(smem + L::SEQS);
+  // a wavefront's results lie where its own pages did
+  auto s_o = [&](int wave, int row) { return (float *)(smem + wave * L::WAVE) + row * (DH + 4); };
+  const int tid0 = threadIdx.x, wv = __builtin_amdgcn_readfirstlane(tid0 >> 6);
+  const int G = a.group;
+  // workgroups are dealt to the eight XCDs in turn: neighbours on the line, which may read the same pages, on one of them
+  const int me = (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
+  int total = 0, longest = 0, first = 0, before = 0;
+  {
+    Batch s;
+    for (look(a, s);;) {
+      int c = s.tiles ? s.cost : 0;
+      for (int o = 32; o > 0; o >>= 1) c = max(c, __shfl_xor(c, o, 64));
+      longest = max(longest, __builtin_amdgcn_readfirstlane(c));
+      total = __builtin_amdgcn_readlane(s.upto, 63);
+      if (s.first == 0) s.put(s_seqs[wv]);
+      if (s.first + 64 >= a.n_seqs) break;
+      s.before = total;
+      s.first += 64;
+      look(a, s);
+    }
+  }
+  const int per = max((int)(((unsigned)total + gridDim.x - 1) / gridDim.x), (longest + kMaxShares - 2) / (kMaxShares - 1));
+  const int x0 = (int)min((int64_t)me * per, (int64_t)total), x1 = min(total - x0, per) + x0;
+  for (int x = x0; x < x1;) {
+  Job w;
+  if (!find_job(a, first, before, s_seqs[wv], x, w)) break;
+  x = w.at + w.cost;
+  // (what hangs on the lane alone is worked out for each job: kept from being moved in front of the loop, where it would hold registers)
+  int lane = tid0 & 63;
+  asm volatile("" : "+v"(lane));
+  const int n = lane & 15, g = lane >> 4;
   // this lane's row
   const int rho = w.tile * kTileRows + n, j = rho / G;
   const bool active = j < w.rows;
@@ -140,10 +178,25 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
   const int j1 = min(w.rows - 1, (w.tile * kTileRows + kTileRows - 1) / G), j0 = w.tile * kTileRows / G;
   const int last = (int)min((int64_t)w.len - w.rows + j1, all - 1), least = (int)min((int64_t)w.len - w.rows + j0, all - 1);
   const int pages = a.n_pages > 0 && last >= 0 ? last / kKvPageRows + 1 : 0;
-  const int shares = max(1, (pages + w.per - 1) / w.per);  // (at most w.shares: a row of the sequence's last tile sees the most)
-  if (w.share >= shares) return;
-  const int p0 = w.share * w.per, p1 = min(pages, p0 + w.per);
+  // its pieces lie on the line behind the one that stands for the rest (a job without pages is one piece of none)
+  const int pieces = max(1, pages + (1 << a.piece_log2) - 1 >> a.piece_log2), line = w.at + 1;
+  const int owner = line / per, shares = (line + pieces - 1) / per - owner + 1, share = me - owner;
+  const int from_piece = max(x0 - line, 0), to_piece = min(x1 - line, pieces);
+  if (from_piece >= to_piece) continue;
+  const int p0 = from_piece << a.piece_log2, p1 = (int)min((int64_t)pages, (int64_t)to_piece << a.piece_log2);
 
+  // page ids of the next 64 pages of this wavefront, one a lane
+  const int *table = a.tables + (int64_t)w.seq * a.table_stride;
+  int ids = 0, ids_from = -1;
+  auto page_id = [&](int k) {  // k: this wavefront's k-th page (the same in every lane)
+    if (ids_from < 0 || k >= ids_from + 64) {
+      ids_from = k;
+      const int p = p0 + wv + 4 * (k + lane);
+      ids = p < p1 ? table[p] : -1;
+      asm volatile("" : "+v"(ids));  // (waited for here: behind the branch it would be waited for with all pages on their way, page after page)
+    }
+    return __builtin_amdgcn_readlane(ids, k - ids_from);
+  };
   half8 q_hi[NB], q_lo[NB];
   float weight;
   {
@@ -191,50 +244,28 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
   float m = -INFINITY, l = 0.0f;
   int c = 100;  // (no scale seen)
 
-  // page ids of the next 64 pages of this wavefront, one a lane
-  const int *table = a.tables + (int64_t)w.seq * a.table_stride;
-  const int head_bytes = kv4_head_bytes(DH);
-  int ids = 0, ids_from = -1;
-  auto page_id = [&](int k) {  // k: this wavefront's k-th page (the same in every lane)
-    if (ids_from < 0 || k >= ids_from + 64) {
-      ids_from = k;
-      const int p = p0 + wv + 4 * (k + lane);
-      ids = p < p1 ? table[p] : -1;
+  const int mine = p0 + wv < p1 ? (p1 - p0 - wv + 3) / 4 : 0;  // pages of this wavefront
+  auto valid = [&](int id) { return id >= 0 && id < a.n_pages; };
+  const unsigned char *ring = smem + wv * L::WAVE;
+  const unsigned ring_at = (unsigned)(size_t)(__attribute__((address_space(3))) const unsigned char *)ring;
+  // a head's part of a page (an absent page's is page 0's: its rows are masked)
+  auto ask = [&](const unsigned char *pool, int id, unsigned to) {
+    const unsigned char *p = uniform(pool + ((int64_t)(valid(id) ? id : 0) * a.Hkv + w.head) * L::HEAD);
+#pragma unroll
+    for (int i = 0; i < NB; i++) dma16(p + 1024 * i, 16 * lane, to + 1024 * i);
+    if (NB > 1) {
+#pragma unroll
+      for (int i = 0; i < NB / 2; i++) dma4(p + 1024 * NB + 256 * i, 4 * lane, to + 1024 * NB + 256 * i);
+    } else if (lane < 32) {
+      dma4(p + 1024, 4 * lane, to + 1024);
     }
-    return __builtin_amdgcn_readlane(ids, k - ids_from);
   };
-  // A page's quants come straight to the lanes that multiply them; its scales, which 16 lanes share, come as one piece a lane
-  // and go through LDS (read by the lanes from memory they were 64 registers and 16 loads a page).
-  typedef uint32_t kdw __attribute__((ext_vector_type(NB)));
-  typedef unsigned short sdw __attribute__((ext_vector_type(NB)));
-  kdw kq[4];
-  u32x4 vq[NB];
-  sdw ks, vs;
-  int id_k = -1, id_v = -1;
-  auto ask_k = [&](int k) {
-    id_k = page_id(k);
-    const unsigned char *p = a.k_pages + ((int64_t)(id_k >= 0 && id_k < a.n_pages ? id_k : 0) * a.Hkv + w.head) * head_bytes;
-#pragma unroll
-    for (int s = 0; s < 4; s++) kq[s] = *(const kdw *)(p + kv4_key_offset(16 * s + n, g, 0, DH));
-    ks = *(const sdw *)(p + 32 * DH + lane * NB * 2);
-  };
-  auto ask_v = [&](int id) {
-    id_v = id;
-    const unsigned char *p = a.v_pages + ((int64_t)(id >= 0 && id < a.n_pages ? id : 0) * a.Hkv + w.head) * head_bytes;
-#pragma unroll
-    for (int b = 0; b < NB; b++) vq[b] = *(const u32x4 *)(p + (b * 16 + n) * kKvPageRows + 16 * g);
-    vs = *(const sdw *)(p + 32 * DH + lane * NB * 2);
-  };
-  // the scales of block b, rows 16 t + 4 g ..
-  auto scales = [&](int which, int t, int b) {
-    return *(const half4 *)(s_scale[wv][which] + ((4 * t + g) * NB + b) * 8);
-  };
+  auto ask_k = [&](int id, int k) { ask(a.k_pages, id, ring_at + (k & 1) * L::SLOT); };
+  auto ask_v = [&](int id, int k) { ask(a.v_pages, id, ring_at + (k & 1) * L::SLOT + L::HEAD); };
+  int id0 = page_id(0), id1 = mine > 1 ? page_id(1) : -1, id2 = -1;
+  if (mine > 0) ask_k(id0, 0), ask_v(id0, 0);
+  if (mine > 1) ask_k(id1, 1), ask_v(id1, 1);
 
-  const int mine = p0 + wv < p1 ? (p1 - p0 - wv + 3) / 4 : 0;
-  if (mine > 0) {
-    ask_k(0);
-    ask_v(id_k);
-  }
   // numbers that the compiler does not see through: a * half + zero and half * minus + a are then one mixed instruction each, where a product
   // or a difference is a conversion more
   float zero = 0.0f, minus = -1.0f;
@@ -250,26 +281,36 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
   auto one_page = [&](auto whole, int k) {
     constexpr bool FULL = decltype(whole)::value;  // every row of the tile sees every row of the page
     const int page = p0 + wv + 4 * k;
-    const int from = FULL ? 0 : id_v >= 0 && id_v < a.n_pages ? page * kKvPageRows : INT_MAX - kKvPageRows;  // (absent: behind every limit)
-    *(sdw *)(s_scale[wv][0] + lane * NB * 2) = ks;
-    *(sdw *)(s_scale[wv][1] + lane * NB * 2) = vs;
-    const sdw vs_now = vs;
+    const int from = FULL ? 0 : valid(id0) ? page * kKvPageRows : INT_MAX - kKvPageRows;  // (absent: behind every limit)
+    const unsigned char *kp = ring + (k & 1) * L::SLOT, *vp = kp + L::HEAD;
+    // the scales of block b, rows 16 t + 4 g ..
+    auto scales = [&](const unsigned char *p, int t, int b) { return *(const half4 *)(p + 32 * DH + ((4 * t + g) * NB + b) * 8); };
+    typedef uint32_t kdw __attribute__((ext_vector_type(NB)));
+    typedef unsigned short sdw __attribute__((ext_vector_type(NB)));
+    // younger than this page's keys: its values, and both of the next page's
+    if (k + 1 < mine) wait_loads<3 * L::REQUESTS>();
+    else wait_loads<L::REQUESTS>();
     f32x4 s[4];
 #pragma unroll
     for (int t = 0; t < 4; t++) {
       s[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      const kdw kq = *(const kdw *)(kp + kv4_key_offset(16 * t + n, g, 0, DH));
 #pragma unroll
       for (int b = 0; b < NB; b++) {
-        const uint32_t u = kq[t][b] ^ 0x88888888u;
+        const uint32_t u = kq[b] ^ 0x88888888u;
         const half8 kk = numbers(u, u >> 4, u >> 8, u >> 12);
         f32x4 x = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk, q_lo[b], f32x4{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
         x = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk, q_hi[b], x, 0, 0, 0);
-        const half4 d = scales(0, t, b);
+        const half4 d = scales(kp, t, b);
 #pragma unroll
         for (int i = 0; i < 4; i++) s[t][i] = fmaf(x[i], (float)d[i], s[t][i]);
       }
     }
-    if (k + 1 < mine) ask_k(k + 1);
+    wait_lds();
+    if (k + 2 < mine) {
+      id2 = page_id(k + 2);
+      ask_k(id2, k);
+    }
     float top = -INFINITY;
 #pragma unroll
     for (int t = 0; t < 4; t++)
@@ -287,7 +328,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
 #pragma unroll
       for (int b = 0; b < NB; b++) o[b][0] *= corr, o[b][1] *= corr;
     }
+    if (k + 2 < mine) wait_loads<3 * L::REQUESTS>();
+    else if (k + 1 < mine) wait_loads<2 * L::REQUESTS>();
+    else wait_loads<0>();
     {
+      const sdw vs_now = *(const sdw *)(vp + 32 * DH + lane * NB * 2);
       float d = 0.0f;  // the largest scale of the page's rows that are there (each lane has a piece of the page's scales)
 #pragma unroll
       for (int x = 0; x < NB; x++) {
@@ -316,10 +361,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
       }
 #pragma unroll
     for (int b = 0; b < NB; b++) {
-      u32x4 hi[2], lo[2];  // rows 16 t + 4 g + (0, 2, 1, 3), t = 0 1 and 2 3
+      u32x4 vq, hi[2], lo[2];  // rows 16 t + 4 g + (0, 2, 1, 3), t = 0 1 and 2 3
 #pragma unroll
       for (int t = 0; t < 4; t++) {
-        const half4 d = scales(1, t, b);
+        const half4 d = scales(vp, t, b);
         float x[4];
 #pragma unroll
         for (int i = 0; i < 4; i++) {
@@ -337,7 +382,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
 #pragma unroll
       for (int part = 0; part < 2; part++) {
         const half8 ph = __builtin_bit_cast(half8, hi[part]), pl = __builtin_bit_cast(half8, lo[part]);
-        const uint32_t u0 = vq[b][2 * part] ^ 0x88888888u, u1 = vq[b][2 * part + 1] ^ 0x88888888u;
+        if (part == 0) vq = *(const u32x4 *)(vp + (b * 16 + n) * kKvPageRows + 16 * g);
+        const uint32_t u0 = vq[2 * part] ^ 0x88888888u, u1 = vq[2 * part + 1] ^ 0x88888888u;
 #pragma unroll
         for (int half = 0; half < 2; half++) {
           const half8 vv = numbers(u0 >> (4 * half), u0 >> (4 * half + 8), u1 >> (4 * half), u1 >> (4 * half + 8));
@@ -346,74 +392,111 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
         }
       }
     }
-    if (k + 1 < mine) ask_v(id_k);
+    wait_lds();
+    if (k + 2 < mine) ask_v(id2, k);
+    id0 = id1, id1 = id2;
   };
   for (int k = 0; k < mine; k++) {
-    if (id_v >= 0 && id_v < a.n_pages && (p0 + wv + 4 * k) * kKvPageRows + kKvPageRows - 1 <= least) one_page(std::true_type(), k);
+    if (valid(id0) && (p0 + wv + 4 * k) * kKvPageRows + kKvPageRows - 1 <= least) one_page(std::true_type(), k);
     else one_page(std::false_type(), k);
   }
   l += __shfl_xor(l, 16, 64);
   l += __shfl_xor(l, 32, 64);
 
-  // the four wavefronts' results meet
+  // the four wavefronts' results meet (and what hangs on the thread alone, here)
+  int tid = tid0;
+  asm volatile("" : "+v"(tid));
+  const int nr = min(kTileRows, w.rows * G - w.tile * kTileRows);  // rows of the tile that there are
   if (g == 0) s_m[wv][n] = m * weight - (float)c, s_l[wv][n] = l;
+  if (n < nr) {
 #pragma unroll
-  for (int b = 0; b < NB; b++)
+    for (int b = 0; b < NB; b++)
 #pragma unroll
-    for (int half = 0; half < 2; half++) *(f32x4 *)&s_o[wv][n][b * 32 + half * 16 + 4 * g] = o[b][half];
+      for (int half = 0; half < 2; half++) *(f32x4 *)(s_o(wv, n) + b * 32 + half * 16 + 4 * g) = o[b][half];
+  }
   __syncthreads();
-  float *record = a.parts + (int64_t)(w.slot + w.share) * kTileRows * (DH + 2);
-  if (tid < kTileRows) {
-    float M = -INFINITY, L = 0.0f;
+  // a share that goes on from the workgroup before, and one that goes on in the next: a workgroup has one of each at most
+  auto record_of = [&](int k) { return a.parts + (int64_t)(2 * (owner + k) + (k == 0)) * kTileRows * (DH + 2); };
+  auto weight_of = [](float mk, float lk, float M) { return mk > -INFINITY ? __builtin_amdgcn_exp2f(mk - M) : lk == lk ? 0.0f : 1.0f; };  // (a NaN stays one)
+  if (tid < nr) {
+    float M = -INFINITY, sum = 0.0f;
+#pragma unroll
     for (int x = 0; x < 4; x++) M = fmaxf(M, s_m[x][tid]);
+#pragma unroll
     for (int x = 0; x < 4; x++) {
-      const float e = s_m[x][tid] > -INFINITY ? __builtin_amdgcn_exp2f(s_m[x][tid] - M) : s_l[x][tid] == s_l[x][tid] ? 0.0f : 1.0f;
+      const float e = weight_of(s_m[x][tid], s_l[x][tid], M);
       s_w[x][tid] = e;
-      L = fmaf(e, s_l[x][tid], L);
+      sum = fmaf(e, s_l[x][tid], sum);
     }
-    s_sum[tid] = L;
+    s_sum[tid] = sum;
     if (shares > 1) {
-      __hip_atomic_store(record + kTileRows * DH + tid, M, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      __hip_atomic_store(record + kTileRows * (DH + 1) + tid, L, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      float *to = record_of(share) + kTileRows * DH + 2 * tid;
+      __hip_atomic_store((unsigned long long *)to, __builtin_bit_cast(unsigned long long, (f32x2){M, sum}), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
   }
   __syncthreads();
-  for (int e = tid; e < kTileRows * DH; e += 256) {
-    const int r = e / DH, c = e % DH, rr = w.tile * kTileRows + r, jj = rr / G;
-    float x = 0.0f;
-    for (int k = 0; k < 4; k++) x = fmaf(s_w[k][r], s_o[k][r][c], x);
+  // where a pair of channels of a tile's row goes
+  auto out_at = [&](int r, int c) {
+    const int rr = w.tile * kTileRows + r, jj = rr / G;
+    return a.out + ((int64_t)(w.row0 + jj) * a.H + w.head * G + rr - jj * G) * DH + c;
+  };
+  for (int e = tid; e < nr * DH / 2; e += 256) {
+    const int r = e / (DH / 2), c = e % (DH / 2) * 2;
+    f32x2 x = {0.0f, 0.0f};
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      const f32x2 y = *(const f32x2 *)(s_o(k, r) + c);
+      x[0] = fmaf(s_w[k][r], y[0], x[0]), x[1] = fmaf(s_w[k][r], y[1], x[1]);
+    }
     if (shares > 1) {
-      __hip_atomic_store(record + e, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    } else if (jj < w.rows) {
-      const float L = s_sum[r];
-      a.out[((int64_t)(w.row0 + jj) * a.H + w.head * G + rr - jj * G) * DH + c] = L != 0.0f ? x / L : 0.0f;
+      __hip_atomic_store((unsigned long long *)(record_of(share) + 2 * e), __builtin_bit_cast(unsigned long long, x), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    } else {
+      const float sum = s_sum[r];
+      *(f2_any *)out_at(r, c) = sum != 0.0f ? f2_any{x[0] / sum, x[1] / sum} : f2_any{0.0f, 0.0f};
     }
   }
-  if (shares == 1) return;
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this thread's device-scope stores have reached memory
-  __syncthreads();
-  if (tid == 0) s_ticket = __hip_atomic_fetch_add(a.tickets + w.slot, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  __syncthreads();
-  if (s_ticket != shares - 1) return;  // (uniform)
-  // the last of the job's workgroups adds the shares up, in their order
-  if (tid == 0) __hip_atomic_store(a.tickets + w.slot, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);  // the next call counts again
-  const float *records = a.parts + (int64_t)w.slot * kTileRows * (DH + 2);
-  for (int e = tid; e < kTileRows * DH; e += 256) {
-    const int r = e / DH, c = e % DH, rr = w.tile * kTileRows + r, jj = rr / G;
-    if (jj >= w.rows) continue;
-    float M = -INFINITY, L = 0.0f, x = 0.0f;
-    for (int k = 0; k < shares; k++)
-      M = fmaxf(M, __hip_atomic_load(records + (int64_t)k * kTileRows * (DH + 2) + kTileRows * DH + r, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
-    for (int k = 0; k < shares; k++) {
-      const float *rec = records + (int64_t)k * kTileRows * (DH + 2);
-      const float mk = __hip_atomic_load(rec + kTileRows * DH + r, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      const float lk = __hip_atomic_load(rec + kTileRows * (DH + 1) + r, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      const float xk = __hip_atomic_load(rec + e, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      const float f = mk > -INFINITY ? __builtin_amdgcn_exp2f(mk - M) : lk == lk ? 0.0f : 1.0f;
-      L = fmaf(f, lk, L);
-      x = fmaf(f, xk, x);
+  if (shares > 1) {
+    int *tickets = a.tickets + 2 * owner;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this thread's device-scope stores have reached memory
+    __syncthreads();
+    if (tid == 0) *s_ticket = __hip_atomic_fetch_add(tickets, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    if (*s_ticket == shares - 1) {  // (uniform) the last of the job's workgroups adds the shares up, in their order
+      if (tid == 0) __hip_atomic_store(tickets, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);  // the next call counts again
+      // maxima and sums of all shares, asked for at once; then the outputs, eight shares at a time: a load after the other would be a round
+      // trip to memory for each share
+      f32x2 (*ml)[kTileRows] = (f32x2 (*)[kTileRows])smem;
+#pragma unroll
+      for (int k0 = 0; k0 < kMaxShares; k0 += 16) {
+        const int k = k0 + (tid >> 4), r = tid & 15;
+        if (k < shares && r < nr)
+          ml[k][r] = __builtin_bit_cast(f32x2, __hip_atomic_load((const unsigned long long *)(record_of(k) + kTileRows * DH + 2 * r), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+      }
+      __syncthreads();
+      for (int e = tid; e < nr * DH / 2; e += 256) {
+        const int r = e / (DH / 2), c = e % (DH / 2) * 2;
+        float M = -INFINITY, sum = 0.0f;
+        for (int k = 0; k < shares; k++) M = fmaxf(M, ml[k][r][0]);
+        f32x2 x = {0.0f, 0.0f};
+        for (int k0 = 0; k0 < shares; k0 += 8) {
+          unsigned long long y[8];
+#pragma unroll
+          for (int k = 0; k < 8; k++) y[k] = __hip_atomic_load((const unsigned long long *)(record_of(min(k0 + k, shares - 1)) + 2 * e), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+#pragma unroll
+          for (int k = 0; k < 8; k++) {
+            if (k0 + k < shares) {
+              const f32x2 z = __builtin_bit_cast(f32x2, y[k]), s = ml[k0 + k][r];
+              const float f = weight_of(s[0], s[1], M);
+              sum = fmaf(f, s[1], sum);
+              x[0] = fmaf(f, z[0], x[0]), x[1] = fmaf(f, z[1], x[1]);
+            }
+          }
+        }
+        *(f2_any *)out_at(r, c) = sum != 0.0f ? f2_any{x[0] / sum, x[1] / sum} : f2_any{0.0f, 0.0f};
+      }
     }
-    a.out[((int64_t)(w.row0 + jj) * a.H + w.head * G + rr - jj * G) * DH + c] = L != 0.0f ? x / L : 0.0f;
+  }
+  __syncthreads();  // the next job's results go through the same LDS
   }
 }
 
@@ -442,16 +525,20 @@ int cthip_sdpa_paged_q4(float *out, const float *q, int64_t q_stride, const void
   // rows of a tile share a key / value head: at most this many tiles of all sequences, and as many jobs a head
   const int64_t tiles = (int64_t)n_rows * (H / Hkv) / kTileRows + (n_seqs < n_rows ? n_seqs : n_rows), jobs = tiles * Hkv;
   if (jobs > (1 << 28)) return fail(CTHIP_E_UNSUPPORTED, "cthip_sdpa_paged_q4: %d rows of %d heads in one call", n_rows, H);
-  int unit = 0;
-  while (jobs * ((table_stride >> unit) + 1) > INT_MAX) unit++;
-  const Kv4Attn a = {out,   q,      (const unsigned char *)k_pages, (const unsigned char *)v_pages, tables, lens, starts, q_stride, n_pages, table_stride, n_seqs, n_rows, H, Hkv,
-                     unit,  (int *)workspace, (float *)workspace + kSplitSlots};
-  const dim3 grid((unsigned)(jobs + kTargetGroups)), block(256);
+  int piece = 2;
+  while (jobs * ((table_stride >> piece) + 2) > INT_MAX / 2) piece++;
+  // as many workgroups as run at once (two, three or four a compute unit for their registers), a multiple of the XCDs
+  const int at_once = std::min(kSplitSlots / 2, state().compute_units * (Dh == 128 ? 2 : Dh == 64 ? 3 : 4) / 8 * 8);
+  const Kv4Attn a = {out,     q,     (const unsigned char *)k_pages, (const unsigned char *)v_pages, tables, lens, starts, q_stride, n_pages, table_stride, n_seqs, n_rows, H, Hkv,
+                     H / Hkv, piece, (int *)workspace, (float *)workspace + kSplitSlots};
+  const dim3 grid((unsigned)at_once), block(256);
+#define ATT(DH_) hipLaunchKernelGGL(k_kv4_attn<DH_>, grid, block, Kv4Lds<DH_>::BYTES, state().stream, a)
   switch (Dh) {
-    case 32: hipLaunchKernelGGL(k_kv4_attn<32>, grid, block, 0, state().stream, a); break;
-    case 64: hipLaunchKernelGGL(k_kv4_attn<64>, grid, block, 0, state().stream, a); break;
-    default: hipLaunchKernelGGL(k_kv4_attn<128>, grid, block, 0, state().stream, a); break;
+    case 32: ATT(32); break;
+    case 64: ATT(64); break;
+    default: ATT(128); break;
   }
+#undef ATT
   CTHIP_LAUNCH_CHECK();
   return 0;
 }
