@@ -31,6 +31,7 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kTileRows = 16;       // rows (query row, query head of the group) of a tile
 constexpr int kSplitSlots = 2048;   // records of shares in the workspace, two a workgroup
+constexpr int kJobPieces = 1;       // what a job costs besides its pages, in pieces of them
 constexpr int kMaxShares = 64;      // of one tile: their records are added up by one workgroup
 
 // sum over the lanes up to this one
@@ -45,7 +46,7 @@ __device__ __forceinline__ int wave_scan_int(int v) {
 }
 
 // Which part of the batch a workgroup takes.  A job is a tile of rows of one key / value head of one sequence.  Its cost is
-// its pages in pieces of `piece` (four, one a wavefront, or more where numbers would not fit 32 bits) and one piece for what a job costs
+// its pages in pieces of `piece` (four, one a wavefront, or more where numbers would not fit 32 bits) and kJobPieces for what a job costs
 // besides; the jobs' costs laid end to end are cut into as many equal parts as workgroups run at once, so that a long sequence is
 // shared by many workgroups and many short ones go to one.  The lengths are on the device only: every wavefront works
 // the division out for itself, 64 sequences at a time.
@@ -72,7 +73,7 @@ __device__ __forceinline__ void look(const Kv4Attn &a, Batch &s) {
   }
   s.tiles = (s.rows * a.group + kTileRows - 1) / kTileRows;
   const int pages = a.n_pages > 0 && s.len > 0 ? (int)min(((unsigned)s.len + kKvPageRows - 1) / kKvPageRows, (unsigned)a.table_stride) : 0;
-  s.cost = (pages + (1 << a.piece_log2) - 1 >> a.piece_log2) + 1;
+  s.cost = (pages + (1 << a.piece_log2) - 1 >> a.piece_log2) + kJobPieces;
   s.upto = s.before + wave_scan_int(s.tiles * a.Hkv * s.cost);
 }
 struct Job {
@@ -112,11 +113,13 @@ __device__ __forceinline__ bool find_job(const Kv4Attn &a, int &first, int &befo
   return true;
 }
 
-// The pages come straight into LDS, two of them on their way beside the one that is worked on: a wavefront's ring of two, each the
-// keys and the values of a head as they lie in memory.
+// The pages come straight into LDS, a wavefront's own ring: each the keys and the values of a head as they lie in memory.  A page's keys
+// give way to those of the page DEPTH further on as soon as the scores are there, its values when the outputs are.
 template <int DH>
 struct Kv4Lds {
-  static constexpr int HEAD = 36 * DH, SLOT = 2 * HEAD, WAVE = 2 * SLOT, STATS = 4 * WAVE, SEQS = STATS + 14 * kTileRows * 4, BYTES = SEQS + 4 * 6 * 64 * 4;
+  static constexpr int DEPTH = 1;  // pages of a ring
+  static constexpr int HEAD = 36 * DH, SLOT = 2 * HEAD, WAVE = DEPTH * SLOT, STATS = 4 * WAVE, SEQS = STATS + 14 * kTileRows * 4, Q = SEQS + 4 * 6 * 64 * 4,
+                       BYTES = Q + DH / 32 * 2048;
   static constexpr int REQUESTS = DH / 32 + (DH / 32 + 1) / 2;  // of a head's part of a page: 16 bytes a lane, then 4
   static_assert(WAVE >= kTileRows * (DH + 4) * 4 && 4 * WAVE >= 8 * kMaxShares * kTileRows, "results and shares in the pages' place");
 };
@@ -126,11 +129,11 @@ struct Kv4Lds {
 //   scores  Numbers as fp16 integers, q as two fp16 terms (22 bits of the row's largest); a block's scale is applied to its 32-wide
 //           partial sum.  (The nibbles as they stand are fp16 subnormals n 2^-24 and would need no conversion, but the matrix
 //           instruction adds products of subnormals with five bits less: 2.8e-6 of a score instead of 6e-8.)
-//   output  2^c p d as two fp16 terms (22 bits of each), values as exact fp16 integers, fp32 accumulators.  2^c brings the largest
-//           scale seen so far to 2^13: products down to 2^-27 of p = 1 at that scale keep their 22 bits, smaller ones lie on a grid
-//           of 2^-38 of it.  It goes into the exponent of p, so that sums and outputs carry it alike.
+//   output  2^14 p as two fp16 terms, times the scale d as two again (the rounded product, what that leaves, the second term's): 22
+//           bits of each p d, or a grid of 2^-24 where it is smaller than 2^-2 of 2^14 p d.  Values as exact fp16 integers, fp32
+//           accumulators.  Scales outside 2^-9 .. 2 are brought there by 2^f first (products stay below fp16's 65504).
 template <int DH>
-__global__ __launch_bounds__(256, DH == 128 ? 2 : DH == 64 ? 3 : 4) void k_kv4_attn(Kv4Attn a) {
+__global__ __launch_bounds__(256, DH == 128 ? 3 : 4) void k_kv4_attn(Kv4Attn a) {
   using L = Kv4Lds<DH>;
   constexpr int NB = DH / 32;
   extern __shared__ __align__(16) unsigned char smem[];
@@ -178,8 +181,8 @@ __global__ __launch_bounds__(256, DH == 128 ? 2 : DH == 64 ? 3 : 4) void k_kv4_a
   const int j1 = min(w.rows - 1, (w.tile * kTileRows + kTileRows - 1) / G), j0 = w.tile * kTileRows / G;
   const int last = (int)min((int64_t)w.len - w.rows + j1, all - 1), least = (int)min((int64_t)w.len - w.rows + j0, all - 1);
   const int pages = a.n_pages > 0 && last >= 0 ? last / kKvPageRows + 1 : 0;
-  // its pieces lie on the line behind the one that stands for the rest (a job without pages is one piece of none)
-  const int pieces = max(1, pages + (1 << a.piece_log2) - 1 >> a.piece_log2), line = w.at + 1;
+  // its pieces lie on the line behind those that stand for the rest (a job without pages is one piece of none)
+  const int pieces = max(1, pages + (1 << a.piece_log2) - 1 >> a.piece_log2), line = w.at + kJobPieces;
   const int owner = line / per, shares = (line + pieces - 1) / per - owner + 1, share = me - owner;
   const int from_piece = max(x0 - line, 0), to_piece = min(x1 - line, pieces);
   if (from_piece >= to_piece) continue;
@@ -187,9 +190,9 @@ __global__ __launch_bounds__(256, DH == 128 ? 2 : DH == 64 ? 3 : 4) void k_kv4_a
 
   // page ids of the next 64 pages of this wavefront, one a lane
   const int *table = a.tables + (int64_t)w.seq * a.table_stride;
-  int ids = 0, ids_from = -1;
+  int ids, ids_from;
   auto page_id = [&](int k) {  // k: this wavefront's k-th page (the same in every lane)
-    if (ids_from < 0 || k >= ids_from + 64) {
+    if (k >= ids_from + 64) {
       ids_from = k;
       const int p = p0 + wv + 4 * (k + lane);
       ids = p < p1 ? table[p] : -1;
@@ -197,54 +200,12 @@ __global__ __launch_bounds__(256, DH == 128 ? 2 : DH == 64 ? 3 : 4) void k_kv4_a
     }
     return __builtin_amdgcn_readlane(ids, k - ids_from);
   };
-  half8 q_hi[NB], q_lo[NB];
-  float weight;
-  {
-    float x[NB][8];
-    const float *src = a.q + (int64_t)(w.row0 + (active ? j : 0)) * a.q_stride + head * DH;
-    float top = 0.0f;
-    bool odd = false;
-#pragma unroll
-    for (int b = 0; b < NB; b++) {
-      f4_any u = *(const f4_any *)(src + b * 32 + g * 8), v = *(const f4_any *)(src + b * 32 + g * 8 + 4);
-#pragma unroll
-      for (int e = 0; e < 4; e++) {
-        x[b][e] = active ? u[e] : 0.0f, x[b][4 + e] = active ? v[e] : 0.0f;
-        top = fmaxf(top, fmaxf(fabsf(x[b][e]), fabsf(x[b][4 + e])));
-        odd = odd || !(fabsf(x[b][e]) < INFINITY) || !(fabsf(x[b][4 + e]) < INFINITY);
-      }
-    }
-    top = fmaxf(top, __shfl_xor(top, 16, 64));
-    top = fmaxf(top, __shfl_xor(top, 32, 64));
-    int bad = odd;
-    bad |= __shfl_xor(bad, 16, 64);
-    bad |= __shfl_xor(bad, 32, 64);
-    // a power of two that brings the row's largest into [2^9, 2^10): fp16's own 11 bits, and 11 below them
-    int e = top > 0.0f ? ilogbf(top) : 0;
-    if (bad) e = 0;
-    const float up = ldexpf(1.0f, 9 - e > 126 ? 126 : 9 - e);
-#pragma unroll
-    for (int b = 0; b < NB; b++) {
-#pragma unroll
-      for (int k = 0; k < 8; k++) {
-        // the order in which a dword's nibbles come apart: channels 0 2 4 6 1 3 5 7
-        const int ch = k < 4 ? (k & 1) * 2 + (k >> 1) * 4 : 1 + (k & 1) * 2 + ((k - 4) >> 1) * 4;
-        const float y = bad ? 0.0f : x[b][ch] * up;
-        q_hi[b][k] = (_Float16)y;
-        q_lo[b][k] = (_Float16)(y - (float)q_hi[b][k]);
-      }
-    }
-    // scores as powers of two: log2(e) / sqrt(DH), and the powers of two taken off again
-    weight = bad ? NAN : 1.44269504f / sqrtf((float)DH) / up;
-  }
-
-  f32x4 o[NB][2];
-#pragma unroll
-  for (int b = 0; b < NB; b++) o[b][0] = o[b][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  float m = -INFINITY, l = 0.0f;
-  int c = 100;  // (no scale seen)
-
   const int mine = p0 + wv < p1 ? (p1 - p0 - wv + 3) / 4 : 0;  // pages of this wavefront
+  {
+    const int p = p0 + wv + 4 * lane;
+    ids_from = 0;
+    ids = p < p1 ? table[p] : -1;
+  }
   auto valid = [&](int id) { return id >= 0 && id < a.n_pages; };
   const unsigned char *ring = smem + wv * L::WAVE;
   const unsigned ring_at = (unsigned)(size_t)(__attribute__((address_space(3))) const unsigned char *)ring;
@@ -260,65 +221,125 @@ __global__ __launch_bounds__(256, DH == 128 ? 2 : DH == 64 ? 3 : 4) void k_kv4_a
       dma4(p + 1024, 4 * lane, to + 1024);
     }
   };
-  auto ask_k = [&](int id, int k) { ask(a.k_pages, id, ring_at + (k & 1) * L::SLOT); };
-  auto ask_v = [&](int id, int k) { ask(a.v_pages, id, ring_at + (k & 1) * L::SLOT + L::HEAD); };
-  int id0 = page_id(0), id1 = mine > 1 ? page_id(1) : -1, id2 = -1;
-  if (mine > 0) ask_k(id0, 0), ask_v(id0, 0);
-  if (mine > 1) ask_k(id1, 1), ask_v(id1, 1);
+  auto ask_k = [&](int id, int k) { ask(a.k_pages, id, ring_at + k % L::DEPTH * L::SLOT); };
+  auto ask_v = [&](int id, int k) { ask(a.v_pages, id, ring_at + k % L::DEPTH * L::SLOT + L::HEAD); };
+  int id[L::DEPTH + 1];  // of the page that is worked on, and of those behind it
+#pragma unroll
+  for (int k = 0; k < L::DEPTH; k++) {
+    id[k] = k < mine ? page_id(k) : -1;
+    if (k < mine) ask_k(id[k], k), ask_v(id[k], k);
+  }
 
-  // numbers that the compiler does not see through: a * half + zero and half * minus + a are then one mixed instruction each, where a product
-  // or a difference is a conversion more
-  float zero = 0.0f, minus = -1.0f;
-  asm volatile("" : "+s"(zero), "+s"(minus));
-  // Nibbles 0 and 4 of four dwords as numbers -8 .. 7: set behind 0x6400 they read 1024 + n, n the nibble with its upper bit flipped.  (The mask
-  // and 0x6400 in registers of both kinds: one instruction for the and and the or.)
-  uint32_t nibbles = 0x000F000Fu, thousand = 0x64006400u;
-  asm volatile("" : "+s"(nibbles), "+v"(thousand));
-  auto numbers = [&](uint32_t u0, uint32_t u1, uint32_t u2, uint32_t u3) {
-    const u32x4 raw = {(u0 & nibbles) | thousand, (u1 & nibbles) | thousand, (u2 & nibbles) | thousand, (u3 & nibbles) | thousand};
-    return __builtin_bit_cast(half8, raw) - (_Float16)1032.0f;
-  };
-  auto one_page = [&](auto whole, int k) {
-    constexpr bool FULL = decltype(whole)::value;  // every row of the tile sees every row of the page
+  // The row's query as two fp16 terms, in LDS as the matrix instructions take them: [block][term][lane][8].  (Held in registers they are a
+  // quarter of what a wavefront has.)  Every wavefront looks at the whole row, block b is wavefront b's to convert.
+  float weight;
+  {
+    float x[NB][8], mine8[8];
+    const float *src = a.q + (int64_t)(w.row0 + (active ? j : 0)) * a.q_stride + head * DH;
+    float top = 0.0f;
+    bool odd = false;
+#pragma unroll
+    for (int b = 0; b < NB; b++) {
+      f4_any u = *(const f4_any *)(src + b * 32 + g * 8), v = *(const f4_any *)(src + b * 32 + g * 8 + 4);
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        x[b][e] = active ? u[e] : 0.0f, x[b][4 + e] = active ? v[e] : 0.0f;
+        top = fmaxf(top, fmaxf(fabsf(x[b][e]), fabsf(x[b][4 + e])));
+        odd = odd || !(fabsf(x[b][e]) < INFINITY) || !(fabsf(x[b][4 + e]) < INFINITY);
+      }
+#pragma unroll
+      for (int e = 0; e < 8; e++) mine8[e] = b == 0 || wv == b ? x[b][e] : mine8[e];
+    }
+    top = fmaxf(top, __shfl_xor(top, 16, 64));
+    top = fmaxf(top, __shfl_xor(top, 32, 64));
+    int bad = odd;
+    bad |= __shfl_xor(bad, 16, 64);
+    bad |= __shfl_xor(bad, 32, 64);
+    // a power of two that brings the row's largest into [2^9, 2^10): fp16's own 11 bits, and 11 below them
+    int e = top > 0.0f ? ilogbf(top) : 0;
+    if (bad) e = 0;
+    const float up = ldexpf(1.0f, 9 - e > 126 ? 126 : 9 - e);
+    if (wv < NB) {
+      half8 hi, lo;
+#pragma unroll
+      for (int k = 0; k < 8; k++) {
+        // the order in which a dword's nibbles come apart: channels 0 2 4 6 1 3 5 7
+        const int ch = k < 4 ? (k & 1) * 2 + (k >> 1) * 4 : 1 + (k & 1) * 2 + ((k - 4) >> 1) * 4;
+        const float y = bad ? 0.0f : mine8[ch] * up;
+        hi[k] = (_Float16)y;
+        lo[k] = (_Float16)(y - (float)hi[k]);
+      }
+      *(half8 *)(smem + L::Q + wv * 2048 + lane * 16) = hi;
+      *(half8 *)(smem + L::Q + wv * 2048 + 1024 + lane * 16) = lo;
+    }
+    // scores as powers of two: log2(e) / sqrt(DH), and the powers of two taken off again
+    weight = bad ? NAN : 1.44269504f / sqrtf((float)DH) / up;
+  }
+
+  f32x4 o[NB][2];
+#pragma unroll
+  for (int b = 0; b < NB; b++) o[b][0] = o[b][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  float m = -INFINITY, l = 0.0f;
+  int f = 100;  // the values' scales go in as 2^f d (100: none seen)
+
+  // a number that the compiler does not see through: half * minus + a is then one mixed instruction, where a difference is a conversion more
+  float minus = -1.0f;
+  asm volatile("" : "+s"(minus));
+  // Numbers -8 .. 7 of nibbles: the lower one of a byte set behind 0x6400 reads 1024 + n, the upper one behind 0x5400 reads 64 + n (n the
+  // nibble with its upper bit flipped).  Mask and exponent in registers of both kinds: one instruction for the and and the xor.
+  uint32_t lower = 0x000F000Fu, upper = 0x00F000F0u, e_lower = 0x64086408u, e_upper = 0x54805480u;
+  asm volatile("" : "+s"(lower), "+s"(upper), "+v"(e_lower), "+v"(e_upper));
+  auto lower_of = [&](uint32_t u) { return __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2v, (u & lower) ^ e_lower) - (_Float16)1032.0f); };
+  auto upper_of = [&](uint32_t u) { return __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2v, (u & upper) ^ e_upper) - (_Float16)72.0f); };
+  __syncthreads();
+  for (int k = 0; k < mine; k++) {
     const int page = p0 + wv + 4 * k;
-    const int from = FULL ? 0 : valid(id0) ? page * kKvPageRows : INT_MAX - kKvPageRows;  // (absent: behind every limit)
-    const unsigned char *kp = ring + (k & 1) * L::SLOT, *vp = kp + L::HEAD;
+    const int from = valid(id[0]) ? page * kKvPageRows : INT_MAX - (kKvPageRows - 1);  // (absent: behind every limit)
+    const bool whole = from + kKvPageRows - 1 <= least;                            // every row of the tile sees every row of the page (uniform)
+    const unsigned char *kp = ring + k % L::DEPTH * L::SLOT, *vp = kp + L::HEAD;
     // the scales of block b, rows 16 t + 4 g ..
     auto scales = [&](const unsigned char *p, int t, int b) { return *(const half4 *)(p + 32 * DH + ((4 * t + g) * NB + b) * 8); };
     typedef uint32_t kdw __attribute__((ext_vector_type(NB)));
     typedef unsigned short sdw __attribute__((ext_vector_type(NB)));
-    // younger than this page's keys: its values, and both of the next page's
-    if (k + 1 < mine) wait_loads<3 * L::REQUESTS>();
+    // younger than this page's keys: its values, and what has been asked for of the pages behind it
+    if (L::DEPTH == 2 && k + 1 < mine) wait_loads<3 * L::REQUESTS>();
     else wait_loads<L::REQUESTS>();
     f32x4 s[4];
+    kdw kq[4];
 #pragma unroll
     for (int t = 0; t < 4; t++) {
       s[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-      const kdw kq = *(const kdw *)(kp + kv4_key_offset(16 * t + n, g, 0, DH));
+      kq[t] = *(const kdw *)(kp + kv4_key_offset(16 * t + n, g, 0, DH));
+    }
 #pragma unroll
-      for (int b = 0; b < NB; b++) {
-        const uint32_t u = kq[b] ^ 0x88888888u;
-        const half8 kk = numbers(u, u >> 4, u >> 8, u >> 12);
-        f32x4 x = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk, q_lo[b], f32x4{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
-        x = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk, q_hi[b], x, 0, 0, 0);
+    for (int b = 0; b < NB; b++) {
+      const half8 q_hi = *(const half8 *)(smem + L::Q + b * 2048 + lane * 16), q_lo = *(const half8 *)(smem + L::Q + b * 2048 + 1024 + lane * 16);
+#pragma unroll
+      for (int t = 0; t < 4; t++) {
+        const uint32_t u = kq[t][b], v = u >> 8;
+        const half8 kk = __builtin_bit_cast(half8, (u32x4){lower_of(u), upper_of(u), lower_of(v), upper_of(v)});  // channels 0 2, 4 6, 1 3, 5 7
+        f32x4 x = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk, q_lo, f32x4{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
+        x = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk, q_hi, x, 0, 0, 0);
         const half4 d = scales(kp, t, b);
 #pragma unroll
         for (int i = 0; i < 4; i++) s[t][i] = fmaf(x[i], (float)d[i], s[t][i]);
       }
     }
     wait_lds();
-    if (k + 2 < mine) {
-      id2 = page_id(k + 2);
-      ask_k(id2, k);
+    if (k + L::DEPTH < mine) {
+      id[L::DEPTH] = page_id(k + L::DEPTH);
+      ask_k(id[L::DEPTH], k);
+    }
+    if (!whole) {
+#pragma unroll
+      for (int t = 0; t < 4; t++)
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+          if (from + 16 * t + 4 * g + i > limit) s[t][i] = -INFINITY;
     }
     float top = -INFINITY;
 #pragma unroll
-    for (int t = 0; t < 4; t++)
-#pragma unroll
-      for (int i = 0; i < 4; i++) {
-        if (!FULL && from + 16 * t + 4 * g + i > limit) s[t][i] = -INFINITY;
-        top = fmaxf(top, s[t][i]);
-      }
+    for (int t = 0; t < 4; t++) top = fmaxf(top, fmaxf(fmaxf(s[t][0], s[t][1]), fmaxf(s[t][2], s[t][3])));
     top = fmaxf(top, __shfl_xor(top, 16, 64));
     top = fmaxf(top, __shfl_xor(top, 32, 64));
     if (__ballot(top > m)) {  // a new maximum in some row
@@ -328,8 +349,16 @@ __global__ __launch_bounds__(256, DH == 128 ? 2 : DH == 64 ? 3 : 4) void k_kv4_a
 #pragma unroll
       for (int b = 0; b < NB; b++) o[b][0] *= corr, o[b][1] *= corr;
     }
-    if (k + 2 < mine) wait_loads<3 * L::REQUESTS>();
-    else if (k + 1 < mine) wait_loads<2 * L::REQUESTS>();
+    const float base = (m > -INFINITY ? m * weight : 0.0f) - 14.0f;
+#pragma unroll
+    for (int t = 0; t < 4; t++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        s[t][i] = __builtin_amdgcn_exp2f(fmaf(s[t][i], weight, -base));
+        l += s[t][i];
+      }
+    if (k + L::DEPTH < mine) wait_loads<(2 * L::DEPTH - 1) * L::REQUESTS>();
+    else if (L::DEPTH == 2 && k + 1 < mine) wait_loads<2 * L::REQUESTS>();
     else wait_loads<0>();
     {
       const sdw vs_now = *(const sdw *)(vp + 32 * DH + lane * NB * 2);
@@ -338,67 +367,71 @@ __global__ __launch_bounds__(256, DH == 128 ? 2 : DH == 64 ? 3 : 4) void k_kv4_a
       for (int x = 0; x < NB; x++) {
         const int flat = lane * NB + x, row = flat / (4 * NB) * 4 + flat % 4;
         const float dx = fabsf(half_bits_to_float(vs_now[x]));
-        if (FULL || from + row <= last) d = fmaxf(d, dx);
+        d = fmaxf(d, whole || from + row <= last ? dx : 0.0f);
       }
       d = fminf(wave_max(d), 65504.0f);
-      const int want = 13 - ((int)(__float_as_uint(d) >> 23) - 127);
-      if (d > 0.0f && want < c) {  // (uniform)
-        const float f = ldexpf(1.0f, want - c);
-        c = want;
-        l *= f;
+      const int e = __builtin_amdgcn_readfirstlane((int)(__float_as_uint(d) >> 23)) - 127;  // (uniform)
+      if (d > 0.0f && f == 100) {
+        f = e >= -9 && e <= 0 ? 0 : min(max(-e, -15), 15);
+      } else if (d > 0.0f && e + f > 0) {
+        const float by = ldexpf(1.0f, -e - f);
+        f = -e;
 #pragma unroll
-        for (int b = 0; b < NB; b++) o[b][0] *= f, o[b][1] *= f;
+        for (int b = 0; b < NB; b++) o[b][0] *= by, o[b][1] *= by;
       }
     }
-    const float base = (m > -INFINITY ? m * weight : 0.0f) - (float)c;
+    // p as two fp16 terms, once for all blocks
+    half2v ph[8], pl[8];
 #pragma unroll
-    for (int t = 0; t < 4; t++)
-#pragma unroll
-      for (int i = 0; i < 4; i++) {
-        s[t][i] = __builtin_amdgcn_exp2f(fmaf(s[t][i], weight, -base));
-        if (!FULL && from + 16 * t + 4 * g + i > limit) s[t][i] = 0.0f;
-        l += s[t][i];
-      }
+    for (int i = 0; i < 8; i++) {
+      const float x0 = s[i >> 1][2 * (i & 1)], x1 = s[i >> 1][2 * (i & 1) + 1];
+      ph[i] = __builtin_convertvector((f32x2){x0, x1}, half2v);
+      pl[i] = __builtin_convertvector((f32x2){fmaf((float)ph[i][0], minus, x0), fmaf((float)ph[i][1], minus, x1)}, half2v);
+    }
+    const _Float16 by = (_Float16)ldexpf(1.0f, f == 100 ? 0 : f);
+    auto outputs = [&](auto plain) {
+    constexpr bool PLAIN = decltype(plain)::value;
 #pragma unroll
     for (int b = 0; b < NB; b++) {
-      u32x4 vq, hi[2], lo[2];  // rows 16 t + 4 g + (0, 2, 1, 3), t = 0 1 and 2 3
-#pragma unroll
-      for (int t = 0; t < 4; t++) {
-        const half4 d = scales(vp, t, b);
-        float x[4];
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-          x[i] = fmaf(s[t][i], (float)d[i], zero);
-          if (!FULL && from + 16 * t + 4 * g + i > limit) x[i] = 0.0f;  // (the scale of a row that is not seen may be anything)
-        }
-#pragma unroll
-        for (int i = 0; i < 2; i++) {
-          const half2v h = __builtin_convertvector((f32x2){x[i], x[i + 2]}, half2v);
-          const f32x2 r = {fmaf((float)h[0], minus, x[i]), fmaf((float)h[1], minus, x[i + 2])};
-          hi[t >> 1][2 * (t & 1) + i] = __builtin_bit_cast(uint32_t, h);
-          lo[t >> 1][2 * (t & 1) + i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(r, half2v));
-        }
-      }
+      const u32x4 vq = *(const u32x4 *)(vp + (b * 16 + n) * kKvPageRows + 16 * g);
 #pragma unroll
       for (int part = 0; part < 2; part++) {
-        const half8 ph = __builtin_bit_cast(half8, hi[part]), pl = __builtin_bit_cast(half8, lo[part]);
-        if (part == 0) vq = *(const u32x4 *)(vp + (b * 16 + n) * kKvPageRows + 16 * g);
-        const uint32_t u0 = vq[2 * part] ^ 0x88888888u, u1 = vq[2 * part + 1] ^ 0x88888888u;
+        half2v xh[4], xl[4];  // p d: the rounded product of the first term, what that leaves, and the second term's
 #pragma unroll
-        for (int half = 0; half < 2; half++) {
-          const half8 vv = numbers(u0 >> (4 * half), u0 >> (4 * half + 8), u1 >> (4 * half), u1 >> (4 * half + 8));
-          o[b][half] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vv, pl, o[b][half], 0, 0, 0);
-          o[b][half] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vv, ph, o[b][half], 0, 0, 0);
+        for (int i = 0; i < 4; i++) {
+          const half4 d4 = scales(vp, 2 * part + (i >> 1), b);
+          half2v d = i & 1 ? half2v{d4[2], d4[3]} : half2v{d4[0], d4[1]};
+          if (!PLAIN) {
+            d = d * (half2v){by, by};
+            const int at = from + 16 * (2 * part + (i >> 1)) + 4 * g + 2 * (i & 1);
+            if (at > limit) d[0] = (_Float16)0.0f;  // (the scale of a row that is not seen may be anything)
+            if (at + 1 > limit) d[1] = (_Float16)0.0f;
+          }
+          xh[i] = ph[4 * part + i] * d;
+          xl[i] = __builtin_elementwise_fma(pl[4 * part + i], d, __builtin_elementwise_fma(ph[4 * part + i], d, -xh[i]));
         }
+        const half8 hi = __builtin_bit_cast(half8, (u32x4){__builtin_bit_cast(uint32_t, xh[0]), __builtin_bit_cast(uint32_t, xh[1]), __builtin_bit_cast(uint32_t, xh[2]),
+                                                           __builtin_bit_cast(uint32_t, xh[3])});
+        const half8 lo = __builtin_bit_cast(half8, (u32x4){__builtin_bit_cast(uint32_t, xl[0]), __builtin_bit_cast(uint32_t, xl[1]), __builtin_bit_cast(uint32_t, xl[2]),
+                                                           __builtin_bit_cast(uint32_t, xl[3])});
+        // bytes 0 1 and 2 3 of a dword as halves
+        const uint32_t u0 = __builtin_amdgcn_perm(0, vq[2 * part], 0x0C010C00u), u1 = __builtin_amdgcn_perm(0, vq[2 * part], 0x0C030C02u);
+        const uint32_t u2 = __builtin_amdgcn_perm(0, vq[2 * part + 1], 0x0C010C00u), u3 = __builtin_amdgcn_perm(0, vq[2 * part + 1], 0x0C030C02u);
+        const half8 v0 = __builtin_bit_cast(half8, (u32x4){lower_of(u0), lower_of(u1), lower_of(u2), lower_of(u3)});
+        const half8 v1 = __builtin_bit_cast(half8, (u32x4){upper_of(u0), upper_of(u1), upper_of(u2), upper_of(u3)});
+        o[b][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, lo, o[b][0], 0, 0, 0);
+        o[b][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, lo, o[b][1], 0, 0, 0);
+        o[b][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, hi, o[b][0], 0, 0, 0);
+        o[b][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, hi, o[b][1], 0, 0, 0);
       }
     }
+    };
+    if (whole && f == 0) outputs(std::true_type());
+    else outputs(std::false_type());
     wait_lds();
-    if (k + 2 < mine) ask_v(id2, k);
-    id0 = id1, id1 = id2;
-  };
-  for (int k = 0; k < mine; k++) {
-    if (valid(id0) && (p0 + wv + 4 * k) * kKvPageRows + kKvPageRows - 1 <= least) one_page(std::true_type(), k);
-    else one_page(std::false_type(), k);
+    if (k + L::DEPTH < mine) ask_v(id[L::DEPTH], k);
+#pragma unroll
+    for (int i = 0; i < L::DEPTH; i++) id[i] = id[i + 1];
   }
   l += __shfl_xor(l, 16, 64);
   l += __shfl_xor(l, 32, 64);
@@ -407,12 +440,13 @@ __global__ __launch_bounds__(256, DH == 128 ? 2 : DH == 64 ? 3 : 4) void k_kv4_a
   int tid = tid0;
   asm volatile("" : "+v"(tid));
   const int nr = min(kTileRows, w.rows * G - w.tile * kTileRows);  // rows of the tile that there are
-  if (g == 0) s_m[wv][n] = m * weight - (float)c, s_l[wv][n] = l;
+  if (g == 0) s_m[wv][n] = m * weight, s_l[wv][n] = l;
+  const float back = ldexpf(1.0f, f == 100 ? 0 : -f);
   if (n < nr) {
 #pragma unroll
     for (int b = 0; b < NB; b++)
 #pragma unroll
-      for (int half = 0; half < 2; half++) *(f32x4 *)(s_o(wv, n) + b * 32 + half * 16 + 4 * g) = o[b][half];
+      for (int half = 0; half < 2; half++) *(f32x4 *)(s_o(wv, n) + b * 32 + half * 16 + 4 * g) = o[b][half] * back;
   }
   __syncthreads();
   // a share that goes on from the workgroup before, and one that goes on in the next: a workgroup has one of each at most
@@ -526,9 +560,9 @@ int cthip_sdpa_paged_q4(float *out, const float *q, int64_t q_stride, const void
   const int64_t tiles = (int64_t)n_rows * (H / Hkv) / kTileRows + (n_seqs < n_rows ? n_seqs : n_rows), jobs = tiles * Hkv;
   if (jobs > (1 << 28)) return fail(CTHIP_E_UNSUPPORTED, "cthip_sdpa_paged_q4: %d rows of %d heads in one call", n_rows, H);
   int piece = 2;
-  while (jobs * ((table_stride >> piece) + 2) > INT_MAX / 2) piece++;
-  // as many workgroups as run at once (two, three or four a compute unit for their registers), a multiple of the XCDs
-  const int at_once = std::min(kSplitSlots / 2, state().compute_units * (Dh == 128 ? 2 : Dh == 64 ? 3 : 4) / 8 * 8);
+  while (jobs * ((table_stride >> piece) + 1 + kJobPieces) > INT_MAX / 2) piece++;
+  // as many workgroups as run at once (three or four a compute unit for their registers and pages), a multiple of the XCDs
+  const int at_once = std::min(kSplitSlots / 2, state().compute_units * (Dh == 128 ? 3 : 4) / 8 * 8);
   const Kv4Attn a = {out,     q,     (const unsigned char *)k_pages, (const unsigned char *)v_pages, tables, lens, starts, q_stride, n_pages, table_stride, n_seqs, n_rows, H, Hkv,
                      H / Hkv, piece, (int *)workspace, (float *)workspace + kSplitSlots};
   const dim3 grid((unsigned)at_once), block(256);
