@@ -117,9 +117,10 @@ __global__ __launch_bounds__(kPlanThreads) void k_kv_plan(int *__restrict__ slot
 
 // ---- rows into the cache ----
 // Four lanes hold a block of 32 channels, eight each.  d = m / -8 as fp16, m the value of largest magnitude (the positive one
-// of two), kept finite; q = floor(x / d + 8.5) within 0 .. 15, d being the scale as it is STORED.  The quotient is taken by a
-// reciprocal and then held against the borders (q - 8.5) d and (q - 7.5) d, which are exact in fp32 (5 bits times 11): the
-// number is the one of real arithmetic whatever the reciprocal's rounding.  A block with an infinity or a NaN has a NaN scale.
+// of two), kept finite; u = floor(x / d + 1/2) within -8 .. 7, d being the scale as it is STORED.  The quotient is taken by a
+// reciprocal, and what it leaves, x - u d, is exact in fp32 (u d has 15 bits, and what is left of x where u is not 0 no more than x has):
+// where that is not within half a step, u moves by one, so the number is the one of real arithmetic whatever the reciprocal's
+// rounding.  A block with an infinity or a NaN has a NaN scale.
 __device__ __forceinline__ float quad_max(float v) {
   v = fmaxf(v, dpp_f<0xB1>(v));
   return fmaxf(v, dpp_f<0x4E>(v));
@@ -141,86 +142,234 @@ __device__ __forceinline__ uint32_t kv4_quantise8(const float *x, unsigned short
   const float d = (float)d16, ds = fabsf(d);
   scale = odd != 0.0f ? (unsigned short)0x7E00 : __builtin_bit_cast(unsigned short, d16);
   if (odd != 0.0f || ds == 0.0f) return 0u;
-  const float inv = 1.0f / ds;
-  uint32_t w = 0;
+  const float inv = 1.0f / ds, half = 0.5f * ds;
+  float u[8], xs[8];
+  bool off = false;
 #pragma unroll
   for (int e = 0; e < 8; e++) {
-    const float xs = d < 0.0f ? -x[e] : x[e];
-    float t = fminf(fmaxf(floorf(fmaf(xs, inv, 8.5f)), 0.0f), 15.0f);
-    if (t > 0.0f && xs < (t - 8.5f) * ds) t -= 1.0f;
-    else if (t < 15.0f && xs >= (t - 7.5f) * ds) t += 1.0f;
-    w |= ((uint32_t)(int)t ^ 8u) << (4 * e);
+    xs[e] = d < 0.0f ? -x[e] : x[e];
+    u[e] = floorf(fmaf(xs[e], inv, 0.5f));
+    const float left = fmaf(-u[e], ds, xs[e]);
+    off = off || left >= half || left < -half;
   }
-  return w;
+  if (off) {  // (seldom: within 2^-20 of a border)
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      const float left = fmaf(-u[e], ds, xs[e]);
+      u[e] += left >= half ? 1.0f : left < -half ? -1.0f : 0.0f;
+    }
+  }
+  // four numbers as one of base 16; with 8 added to each the digits are nibbles
+  float lo4 = 0.0f, hi4 = 0.0f;
+#pragma unroll
+  for (int e = 3; e >= 0; e--) {
+    lo4 = fmaf(lo4, 16.0f, fminf(fmaxf(u[e], -8.0f), 7.0f));
+    hi4 = fmaf(hi4, 16.0f, fminf(fmaxf(u[4 + e], -8.0f), 7.0f));
+  }
+  return ((uint32_t)((int)lo4 + 0x8888) | (uint32_t)((int)hi4 + 0x8888) << 16) ^ 0x88888888u;
 }
 
-// one row per blockIdx.x, keys (blockIdx.z = 0) or values; a thread per eight channels
-__global__ __launch_bounds__(256) void k_kv4_append(unsigned char *__restrict__ kp, unsigned char *__restrict__ vp, const float *__restrict__ kr,
-                                                    const float *__restrict__ vr, int64_t k_stride, int64_t v_stride,
-                                                    const int *__restrict__ slots, int n_pages, int kv, int dh) {
-  const int e8 = blockIdx.y * 256 + threadIdx.x;  // eighth of the row
-  if (e8 >= kv * dh / 8) return;                   // (kv * dh / 8 is a multiple of 4: whole quads leave)
-  const int slot = slots[blockIdx.x];
-  if (slot < 0 || slot >= n_pages * kKvPageRows) return;
-  const bool values = blockIdx.z != 0;
-  const float *src = (values ? vr + blockIdx.x * v_stride : kr + blockIdx.x * k_stride) + 8 * e8;
-  float x[8];
+struct Kv4Rows {
+  unsigned char *k_pages, *v_pages;
+  const float *k_in, *v_in;  // into the cache
+  float *k_out, *v_out;      // out of it
+  int64_t k_stride, v_stride;
+  const int *slots;
+  int n_rows, n_pages, kv;
+};
+// nibbles 0 .. 3 of a dword as the low halves of its bytes
+__device__ __forceinline__ uint32_t spread4(uint32_t w) { return (w & 0xF) | (w & 0xF0) << 4 | (w & 0xF00) << 8 | (w & 0xF000) << 12; }
+// The quad of lanes that holds a value block: lanes 0 and 1 its channels 0 .. 15, 2 and 3 their partners.  Each lane gets the four bytes of
+// four channels, the first of which is returned.
+__device__ __forceinline__ int value_bytes(uint32_t w, int g, unsigned char *bytes) {
+  const uint32_t other = __builtin_bit_cast(uint32_t, dpp_f<0x4E>(__builtin_bit_cast(float, w)));
+  const uint32_t low = g < 2 ? w : other, high = g < 2 ? other : w;
+  const int j0 = g < 2 ? 0 : 4;
+#pragma unroll
+  for (int j = 0; j < 4; j++) bytes[j] = (unsigned char)(((low >> 4 * (j0 + j)) & 15u) | ((high >> 4 * (j0 + j)) & 15u) << 4);
+  return 8 * (g & 1) + j0;
+}
+__device__ __forceinline__ void load8(const float *src, float *x) {
   *(f4_any *)x = *(const f4_any *)src;
   *(f4_any *)(x + 4) = *(const f4_any *)(src + 4);
-  unsigned short d;
-  const uint32_t w = kv4_quantise8(x, d);
-  const int row = slot % kKvPageRows, h = 8 * e8 / dh, c8 = e8 - h * (dh / 8), b = c8 >> 2, g = c8 & 3;
-  unsigned char *head = (values ? vp : kp) + ((int64_t)(slot / kKvPageRows) * kv + h) * kv4_head_bytes(dh);
-  if (g == 0) *(unsigned short *)(head + kv4_scale_offset(row, b, dh)) = d;
-  if (!values) {
-    // bytes j: channel j low, channel 4 + j high
-    const uint32_t lo = (w & 0xF) | (w & 0xF0) << 4 | (w & 0xF00) << 8 | (w & 0xF000) << 12;
-    const uint32_t hi = w >> 16, up = (hi & 0xF) | (hi & 0xF0) << 4 | (hi & 0xF00) << 8 | (hi & 0xF000) << 12;
-    *(uint32_t *)(head + kv4_key_offset(row, g, b, dh)) = lo | up << 4;
-  } else {
-    // lanes 0 and 1 of the quad hold channels 0 .. 15 of the block, 2 and 3 their partners; each lane stores four bytes
-    const uint32_t other = __builtin_bit_cast(uint32_t, dpp_f<0x4E>(__builtin_bit_cast(float, w)));
-    const uint32_t low = g < 2 ? w : other, high = g < 2 ? other : w;
-    const int j0 = g < 2 ? 0 : 4, c = 8 * (g & 1) + j0;
+}
+__device__ __forceinline__ void key_values(uint32_t w, float d, float *x) {
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
-      const int sh = 4 * (j0 + j);
-      head[kv4_value_offset(row, b, c + j)] = (unsigned char)(((low >> sh) & 15u) | ((high >> sh) & 15u) << 4);
-    }
+  for (int j = 0; j < 4; j++) {
+    x[j] = d * (float)((int)(w << (28 - 8 * j)) >> 28);
+    x[4 + j] = d * (float)((int)(w << (24 - 8 * j)) >> 28);
   }
 }
 
-// ---- rows of the cache back as fp32, by their slots ----
-__global__ __launch_bounds__(256) void k_kv4_rows(float *__restrict__ ko, float *__restrict__ vo, const unsigned char *__restrict__ kp,
-                                                  const unsigned char *__restrict__ vp, const int *__restrict__ slots, int n_pages, int kv, int dh) {
-  const int e8 = blockIdx.y * 256 + threadIdx.x;
-  if (e8 >= kv * dh / 8) return;
-  const int slot = slots[blockIdx.x];
-  if (slot < 0 || slot >= n_pages * kKvPageRows) return;
+// Few rows: one row per blockIdx.x, keys (blockIdx.z = 0) or values; a thread per eight channels
+template <bool IN>
+__global__ __launch_bounds__(256) void k_kv4_rows(Kv4Rows a, int dh) {
+  const int e8 = blockIdx.y * 256 + threadIdx.x;  // eighth of the row
+  if (e8 >= a.kv * dh / 8) return;                 // (kv * dh / 8 is a multiple of 4: whole quads leave)
+  const int slot = a.slots[blockIdx.x];
+  if (slot < 0 || slot >= a.n_pages * kKvPageRows) return;
   const bool values = blockIdx.z != 0;
-  float *out = values ? vo : ko;
-  if (!out) return;
   const int row = slot % kKvPageRows, h = 8 * e8 / dh, c8 = e8 - h * (dh / 8), b = c8 >> 2, g = c8 & 3;
-  const unsigned char *head = (values ? vp : kp) + ((int64_t)(slot / kKvPageRows) * kv + h) * kv4_head_bytes(dh);
-  const float d = half_bits_to_float(*(const unsigned short *)(head + kv4_scale_offset(row, b, dh)));
+  unsigned char *head = (values ? a.v_pages : a.k_pages) + ((int64_t)(slot / kKvPageRows) * a.kv + h) * kv4_head_bytes(dh);
   float x[8];
-  if (!values) {
-    const uint32_t w = *(const uint32_t *)(head + kv4_key_offset(row, g, b, dh));
+  if (IN) {
+    load8((values ? a.v_in + blockIdx.x * a.v_stride : a.k_in + blockIdx.x * a.k_stride) + 8 * e8, x);
+    unsigned short d;
+    const uint32_t w = kv4_quantise8(x, d);
+    if (g == 0) *(unsigned short *)(head + kv4_scale_offset(row, b, dh)) = d;
+    if (!values) {
+      *(uint32_t *)(head + kv4_key_offset(row, g, b, dh)) = spread4(w) | spread4(w >> 16) << 4;
+    } else {
+      unsigned char bytes[4];
+      const int c = value_bytes(w, g, bytes);
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
-      x[j] = d * (float)((int)(w << (28 - 8 * j)) >> 28);
-      x[4 + j] = d * (float)((int)(w << (24 - 8 * j)) >> 28);
+      for (int j = 0; j < 4; j++) head[kv4_value_offset(row, b, c + j)] = bytes[j];
     }
   } else {
+    float *out = values ? a.v_out : a.k_out;
+    if (!out) return;
+    const float d = half_bits_to_float(*(const unsigned short *)(head + kv4_scale_offset(row, b, dh)));
+    if (!values) {
+      key_values(*(const uint32_t *)(head + kv4_key_offset(row, g, b, dh)), d, x);
+    } else {
 #pragma unroll
-    for (int j = 0; j < 8; j++) {
-      const int v = head[kv4_value_offset(row, b, 8 * (g & 1) + j)];
-      x[j] = d * (float)((int)((uint32_t)v << (g < 2 ? 28 : 24)) >> 28);
+      for (int j = 0; j < 8; j++) x[j] = d * (float)((int)((uint32_t)head[kv4_value_offset(row, b, 8 * (g & 1) + j)] << (g < 2 ? 28 : 24)) >> 28);
+    }
+    float *dst = out + (int64_t)blockIdx.x * a.kv * dh + 8 * e8;
+    *(f4_any *)dst = *(const f4_any *)x;
+    *(f4_any *)(dst + 4) = *(const f4_any *)(x + 4);
+  }
+}
+
+// Many rows: 64 consecutive ones of one head a workgroup.  Where their slots follow one another -- a piece of a prompt: the end of a page and
+// the beginning of another, or a whole one -- values and scales go through LDS, where they lie as in a page, and four rows at a time
+// between there and memory: row by row they are single bytes, each in a line of its own.
+template <int DH, bool IN>
+__global__ __launch_bounds__(256) void k_kv4_rows64(Kv4Rows a) {
+  constexpr int NB = DH / 32, TPR = DH / 8, LINE = kKvPageRows + 4;  // (lines of 17 dwords: a row's bytes lie in different banks)
+  __shared__ int s_slot[kKvPageRows];
+  __shared__ __align__(16) unsigned char s_v[DH / 2 * LINE];
+  __shared__ __align__(16) unsigned short s_d[kKvPageRows * NB];  // [row / 4][block][row % 4]
+  const int tid = threadIdx.x, r0 = blockIdx.x * kKvPageRows, count = min(kKvPageRows, a.n_rows - r0), h = blockIdx.y;
+  const bool values = blockIdx.z != 0;
+  if (!IN && !(values ? a.v_out : a.k_out)) return;
+  if (tid < kKvPageRows) s_slot[tid] = tid < count ? a.slots[r0 + tid] : -1;
+  __syncthreads();
+  const int first = s_slot[0], o = first & (kKvPageRows - 1), split = kKvPageRows - o;  // rows split .. lie in a second page
+  const int page_a = first / kKvPageRows, page_b = split < count ? s_slot[split] / kKvPageRows : page_a;
+  bool fine = true;
+  if (tid < count) {
+    const int slot = s_slot[tid];
+    fine = slot >= 0 && slot < a.n_pages * kKvPageRows && slot / kKvPageRows == (tid < split ? page_a : page_b) && (slot & (kKvPageRows - 1)) == ((o + tid) & (kKvPageRows - 1));
+  }
+  const bool follow = __syncthreads_and(fine);  // every slot one behind the other
+  unsigned char *pool = values ? a.v_pages : a.k_pages;
+  auto head_of = [&](int page) { return pool + ((int64_t)page * a.kv + h) * kv4_head_bytes(DH); };
+  auto there = [&](int row) { return ((row - o) & (kKvPageRows - 1)) < count; };  // row of a page: whether it is one of ours
+  auto home = [&](int row) { return head_of(row >= o ? page_a : page_b); };
+  // the pages' values (four rows of a channel pair a dword, which in a page lie one behind the other) and scales
+  auto exchange = [&]() {
+    for (int d = tid; values && d < DH / 2 * 16; d += 256) {
+      const int line = d >> 4, q = d & 15, row = 16 * (q & 3) + 4 * (q >> 2);
+      unsigned char *mine = s_v + line * LINE + 4 * q;
+      if (there(row) && there(row + 3) && (row + 3 < o || row >= o)) {
+        uint32_t *p = (uint32_t *)(home(row) + 4 * d);
+        if (IN) *p = *(const uint32_t *)mine;
+        else *(uint32_t *)mine = *p;
+      } else {
+        for (int i = 0; i < 4; i++)
+          if (there(row + i)) {
+            unsigned char *p = home(row + i) + 4 * d + i;
+            if (IN) *p = mine[i];
+            else mine[i] = *p;
+          }
+      }
+    }
+    for (int d = tid; d < 16 * NB; d += 256) {
+      const int row = d / NB * 4;
+      unsigned short *mine = s_d + 4 * d;
+      if (there(row) && there(row + 3) && (row + 3 < o || row >= o)) {
+        uint2 *p = (uint2 *)(home(row) + 32 * DH + 8 * d);
+        if (IN) *p = *(const uint2 *)mine;
+        else *(uint2 *)mine = *p;
+      } else {
+        for (int i = 0; i < 4; i++)
+          if (there(row + i)) {
+            unsigned short *p = (unsigned short *)(home(row + i) + 32 * DH + 8 * d) + i;
+            if (IN) *p = mine[i];
+            else mine[i] = *p;
+          }
+      }
+    }
+  };
+  if (!IN && follow) {
+    exchange();
+    __syncthreads();
+  }
+  const int c8 = tid % TPR, b = c8 >> 2, g = c8 & 3;
+#pragma unroll
+  for (int pass = 0; pass < kKvPageRows / (256 / TPR); pass++) {
+    const int r = pass * (256 / TPR) + tid / TPR;
+    const int slot = r < count ? s_slot[r] : -1, row = slot & (kKvPageRows - 1);
+    if (slot < 0 || slot >= a.n_pages * kKvPageRows) continue;  // (whole quads)
+    unsigned char *head = head_of(slot / kKvPageRows);
+    unsigned short *scale = follow ? s_d + ((row >> 2) * NB + b) * 4 + (row & 3) : (unsigned short *)(head + kv4_scale_offset(row, b, DH));
+    float x[8];
+    if (IN) {
+      load8((values ? a.v_in + (r0 + r) * a.v_stride : a.k_in + (r0 + r) * a.k_stride) + h * DH + 8 * c8, x);
+      unsigned short d;
+      const uint32_t w = kv4_quantise8(x, d);
+      if (g == 0) *scale = d;
+      if (!values) {
+        *(uint32_t *)(head + kv4_key_offset(row, g, b, DH)) = spread4(w) | spread4(w >> 16) << 4;
+      } else {
+        unsigned char bytes[4];
+        const int c = value_bytes(w, g, bytes);
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          if (follow) s_v[(b * 16 + c + j) * LINE + kv4_value_place(row)] = bytes[j];
+          else head[kv4_value_offset(row, b, c + j)] = bytes[j];
+        }
+      }
+    } else {
+      const float d = half_bits_to_float(*scale);
+      if (!values) {
+        key_values(*(const uint32_t *)(head + kv4_key_offset(row, g, b, DH)), d, x);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+          const int line = b * 16 + 8 * (g & 1) + j;
+          const unsigned char byte = follow ? s_v[line * LINE + kv4_value_place(row)] : head[line * kKvPageRows + kv4_value_place(row)];
+          x[j] = d * (float)((int)((uint32_t)byte << (g < 2 ? 28 : 24)) >> 28);
+        }
+      }
+      float *dst = (values ? a.v_out : a.k_out) + ((int64_t)(r0 + r) * a.kv + h) * DH + 8 * c8;
+      *(f4_any *)dst = *(const f4_any *)x;
+      *(f4_any *)(dst + 4) = *(const f4_any *)(x + 4);
     }
   }
-  float *dst = out + (int64_t)blockIdx.x * kv * dh + 8 * e8;
-  *(f4_any *)dst = *(const f4_any *)x;
-  *(f4_any *)(dst + 4) = *(const f4_any *)(x + 4);
+  if (IN && follow) {
+    __syncthreads();
+    exchange();
+  }
+}
+
+template <bool IN>
+static int launch_kv4_rows(const Kv4Rows &a, int dh) {
+  const int eighths = a.kv * dh / 8;
+  // Rows of a decode step, one a sequence, or a page's worth and more: XX
+  if (a.n_rows < 2 * kKvPageRows) {
+    hipLaunchKernelGGL(k_kv4_rows<IN>, dim3((unsigned)a.n_rows, (unsigned)((eighths + 255) / 256), 2), dim3(256), 0, state().stream, a, dh);
+  } else {
+    const dim3 grid((unsigned)((a.n_rows + kKvPageRows - 1) / kKvPageRows), (unsigned)a.kv, 2);
+#define ROWS(DH_) hipLaunchKernelGGL((k_kv4_rows64<DH_, IN>), grid, dim3(256), 0, state().stream, a)
+    if (dh == 32) ROWS(32);
+    else if (dh == 64) ROWS(64);
+    else ROWS(128);
+#undef ROWS
+  }
+  CTHIP_LAUNCH_CHECK();
+  return 0;
 }
 
 // ---- reordering of beams ----
@@ -325,11 +474,7 @@ int cthip_kv_append_paged_q4(void *k_pages, void *v_pages, const float *k_rows, 
   if (n_rows == 0 || n_pages == 0) return 0;
   CTHIP_ARG(k_pages && v_pages && k_rows && v_rows && slots);
   CTHIP_ARG(aligned16(k_pages) && aligned16(v_pages) && k_stride >= (int64_t)kv_heads * head_dim && v_stride >= (int64_t)kv_heads * head_dim);
-  const int eighths = kv_heads * head_dim / 8;
-  hipLaunchKernelGGL(k_kv4_append, dim3((unsigned)n_rows, (unsigned)((eighths + 255) / 256), 2), dim3(256), 0, state().stream, (unsigned char *)k_pages,
-                     (unsigned char *)v_pages, k_rows, v_rows, k_stride, v_stride, slots, n_pages, kv_heads, head_dim);
-  CTHIP_LAUNCH_CHECK();
-  return 0;
+  return launch_kv4_rows<true>({(unsigned char *)k_pages, (unsigned char *)v_pages, k_rows, v_rows, nullptr, nullptr, k_stride, v_stride, slots, n_rows, n_pages, kv_heads}, head_dim);
 }
 
 int cthip_kv_rows_paged_q4(float *k_rows, float *v_rows, const void *k_pages, const void *v_pages, const int *slots, int n_rows, int n_pages, int kv_heads,
@@ -339,11 +484,7 @@ int cthip_kv_rows_paged_q4(float *k_rows, float *v_rows, const void *k_pages, co
   if (!kv4_shape_ok(kv_heads, head_dim)) return fail(CTHIP_E_UNSUPPORTED, "cthip_kv_rows_paged_q4: %d heads of %d (head sizes 32, 64, 128)", kv_heads, head_dim);
   if (n_rows == 0 || n_pages == 0 || (!k_rows && !v_rows)) return 0;
   CTHIP_ARG(slots && (!k_rows || k_pages) && (!v_rows || v_pages) && aligned16(k_pages) && aligned16(v_pages));
-  const int eighths = kv_heads * head_dim / 8;
-  hipLaunchKernelGGL(k_kv4_rows, dim3((unsigned)n_rows, (unsigned)((eighths + 255) / 256), 2), dim3(256), 0, state().stream, k_rows, v_rows,
-                     (const unsigned char *)k_pages, (const unsigned char *)v_pages, slots, n_pages, kv_heads, head_dim);
-  CTHIP_LAUNCH_CHECK();
-  return 0;
+  return launch_kv4_rows<false>({(unsigned char *)k_pages, (unsigned char *)v_pages, nullptr, nullptr, k_rows, v_rows, 0, 0, slots, n_rows, n_pages, kv_heads}, head_dim);
 }
 
 int cthip_beam_reorder_paged_q4(int *tables_out, int *history_out, void *k_pages, void *v_pages, int n_layers, int n_pages, const int *tables, int table_stride,
