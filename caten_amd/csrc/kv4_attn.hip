@@ -293,6 +293,15 @@ __global__ __launch_bounds__(256, DH == 128 ? 3 : 4) void k_kv4_attn(Kv4Attn a) 
   auto upper_of = [&](uint32_t u) { return __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2v, (u & upper) ^ e_upper) - (_Float16)72.0f); };
   __syncthreads();
   for (int k = 0; k < mine; k++) {
+    {
+      // Of the wavefronts on a SIMD the oldest goes first, and what it gains the others lose: the last workgroup of a compute unit ended at
+      // twice the first one's time, the SIMDs to itself.  So who has more left goes first, by quarters of a part.
+      const int left = 4 * (x1 - line - from_piece - (k << 2 >> a.piece_log2));
+      if (left > 3 * per) __builtin_amdgcn_s_setprio(3);
+      else if (left > 2 * per) __builtin_amdgcn_s_setprio(2);
+      else if (left > per) __builtin_amdgcn_s_setprio(1);
+      else __builtin_amdgcn_s_setprio(0);
+    }
     const int page = p0 + wv + 4 * k;
     const int from = valid(id[0]) ? page * kKvPageRows : INT_MAX - (kKvPageRows - 1);  // (absent: behind every limit)
     const bool whole = from + kKvPageRows - 1 <= least;                            // every row of the tile sees every row of the page (uniform)
