@@ -34,6 +34,14 @@ constexpr int kSplitSlots = 2048;   // records of shares in the workspace, two a
 constexpr int kJobPieces = 1;       // what a job costs besides its pages, in pieces of them
 constexpr int kMaxShares = 64;      // of one tile: their records are added up by one workgroup
 
+// floor(x / d) where that is below 2^21, x below 2^30: the quotient by a reciprocal is off by one at most, which what it leaves shows.  (A division
+// of integers is forty instructions that nothing runs beside.)
+__device__ __forceinline__ int fast_div(int x, int d) {
+  const int q = (int)((float)x * __builtin_amdgcn_rcpf((float)d)), left = x - q * d;
+  return q + (left >= d ? 1 : 0) - (left < 0 ? 1 : 0);
+}
+__device__ __forceinline__ int uniform_fast_div(int x, int d) { return __builtin_amdgcn_readfirstlane(fast_div(x, d)); }
+
 // sum over the lanes up to this one
 __device__ __forceinline__ int wave_scan_int(int v) {
   v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);  // row_shr:1
@@ -82,10 +90,7 @@ struct Job {
   int at, cost;         // its place on the line of all costs
 };
 // the job at a place on the line, which lies in front of its end
-__device__ __forceinline__ bool find_job(const Kv4Attn &a, int &first, int &before, int (*kept)[64], int place, Job &j) {
-  Batch s;
-  s.first = first, s.before = before;
-  s.get(kept);
+__device__ __forceinline__ bool find_job(const Kv4Attn &a, Batch &s, int (*kept)[64], int place, Job &j) {
   unsigned long long past;
   while (!(past = __ballot(s.upto > place))) {
     if (s.first + 64 >= a.n_seqs) return false;
@@ -94,16 +99,15 @@ __device__ __forceinline__ bool find_job(const Kv4Attn &a, int &first, int &befo
     look(a, s);
     s.put(kept);
   }
-  first = s.first, before = s.before;
   const int l = (int)__builtin_ctzll(past);
   const int tiles = __builtin_amdgcn_readlane(s.tiles, l), all = tiles * a.Hkv;
   j.cost = __builtin_amdgcn_readlane(s.cost, l);
-  const int start = __builtin_amdgcn_readlane(s.upto, l) - all * j.cost, job = (place - start) / j.cost;
+  const int start = __builtin_amdgcn_readlane(s.upto, l) - all * j.cost, job = uniform_fast_div(place - start, j.cost);
   // (starts that overlap can sum to anything: such rows are nobody's)
   if (place < start || job >= all) return false;
   j.at = start + job * j.cost;
   j.seq = s.first + l;
-  j.head = job / tiles;
+  j.head = tiles == 1 ? job : uniform_fast_div(job, tiles);
   // tiles from both ends in turn: in a prompt's own pages late rows see more than early ones, and a workgroup gets some of each
   const int t = job - j.head * tiles;
   j.tile = t & 1 ? tiles - 1 - (t >> 1) : t >> 1;
@@ -113,12 +117,12 @@ __device__ __forceinline__ bool find_job(const Kv4Attn &a, int &first, int &befo
   return true;
 }
 
-// The pages come straight into LDS, a wavefront's own ring: each the keys and the values of a head as they lie in memory.  A page's keys
-// give way to those of the page DEPTH further on as soon as the scores are there, its values when the outputs are.
+// The pages come straight into LDS, into a wavefront's own place: the keys and the values of a head as they lie in memory.  A page's
+// key quants are taken to registers when their turn comes, and the next page's are asked for at once; the rest follows when the scores, or the
+// outputs, are there.
 template <int DH>
 struct Kv4Lds {
-  static constexpr int DEPTH = 1;  // pages of a ring
-  static constexpr int HEAD = 36 * DH, SLOT = 2 * HEAD, WAVE = DEPTH * SLOT, STATS = 4 * WAVE, SEQS = STATS + 14 * kTileRows * 4, Q = SEQS + 4 * 6 * 64 * 4,
+  static constexpr int HEAD = 36 * DH, WAVE = 2 * HEAD, STATS = 4 * WAVE, SEQS = STATS + 14 * kTileRows * 4, Q = SEQS + 4 * 6 * 64 * 4,
                        BYTES = Q + DH / 32 * 2048;
   static constexpr int REQUESTS = DH / 32 + (DH / 32 + 1) / 2;  // of a head's part of a page: 16 bytes a lane, then 4
   static_assert(WAVE >= kTileRows * (DH + 4) * 4 && 4 * WAVE >= 8 * kMaxShares * kTileRows, "results and shares in the pages' place");
@@ -146,44 +150,48 @@ __global__ __launch_bounds__(256, DH == 128 ? 3 : 4) void k_kv4_attn(Kv4Attn a) 
   const int G = a.group;
   // workgroups are dealt to the eight XCDs in turn: neighbours on the line, which may read the same pages, on one of them
   const int me = (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
-  int total = 0, longest = 0, first = 0, before = 0;
-  {
-    Batch s;
-    for (look(a, s);;) {
-      int c = s.tiles ? s.cost : 0;
-      for (int o = 32; o > 0; o >>= 1) c = max(c, __shfl_xor(c, o, 64));
-      longest = max(longest, __builtin_amdgcn_readfirstlane(c));
-      total = __builtin_amdgcn_readlane(s.upto, 63);
-      if (s.first == 0) s.put(s_seqs[wv]);
-      if (s.first + 64 >= a.n_seqs) break;
-      s.before = total;
-      s.first += 64;
-      look(a, s);
-    }
+  int total = 0, longest = 0;
+  Batch s;
+  for (look(a, s);;) {
+    int c = s.tiles ? s.cost : 0;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) c = max(c, __shfl_xor(c, o, 64));
+    longest = max(longest, __builtin_amdgcn_readfirstlane(c));
+    total = __builtin_amdgcn_readlane(s.upto, 63);
+    if (s.first + 64 >= a.n_seqs) break;
+    s.before = total;
+    s.first += 64;
+    look(a, s);
   }
-  const int per = max((int)(((unsigned)total + gridDim.x - 1) / gridDim.x), (longest + kMaxShares - 2) / (kMaxShares - 1));
+  if (s.first) {
+    s.first = 0, s.before = 0;
+    look(a, s);
+  }
+  s.put(s_seqs[wv]);
+  const int per = max(uniform_fast_div(total + (int)gridDim.x - 1, (int)gridDim.x), (longest + kMaxShares - 2) / (kMaxShares - 1));
   const int x0 = (int)min((int64_t)me * per, (int64_t)total), x1 = min(total - x0, per) + x0;
   for (int x = x0; x < x1;) {
   Job w;
-  if (!find_job(a, first, before, s_seqs[wv], x, w)) break;
+  if (x != x0) s.get(s_seqs[wv]);
+  if (!find_job(a, s, s_seqs[wv], x, w)) break;
   x = w.at + w.cost;
   // (what hangs on the lane alone is worked out for each job: kept from being moved in front of the loop, where it would hold registers)
   int lane = tid0 & 63;
   asm volatile("" : "+v"(lane));
   const int n = lane & 15, g = lane >> 4;
   // this lane's row
-  const int rho = w.tile * kTileRows + n, j = rho / G;
+  const int rho = w.tile * kTileRows + n, j = fast_div(rho, G);
   const bool active = j < w.rows;
   const int head = w.head * G + rho - j * G;
   const int64_t all = (int64_t)a.table_stride * kKvPageRows;
   const int limit = active ? (int)min((int64_t)w.len - w.rows + j, all - 1) : -1;  // the last key it sees
   // pages that any row / every row of the tile sees (rows rise with n)
-  const int j1 = min(w.rows - 1, (w.tile * kTileRows + kTileRows - 1) / G), j0 = w.tile * kTileRows / G;
+  const int j1 = min(w.rows - 1, uniform_fast_div(w.tile * kTileRows + kTileRows - 1, G)), j0 = uniform_fast_div(w.tile * kTileRows, G);
   const int last = (int)min((int64_t)w.len - w.rows + j1, all - 1), least = (int)min((int64_t)w.len - w.rows + j0, all - 1);
   const int pages = a.n_pages > 0 && last >= 0 ? last / kKvPageRows + 1 : 0;
   // its pieces lie on the line behind those that stand for the rest (a job without pages is one piece of none)
   const int pieces = max(1, pages + (1 << a.piece_log2) - 1 >> a.piece_log2), line = w.at + kJobPieces;
-  const int owner = line / per, shares = (line + pieces - 1) / per - owner + 1, share = me - owner;
+  const int owner = uniform_fast_div(line, per), shares = uniform_fast_div(line + pieces - 1, per) - owner + 1, share = me - owner;
   const int from_piece = max(x0 - line, 0), to_piece = min(x1 - line, pieces);
   if (from_piece >= to_piece) continue;
   const int p0 = from_piece << a.piece_log2, p1 = (int)min((int64_t)pages, (int64_t)to_piece << a.piece_log2);
@@ -210,24 +218,27 @@ __global__ __launch_bounds__(256, DH == 128 ? 3 : 4) void k_kv4_attn(Kv4Attn a) 
   const unsigned char *ring = smem + wv * L::WAVE;
   const unsigned ring_at = (unsigned)(size_t)(__attribute__((address_space(3))) const unsigned char *)ring;
   // a head's part of a page (an absent page's is page 0's: its rows are masked)
-  auto ask = [&](const unsigned char *pool, int id, unsigned to) {
+  auto ask_quants = [&](const unsigned char *pool, int id, unsigned to) {
     const unsigned char *p = uniform(pool + ((int64_t)(valid(id) ? id : 0) * a.Hkv + w.head) * L::HEAD);
 #pragma unroll
     for (int i = 0; i < NB; i++) dma16(p + 1024 * i, 16 * lane, to + 1024 * i);
+  };
+  auto ask_scales = [&](const unsigned char *pool, int id, unsigned to) {
+    const unsigned char *p = uniform(pool + ((int64_t)(valid(id) ? id : 0) * a.Hkv + w.head) * L::HEAD) + 1024 * NB;
     if (NB > 1) {
 #pragma unroll
-      for (int i = 0; i < NB / 2; i++) dma4(p + 1024 * NB + 256 * i, 4 * lane, to + 1024 * NB + 256 * i);
+      for (int i = 0; i < NB / 2; i++) dma4(p + 256 * i, 4 * lane, to + 1024 * NB + 256 * i);
     } else if (lane < 32) {
-      dma4(p + 1024, 4 * lane, to + 1024);
+      dma4(p, 4 * lane, to + 1024);
     }
   };
-  auto ask_k = [&](int id, int k) { ask(a.k_pages, id, ring_at + k % L::DEPTH * L::SLOT); };
-  auto ask_v = [&](int id, int k) { ask(a.v_pages, id, ring_at + k % L::DEPTH * L::SLOT + L::HEAD); };
-  int id[L::DEPTH + 1];  // of the page that is worked on, and of those behind it
-#pragma unroll
-  for (int k = 0; k < L::DEPTH; k++) {
-    id[k] = k < mine ? page_id(k) : -1;
-    if (k < mine) ask_k(id[k], k), ask_v(id[k], k);
+  const unsigned char *const kp = ring, *const vp = ring + L::HEAD;
+  const unsigned k_at = ring_at, v_at = ring_at + L::HEAD;
+  int id = -1, next = -1;  // of the page that is worked on, and of the one behind it
+  if (mine > 0) {
+    id = page_id(0);
+    ask_quants(a.k_pages, id, k_at), ask_scales(a.k_pages, id, k_at);
+    ask_quants(a.v_pages, id, v_at), ask_scales(a.v_pages, id, v_at);
   }
 
   // The row's query as two fp16 terms, in LDS as the matrix instructions take them: [block][term][lane][8].  (Held in registers they are a
@@ -255,10 +266,9 @@ __global__ __launch_bounds__(256, DH == 128 ? 3 : 4) void k_kv4_attn(Kv4Attn a) 
     int bad = odd;
     bad |= __shfl_xor(bad, 16, 64);
     bad |= __shfl_xor(bad, 32, 64);
-    // a power of two that brings the row's largest into [2^9, 2^10): fp16's own 11 bits, and 11 below them
-    int e = top > 0.0f ? ilogbf(top) : 0;
-    if (bad) e = 0;
-    const float up = ldexpf(1.0f, 9 - e > 126 ? 126 : 9 - e);
+    // 2^(9 - e), e the exponent of the row's largest, brings that into [2^9, 2^10): fp16's own 11 bits, and 11 below them
+    const int e = min(max((int)(__float_as_uint(top) >> 23) - 127, -100), 127);
+    const float up = __uint_as_float((unsigned)(127 + 9 - e) << 23), down = __uint_as_float((unsigned)(127 - 9 + e) << 23);
     if (wv < NB) {
       half8 hi, lo;
 #pragma unroll
@@ -272,8 +282,8 @@ __global__ __launch_bounds__(256, DH == 128 ? 3 : 4) void k_kv4_attn(Kv4Attn a) 
       *(half8 *)(smem + L::Q + wv * 2048 + lane * 16) = hi;
       *(half8 *)(smem + L::Q + wv * 2048 + 1024 + lane * 16) = lo;
     }
-    // scores as powers of two: log2(e) / sqrt(DH), and the powers of two taken off again
-    weight = bad ? NAN : 1.44269504f / sqrtf((float)DH) / up;
+    // scores as powers of two: log2(e) / sqrt(DH), and the power of two taken off again
+    weight = bad ? NAN : (DH == 32 ? 0.25503487f : DH == 64 ? 0.18033688f : 0.12751743f) * down;
   }
 
   f32x4 o[NB][2];
@@ -303,16 +313,15 @@ __global__ __launch_bounds__(256, DH == 128 ? 3 : 4) void k_kv4_attn(Kv4Attn a) 
       else __builtin_amdgcn_s_setprio(0);
     }
     const int page = p0 + wv + 4 * k;
-    const int from = valid(id[0]) ? page * kKvPageRows : INT_MAX - (kKvPageRows - 1);  // (absent: behind every limit)
+    const int from = valid(id) ? page * kKvPageRows : INT_MAX - (kKvPageRows - 1);  // (absent: behind every limit)
     const bool whole = from + kKvPageRows - 1 <= least;                            // every row of the tile sees every row of the page (uniform)
-    const unsigned char *kp = ring + k % L::DEPTH * L::SLOT, *vp = kp + L::HEAD;
     // the scales of block b, rows 16 t + 4 g ..
     auto scales = [&](const unsigned char *p, int t, int b) { return *(const half4 *)(p + 32 * DH + ((4 * t + g) * NB + b) * 8); };
     typedef uint32_t kdw __attribute__((ext_vector_type(NB)));
     typedef unsigned short sdw __attribute__((ext_vector_type(NB)));
-    // younger than this page's keys: its values, and what has been asked for of the pages behind it
-    if (L::DEPTH == 2 && k + 1 < mine) wait_loads<3 * L::REQUESTS>();
-    else wait_loads<L::REQUESTS>();
+    wait_loads<L::REQUESTS>();  // (younger than this page's keys: its values)
+    const bool more = k + 1 < mine;
+    if (more) next = page_id(k + 1);
     f32x4 s[4];
     kdw kq[4];
 #pragma unroll
@@ -320,6 +329,8 @@ __global__ __launch_bounds__(256, DH == 128 ? 3 : 4) void k_kv4_attn(Kv4Attn a) 
       s[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
       kq[t] = *(const kdw *)(kp + kv4_key_offset(16 * t + n, g, 0, DH));
     }
+    wait_lds();
+    if (more) ask_quants(a.k_pages, next, k_at);
 #pragma unroll
     for (int b = 0; b < NB; b++) {
       const half8 q_hi = *(const half8 *)(smem + L::Q + b * 2048 + lane * 16), q_lo = *(const half8 *)(smem + L::Q + b * 2048 + 1024 + lane * 16);
@@ -335,10 +346,7 @@ __global__ __launch_bounds__(256, DH == 128 ? 3 : 4) void k_kv4_attn(Kv4Attn a) 
       }
     }
     wait_lds();
-    if (k + L::DEPTH < mine) {
-      id[L::DEPTH] = page_id(k + L::DEPTH);
-      ask_k(id[L::DEPTH], k);
-    }
+    if (more) ask_scales(a.k_pages, next, k_at);
     if (!whole) {
 #pragma unroll
       for (int t = 0; t < 4; t++)
@@ -366,8 +374,7 @@ __global__ __launch_bounds__(256, DH == 128 ? 3 : 4) void k_kv4_attn(Kv4Attn a) 
         s[t][i] = __builtin_amdgcn_exp2f(fmaf(s[t][i], weight, -base));
         l += s[t][i];
       }
-    if (k + L::DEPTH < mine) wait_loads<(2 * L::DEPTH - 1) * L::REQUESTS>();
-    else if (L::DEPTH == 2 && k + 1 < mine) wait_loads<2 * L::REQUESTS>();
+    if (more) wait_loads<L::REQUESTS>();  // (younger than this page's values: the next one's keys)
     else wait_loads<0>();
     {
       const sdw vs_now = *(const sdw *)(vp + 32 * DH + lane * NB * 2);
@@ -438,9 +445,8 @@ __global__ __launch_bounds__(256, DH == 128 ? 3 : 4) void k_kv4_attn(Kv4Attn a) 
     if (whole && f == 0) outputs(std::true_type());
     else outputs(std::false_type());
     wait_lds();
-    if (k + L::DEPTH < mine) ask_v(id[L::DEPTH], k);
-#pragma unroll
-    for (int i = 0; i < L::DEPTH; i++) id[i] = id[i + 1];
+    if (more) ask_quants(a.v_pages, next, v_at), ask_scales(a.v_pages, next, v_at);
+    id = next;
   }
   l += __shfl_xor(l, 16, 64);
   l += __shfl_xor(l, 32, 64);
@@ -480,7 +486,7 @@ __global__ __launch_bounds__(256, DH == 128 ? 3 : 4) void k_kv4_attn(Kv4Attn a) 
   __syncthreads();
   // where a pair of channels of a tile's row goes
   auto out_at = [&](int r, int c) {
-    const int rr = w.tile * kTileRows + r, jj = rr / G;
+    const int rr = w.tile * kTileRows + r, jj = fast_div(rr, G);
     return a.out + ((int64_t)(w.row0 + jj) * a.H + w.head * G + rr - jj * G) * DH + c;
   };
   for (int e = tid; e < nr * DH / 2; e += 256) {
@@ -567,7 +573,7 @@ int cthip_sdpa_paged_q4(float *out, const float *q, int64_t q_stride, const void
   CTHIP_ARG((((uintptr_t)k_pages | (uintptr_t)v_pages | (uintptr_t)workspace) & 15) == 0);
   // rows of a tile share a key / value head: at most this many tiles of all sequences, and as many jobs a head
   const int64_t tiles = (int64_t)n_rows * (H / Hkv) / kTileRows + (n_seqs < n_rows ? n_seqs : n_rows), jobs = tiles * Hkv;
-  if (jobs > (1 << 28)) return fail(CTHIP_E_UNSUPPORTED, "cthip_sdpa_paged_q4: %d rows of %d heads in one call", n_rows, H);
+  if (jobs > (1 << 21)) return fail(CTHIP_E_UNSUPPORTED, "cthip_sdpa_paged_q4: %d rows of %d heads in one call", n_rows, H);
   int piece = 2;
   while (jobs * ((table_stride >> piece) + 1 + kJobPieces) > INT_MAX / 2) piece++;
   // as many workgroups as run at once (three or four a compute unit for their registers and pages), a multiple of the XCDs
