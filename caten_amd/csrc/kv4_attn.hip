@@ -42,7 +42,7 @@ __device__ __forceinline__ int fast_div(int x, int d) {
 }
 __device__ __forceinline__ int uniform_fast_div(int x, int d) { return __builtin_amdgcn_readfirstlane(fast_div(x, d)); }
 
-// sum over the lanes up to this one
+// sum, and maximum, over the lanes up to this one
 __device__ __forceinline__ int wave_scan_int(int v) {
   v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);  // row_shr:1
   v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);
@@ -50,6 +50,15 @@ __device__ __forceinline__ int wave_scan_int(int v) {
   v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true);
   v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);  // row_bcast:15 into rows 1 and 3
   v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);  // row_bcast:31 into rows 2 and 3
+  return v;
+}
+__device__ __forceinline__ int wave_scan_max(int v) {
+  v = max(v, __builtin_amdgcn_update_dpp(v, v, 0x111, 0xF, 0xF, false));  // (a lane that gets nothing: its own)
+  v = max(v, __builtin_amdgcn_update_dpp(v, v, 0x112, 0xF, 0xF, false));
+  v = max(v, __builtin_amdgcn_update_dpp(v, v, 0x114, 0xF, 0xF, false));
+  v = max(v, __builtin_amdgcn_update_dpp(v, v, 0x118, 0xF, 0xF, false));
+  v = max(v, __builtin_amdgcn_update_dpp(v, v, 0x142, 0xA, 0xF, false));
+  v = max(v, __builtin_amdgcn_update_dpp(v, v, 0x143, 0xC, 0xF, false));
   return v;
 }
 
@@ -60,6 +69,7 @@ __device__ __forceinline__ int wave_scan_int(int v) {
 // the division out for itself, 64 sequences at a time.
 struct Batch {
   int first = 0, before = 0;  // of the 64 sequences in the lanes: the first, and the cost in front of it
+  int reach = 0;              // the largest start up to the last of them
   int len, row0, rows, tiles, cost, upto;  // this lane's; cost: of one job; upto: of all up to the end of this sequence
   // A wavefront keeps them in LDS while it works on a job: they are needed again for the next one only.
   __device__ __forceinline__ void put(int (*to)[64]) const {
@@ -73,15 +83,16 @@ struct Batch {
 };
 __device__ __forceinline__ void look(const Kv4Attn &a, Batch &s) {
   const int i = s.first + (int)(threadIdx.x & 63);
-  s.len = 0, s.row0 = 0, s.rows = 0;
-  if (i < a.n_seqs) {
-    s.len = a.lens[i], s.row0 = a.starts[i];
-    const int end = min(a.starts[i + 1], a.n_rows);
-    s.rows = s.row0 >= 0 && end > s.row0 ? end - s.row0 : 0;
-  }
+  s.len = 0, s.row0 = 0;
+  int end = 0;
+  if (i < a.n_seqs) s.len = max(a.lens[i], 0), s.row0 = a.starts[i], end = min(a.starts[i + 1], a.n_rows);
+  // (rows in front of an earlier sequence's are nobody's: no row is two sequences', and the costs of all stay within their bound)
+  const int reach = max(s.reach, wave_scan_max(s.row0));
+  s.reach = __builtin_amdgcn_readlane(reach, 63);
+  s.rows = s.row0 == reach && end > s.row0 ? end - s.row0 : 0;
   s.tiles = (s.rows * a.group + kTileRows - 1) / kTileRows;
   const int pages = a.n_pages > 0 && s.len > 0 ? (int)min(((unsigned)s.len + kKvPageRows - 1) / kKvPageRows, (unsigned)a.table_stride) : 0;
-  s.cost = (pages + (1 << a.piece_log2) - 1 >> a.piece_log2) + kJobPieces;
+  s.cost = max(1, pages + (1 << a.piece_log2) - 1 >> a.piece_log2) + kJobPieces;  // (without keys there is still a row to write)
   s.upto = s.before + wave_scan_int(s.tiles * a.Hkv * s.cost);
 }
 struct Job {
@@ -103,8 +114,6 @@ __device__ __forceinline__ bool find_job(const Kv4Attn &a, Batch &s, int (*kept)
   const int tiles = __builtin_amdgcn_readlane(s.tiles, l), all = tiles * a.Hkv;
   j.cost = __builtin_amdgcn_readlane(s.cost, l);
   const int start = __builtin_amdgcn_readlane(s.upto, l) - all * j.cost, job = uniform_fast_div(place - start, j.cost);
-  // (starts that overlap can sum to anything: such rows are nobody's)
-  if (place < start || job >= all) return false;
   j.at = start + job * j.cost;
   j.seq = s.first + l;
   j.head = tiles == 1 ? job : uniform_fast_div(job, tiles);
@@ -164,7 +173,7 @@ __global__ __launch_bounds__(256, DH == 128 ? 3 : 4) void k_kv4_attn(Kv4Attn a) 
     look(a, s);
   }
   if (s.first) {
-    s.first = 0, s.before = 0;
+    s.first = 0, s.before = 0, s.reach = 0;
     look(a, s);
   }
   s.put(s_seqs[wv]);
@@ -292,6 +301,10 @@ __global__ __launch_bounds__(256, DH == 128 ? 3 : 4) void k_kv4_attn(Kv4Attn a) 
   float m = -INFINITY, l = 0.0f;
   int f = 100;  // the values' scales go in as 2^f d (100: none seen)
 
+  // What a row's weights are taken against: 2^(m weight - base) = 2^14.  The base is used as it is rounded wherever weights of different maxima
+  // meet, so its rounding cancels.
+  auto base_of = [&](float top) { return top > -INFINITY ? fmaf(top, weight, -14.0f) : -14.0f; };
+
   // a number that the compiler does not see through: half * minus + a is then one mixed instruction, where a difference is a conversion more
   float minus = -1.0f;
   asm volatile("" : "+s"(minus));
@@ -360,20 +373,27 @@ __global__ __launch_bounds__(256, DH == 128 ? 3 : 4) void k_kv4_attn(Kv4Attn a) 
     top = fmaxf(top, __shfl_xor(top, 16, 64));
     top = fmaxf(top, __shfl_xor(top, 32, 64));
     if (__ballot(top > m)) {  // a new maximum in some row
-      const float m_new = fmaxf(m, top), corr = m_new > -INFINITY ? __builtin_amdgcn_exp2f((m - m_new) * weight) : 1.0f;
+      const float m_new = fmaxf(m, top), corr = m > -INFINITY ? __builtin_amdgcn_exp2f(base_of(m) - base_of(m_new)) : 0.0f;
       m = m_new;
       l *= corr;
 #pragma unroll
       for (int b = 0; b < NB; b++) o[b][0] *= corr, o[b][1] *= corr;
     }
-    const float base = (m > -INFINITY ? m * weight : 0.0f) - 14.0f;
+    const float base = base_of(m);
+    if (__ballot(!(fabsf(base) < 4194304.0f))) {  // (seldom: where the base's rounding is a power of two that matters)
+      const float from_m = m > -INFINITY ? m : 0.0f;
 #pragma unroll
-    for (int t = 0; t < 4; t++)
+      for (int t = 0; t < 4; t++)
 #pragma unroll
-      for (int i = 0; i < 4; i++) {
-        s[t][i] = __builtin_amdgcn_exp2f(fmaf(s[t][i], weight, -base));
-        l += s[t][i];
-      }
+        for (int i = 0; i < 4; i++) s[t][i] = __builtin_amdgcn_exp2f(fmaf(s[t][i] - from_m, weight, 14.0f));
+    } else {
+#pragma unroll
+      for (int t = 0; t < 4; t++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) s[t][i] = __builtin_amdgcn_exp2f(fmaf(s[t][i], weight, -base));
+    }
+#pragma unroll
+    for (int t = 0; t < 4; t++) l += (s[t][0] + s[t][1]) + (s[t][2] + s[t][3]);
     if (more) wait_loads<L::REQUESTS>();  // (younger than this page's values: the next one's keys)
     else wait_loads<0>();
     {
@@ -455,7 +475,7 @@ __global__ __launch_bounds__(256, DH == 128 ? 3 : 4) void k_kv4_attn(Kv4Attn a) 
   int tid = tid0;
   asm volatile("" : "+v"(tid));
   const int nr = min(kTileRows, w.rows * G - w.tile * kTileRows);  // rows of the tile that there are
-  if (g == 0) s_m[wv][n] = m * weight, s_l[wv][n] = l;
+  if (g == 0) s_m[wv][n] = m > -INFINITY ? base_of(m) : -INFINITY, s_l[wv][n] = l;
   const float back = ldexpf(1.0f, f == 100 ? 0 : -f);
   if (n < nr) {
 #pragma unroll
@@ -573,11 +593,12 @@ int cthip_sdpa_paged_q4(float *out, const float *q, int64_t q_stride, const void
   CTHIP_ARG((((uintptr_t)k_pages | (uintptr_t)v_pages | (uintptr_t)workspace) & 15) == 0);
   // rows of a tile share a key / value head: at most this many tiles of all sequences, and as many jobs a head
   const int64_t tiles = (int64_t)n_rows * (H / Hkv) / kTileRows + (n_seqs < n_rows ? n_seqs : n_rows), jobs = tiles * Hkv;
-  if (jobs > (1 << 21)) return fail(CTHIP_E_UNSUPPORTED, "cthip_sdpa_paged_q4: %d rows of %d heads in one call", n_rows, H);
-  int piece = 2;
-  while (jobs * ((table_stride >> piece) + 1 + kJobPieces) > INT_MAX / 2) piece++;
+  if (jobs > (1 << 21) || n_rows > (1 << 20))
+    return fail(CTHIP_E_UNSUPPORTED, "cthip_sdpa_paged_q4: %d rows of %d heads in one call (at most 2^20 rows, and 2^21 tiles of 16 heads of them)", n_rows, H);
   // as many workgroups as run at once (three or four a compute unit for their registers and pages), a multiple of the XCDs
   const int at_once = std::min(kSplitSlots / 2, state().compute_units * (Dh == 128 ? 3 : 4) / 8 * 8);
+  int piece = 2;  // (the line is shorter than 2^30, and a workgroup's part of it below what fast_div holds for)
+  while (jobs * ((table_stride >> piece) + 1 + kJobPieces) > std::min((int64_t)INT_MAX / 2, (int64_t)at_once << 20)) piece++;
   const Kv4Attn a = {out,     q,     (const unsigned char *)k_pages, (const unsigned char *)v_pages, tables, lens, starts, q_stride, n_pages, table_stride, n_seqs, n_rows, H, Hkv,
                      H / Hkv, piece, (int *)workspace, (float *)workspace + kSplitSlots};
   const dim3 grid((unsigned)at_once), block(256);

@@ -113,6 +113,17 @@ def _fill(cache, byte):
         _lib.check(_lib.load().cthip_memset(pool.ptr, byte, pool.nbytes))
 
 
+def attend_over(value, cache, q, tables, lens, starts):
+    """PagedCacheQ4.attend into an array that holds `value`."""
+    from caten_amd import _lib, ops
+    n, H, dh = q.shape
+    dq, dt, dl, ds = (ops.DeviceArray.from_numpy(np.ascontiguousarray(a, t)) for a, t in ((q, np.float32), (tables, np.int32), (lens, np.int32), (starts, np.int32)))
+    out = ops.DeviceArray.from_numpy(np.full(q.shape, value, np.float32))
+    _lib.check(_lib.load().cthip_sdpa_paged_q4(out.ptr, dq.ptr, H * dh, cache.k.ptr, cache.v.ptr, cache.n_pages, dt.ptr, tables.shape[1], dl.ptr, ds.ptr, len(lens), n, H, cache.kv_heads, dh,
+                                               cache.workspace.ptr))
+    return out.numpy()
+
+
 # ------------------------------------------------------------------------------------------------------------- planning
 
 
@@ -165,7 +176,7 @@ def test_plan_out_of_place_leaves_its_inputs():
 # ------------------------------------------------------------------------------------------------------- rows in and out
 
 
-@pytest.mark.parametrize("kv,dh,rows", [(1, 32, 1), (12, 64, 48), (3, 32, 200), (8, 128, 130), (32, 128, 3), (5, 64, 1000)])
+@pytest.mark.parametrize("kv,dh,rows", [(1, 32, 1), (12, 64, 48), (3, 32, 200), (8, 128, 130), (32, 128, 3), (5, 64, 1000), (17, 64, 1100), (32, 32, 1024), (8, 128, 1025)])
 def test_rows_in_and_out(kv, dh, rows):
     print(f"case: rows {kv} heads of {dh}, {rows} rows", flush=True)
     from caten_amd import ops
@@ -236,6 +247,59 @@ def test_strided_rows_and_slots_outside_the_pool():
     _lib.check(lib.cthip_kv_rows_paged_q4(None, out.ptr, None, cache.v.ptr, ds.ptr, rows, 2, kv, dh))
     got = out.numpy()
     assert (got[~fine] == 7.0).all() and not (got[fine] == 7.0).any()
+
+
+@pytest.mark.parametrize("kv,dh,offset,rows", [(3, 64, 17, 200), (40, 32, 0, 900), (17, 64, 17, 1000), (9, 128, 63, 1000), (33, 64, 1, 513), (64, 32, 61, 640), (8, 128, 0, 64 * 16 + 3)])
+def test_rows_of_a_prompt(kv, dh, offset, rows):
+    """Slots that follow one another, from anywhere in a page on, pages in any order; one row of the third 64 is left out."""
+    print(f"case: prompt of {rows} rows from row {offset} on, {kv} heads of {dh}", flush=True)
+    from caten_amd import ops
+    rng = np.random.default_rng(offset + rows)
+    cache = ops.PagedCacheQ4(-(-(offset + rows) // PAGE) + 2, kv, dh)
+    _fill(cache, 0x5a)
+    pages = rng.permutation(cache.n_pages)
+    at = offset + np.arange(rows)
+    slots = (pages[at // PAGE] * PAGE + at % PAGE).astype(np.int32)
+    left_out = 140 if rows > 180 else rows - 1
+    there = np.arange(rows) != left_out
+    others = np.setdiff1d(np.arange(cache.n_pages * PAGE), slots[there]).astype(np.int32)
+    before = cache.rows(others)
+    k, v = (rng.normal(0, 1, (rows, kv, dh)).astype(np.float32) for _ in range(2))
+    given = np.where(there, slots, -1)
+    cache.append(k, v, given)
+    got_k, got_v = cache.rows(given)
+    assert np.array_equal(got_k[there], quantised(k[there])) and np.array_equal(got_v[there], quantised(v[there]))
+    assert not got_k[left_out].any() and not got_v[left_out].any()
+    one_by_one = [cache.rows(given[i:i + 1]) for i in range(0, rows, 37)]  # (a few rows take another kernel)
+    assert all(np.array_equal(a[0], got_k[i]) and np.array_equal(b[0], got_v[i]) for i, (a, b) in zip(range(0, rows, 37), one_by_one))
+    assert all(np.array_equal(a, b) for a, b in zip(before, cache.rows(others)))
+    # the same rows, one at a time, are the same bytes
+    whole = cache.k.numpy(), cache.v.numpy()
+    _fill(cache, 0x5a)
+    for i in range(0, rows, 100):
+        cache.append(k[i:i + 100], v[i:i + 100], given[i:i + 100])
+    assert np.array_equal(whole[0], cache.k.numpy()) and np.array_equal(whole[1], cache.v.numpy())
+
+
+def test_places_past_32_bits():
+    """A pool of more than 2^32 bytes, its last pages in use."""
+    from caten_amd import ops
+    rng = np.random.default_rng(21)
+    kv, dh, n_pages = 32, 128, 30000  # 4.4 GB a pool
+    cache = ops.PagedCacheQ4(n_pages, kv, dh)
+    lens, H = [130, 200], 32
+    tables = np.array([[n_pages - 1, 3, n_pages - 2, -1], [n_pages - 3, n_pages - 4, 5, n_pages - 5]], np.int32)
+    held = []
+    for i, n in enumerate(lens):
+        slots = np.array([tables[i, t // PAGE] * PAGE + t % PAGE for t in range(n)], np.int32)
+        k, v = (rng.normal(0, 1, (n, kv, dh)).astype(np.float32) for _ in range(2))
+        cache.append(k, v, slots)
+        held.append(cache.rows(slots))
+        assert np.array_equal(held[-1][0], quantised(k)) and np.array_equal(held[-1][1], quantised(v))
+    q = rng.normal(0, 1, (2, H, dh)).astype(np.float32)
+    got = cache.attend(q, tables, lens, [0, 1, 2])
+    for i, (k, v) in enumerate(held):
+        close(got[i:i + 1], *attention(q[i:i + 1], k, v))
 
 
 # ------------------------------------------------------------------------------------------------------------ attention
@@ -316,6 +380,132 @@ def test_rows_that_see_nothing_and_rows_behind_the_last(H, kv, rows):
         t = 200 - rows + r + 1
         keep = [x for x in range(t) if x // PAGE != 1]
         close(got[r:r + 1], *attention(q[r:r + 1], k[keep], v[keep]))
+
+
+def test_a_very_long_sequence():
+    """More pages than a wavefront holds the ids of: over a million keys of one narrow head."""
+    from caten_amd import ops
+    rng = np.random.default_rng(22)
+    T, kv, dh, H = 1100000, 1, 32, 3
+    n_pages = -(-T // PAGE)
+    cache = ops.PagedCacheQ4(n_pages, kv, dh)
+    tables = rng.permutation(n_pages).astype(np.int32)[None]
+    slots = (tables[0].astype(np.int64)[np.arange(T) // PAGE] * PAGE + np.arange(T) % PAGE).astype(np.int32)
+    k, v = (rng.standard_normal((T, kv, dh), np.float32) for _ in range(2))
+    k[::, 0] *= (1 + np.arange(T) % 3)[:, None]
+    cache.append(k, v, slots)
+    k, v = cache.rows(slots)
+    q = rng.normal(0, 1, (2, H, dh)).astype(np.float32)
+    got = cache.attend(q, tables, [T], [0, 2])
+    want, size, big = attention(q, k, v)
+    # sums of 1.1e6 positive terms in 63 x 4 pieces of some 70 pages: off by a few hundred roundings of 2^-24 at most, against 2^-16 allowed for
+    close(got, want, size, big)
+
+
+@pytest.mark.parametrize("H,kv,dh", [(4, 2, 64), (16, 1, 128), (3, 3, 32)])
+@pytest.mark.parametrize("rows", [1, 20])
+@pytest.mark.parametrize("factors", [(1e-6,), (1e-3,), (30,), (1e5,), (1e-4, 1, 1e3), (1e3, 1, 1e-2), (0, 1), (1, 0, 50)])
+def test_sizes_of_values(H, kv, dh, rows, factors):
+    """Values from where a block's scale is subnormal to where it is the largest there is, alike or different page by page."""
+    from caten_amd import ops
+    rng = np.random.default_rng(dh + rows)
+    T = 40 * PAGE + 30
+    cache, tables, starts, held = batch(rng, [T], [rows], kv, dh)
+    slots = np.array([tables[0, t // PAGE] * PAGE + t % PAGE for t in range(T)], np.int32)
+    factor = np.array(factors)[np.arange(T) // PAGE * len(factors) // (T // PAGE + 1)].astype(np.float32)
+    k, v = held[0][0], held[0][1] * factor[:, None, None]
+    cache.append(k, v, slots)
+    k, v = cache.rows(slots)
+    q = rng.normal(0, 1, (rows, H, dh)).astype(np.float32)
+    close(cache.attend(q, tables, [T], starts), *attention(q, k, v))
+
+
+@pytest.mark.parametrize("factor", [1e-30, 1e-4, 3e3, 1e6, 1e9, 1e25])
+def test_sizes_of_queries(factor):
+    """Scores that are all alike, and scores of which the largest alone counts, up to where fp32 does not tell neighbours apart."""
+    rng = np.random.default_rng(24)
+    for H, kv, dh, rows in ((4, 2, 64, 1), (8, 1, 32, 20)):
+        T = 500
+        cache, tables, starts, held = batch(rng, [T], [rows], kv, dh)
+        q = (rng.normal(0, 1, (rows, H, dh)) * factor).astype(np.float32)
+        got = cache.attend(q, tables, [T], starts)
+        want, size, big = attention(q, *held[0])
+        if factor < 1e5:
+            close(got, want, size, big)
+            continue
+        # a score is off by what 2^-22 of its terms' sum is: keys that near the largest may have any share, others none
+        for r in range(rows):
+            for h in range(H):
+                k, v = (a[:T - rows + r + 1, h // (H // kv)].astype(np.float64) for a in held[0])
+                s = k @ q[r, h].astype(np.float64) / np.sqrt(dh)
+                near = s >= s.max() - size[r, h] * 2.0 ** -19 - 20
+                assert np.isfinite(got[r, h]).all()
+                slack = big[r, h] * 2.0 ** -15
+                assert (got[r, h] >= v[near].min(0) - slack).all() and (got[r, h] <= v[near].max(0) + slack).all()
+
+
+def test_starts_in_any_order():
+    """Rows in front of an earlier sequence's are nobody's; a negative length is none.  The workspace stays as it was."""
+    rng = np.random.default_rng(25)
+    kv, dh, H = 2, 64, 4
+    lens = [5000, 300, 200, 100] + [40] * 100
+    cache, tables, _, held = batch(rng, lens, [0] * len(lens), kv, dh)
+    n = 12
+    q = rng.normal(0, 1, (n, H, dh)).astype(np.float32)
+
+    def call(starts, lens):
+        return attend_over(7.0, cache, q, tables, lens, starts)
+
+    def whose(got, rows, i):
+        close(got[rows], *attention(q[rows], *held[i]))
+
+    got = call([0, 2, 1, 3, 4] + [4] * 100, lens)  # sequence 1 ends in front of its start, sequence 2's row 1 is sequence 0's
+    whose(got, slice(0, 2), 0)
+    whose(got, slice(3, 4), 3)
+    assert (got[2] == 7.0).all() and (got[4:] == 7.0).all()
+    got = call([-3, 2, 4, 2 ** 31 - 1, 5] + [0] * 99 + [3], lens)
+    whose(got, slice(2, 4), 1)
+    whose(got, slice(4, 12), 2)
+    assert (got[:2] == 7.0).all()
+    many = [0] * 70 + [9] + [1, 9, 10] * 10 + [4, 12, 11]  # behind the first 64
+    got = call(many + [11], lens)
+    whose(got, slice(0, 9), 69)
+    owner = [i for i in range(len(lens)) if many[i] == 9 and (many + [11])[i + 1] == 10][0]
+    whose(got, slice(9, 10), owner)
+    starts = np.minimum(np.arange(len(lens) + 1), 4)
+    got = call(starts, [5000, -1, -2 ** 31, 100] + [40] * 100)
+    whose(got, slice(0, 1), 0)
+    whose(got, slice(3, 4), 3)
+    assert not got[1:3].any()
+    assert not cache.workspace.numpy()[:4 * 2048].any()
+
+
+@pytest.mark.parametrize("H,kv,dh", [(4, 4, 32), (20, 1, 64), (8, 2, 128)])
+def test_sequences_without_keys(H, kv, dh):
+    """Their rows are zero, wherever they lie between the others."""
+    rng = np.random.default_rng(H)
+    for n, share in ((1, 1.0), (5, 0.5), (700, 0.5), (700, 1.0)):
+        lens = np.where(rng.uniform(0, 1, n) < share, 0, rng.integers(1, 300, n))
+        rows = np.where(lens == 0, rng.integers(1, 4, n), np.minimum(lens, rng.integers(0, 3, n)))
+        cache, tables, starts, held = batch(rng, list(lens), list(rows), kv, dh)
+        q = rng.normal(0, 1, (rows.sum(), H, dh)).astype(np.float32)
+        got = attend_over(7.0, cache, q, tables, lens, starts)
+        for i, (k, v) in enumerate(held):
+            mine = slice(starts[i], starts[i + 1])
+            if lens[i] == 0:
+                assert not got[mine].any()
+            else:
+                close(got[mine], *attention(q[mine], k, v))
+
+
+def test_nothing_in_the_pool():
+    from caten_amd import _lib, ops
+    lib, out = _lib.init(), ops.DeviceArray.from_numpy(np.full((3, 2, 32), 7.0, np.float32))
+    ws = ops.DeviceArray((int(lib.cthip_sdpa_paged_q4_workspace(32)),), np.uint8)
+    q, t, lens, starts = (ops.DeviceArray.from_numpy(a) for a in (np.ones((3, 2, 32), np.float32), np.zeros((2, 4), np.int32), np.array([9, 0], np.int32), np.array([0, 1, 2], np.int32)))
+    _lib.check(lib.cthip_sdpa_paged_q4(out.ptr, q.ptr, 64, None, None, 0, t.ptr, 4, lens.ptr, starts.ptr, 2, 3, 2, 1, 32, ws.ptr))
+    got = out.numpy()
+    assert not got[:2].any() and (got[2] == 7.0).all()
 
 
 def test_more_rows_than_keys_and_a_table_that_is_too_short():
@@ -537,7 +727,9 @@ def test_refusals():
     for change in (dict(out=None), dict(q=None), dict(k=None), dict(v=None), dict(tables=None), dict(lens=None), dict(starts=None), dict(ws=None), dict(ws=p + 4), dict(k=p + 8), dict(qs=127), dict(n=-1),
                    dict(rows=-1), dict(stride=0), dict(H=3), dict(H=0), dict(pages=-1)):
         refused(bad, lib.cthip_sdpa_paged_q4, *attend(**change))
-    for change in (dict(dh=96, qs=1000), dict(n=4097)):
+    refused(no, lib.cthip_kv_append_paged_q4, *append(rows=2 ** 28 + 1))
+    refused(no, lib.cthip_kv_rows_paged_q4, *rows(rows=2 ** 28 + 1))
+    for change in (dict(dh=96, qs=1000), dict(n=4097), dict(rows=2 ** 20 + 1), dict(rows=2 ** 20, H=128, kv=1, qs=4096), dict(H=65536, kv=65536, qs=2 ** 21)):
         refused(no, lib.cthip_sdpa_paged_q4, *attend(**change))
     # nothing to do
     _lib.check(lib.cthip_kv_append_paged_q4(*append(rows=0, k=None)))
