@@ -1,10 +1,10 @@
 // Beam search's selection: the n_beams best of (beam, token) by score[beam] + log softmax(logits[beam])[token].  The reference
 // decodes greedily (apps/gpt2/gpt2.lisp:97-113); this is its !argmax (api/high-level-ops.lisp:314-343) for several hypotheses.
 //
-// The logits are read once: a row is cut into slices, a workgroup holds a slice in registers, 8 or 32 values a thread, and leaves its
+// The logits are read once: a row is cut into slices, a workgroup holds a slice in registers, 16 or 32 values a thread, and leaves its
 // maximum, its sum of exponentials and its n_beams best in order.  A second launch joins the rows' sums and merges the sorted lists,
 // a workgroup a request.  (As one launch, the last of a request's workgroups merging, stores had to reach memory and a ticket be
-// drawn before a workgroup could end, and the merge's registers were everybody's: 62 us instead of XX for 48 x 8 beams of 32000.)
+// drawn before a workgroup could end, and the merge's registers were everybody's: 62 us instead of 26 for 48 x 8 beams of 32000.)
 // Everything behind the exponentials is in 64 bits: between beams, candidates are compared by sums that a rounding could turn round.
 #include <algorithm>
 
@@ -380,16 +380,17 @@ int cthip_beam_select(int *tokens, int *parents, float *scores_out, int *finishe
                       const int *finished, int n_batch, int n_beams, int vocab, int eos, void *workspace) {
   CTHIP_REQUIRE_INIT();
   CTHIP_ARG(n_batch >= 0 && n_beams >= 1 && vocab >= 1 && vocab >= n_beams && vocab <= (1 << 30) && logits_stride >= vocab && eos >= -1 && eos < vocab);
-  if (n_beams > kMaxSelectBeams || (int64_t)n_batch * n_beams > (1 << 24))
-    return fail(CTHIP_E_UNSUPPORTED, "cthip_beam_select: %d x %d beams (at most %d, and 2^24 in all)", n_batch, n_beams, kMaxSelectBeams);
+  if (n_beams > kMaxSelectBeams || (int64_t)n_batch * n_beams > (1 << 18))
+    return fail(CTHIP_E_UNSUPPORTED, "cthip_beam_select: %d x %d beams (at most %d, and 2^18 in all)", n_batch, n_beams, kMaxSelectBeams);
   CTHIP_ARG(eos >= 0 || !finished);
   if (n_batch == 0) return 0;
   CTHIP_ARG(tokens && parents && scores_out && logits && scores && workspace && ((uintptr_t)workspace & 15) == 0);
   CTHIP_ARG(scores_out != scores && (!finished_out || finished_out != finished));
-  // A slice is what a workgroup holds in registers (rows that need more than 32 of them have longer ones): 8 values a thread while that is
-  // at most four workgroups a compute unit, 32 otherwise
+  // A slice is what a workgroup holds in registers (rows that need more than kMaxSlices have longer ones): 16 values a thread while that is at most
+  // four workgroups a compute unit, 32 otherwise.  4 beams of 50257: 10.0 us with 16 values, 10.8 with 32; 64 of 50257: 11.9 and 11.8; 384 of
+  // 32000: 26.5 and 25.2; 128 of 128256: 34.9 and 30.6.
   const int64_t rows = (int64_t)n_batch * n_beams;
-  const int small = (vocab + 8 * kSelectThreads - 1) / (8 * kSelectThreads);
+  const int small = (vocab + 16 * kSelectThreads - 1) / (16 * kSelectThreads);
   const bool few = small <= kMaxSlices && rows * small <= 4 * state().compute_units;
   const int slices = few ? small : std::min(kMaxSlices, (vocab + 32 * kSelectThreads - 1) / (32 * kSelectThreads));
   const int slice = ((vocab + slices - 1) / slices + 3) / 4 * 4;
@@ -397,7 +398,7 @@ int cthip_beam_select(int *tokens, int *parents, float *scores_out, int *finishe
   const int list_bytes = entries <= kMergeList ? (int)sizeof(BeamPair) * entries : 0;
   const BeamArgs a = {tokens, parents, scores_out, finished_out, logits, logits_stride, scores, finished, n_batch, n_beams, vocab, eos, in_use, slice,
                       (unsigned char *)workspace, list_bytes};
-  if (few) hipLaunchKernelGGL(k_beam_slice<8>, dim3((unsigned)(rows * in_use)), dim3(kSelectThreads), 0, state().stream, a);
+  if (few) hipLaunchKernelGGL(k_beam_slice<16>, dim3((unsigned)(rows * in_use)), dim3(kSelectThreads), 0, state().stream, a);
   else hipLaunchKernelGGL(k_beam_slice<32>, dim3((unsigned)(rows * in_use)), dim3(kSelectThreads), 0, state().stream, a);
   CTHIP_LAUNCH_CHECK();
   hipLaunchKernelGGL(k_beam_merge, dim3((unsigned)n_batch), dim3(kSelectThreads), (unsigned)(list_bytes + 16 * n_beams * in_use), state().stream, a);

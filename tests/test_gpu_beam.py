@@ -61,6 +61,26 @@ def test_select(n, K, V):
     check(logits, scores, done, eos=0)
 
 
+@pytest.mark.parametrize("n,K,V", [(1, 32, 131072), (1, 14, 250001), (2, 2, 300007), (1, 3, 600000)])
+def test_long_rows(n, K, V):
+    """More lists than the merge keeps by it, rows of more than 32 slices' registers."""
+    print(f"case: long rows, {n} x {K} beams of {V}", flush=True)
+    rng = np.random.default_rng(V)
+    logits = rng.standard_normal((n, K, V), np.float32)
+    logits[:, :, -3:] += 4
+    scores = -np.sort(rng.uniform(0, 2, (n, K)).astype(np.float32), 1)
+    check(logits, scores)
+    check(np.round(logits), scores, (rng.uniform(0, 1, (n, K)) < 0.4).astype(np.int32), eos=V - 1)
+
+
+def test_more_equal_candidates_than_the_merge_holds():
+    """32 beams, each with 32 tokens of one logit, all scores alike: 1024 equal candidates."""
+    logits = np.zeros((2, 32, 4000), np.float32)
+    logits[0, :, 100:140] = 9.0
+    logits[1, 5:, 7:3000:90] = 9.0
+    check(logits, np.zeros((2, 32), np.float32))
+
+
 def test_first_step():
     """Beams that all hold the prompt: only the first counts."""
     rng = np.random.default_rng(1)
@@ -228,6 +248,42 @@ def test_reorder(n, K, layers, kv, dh):
                 assert len(set(want[i * K:(i + 1) * K, t // PAGE])) == K
 
 
+def test_captured_reordering():
+    """A replay with other parents and lengths is that call; tables go to and fro."""
+    from caten_amd import _lib, ops
+    lib, rng = _lib.init(), np.random.default_rng(7)
+    stream = C.c_void_p(lib.cthip_stream())
+    n, K, layers, kv, dh, table = 2, 4, 3, 2, 32, 3
+    n_pages = n * K * table
+    cache = ops.PagedCacheQ4(n_pages, kv, dh, layers)
+    tables = rng.permutation(n_pages).reshape(n * K, table).astype(np.int32)
+    for i in range(n):
+        tables[i * K:(i + 1) * K, 0] = tables[i * K, 0]
+    dt, dl, dp = ops.DeviceArray.from_numpy(tables), ops.DeviceArray((n,), np.int32), ops.DeviceArray((n, K), np.int32)
+    out, hist, dh_out = ops.DeviceArray(tables.shape, np.int32), ops.DeviceArray.from_numpy(rng.integers(0, 99, (n * K, 5)).astype(np.int32)), ops.DeviceArray((n * K, 5), np.int32)
+    tokens, step = ops.DeviceArray.from_numpy(np.arange(n * K, dtype=np.int32)), ops.DeviceArray.from_numpy(np.array([2], np.int32))
+    call = lambda: _lib.check(lib.cthip_beam_reorder_paged_q4(out.ptr, dh_out.ptr, cache.k.ptr, cache.v.ptr, layers, n_pages, dt.ptr, table, dl.ptr, dp.ptr, n, K, kv, dh, hist.ptr, 5,
+                                                              tokens.ptr, step.ptr))
+    graph, run = C.c_void_p(), C.c_void_p()
+    assert lib.hipStreamBeginCapture(stream, 1) == 0
+    call()
+    assert lib.hipStreamEndCapture(stream, C.byref(graph)) == 0
+    assert lib.hipGraphInstantiate(C.byref(run), graph, None, None, C.c_size_t(0)) == 0
+    for _ in range(4):
+        parents, lens = rng.integers(0, K, (n, K)).astype(np.int32), rng.integers(65, 128, n).astype(np.int32)
+        fill = [rng.integers(0, 256, p.shape).astype(np.uint8) for p in (cache.k, cache.v)]
+        for to, x in zip((cache.k, cache.v, dp, dl), fill + [parents, lens]):
+            _lib.check(lib.cthip_h2d(to.ptr, x.ctypes.data, x.nbytes))
+        want, pools = reorder_by_hand(tables, lens, parents, *fill)
+        assert lib.hipGraphLaunch(run, stream) == 0
+        assert np.array_equal(out.numpy(), want) and np.array_equal(cache.k.numpy(), pools[0]) and np.array_equal(cache.v.numpy(), pools[1])
+        got = dh_out.numpy()
+        call()
+        assert np.array_equal(out.numpy(), want) and np.array_equal(dh_out.numpy(), got) and np.array_equal(got[:, 2], np.arange(n * K))
+    lib.hipGraphExecDestroy(run)
+    lib.hipGraphDestroy(graph)
+
+
 def test_a_search_as_a_whole():
     """plan, append, attention, select, reorder, step after step on the device; against a search that keeps every hypothesis's
     own dense cache: the same tokens and scores, across a border of two pages."""
@@ -307,7 +363,7 @@ def test_refusals():
     for change in (dict(t=None), dict(par=None), dict(s_out=None), dict(x=None), dict(s=None), dict(ws=None), dict(ws=p + 4), dict(stride=9), dict(n=-1), dict(K=0), dict(V=1), dict(V=0), dict(eos=10),
                    dict(eos=-2), dict(eos=-1), dict(s=p), dict(f=p)):
         refused(bad, lib.cthip_beam_select, *select(**change))
-    for change in (dict(K=33, V=100, stride=100), dict(n=1 << 24)):
+    for change in (dict(K=33, V=100, stride=100), dict(n=(1 << 17) + 1)):
         refused(no, lib.cthip_beam_select, *select(**change))
     reorder = lambda **k: [dict(dict(to=p, ho=p, k=p, v=p, layers=1, pages=1, t=r, stride=1, lens=p, par=p, n=1, K=2, kv=1, dh=32, h=r, cols=4, tok=p, step=p), **k)[x] for x in
                            ("to", "ho", "k", "v", "layers", "pages", "t", "stride", "lens", "par", "n", "K", "kv", "dh", "h", "cols", "tok", "step")]
