@@ -89,13 +89,12 @@ __global__ __launch_bounds__(kSelectThreads) void k_beam_slice(BeamArgs a) {
         }
       }
       if (tid == 0) s_count = 0;
-      float mine = -INFINITY, four[VPT / 4];
+      float mine = -INFINITY;
 #pragma unroll
       for (int j = 0; j < VPT / 4; j++) {
 #pragma unroll
         for (int e = 0; e < 4; e++) v[4 * j + e] = beam_logit(v[4 * j + e]);
-        four[j] = fmaxf(fmaxf(v[4 * j], v[4 * j + 1]), fmaxf(v[4 * j + 2], v[4 * j + 3]));
-        mine = fmaxf(mine, four[j]);
+        mine = fmaxf(mine, fmaxf(fmaxf(v[4 * j], v[4 * j + 1]), fmaxf(v[4 * j + 2], v[4 * j + 3])));
       }
       // The K-th largest of a wavefront's 64 maxima: at least K values are that large, so it bounds the K-th best from below; of the four
       // wavefronts' the largest does.
@@ -126,17 +125,14 @@ __global__ __launch_bounds__(kSelectThreads) void k_beam_slice(BeamArgs a) {
       top = new_top;
       // candidates, in any order
       int more = 0;
+      if (mine >= bound) {  // (seldom)
 #pragma unroll
-      for (int j = 0; j < VPT / 4; j++) {
-        if (four[j] >= bound) {  // (seldom)
-#pragma unroll
-          for (int e = 0; e < 4; e++) {
-            const int at = c0 + 4 * (tid + kSelectThreads * j) + e;
-            if (v[4 * j + e] >= bound && at < v1) {
-              const int to = atomicAdd(&s_count, 1);
-              if (to < kSelectList) list[to] = {v[4 * j + e], at};
-              else more = 1;
-            }
+        for (int e = 0; e < VPT; e++) {
+          const int at = c0 + 4 * (tid + kSelectThreads * (e >> 2)) + (e & 3);
+          if (v[e] >= bound && at < v1) {
+            const int to = atomicAdd(&s_count, 1);
+            if (to < kSelectList) list[to] = {v[e], at};
+            else more = 1;
           }
         }
       }
