@@ -42,6 +42,13 @@ __device__ __forceinline__ int fast_div(int x, int d) {
 }
 __device__ __forceinline__ int uniform_fast_div(int x, int d) { return __builtin_amdgcn_readfirstlane(fast_div(x, d)); }
 
+// of three, NaN ignored (fmaxf would first have each operand made a quiet number: an instruction more for each)
+__device__ __forceinline__ float max3(float x, float y, float z) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(x), "v"(y), "v"(z));
+  return r;
+}
+
 // sum, and maximum, over the lanes up to this one
 __device__ __forceinline__ int wave_scan_int(int v) {
   v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);  // row_shr:1
@@ -60,6 +67,16 @@ __device__ __forceinline__ int wave_scan_max(int v) {
   v = max(v, __builtin_amdgcn_update_dpp(v, v, 0x142, 0xA, 0xF, false));
   v = max(v, __builtin_amdgcn_update_dpp(v, v, 0x143, 0xC, 0xF, false));
   return v;
+}
+
+// the larger of this lane's and the one's 16, or 32, lanes away
+__device__ __forceinline__ float max16(float v) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float max32(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
 // Which part of the batch a workgroup takes.  A job is a tile of rows of one key / value head of one sequence.  Its cost is
@@ -367,11 +384,10 @@ __global__ __launch_bounds__(256, DH == 128 ? 3 : 4) void k_kv4_attn(Kv4Attn a) 
         for (int i = 0; i < 4; i++)
           if (from + 16 * t + 4 * g + i > limit) s[t][i] = -INFINITY;
     }
-    float top = -INFINITY;
+    float top = max3(s[0][0], s[0][1], s[0][2]);
 #pragma unroll
-    for (int t = 0; t < 4; t++) top = fmaxf(top, fmaxf(fmaxf(s[t][0], s[t][1]), fmaxf(s[t][2], s[t][3])));
-    top = fmaxf(top, __shfl_xor(top, 16, 64));
-    top = fmaxf(top, __shfl_xor(top, 32, 64));
+    for (int e = 3; e < 15; e += 2) top = max3(top, s[e / 4][e % 4], s[(e + 1) / 4][(e + 1) % 4]);
+    top = max32(max16(fmaxf(top, s[3][3])));  // (no assembly in front of the exchange of lanes: the waits it needs are the compiler's)
     if (__ballot(top > m)) {  // a new maximum in some row
       const float m_new = fmaxf(m, top), corr = m > -INFINITY ? __builtin_amdgcn_exp2f(base_of(m) - base_of(m_new)) : 0.0f;
       m = m_new;
@@ -396,8 +412,12 @@ __global__ __launch_bounds__(256, DH == 128 ? 3 : 4) void k_kv4_attn(Kv4Attn a) 
     for (int t = 0; t < 4; t++) l += (s[t][0] + s[t][1]) + (s[t][2] + s[t][3]);
     if (more) wait_loads<L::REQUESTS>();  // (younger than this page's values: the next one's keys)
     else wait_loads<0>();
-    {
-      const sdw vs_now = *(const sdw *)(vp + 32 * DH + lane * NB * 2);
+    const sdw vs_now = *(const sdw *)(vp + 32 * DH + lane * NB * 2);
+    unsigned large = 0;  // scales of 2 and more have this bit of their exponent
+#pragma unroll
+    for (int x = 0; x < NB; x++) large |= vs_now[x] & 0x4000u;
+    bool plain = whole && f == 0 && !__ballot(large);
+    if (!plain) {
       float d = 0.0f;  // the largest scale of the page's rows that are there (each lane has a piece of the page's scales)
 #pragma unroll
       for (int x = 0; x < NB; x++) {
@@ -415,6 +435,7 @@ __global__ __launch_bounds__(256, DH == 128 ? 3 : 4) void k_kv4_attn(Kv4Attn a) 
 #pragma unroll
         for (int b = 0; b < NB; b++) o[b][0] *= by, o[b][1] *= by;
       }
+      plain = whole && f == 0;
     }
     // p as two fp16 terms, once for all blocks
     half2v ph[8], pl[8];
@@ -462,7 +483,7 @@ __global__ __launch_bounds__(256, DH == 128 ? 3 : 4) void k_kv4_attn(Kv4Attn a) 
       }
     }
     };
-    if (whole && f == 0) outputs(std::true_type());
+    if (plain) outputs(std::true_type());
     else outputs(std::false_type());
     wait_lds();
     if (more) ask_quants(a.v_pages, next, v_at), ask_scales(a.v_pages, next, v_at);
