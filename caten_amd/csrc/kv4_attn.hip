@@ -378,16 +378,19 @@ __global__ __launch_bounds__(256, DH == 128 ? 3 : 4) void k_kv4_attn(Kv4Attn a) 
     wait_lds();
     if (more) ask_scales(a.k_pages, next, k_at);
     if (!whole) {
+      int sees = limit - from - 4 * g;  // of the keys 16 t + i: up to this one
+      asm volatile("" : "+v"(sees));
 #pragma unroll
       for (int t = 0; t < 4; t++)
 #pragma unroll
         for (int i = 0; i < 4; i++)
-          if (from + 16 * t + 4 * g + i > limit) s[t][i] = -INFINITY;
+          if (16 * t + i > sees) s[t][i] = -INFINITY;
     }
-    float top = max3(s[0][0], s[0][1], s[0][2]);
+    float tops[5];
 #pragma unroll
-    for (int e = 3; e < 15; e += 2) top = max3(top, s[e / 4][e % 4], s[(e + 1) / 4][(e + 1) % 4]);
-    top = max32(max16(fmaxf(top, s[3][3])));  // (no assembly in front of the exchange of lanes: the waits it needs are the compiler's)
+    for (int e = 0; e < 5; e++) tops[e] = max3(s[3 * e / 4][3 * e % 4], s[(3 * e + 1) / 4][(3 * e + 1) % 4], s[(3 * e + 2) / 4][(3 * e + 2) % 4]);
+    // (no assembly in front of the exchange of lanes: the waits it needs are the compiler's)
+    const float top = max32(max16(fmaxf(max3(tops[0], tops[1], tops[2]), max3(tops[3], tops[4], s[3][3]))));
     if (__ballot(top > m)) {  // a new maximum in some row
       const float m_new = fmaxf(m, top), corr = m > -INFINITY ? __builtin_amdgcn_exp2f(base_of(m) - base_of(m_new)) : 0.0f;
       m = m_new;
