@@ -1,10 +1,9 @@
 // The KV cache of a batch of sequences in 4 bits, in one pool of pages (kv4.hip, kv4_attn.hip): how a page is laid out.
 // A page holds kKvPageRows rows of every key / value head; (n_pages, kv_heads, kv4_head_bytes) bytes for the keys and as
 // many for the values.  A block of 32 channels of a row is one fp16 scale d and 32 numbers -8 .. 7 (GGUF's Q4_0 block with
-// the numbers as two's complement nibbles: a nibble in the upper half of a byte is then 16 times its number as an int8,
-// with no bias to take off again).  A head's part of a page: 32 Dh bytes of quants, then 4 Dh bytes of scales.
+// the numbers as two's complement nibbles).  A head's part of a page: 32 Dh bytes of quants, then 4 Dh bytes of scales.
 //   keys    [row][8-channel group g of a block][block][4 bytes]: a lane that holds one row and one g finds its 8 channels
-//           of every block side by side, and one group's 4 x 8 channels are what one i8 matrix instruction takes per block.
+//           of every block side by side, and one group's 4 x 8 channels are what one matrix instruction takes per block.
 //           Low nibbles: channels 0 .. 3 of the group, high ones 4 .. 7.
 //   values  [block][channel % 16][row, reordered]: transposed, since the product over rows wants many rows of one channel in
 //           a lane.  Low nibbles: channels 0 .. 15 of the block, high ones 16 .. 31.  Row 16 s + 4 g + i lies at 16 g + 4 s + i:

@@ -11,7 +11,9 @@ namespace cthip {
 // starts = exclusive sum of the new rows, pages wanted = ceil((len + new) / 64) - ceil(len / 64), and their exclusive sum says
 // which entries of the free stack a sequence gets.  Every workgroup works the two sums out for itself (n <= 4096 in LDS, at most
 // four sequences a thread) and then finds the sequence of each of its rows by bisection: one launch, nothing to wait for
-// between workgroups.  The row that opens a page enters it into the table.
+// between workgroups.  The row that opens a page enters it into the table.  Bound by latencies: a launch, two sums over 1024
+// threads (data-parallel moves; by exchanges through LDS and 256 rows a workgroup 14.4 us instead of 7.5 for 500 sequences with room for
+// 150000 rows) and a bisection.  64 sequences of a decode step: 4.8 us.
 constexpr int kPlanThreads = 1024, kPlanRows = 2048;  // rows of a workgroup: most decode steps are one workgroup
 
 template <int CTRL, int ROWS>
@@ -127,7 +129,8 @@ __global__ __launch_bounds__(kPlanThreads) void k_kv_plan(int *__restrict__ slot
 // of two), kept finite; u = floor(x / d + 1/2) within -8 .. 7, d being the scale as it is STORED.  The quotient is taken by a
 // reciprocal, and what it leaves, x - u d, is exact in fp32 (u d has 15 bits, and what is left of x where u is not 0 no more than x has):
 // where that is not within half a step, u moves by one, so the number is the one of real arithmetic whatever the reciprocal's
-// rounding.  A block with an infinity or a NaN has a NaN scale.
+// rounding.  A block with an infinity or a NaN has a NaN scale.  Bound by the rows that come in (8 bytes a channel of keys and values):
+// 6001 rows of 8 heads of 128 in 17.2 us, 3.3 TB/s in and out of the card; back as fp32 17.6 us.
 __device__ __forceinline__ float quad_max(float v) {
   v = fmaxf(v, dpp_f<0xB1>(v));
   return fmaxf(v, dpp_f<0x4E>(v));
@@ -387,6 +390,8 @@ static int launch_kv4_rows(const Kv4Rows &a, int dh) {
 // own.  A parent's page goes to its first child as it is; every further child needs a copy, and there are as many pages of
 // beams without a child: the further children take them in order.  A page that is copied from is kept by somebody and is not
 // copied to, so the copies need no order among themselves, and a call repeated on the same tables writes the same bytes.
+// A workgroup a page of a layer, 16 bytes a thread at a time: bound by a launch and a round trip or two where there is little to copy
+// (4.4 us for 4 beams), by the copies else (33 MB in 22 layers: 13 us, four loads a thread asked for at once: 20).
 struct ReorderArgs {
   int *tables_out, *history_out;
   unsigned char *k_pages, *v_pages;

@@ -1,5 +1,18 @@
 // Attention of a ragged batch of query rows over the 4-bit paged cache (layout: kv4.h).  The reference attends one sequence over
 // a dense fp32 cache (external/llm/layers.lisp:3-5,19-33).
+//
+// out = sum_t p_t v_t / sum_t p_t, p_t = exp(q . k_t / sqrt(Dh) - maximum), over one pass of the pages with a running maximum and
+// sum.  One launch: as many workgroups as the card holds, each with an equal part of all (tile of rows, head, page) there are, whatever
+// the lengths; a tile that several workgroups have parts of is joined by the last of them, in their order.
+//
+// What bounds it is the vector unit, not memory: taking the nibbles apart (9 instructions for 8 numbers of a key, 20 for 16 of
+// values), the scales (one a number of the 16 x 64 scores, two terms of p d), exponentials.  Per page and 16 rows 450 instructions at
+// Dh = 64 and some 650 at 128, of 4 cycles each, against 512 and 1024 cycles of matrix instructions and, at Dh = 128, 9 KB.
+//   700-row prompts of 5 sequences, 32 heads over 4 of 64 (25 GFLOP): 112 us, the vector units busy 67 % of it, the matrix units 17 %.
+//   32 sequences of 150 .. 20000, 64 heads over 8 of 128 (159 MB): 48 us = 3.3 TB/s; vector units 47 %, matrix units 14 %; some 12 us are what a
+//   workgroup does before its first page and after its last.
+//   8 sequences of 1500 .. 5000, 32 heads of 128 (93 MB): 30 us = 3.1 TB/s, 15 of a tile's 16 rows empty.
+//   One sequence of 701, 12 heads of 64: 9.5 us, a chain of round trips: lengths, table, page, record, ticket, records.
 #include <algorithm>
 #include <type_traits>
 
@@ -31,7 +44,7 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kTileRows = 16;       // rows (query row, query head of the group) of a tile
 constexpr int kSplitSlots = 2048;   // records of shares in the workspace, two a workgroup
-constexpr int kJobPieces = 1;       // what a job costs besides its pages, in pieces of them
+constexpr int kJobPieces = 1;       // what a job costs besides its pages, in pieces of them (2: 52 us instead of 50, 34 instead of 31, for the batches above)
 constexpr int kMaxShares = 64;      // of one tile: their records are added up by one workgroup
 
 // floor(x / d) where that is below 2^21, x below 2^30: the quotient by a reciprocal is off by one at most, which what it leaves shows.  (A division
@@ -335,7 +348,8 @@ __global__ __launch_bounds__(256, DH == 128 ? 3 : 4) void k_kv4_attn(Kv4Attn a) 
   for (int k = 0; k < mine; k++) {
     {
       // Of the wavefronts on a SIMD the oldest goes first, and what it gains the others lose: the last workgroup of a compute unit ended at
-      // twice the first one's time, the SIMDs to itself.  So who has more left goes first, by quarters of a part.
+      // twice the first one's time, the SIMDs to itself.  So who has more left goes first, by quarters of a part (prompts 122 -> 112 us, the
+      // batches 52 -> 48 and 34 -> 30).
       const int left = 4 * (x1 - line - from_piece - (k << 2 >> a.piece_log2));
       if (left > 3 * per) __builtin_amdgcn_s_setprio(3);
       else if (left > 2 * per) __builtin_amdgcn_s_setprio(2);
@@ -619,7 +633,8 @@ int cthip_sdpa_paged_q4(float *out, const float *q, int64_t q_stride, const void
   const int64_t tiles = (int64_t)n_rows * (H / Hkv) / kTileRows + (n_seqs < n_rows ? n_seqs : n_rows), jobs = tiles * Hkv;
   if (jobs > (1 << 21) || n_rows > (1 << 20))
     return fail(CTHIP_E_UNSUPPORTED, "cthip_sdpa_paged_q4: %d rows of %d heads in one call (at most 2^20 rows, and 2^21 tiles of 16 heads of them)", n_rows, H);
-  // as many workgroups as run at once (three or four a compute unit for their registers and pages), a multiple of the XCDs
+  // as many workgroups as run at once (three or four a compute unit for their registers and pages; with two or three and no spilled register
+  // prompts take 119 us instead of 112, the batches 50 and 32 instead of 48 and 30), a multiple of the XCDs
   const int at_once = std::min(kSplitSlots / 2, state().compute_units * (Dh == 128 ? 3 : 4) / 8 * 8);
   int piece = 2;  // (the line is shorter than 2^30, and a workgroup's part of it below what fast_div holds for)
   while (jobs * ((table_stride >> piece) + 1 + kJobPieces) > std::min((int64_t)INT_MAX / 2, (int64_t)at_once << 20)) piece++;

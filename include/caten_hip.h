@@ -384,7 +384,8 @@ int64_t cthip_kv_page_bytes_q4(int kv_heads, int head_dim); /* of one page of ke
  * free_pages is a stack of n_free[0] page ids: pages are taken from its end, in the order of the sequences, and the array
  * itself is not changed.  A sequence is refused whole -- length kept, slots and positions -1, no pages -- where a count is
  * negative, its table row or max_rows is too short, or too few pages are left; once pages have run out, every later
- * sequence that needs one is refused too.  refused[0] is their number: such a sequence's rows must not be attended.  At most 4096 sequences. */
+ * sequence that needs one is refused too.  refused[0] is their number: such a sequence's rows must not be attended.  At most 4096 sequences,
+ * max_rows 2^30. */
 int cthip_kv_plan_paged(int *slots, int *positions, int *starts, int *tables, int table_stride, int *lens_out, int *n_free_out, int *refused,
                         const int *lens, const int *new_lens, int n_seqs, const int *free_pages, const int *n_free, int max_rows);
 /* Key and value rows (n_rows, kv_heads * head_dim), k_stride / v_stride floats apart (they may be slices of a fused product),
@@ -392,7 +393,7 @@ int cthip_kv_plan_paged(int *slots, int *positions, int *starts, int *tables, in
  * of 32: m = the value of largest magnitude (the positive one of two), d = fp16(m / -8) held within +-65504, number =
  * clamp(floor(x / d + 8.5), 0, 15) - 8, decided exactly; a block with an infinity or a NaN reads back as NaN.
  * cthip_kv_rows_paged_q4 is the way back: (n_rows, kv_heads * head_dim) fp32, contiguous; rows whose slot is outside
- * the pool are left as they were; either of k_rows / v_rows may be NULL. */
+ * the pool are left as they were; either of k_rows / v_rows may be NULL.  At most 2^28 rows. */
 int cthip_kv_append_paged_q4(void *k_pages, void *v_pages, const float *k_rows, const float *v_rows, int64_t k_stride, int64_t v_stride, const int *slots,
                              int n_rows, int n_pages, int kv_heads, int head_dim);
 int cthip_kv_rows_paged_q4(float *k_rows, float *v_rows, const void *k_pages, const void *v_pages, const int *slots, int n_rows, int n_pages, int kv_heads,
@@ -400,8 +401,10 @@ int cthip_kv_rows_paged_q4(float *k_rows, float *v_rows, const void *k_pages, co
 /* Attention (layers.lisp:3-5) of a ragged batch over the cache.  Rows starts[i] .. starts[i + 1] - 1 of q are the last rows of
  * sequence i, which holds lens[i] keys (those rows' own among them): each sees the keys up to its own position.  One row a
  * sequence is a decode step, more are a prompt or a piece of one.  q rows are (H, Dh), q_stride floats apart; out (n_rows, H,
- * Dh) contiguous, not q.  A row that sees no key is zero; rows behind starts[n_seqs] are left as they were; a table entry outside the pool is
- * a page without keys.  fp32 sums; q and the probabilities enter the integer products with 22 bits.
+ * Dh) contiguous, not q.  A row that sees no key is zero; rows behind starts[n_seqs], and those of a sequence that starts in front of an
+ * earlier one's rows, are left as they were; a table entry outside the pool, or a row past the table's end, holds no key.  fp32 sums; q, and the
+ * probabilities times the values' scales, enter the products with 22 bits of a row's largest.  At most 4096 sequences, 2^20 rows and
+ * 2^21 tiles of 16 (row, head) of a key / value head.
  * workspace: cthip_sdpa_paged_q4_workspace(Dh) = 4 * (2048 + 2048 * 16 * (Dh + 2)) bytes, 16-byte aligned, zeroed once
  * (cthip_alloc does); every call leaves it ready for the next.  Calls that may overlap (graphs replayed on other streams) need one each. */
 int64_t cthip_sdpa_paged_q4_workspace(int Dh);
@@ -412,8 +415,9 @@ int cthip_sdpa_paged_q4(float *out, const float *q, int64_t q_stride, const void
  * beam, then to the higher logit, then to the lower token.  NaN logits and scores count as minus infinity, and a
  * candidate of minus infinity is taken only where nothing else is left.  logits rows (n_batch * n_beams, vocab), logits_stride
  * floats apart; scores, finished and the outputs (n_batch, n_beams); parents count within the request; finished_out (may be
- * NULL) = the parent's, or token == eos; eos -1 = none.  n_beams 1 .. 32, vocab >= n_beams.  Not in place.
- * workspace: cthip_beam_select_workspace(...) = 256 + 4 n_batch + 32 n_batch n_beams (24 + 8 n_beams) bytes, as above. */
+ * NULL) = the parent's, or token == eos; eos -1 = none.  n_beams 1 .. 32, vocab >= n_beams, at most 2^18 beams of all requests.  Not in place.
+ * workspace: cthip_beam_select_workspace(...) = 256 + 4 n_batch + 32 n_batch n_beams (24 + 8 n_beams) bytes, 16-byte aligned, whatever
+ * they hold; calls that may overlap need one each. */
 int64_t cthip_beam_select_workspace(int n_batch, int n_beams);
 int cthip_beam_select(int *tokens, int *parents, float *scores_out, int *finished_out, const float *logits, int64_t logits_stride, const float *scores,
                       const int *finished, int n_batch, int n_beams, int vocab, int eos, void *workspace);
