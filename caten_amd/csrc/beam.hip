@@ -223,16 +223,30 @@ __global__ __launch_bounds__(kSelectThreads) void k_beam_merge(BeamArgs a) {
   const unsigned char *recs = a.records + (int64_t)b0 * a.slices * record_bytes;
   const int entries = slices_in_all * K;
   const bool held = entries * (int)sizeof(BeamPair) <= a.list_bytes;
-  if (held)  // (lists of beams that had no use for theirs hold anything, and are not looked at)
-    for (int i = tid; i < entries; i += kSelectThreads) list[i] = ((const BeamPair *)(recs + (int64_t)(i / K) * record_bytes + 24))[i % K];
-  for (int i = tid; i < slices_in_all; i += kSelectThreads) {
+  auto entry = [&](int i) { return ((const BeamPair *)(recs + (int64_t)(i / K) * record_bytes + 24))[i % K]; };
+  // what there is to read is asked for at once; where a thread has more than one of a kind, the others behind it
+  const bool has_entry = held && tid < entries, has_slice = tid < slices_in_all;
+  BeamPair first_entry = {};
+  float first_top = 0.0f, score = 0.0f;
+  double first_sum = 0.0;
+  int done = 0;
+  if (has_entry) first_entry = entry(tid);
+  if (has_slice) first_top = *(const float *)(recs + (int64_t)tid * record_bytes + 8), first_sum = *(const double *)(recs + (int64_t)tid * record_bytes);
+  if (tid < K) score = a.scores[b0 + tid];
+  if (tid < K && a.finished) done = a.finished[b0 + tid];
+  // (lists of beams that had no use for theirs hold anything, and are not looked at)
+  if (has_entry) list[tid] = first_entry;
+  if (has_slice) s_tops[tid] = first_top, s_sums[tid] = first_sum, s_taken[tid] = 0;
+  if (held)
+    for (int i = tid + kSelectThreads; i < entries; i += kSelectThreads) list[i] = entry(i);
+  for (int i = tid + kSelectThreads; i < slices_in_all; i += kSelectThreads) {
     s_tops[i] = *(const float *)(recs + (int64_t)i * record_bytes + 8);
     s_sums[i] = *(const double *)(recs + (int64_t)i * record_bytes);
     s_taken[i] = 0;
   }
   if (tid < K) {
-    const float s = beam_logit(a.scores[b0 + tid]);
-    s_state[tid] = s == -INFINITY ? 0 : a.finished && a.finished[b0 + tid] ? 1 : 2;  // no candidates, one, a row of them
+    const float s = beam_logit(score);
+    s_state[tid] = s == -INFINITY ? 0 : done ? 1 : 2;  // no candidates, one, a row of them
     s_base[tid] = (double)s;
     s_top[tid] = 0.0f;
   }
