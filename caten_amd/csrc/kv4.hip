@@ -390,8 +390,8 @@ static int launch_kv4_rows(const Kv4Rows &a, int dh) {
 // own.  A parent's page goes to its first child as it is; every further child needs a copy, and there are as many pages of
 // beams without a child: the further children take them in order.  A page that is copied from is kept by somebody and is not
 // copied to, so the copies need no order among themselves, and a call repeated on the same tables writes the same bytes.
-// A workgroup a page of a layer, 16 bytes a thread at a time: bound by a launch and a round trip or two where there is little to copy
-// (4.4 us for 4 beams), by the copies else (33 MB in 22 layers: 13 us, four loads a thread asked for at once: 20).
+// Bound by a launch and three round trips (parents, table, page) where there is little to copy: 5.0 us for 4 beams; 24 x 6 beams in 22 layers,
+// 33 MB: 8.7 us (a load for each parent in turn, and a workgroup for each page: 13).
 struct ReorderArgs {
   int *tables_out, *history_out;
   unsigned char *k_pages, *v_pages;
@@ -399,9 +399,10 @@ struct ReorderArgs {
   int table_stride, n_layers, n_pages, beams, cols, page_bytes;
 };
 constexpr int kMaxBeams = 32;
+typedef uint32_t dwords4 __attribute__((ext_vector_type(4)));
 
-// blockIdx.y = beam; blockIdx.x = 0: its row of the table and its history, otherwise the pages of layer (x - 1) / 2.  Who is whose child
-// is worked out from one load of all parents (a load for each in turn: 13 us instead of XX for 24 x 6 beams in 22 layers).
+// blockIdx.y = beam; blockIdx.x = 0: its row of the table and its history, otherwise a page of keys and one of values in layer x - 1.  Who is
+// whose child is worked out from one load of all parents.
 __global__ __launch_bounds__(256) void k_beam_reorder(ReorderArgs a) {
   const int n0 = blockIdx.y / a.beams * a.beams, j = blockIdx.y - n0, tid = threadIdx.x, lane = tid & 63;
   int parent = lane;
@@ -445,11 +446,21 @@ __global__ __launch_bounds__(256) void k_beam_reorder(ReorderArgs a) {
   if (!further || !tail) return;
   const int src = from[last], dst = a.tables[(int64_t)(n0 + owner) * a.table_stride + last];
   if (src < 0 || src >= a.n_pages || dst < 0 || dst >= a.n_pages) return;
-  const int x = blockIdx.x - 1;
-  unsigned char *pool = (x & 1 ? a.v_pages : a.k_pages) + (int64_t)(x >> 1) * a.n_pages * a.page_bytes;
-  const uint4 *s = (const uint4 *)(pool + (int64_t)src * a.page_bytes);
-  uint4 *d = (uint4 *)(pool + (int64_t)dst * a.page_bytes);
-  for (int e = tid; e < a.page_bytes / 16; e += 256) d[e] = s[e];
+  const int layer = blockIdx.x - 1, n = a.page_bytes / 16;
+  for (int values = 0; values < 2; values++) {
+    unsigned char *pool = (values ? a.v_pages : a.k_pages) + (int64_t)layer * a.n_pages * a.page_bytes;
+    const dwords4 *s = (const dwords4 *)(pool + (int64_t)src * a.page_bytes);
+    dwords4 *d = (dwords4 *)(pool + (int64_t)dst * a.page_bytes);
+    for (int e = tid; e < n; e += 4 * 256) {
+      dwords4 v[4];
+#pragma unroll
+      for (int k = 0; k < 4; k++)
+        if (e + 256 * k < n) v[k] = s[e + 256 * k];
+#pragma unroll
+      for (int k = 0; k < 4; k++)
+        if (e + 256 * k < n) d[e + 256 * k] = v[k];
+    }
+  }
 }
 
 }  // namespace cthip
@@ -524,7 +535,7 @@ int cthip_beam_reorder_paged_q4(int *tables_out, int *history_out, void *k_pages
   CTHIP_ARG(!history_out || (history && history_out != history && tokens && step));
   const ReorderArgs a = {tables_out, cols ? history_out : nullptr, (unsigned char *)k_pages, (unsigned char *)v_pages, tables, lens, parents, history, tokens, step,
                          table_stride, n_layers, n_pages, n_beams, cols, kv_heads * kv4_head_bytes(head_dim)};
-  const unsigned copies = n_pages ? 2u * (unsigned)n_layers : 0u;
+  const unsigned copies = n_pages ? (unsigned)n_layers : 0u;
   hipLaunchKernelGGL(k_beam_reorder, dim3(1 + copies, (unsigned)(n_batch * n_beams)), dim3(256), 0, state().stream, a);
   CTHIP_LAUNCH_CHECK();
   return 0;
