@@ -4,7 +4,7 @@
 // The logits are read once: a row is cut into slices, a workgroup holds a slice in registers, 16 or 32 values a thread, and leaves its
 // maximum, its sum of exponentials and its n_beams best in order.  A second launch joins the rows' sums and merges the sorted lists,
 // a workgroup a request.  (As one launch, the last of a request's workgroups merging, stores had to reach memory and a ticket be
-// drawn before a workgroup could end, and the merge's registers were everybody's: 62 us instead of 26 for 48 x 8 beams of 32000.)
+// drawn before a workgroup could end, and the merge's registers were everybody's: 62 us instead of 25 for 48 x 8 beams of 32000.)
 // Where there is much to read, half the time is the logits' way and half what a workgroup does with its slice once it is there -- a
 // bound from below on the n_beams best, found lane by lane, and the candidates' way through LDS: 384 rows of 32000 (49 MB) 17.4 us + 8.4
 // for the merge.  Smaller chunks with the next one on its way while one is worked on (29 - 37 us) do that more often; a looser

@@ -390,7 +390,7 @@ static int launch_kv4_rows(const Kv4Rows &a, int dh) {
 // own.  A parent's page goes to its first child as it is; every further child needs a copy, and there are as many pages of
 // beams without a child: the further children take them in order.  A page that is copied from is kept by somebody and is not
 // copied to, so the copies need no order among themselves, and a call repeated on the same tables writes the same bytes.
-// Bound by a launch and three round trips (parents, table, page) where there is little to copy: 5.0 us for 4 beams; 24 x 6 beams in 22 layers,
+// Bound by a launch and three round trips (parents, table, page) where there is little to copy: 4.6 us for 4 beams; 24 x 6 beams in 22 layers,
 // 33 MB: 8.7 us (a load for each parent in turn, and a workgroup for each page: 13).
 struct ReorderArgs {
   int *tables_out, *history_out;
