@@ -626,7 +626,7 @@ int cthip_sdpa_paged_q4(float *out, const float *q, int64_t q_stride, const void
   if (!kv4_shape_ok(Hkv, Dh) || H > 65535) return fail(CTHIP_E_UNSUPPORTED, "cthip_sdpa_paged_q4: %d heads over %d of %d (at most 65535 heads, head sizes 32, 64, 128)", H, Hkv, Dh);
   if (n_seqs > kKv4MaxSeqs) return fail(CTHIP_E_UNSUPPORTED, "cthip_sdpa_paged_q4: %d sequences in one call (at most %d)", n_seqs, kKv4MaxSeqs);
   if (n_seqs == 0 || n_rows == 0) return 0;
-  CTHIP_ARG(out && q && tables && lens && starts && workspace && q_stride >= (int64_t)H * Dh);
+  CTHIP_ARG(out && q && out != q && tables && lens && starts && workspace && q_stride >= (int64_t)H * Dh);
   CTHIP_ARG(n_pages == 0 || (k_pages && v_pages));
   CTHIP_ARG((((uintptr_t)k_pages | (uintptr_t)v_pages | (uintptr_t)workspace) & 15) == 0);
   // rows of a tile share a key / value head: at most this many tiles of all sequences, and as many jobs a head

@@ -352,6 +352,8 @@ def beam_select(logits, scores, finished=None, eos: int = -1) -> dict:
     logits, scores = np.ascontiguousarray(logits, np.float32), np.ascontiguousarray(scores, np.float32)
     if logits.ndim != 3 or logits.shape[:2] != scores.shape:
         raise ValueError(f"beam_select: logits {logits.shape}, scores {scores.shape}")
+    if finished is not None and np.shape(finished) != scores.shape:
+        raise ValueError(f"beam_select: scores {scores.shape}, finished {np.shape(finished)}")
     n, k, vocab = logits.shape
     size = int(_lib.init().cthip_beam_select_workspace(n, k))
     if size < 0:

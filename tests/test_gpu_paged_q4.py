@@ -155,6 +155,16 @@ def test_plan(n, new, table, spare, max_rows):
         assert np.array_equal(got[key], want[key]), key
 
 
+def test_plan_of_nothing():
+    from caten_amd import ops
+    got = ops.kv_plan(np.zeros(0), np.zeros(0), np.zeros((0, 4)), [7, 8], 5)
+    assert (got["slots"] == -1).all() and (got["positions"] == -1).all() and got["starts"][0] == 0 and got["n_free"] == 2 and got["refused"] == 0
+    got = ops.kv_plan([64, 0, 3], [0, 0, 0], -np.ones((3, 4)), [], 0)
+    assert not got["starts"].any() and list(got["lens"]) == [64, 0, 3] and got["refused"] == 0
+    got = ops.kv_plan([64, 0, 3], [1, 0, 1], np.array([[5, -1], [-1, -1], [6, -1]]), [], 2)  # no page left for the first
+    assert list(got["slots"]) == [-1, 6 * PAGE + 3] and list(got["lens"]) == [64, 0, 4] and got["refused"] == 1
+
+
 def test_plan_out_of_place_leaves_its_inputs():
     from caten_amd import _lib
     from caten_amd.ops import DeviceArray
@@ -722,9 +732,9 @@ def test_refusals():
     for change in (dict(k=None), dict(v=None), dict(slots=None), dict(rows=-1), dict(v=p + 4)):
         refused(bad, lib.cthip_kv_rows_paged_q4, *rows(**change))
     refused(no, lib.cthip_kv_rows_paged_q4, *rows(dh=40))
-    attend = lambda **k: [dict(dict(out=p, q=p, qs=128, k=p, v=p, pages=1, tables=p, stride=1, lens=p, starts=p, n=1, rows=1, H=4, kv=2, dh=32, ws=p), **k)[x] for x in
+    attend = lambda **k: [dict(dict(out=p, q=p + 8192, qs=128, k=p, v=p, pages=1, tables=p, stride=1, lens=p, starts=p, n=1, rows=1, H=4, kv=2, dh=32, ws=p), **k)[x] for x in
                           ("out", "q", "qs", "k", "v", "pages", "tables", "stride", "lens", "starts", "n", "rows", "H", "kv", "dh", "ws")]
-    for change in (dict(out=None), dict(q=None), dict(k=None), dict(v=None), dict(tables=None), dict(lens=None), dict(starts=None), dict(ws=None), dict(ws=p + 4), dict(k=p + 8), dict(qs=127), dict(n=-1),
+    for change in (dict(out=None), dict(q=None), dict(q=p), dict(k=None), dict(v=None), dict(tables=None), dict(lens=None), dict(starts=None), dict(ws=None), dict(ws=p + 4), dict(k=p + 8), dict(qs=127), dict(n=-1),
                    dict(rows=-1), dict(stride=0), dict(H=3), dict(H=0), dict(pages=-1)):
         refused(bad, lib.cthip_sdpa_paged_q4, *attend(**change))
     refused(no, lib.cthip_kv_append_paged_q4, *append(rows=2 ** 28 + 1))
