@@ -96,7 +96,8 @@ __device__ __forceinline__ float max32(float v) {
 // its pages in pieces of `piece` (four, one a wavefront, or more where numbers would not fit 32 bits) and kJobPieces for what a job costs
 // besides; the jobs' costs laid end to end are cut into as many equal parts as workgroups run at once, so that a long sequence is
 // shared by many workgroups and many short ones go to one.  The lengths are on the device only: every wavefront works
-// the division out for itself, 64 sequences at a time.
+// the division out for itself, 64 sequences at a time (0.4 us each: 33 us for 4096 sequences of which one has a row; 57 where each
+// 64 waited for their lengths and were gone through again for a job).
 struct Batch {
   int first = 0, before = 0;  // of the 64 sequences in the lanes: the first, and the cost in front of it
   int reach = 0;              // the largest start up to the last of them
@@ -111,11 +112,16 @@ struct Batch {
     len = from[0][l], row0 = from[1][l], rows = from[2][l], tiles = from[3][l], cost = from[4][l], upto = from[5][l];
   }
 };
-__device__ __forceinline__ void look(const Kv4Attn &a, Batch &s) {
-  const int i = s.first + (int)(threadIdx.x & 63);
-  s.len = 0, s.row0 = 0;
-  int end = 0;
-  if (i < a.n_seqs) s.len = max(a.lens[i], 0), s.row0 = a.starts[i], end = min(a.starts[i + 1], a.n_rows);
+struct Read {  // of a sequence
+  int len = 0, row0 = 0, end = 0;
+  __device__ __forceinline__ Read(const Kv4Attn &a, int first) {
+    const int i = first + (int)(threadIdx.x & 63);
+    if (i < a.n_seqs) len = a.lens[i], row0 = a.starts[i], end = a.starts[i + 1];
+  }
+};
+__device__ __forceinline__ void look(const Kv4Attn &a, const Read &read, Batch &s) {
+  s.len = max(read.len, 0), s.row0 = read.row0;
+  const int end = min(read.end, a.n_rows);
   // (rows in front of an earlier sequence's are nobody's: no row is two sequences', and the costs of all stay within their bound)
   const int reach = max(s.reach, wave_scan_max(s.row0));
   s.reach = __builtin_amdgcn_readlane(reach, 63);
@@ -130,16 +136,17 @@ struct Job {
   int len, rows, row0;  // of the sequence: keys, rows of this step and the first of them
   int at, cost;         // its place on the line of all costs
 };
-// the job at a place on the line, which lies in front of its end
-__device__ __forceinline__ bool find_job(const Kv4Attn &a, Batch &s, int (*kept)[64], int place, Job &j) {
-  unsigned long long past;
-  while (!(past = __ballot(s.upto > place))) {
-    if (s.first + 64 >= a.n_seqs) return false;
-    s.before = __builtin_amdgcn_readlane(s.upto, 63);
-    s.first += 64;
-    look(a, s);
+// the job at a place on the line, which lies in front of its end; fronts: what 64 sequences at a time have in front of them, cost and largest start
+__device__ __forceinline__ bool find_job(const Kv4Attn &a, Batch &s, int (*kept)[64], const int (*fronts)[64], int place, Job &j) {
+  if (place < s.before || place >= __builtin_amdgcn_readlane(s.upto, 63)) {
+    const int lane = threadIdx.x & 63;
+    const int block = __popcll(__ballot(lane * 64 < a.n_seqs && fronts[0][lane] <= place)) - 1;
+    s.first = 64 * block, s.before = __builtin_amdgcn_readfirstlane(fronts[0][block]), s.reach = __builtin_amdgcn_readfirstlane(fronts[1][block]);
+    look(a, Read(a, s.first), s);
     s.put(kept);
   }
+  const unsigned long long past = __ballot(s.upto > place);
+  if (!past) return false;
   const int l = (int)__builtin_ctzll(past);
   const int tiles = __builtin_amdgcn_readlane(s.tiles, l), all = tiles * a.Hkv;
   j.cost = __builtin_amdgcn_readlane(s.cost, l);
@@ -161,7 +168,7 @@ __device__ __forceinline__ bool find_job(const Kv4Attn &a, Batch &s, int (*kept)
 // outputs, are there.
 template <int DH>
 struct Kv4Lds {
-  static constexpr int HEAD = 36 * DH, WAVE = 2 * HEAD, STATS = 4 * WAVE, SEQS = STATS + 14 * kTileRows * 4, Q = SEQS + 4 * 6 * 64 * 4,
+  static constexpr int HEAD = 36 * DH, WAVE = 2 * HEAD, STATS = 4 * WAVE, SEQS = STATS + 14 * kTileRows * 4, FRONTS = SEQS + 4 * 6 * 64 * 4, Q = FRONTS + 2 * 64 * 4,
                        BYTES = Q + DH / 32 * 2048;
   static constexpr int REQUESTS = DH / 32 + (DH / 32 + 1) / 2;  // of a head's part of a page: 16 bytes a lane, then 4
   static_assert(WAVE >= kTileRows * (DH + 4) * 4 && 4 * WAVE >= 8 * kMaxShares * kTileRows, "results and shares in the pages' place");
@@ -183,6 +190,7 @@ __global__ __launch_bounds__(256, DH == 128 ? 3 : 4) void k_kv4_attn(Kv4Attn a) 
   float (*s_m)[kTileRows] = (float (*)[kTileRows])(smem + L::STATS), (*s_l)[kTileRows] = s_m + 4, (*s_w)[kTileRows] = s_m + 8, *s_sum = s_m[12];
   int *s_ticket = (int *)s_m[13];
   int (*s_seqs)[6][64] = (int (*)[6][64])(smem + L::SEQS);
+  int (*s_fronts)[64] = (int (*)[64])(smem + L::FRONTS);  // (every wavefront writes all of it, the same)
   // a wavefront's results lie where its own pages did
   auto s_o = [&](int wave, int row) { return (float *)(smem + wave * L::WAVE) + row * (DH + 4); };
   const int tid0 = threadIdx.x, wv = __builtin_amdgcn_readfirstlane(tid0 >> 6);
@@ -191,28 +199,26 @@ __global__ __launch_bounds__(256, DH == 128 ? 3 : 4) void k_kv4_attn(Kv4Attn a) 
   const int me = (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
   int total = 0, longest = 0;
   Batch s;
-  for (look(a, s);;) {
-    int c = s.tiles ? s.cost : 0;
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) c = max(c, __shfl_xor(c, o, 64));
-    longest = max(longest, __builtin_amdgcn_readfirstlane(c));
+  for (Read read(a, 0);;) {
+    const bool more = s.first + 64 < a.n_seqs;
+    if ((tid0 & 63) == 0) s_fronts[0][s.first >> 6] = s.before, s_fronts[1][s.first >> 6] = s.reach;
+    const Read next(a, more ? s.first + 64 : a.n_seqs);  // (on its way while these are looked at)
+    look(a, read, s);
+    longest = max(longest, s.tiles ? s.cost : 0);
     total = __builtin_amdgcn_readlane(s.upto, 63);
-    if (s.first + 64 >= a.n_seqs) break;
+    if (!more) break;
     s.before = total;
     s.first += 64;
-    look(a, s);
+    read = next;
   }
-  if (s.first) {
-    s.first = 0, s.before = 0, s.reach = 0;
-    look(a, s);
-  }
+  longest = __builtin_amdgcn_readlane(wave_scan_max(longest), 63);
   s.put(s_seqs[wv]);
   const int per = max(uniform_fast_div(total + (int)gridDim.x - 1, (int)gridDim.x), (longest + kMaxShares - 2) / (kMaxShares - 1));
   const int x0 = (int)min((int64_t)me * per, (int64_t)total), x1 = min(total - x0, per) + x0;
   for (int x = x0; x < x1;) {
   Job w;
   if (x != x0) s.get(s_seqs[wv]);
-  if (!find_job(a, s, s_seqs[wv], x, w)) break;
+  if (!find_job(a, s, s_seqs[wv], s_fronts, x, w)) break;
   x = w.at + w.cost;
   // (what hangs on the lane alone is worked out for each job: kept from being moved in front of the loop, where it would hold registers)
   int lane = tid0 & 63;
