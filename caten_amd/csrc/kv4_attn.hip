@@ -8,11 +8,11 @@
 // What bounds it is the vector unit, not memory: taking the nibbles apart (9 instructions for 8 numbers of a key, 20 for 16 of
 // values), the scales (one a number of the 16 x 64 scores, two terms of p d), exponentials.  Per page and 16 rows 450 instructions at
 // Dh = 64 and some 650 at 128, of 4 cycles each, against 512 and 1024 cycles of matrix instructions and, at Dh = 128, 9 KB.
-//   700-row prompts of 5 sequences, 32 heads over 4 of 64 (25 GFLOP): 112 us, the vector units busy 67 % of it, the matrix units 17 %.
+//   700-row prompts of 5 sequences, 32 heads over 4 of 64 (25 GFLOP): 109 us, the vector units busy 67 % of it, the matrix units 17 %.
 //   32 sequences of 150 .. 20000, 64 heads over 8 of 128 (159 MB): 48 us = 3.3 TB/s; vector units 47 %, matrix units 14 %; some 12 us are what a
 //   workgroup does before its first page and after its last.
 //   8 sequences of 1500 .. 5000, 32 heads of 128 (93 MB): 30 us = 3.1 TB/s, 15 of a tile's 16 rows empty.
-//   One sequence of 701, 12 heads of 64: 9.5 us, a chain of round trips: lengths, table, page, record, ticket, records.
+//   One sequence of 701, 12 heads of 64: 8.7 us, a chain of round trips: lengths, table, page, record, ticket, records.
 #include <algorithm>
 #include <type_traits>
 
@@ -211,7 +211,10 @@ __global__ __launch_bounds__(256, DH == 128 ? 3 : 4) void k_kv4_attn(Kv4Attn a) 
   }
   longest = __builtin_amdgcn_readlane(wave_scan_max(longest), 63);
   s.put(s_seqs[wv]);
-  const int per = max(uniform_fast_div(total + (int)gridDim.x - 1, (int)gridDim.x), (longest + L::SHARES - 2) / (L::SHARES - 1));
+  // A part's length: of the whole, or what keeps a tile's shares below their number, or, since its last workgroup reads all of a tile's
+  // records, as many pieces as come out about even with that (sqrt(longest / 20): 32768 keys of one head of 128 27.3 -> 22.5 us, 131072 38.0 -> 34.1).
+  const int even = __builtin_amdgcn_readfirstlane((int)__builtin_sqrtf(0.05f * (float)longest));
+  const int per = max(max(uniform_fast_div(total + (int)gridDim.x - 1, (int)gridDim.x), (longest + L::SHARES - 2) / (L::SHARES - 1)), even);
   // Workgroups are dealt to the eight XCDs in turn.  Neighbours on the line, which may read the same pages and join their shares, on one of
   // them, and all XCDs alike where there are fewer parts than workgroups (one sequence of 2048, 8 heads of 128, 72 parts: 15.3 us on one XCD,
   // 10.8 on eight).
@@ -580,8 +583,8 @@ __global__ __launch_bounds__(256, DH == 128 ? 3 : 4) void k_kv4_attn(Kv4Attn a) 
     if (*s_ticket == shares - 1) {  // (uniform) the last of the job's workgroups adds the shares up, in their order
       if (tid == 0) __hip_atomic_store(tickets, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);  // the next call counts again
       // Maxima and sums of all shares, asked for at once, then the outputs, eight or sixteen shares at a time: a load after the other would be a
-      // round trip to memory for each share.  Up to 16 shares every thread works the weights out for itself (9.5 us for one sequence of 701, 12
-      // heads of 64, against 10.4), else once for all (8192: 14.3 against 15.9).
+      // round trip to memory for each share.  Up to 16 shares every thread works the weights out for itself (9.3 us for one sequence of 701, 12
+      // heads of 64, against 10.4; with all parts on one XCD), else once for all (8192: 14.4 against 15.9).
       if (shares <= 16) {
         f32x2 (*ml)[kTileRows] = (f32x2 (*)[kTileRows])smem;
         if ((tid >> 4) < shares && (tid & 15) < nr)

@@ -342,7 +342,8 @@ def test_several_rows(H, kv, dh, lens, rows):
         close(got[starts[i]:starts[i + 1]], *attention(q[starts[i]:starts[i + 1]], k, v))
 
 
-@pytest.mark.parametrize("H,kv,dh,lens,rows", [(8, 8, 128, [9000, 40], [1, 1]), (8, 2, 64, [12345], [1]), (8, 1, 32, [4100, 4099, 77], [3, 1, 20]), (4, 1, 128, [6000], [40])])
+@pytest.mark.parametrize("H,kv,dh,lens,rows", [(8, 8, 128, [9000, 40], [1, 1]), (8, 2, 64, [12345], [1]), (8, 1, 32, [4100, 4099, 77], [3, 1, 20]), (4, 1, 128, [6000], [40]), (4, 1, 64, [100000], [2]),
+                                               (17, 1, 128, [60000], [1]), (6, 2, 32, [90000, 5], [1, 1])])
 def test_long_sequences(H, kv, dh, lens, rows):
     """Split over workgroups and joined; the sequences' lengths far apart."""
     print(f"case: long {lens} {rows}, {H} heads over {kv} of {dh}", flush=True)
