@@ -61,6 +61,14 @@ __device__ __forceinline__ float max3(float x, float y, float z) {
   return r;
 }
 
+// The lane's number, asked for anew each time: held over the loop over pages it would be kept in memory, and come back as a wait for all
+// loads on their way.
+__device__ __forceinline__ int lane_now() {
+  int l;
+  asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(l));
+  return l;
+}
+
 // sum, and maximum, over the lanes up to this one
 __device__ __forceinline__ int wave_scan_int(int v) {
   v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);  // row_shr:1
@@ -103,18 +111,18 @@ struct Batch {
   int len, row0, rows, tiles, cost, upto;  // this lane's; cost: of one job; upto: of all up to the end of this sequence
   // A wavefront keeps them in LDS while it works on a job: they are needed again for the next one only.
   __device__ __forceinline__ void put(int (*to)[64]) const {
-    const int l = threadIdx.x & 63;
+    const int l = lane_now();
     to[0][l] = len, to[1][l] = row0, to[2][l] = rows, to[3][l] = tiles, to[4][l] = cost, to[5][l] = upto;
   }
   __device__ __forceinline__ void get(const int (*from)[64]) {
-    const int l = threadIdx.x & 63;
+    const int l = lane_now();
     len = from[0][l], row0 = from[1][l], rows = from[2][l], tiles = from[3][l], cost = from[4][l], upto = from[5][l];
   }
 };
 struct Read {  // of a sequence
   int len = 0, row0 = 0, end = 0;
   __device__ __forceinline__ Read(const Kv4Attn &a, int first) {
-    const int i = first + (int)(threadIdx.x & 63);
+    const int i = first + lane_now();
     if (i < a.n_seqs) len = a.lens[i], row0 = a.starts[i], end = a.starts[i + 1];
   }
 };
@@ -138,7 +146,7 @@ struct Job {
 // the job at a place on the line, which lies in front of its end; fronts: what 64 sequences at a time have in front of them, cost and largest start
 __device__ __forceinline__ bool find_job(const Kv4Attn &a, Batch &s, int (*kept)[64], const int (*fronts)[64], int place, Job &j) {
   if (place < s.before || place >= __builtin_amdgcn_readlane(s.upto, 63)) {
-    const int lane = threadIdx.x & 63;
+    const int lane = lane_now();
     const int block = __popcll(__ballot(lane * 64 < a.n_seqs && fronts[0][lane] <= place)) - 1;
     s.first = 64 * block, s.before = __builtin_amdgcn_readfirstlane(fronts[0][block]), s.reach = __builtin_amdgcn_readfirstlane(fronts[1][block]);
     look(a, Read(a, s.first), s);
@@ -180,8 +188,11 @@ struct Kv4Lds {
 //           partial sum.  (The nibbles as they stand are fp16 subnormals n 2^-24 and would need no conversion, but the matrix
 //           instruction adds products of subnormals with five bits less: 2.8e-6 of a score instead of 6e-8.)
 //   output  2^14 p as two fp16 terms, times the scale d as two again (the rounded product, what that leaves, the second term's): 22
-//           bits of each p d, or a grid of 2^-24 where it is smaller than 2^-2 of 2^14 p d.  Values as exact fp16 integers, fp32
-//           accumulators.  Scales outside 2^-9 .. 2 are brought there by 2^f first (products stay below fp16's 65504).
+//           bits of each 2^14 p d, or a grid of 2^-24 where it, or 2^14 p, is below 2^-2.  Values as exact fp16 integers, fp32 accumulators.
+//           Products stay below 2^15 (fp16 ends at 65504) by a power of two f: 2^f d, f > 0, while all scales seen are below 2^-9, which is exact;
+//           2^f p, f >= -4, from a scale of 2 on (on d it would put the page's other scales on fp16's subnormal grid: off by 5 % beside a
+//           value of 4e5 that has no weight).  Pages with a scale of 32 or more take the fp32 matrix instructions, p d as one fp32 number, at an
+//           eighth of the rate (where all pages have one the batches above take 85 and 57 us, the prompts 239).
 template <int DH>
 __global__ __launch_bounds__(256, DH == 128 ? 3 : 4) void k_kv4_attn(Kv4Attn a) {
   using L = Kv4Lds<DH>;
@@ -193,13 +204,13 @@ __global__ __launch_bounds__(256, DH == 128 ? 3 : 4) void k_kv4_attn(Kv4Attn a) 
   int (*s_fronts)[64] = (int (*)[64])(smem + L::FRONTS);  // (every wavefront writes all of it, the same)
   // a wavefront's results lie where its own pages did
   auto s_o = [&](int wave, int row) { return (float *)(smem + wave * L::WAVE) + row * (DH + 4); };
-  const int tid0 = threadIdx.x, wv = __builtin_amdgcn_readfirstlane(tid0 >> 6);
+  const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int G = a.group;
   int total = 0, longest = 0;
   Batch s;
   for (Read read(a, 0);;) {
     const bool more = s.first + 64 < a.n_seqs;
-    if ((tid0 & 63) == 0) s_fronts[0][s.first >> 6] = s.before, s_fronts[1][s.first >> 6] = s.reach;
+    if (lane_now() == 0) s_fronts[0][s.first >> 6] = s.before, s_fronts[1][s.first >> 6] = s.reach;
     const Read next(a, more ? s.first + 64 : a.n_seqs);  // (on its way while these are looked at)
     look(a, read, s);
     longest = max(longest, s.tiles ? s.cost : 0);
@@ -226,9 +237,7 @@ __global__ __launch_bounds__(256, DH == 128 ? 3 : 4) void k_kv4_attn(Kv4Attn a) 
   if (x != x0) s.get(s_seqs[wv]);
   if (!find_job(a, s, s_seqs[wv], s_fronts, x, w)) break;
   x = w.at + w.cost;
-  // (what hangs on the lane alone is worked out for each job: kept from being moved in front of the loop, where it would hold registers)
-  int lane = tid0 & 63;
-  asm volatile("" : "+v"(lane));
+  const int lane = lane_now();
   const int n = lane & 15, g = lane >> 4;
   // this lane's row
   const int rho = w.tile * kTileRows + n, j = fast_div(rho, G);
@@ -341,7 +350,7 @@ __global__ __launch_bounds__(256, DH == 128 ? 3 : 4) void k_kv4_attn(Kv4Attn a) 
 #pragma unroll
   for (int b = 0; b < NB; b++) o[b][0] = o[b][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   float m = -INFINITY, l = 0.0f;
-  int f = 100;  // the values' scales go in as 2^f d (100: none seen)
+  int f = 100;  // outputs are held times 2^f, f in -4 .. 15 (100: no scale seen)
 
   // What a row's weights are taken against: 2^(m weight - base) = 2^14.  The base is used as it is rounded wherever weights of different maxima
   // meet, so its rounding cancels.
@@ -445,7 +454,7 @@ __global__ __launch_bounds__(256, DH == 128 ? 3 : 4) void k_kv4_attn(Kv4Attn a) 
     unsigned large = 0;  // scales of 2 and more have this bit of their exponent
 #pragma unroll
     for (int x = 0; x < NB; x++) large |= vs_now[x] & 0x4000u;
-    bool plain = whole && f == 0 && !__ballot(large);
+    bool plain = whole && f == 0 && !__ballot(large), wide = false;
     if (!plain) {
       float d = 0.0f;  // the largest scale of the page's rows that are there (each lane has a piece of the page's scales)
 #pragma unroll
@@ -456,27 +465,30 @@ __global__ __launch_bounds__(256, DH == 128 ? 3 : 4) void k_kv4_attn(Kv4Attn a) 
       }
       d = fminf(wave_max(d), 65504.0f);
       const int e = __builtin_amdgcn_readfirstlane((int)(__float_as_uint(d) >> 23)) - 127;  // (uniform)
+      const int fits = e > 0 ? max(-e, -4) : e >= -9 ? 0 : min(-e, 15);  // the power of two that this page asks for
       if (d > 0.0f && f == 100) {
-        f = e >= -9 && e <= 0 ? 0 : min(max(-e, -15), 15);
-      } else if (d > 0.0f && e + f > 0) {
-        const float by = ldexpf(1.0f, -e - f);
-        f = -e;
+        f = fits;
+      } else if (d > 0.0f && e + f > 0 && f > -4) {
+        const float by = ldexpf(1.0f, max(-e, -4) - f);
+        f = max(-e, -4);
 #pragma unroll
         for (int b = 0; b < NB; b++) o[b][0] *= by, o[b][1] *= by;
       }
+      wide = e > 4;
       plain = whole && f == 0;
     }
+    const float p_by = ldexpf(1.0f, min(f, 0));
+    auto outputs = [&](auto plain) {
+    constexpr bool PLAIN = decltype(plain)::value;
+    const _Float16 by = (_Float16)ldexpf(1.0f, f == 100 ? 0 : max(f, 0));
     // p as two fp16 terms, once for all blocks
     half2v ph[8], pl[8];
 #pragma unroll
     for (int i = 0; i < 8; i++) {
-      const float x0 = s[i >> 1][2 * (i & 1)], x1 = s[i >> 1][2 * (i & 1) + 1];
+      const float x0 = s[i >> 1][2 * (i & 1)] * (PLAIN ? 1.0f : p_by), x1 = s[i >> 1][2 * (i & 1) + 1] * (PLAIN ? 1.0f : p_by);
       ph[i] = __builtin_convertvector((f32x2){x0, x1}, half2v);
       pl[i] = __builtin_convertvector((f32x2){fmaf((float)ph[i][0], minus, x0), fmaf((float)ph[i][1], minus, x1)}, half2v);
     }
-    const _Float16 by = (_Float16)ldexpf(1.0f, f == 100 ? 0 : f);
-    auto outputs = [&](auto plain) {
-    constexpr bool PLAIN = decltype(plain)::value;
 #pragma unroll
     for (int b = 0; b < NB; b++) {
       const u32x4 vq = *(const u32x4 *)(vp + (b * 16 + n) * kKvPageRows + 16 * g);
@@ -512,7 +524,26 @@ __global__ __launch_bounds__(256, DH == 128 ? 3 : 4) void k_kv4_attn(Kv4Attn a) 
       }
     }
     };
-    if (plain) outputs(std::true_type());
+    // large scales: four keys 16 t + 4 g + i, one of each lane group, an instruction
+    auto outputs_wide = [&]() {
+#pragma unroll 1
+      for (int t = 0; t < 4; t++) {  // (the first of the scores each time, in turn: little code)
+#pragma unroll
+        for (int b = 0; b < NB; b++) {
+          const uint32_t u = *(const uint32_t *)(vp + (b * 16 + n) * kKvPageRows + 16 * g + 4 * t);
+          const half4 d = scales(vp, t, b);
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            const float x = from + 16 * t + 4 * g + i > limit ? 0.0f : s[0][i] * ((float)d[i] * p_by);
+            o[b][0] = __builtin_amdgcn_mfma_f32_16x16x4f32((float)((int)(u << (28 - 8 * i)) >> 28), x, o[b][0], 0, 0, 0);
+            o[b][1] = __builtin_amdgcn_mfma_f32_16x16x4f32((float)((int)(u << (24 - 8 * i)) >> 28), x, o[b][1], 0, 0, 0);
+          }
+        }
+        s[0] = s[1], s[1] = s[2], s[2] = s[3];
+      }
+    };
+    if (wide) outputs_wide();
+    else if (plain) outputs(std::true_type());
     else outputs(std::false_type());
     wait_lds();
     if (more) ask_quants(a.v_pages, next, v_at), ask_scales(a.v_pages, next, v_at);
@@ -521,17 +552,16 @@ __global__ __launch_bounds__(256, DH == 128 ? 3 : 4) void k_kv4_attn(Kv4Attn a) 
   l += __shfl_xor(l, 16, 64);
   l += __shfl_xor(l, 32, 64);
 
-  // the four wavefronts' results meet (and what hangs on the thread alone, here)
-  int tid = tid0;
-  asm volatile("" : "+v"(tid));
+  // the four wavefronts' results meet
+  const int tid = wv * 64 + lane_now(), n_out = tid & 15, g_out = (tid >> 4) & 3;
   const int nr = min(kTileRows, w.rows * G - w.tile * kTileRows);  // rows of the tile that there are
-  if (g == 0) s_m[wv][n] = m > -INFINITY ? base_of(m) : -INFINITY, s_l[wv][n] = l;
+  if (g_out == 0) s_m[wv][n_out] = m > -INFINITY ? base_of(m) : -INFINITY, s_l[wv][n_out] = l;
   const float back = ldexpf(1.0f, f == 100 ? 0 : -f);
-  if (n < nr) {
+  if (n_out < nr) {
 #pragma unroll
     for (int b = 0; b < NB; b++)
 #pragma unroll
-      for (int half = 0; half < 2; half++) *(f32x4 *)(s_o(wv, n) + b * 32 + half * 16 + 4 * g) = o[b][half] * back;
+      for (int half = 0; half < 2; half++) *(f32x4 *)(s_o(wv, n_out) + b * 32 + half * 16 + 4 * g_out) = o[b][half] * back;
   }
   __syncthreads();
   // a share that goes on from the workgroup before, and one that goes on in the next: a workgroup has one of each at most

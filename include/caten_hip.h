@@ -402,9 +402,9 @@ int cthip_kv_rows_paged_q4(float *k_rows, float *v_rows, const void *k_pages, co
  * sequence i, which holds lens[i] keys (those rows' own among them): each sees the keys up to its own position.  One row a
  * sequence is a decode step, more are a prompt or a piece of one.  q rows are (H, Dh), q_stride floats apart; out (n_rows, H,
  * Dh) contiguous, not q.  A row that sees no key is zero; rows behind starts[n_seqs], and those of a sequence that starts in front of an
- * earlier one's rows, are left as they were; a table entry outside the pool, or a row past the table's end, holds no key.  fp32 sums; q, and the
- * probabilities times the values' scales, enter the products with 22 bits of a row's largest.  At most 4096 sequences, 2^20 rows and
- * 2^21 tiles of 16 (row, head) of a key / value head.
+ * earlier one's rows, are left as they were; a table entry outside the pool, or a row past the table's end, holds no key.  fp32 sums; q enters the
+ * products with 22 bits of a row's largest, a probability times a value's scale with 22 bits of its own, or off by 2^-35 (1 + scale) where that is more
+ * (the largest probability being 1).  At most 4096 sequences, 2^20 rows and 2^21 tiles of 16 (row, head) of a key / value head.
  * workspace: cthip_sdpa_paged_q4_workspace(Dh) = 4 * (2048 + 2048 * 16 * (Dh + 2)) bytes, 16-byte aligned, zeroed once
  * (cthip_alloc does); every call leaves it ready for the next.  Calls that may overlap (graphs replayed on other streams) need one each. */
 int64_t cthip_sdpa_paged_q4_workspace(int Dh);

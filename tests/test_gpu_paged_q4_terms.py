@@ -1,0 +1,151 @@
+"""Attention over the 4-bit paged cache where every rounding can be counted: few keys have a weight at all, so sums have few
+terms and the bound is near what the products themselves lose.  Held against the definition in NumPy, in 64 bits, channel by
+channel: a channel's error is measured by its own weighted values, not by the largest of the head."""
+import numpy as np
+import pytest
+
+from tests.test_gpu_paged_q4 import PAGE, batch
+
+pytestmark = pytest.mark.gpu
+
+
+def sparse_keys(rng, T, kv, dh, live):
+    """Keys of which all but `live` score some hundreds below the others for queries from `gated_queries` (their weights are
+    exactly zero in fp32), the live ones with two channels a block that are not zero."""
+    k = np.zeros((T, kv, dh), np.float32)
+    k[:, :, 0] = -4000.0
+    for t in live:
+        k[t] = 0.0
+        for h in range(kv):
+            for b in range(dh // 32):
+                k[t, h, 32 * b + 1 + rng.permutation(31)[:2]] = rng.normal(0, 2.0, 2)
+    return k
+
+
+def gated_queries(rng, rows, H, dh):
+    q = rng.normal(0, 1, (rows, H, dh)).astype(np.float32)
+    q[:, :, 0] = 2.0
+    return q
+
+
+def channels(q, k, v, p_of=None, q_of=None):
+    """(out, tolerance) of the last rows of a sequence, channel by channel; p_of / q_of: what a poorer kernel would make of
+    weights relative to the largest, and of queries.
+
+    Of one live key, per unit of its weighted value:
+      q     two fp16 terms of the row's largest: off by 2^-23 of it; times the key's channels: q_err
+      score a sum of 2 channels a block in two terms (4 additions a block), a scale and an addition a block, a weight: 6 NB + 2 roundings of
+            2^-23 (a matrix instruction may cut off) of the terms' sum
+      exponential  the argument, below 16 for weights above 2^-30, rounded: ln 2 * 16 * 2^-24 < 2^-20; itself 2^-22
+      p d   p as two terms 2^-22, the products' second term 2^-22; the fp32 form less.  Half a step of fp16's grid of 2^-24 in 2^10 p,
+            times a value below 512 (pages with larger scales take the fp32 form): 2^-35 of that; in 2^10 p d, times a number up to 8: 2^-32
+      sums  of L live keys and their terms over wavefronts and shares: 2 L + 8 roundings of 2^-23
+    An error of a weight counts twice: above and below the line."""
+    q, k, v = (np.asarray(a, np.float64) for a in (q, k, v))
+    rows, H, dh = q.shape
+    T, G, NB = k.shape[0], H // k.shape[1], dh // 32
+    out, tol = np.zeros(q.shape), np.zeros(q.shape)
+    used = q if q_of is None else q_of(q)
+    for r in range(rows):
+        t = T - rows + r + 1
+        for h in range(H):
+            kk, vv = k[:t, h // G], v[:t, h // G]
+            s = kk @ used[r, h] / np.sqrt(dh)
+            live = s > s.max() - 100
+            p = np.exp(s - s.max())
+            if p_of is not None:
+                p = p_of(p)
+            out[r, h] = p[live] @ vv[live] / p[live].sum()
+            size = (np.abs(kk[live]) @ np.abs(q[r, h])).max() / np.sqrt(dh)
+            q_err = np.abs(kk[live]).sum(1).max() * np.abs(q[r, h]).max() * 2.0 ** -23 / np.sqrt(dh)
+            one = q_err + size * (6 * NB + 2) * 2.0 ** -23 + 2.0 ** -20 + 2.0 ** -22 + 2.0 ** -21
+            L = live.sum()
+            tol[r, h] = p[live] @ np.abs(vv[live]) / p[live].sum() * (2 * one + (2 * L + 8) * 2.0 ** -23 + 2.0 ** -24) + L * (2.0 ** -32 + 2.0 ** -35 * np.minimum(np.abs(vv[live]).max(0), 512))
+    return out, tol
+
+
+def check(got, q, k, v):
+    want, tol = channels(q, k, v)
+    assert np.isfinite(got).all()
+    worst = np.abs(got - want) / tol
+    print("share of the tolerance:", float(worst.max()), flush=True)
+    assert (worst <= 1).all(), float(worst.max())
+    return want, tol
+
+
+def sequence(rng, T, rows, kv, dh, live, sizes):
+    """A sequence with sparse keys and values of `sizes` (T, kv, dh); (cache, tables, starts, keys, values as held)."""
+    cache, tables, starts, _ = batch(rng, [T], [rows], kv, dh)
+    slots = np.array([tables[0, t // PAGE] * PAGE + t % PAGE for t in range(T)], np.int32)
+    v = (rng.normal(0, 1, (T, kv, dh)) * sizes).astype(np.float32)
+    cache.append(sparse_keys(rng, T, kv, dh, live), v, slots)
+    k, v = cache.rows(slots)
+    return cache, tables, starts, k, v
+
+
+LIVE = [3, 40, 70, 100, 130, 200, 260, 290]
+
+
+@pytest.mark.parametrize("H,kv,dh", [(4, 2, 64), (16, 1, 128), (3, 3, 64), (32, 4, 128)])
+@pytest.mark.parametrize("rows", [1, 20])
+@pytest.mark.parametrize("large,small", [(100, 0.01), (1000, 0.01), (1e4, 0.05), (1.8e4, 1.0), (4e5, 0.05), (30, 3e-3)])
+def test_a_block_of_large_values_beside_small_ones(H, kv, dh, rows, large, small):
+    """Channels 32 .. 63 large, the others small: in all pages, or in one of them."""
+    rng = np.random.default_rng(int(large) + dh + rows)
+    T = 340
+    for pages in (range(6), [0], [3]):
+        sizes = np.full((T, kv, dh), small)
+        for page in pages:
+            sizes[PAGE * page:PAGE * (page + 1), :, 32:64] = large
+        cache, tables, starts, k, v = sequence(rng, T, rows, kv, dh, LIVE, sizes)
+        q = gated_queries(rng, rows, H, dh)
+        check(cache.attend(q, tables, [T], starts), q, k, v)
+
+
+@pytest.mark.parametrize("H,kv,dh", [(6, 2, 32), (4, 2, 64), (16, 1, 128), (3, 3, 128)])
+@pytest.mark.parametrize("rows", [1, 20])
+@pytest.mark.parametrize("size", [20, 4.7e3, 2.4e4, 3.9e5])
+def test_a_large_row_without_weight(H, kv, dh, rows, size):
+    """One row of large values that no query has a weight for, in the first page, in a later one, in the last: the others' results
+    do not depend on it."""
+    rng = np.random.default_rng(int(size) + dh + rows)
+    T = 340
+    for row in (5, 150, 310):
+        sizes = np.full((T, kv, dh), 0.05)
+        sizes[row] = size
+        cache, tables, starts, k, v = sequence(rng, T, rows, kv, dh, LIVE, sizes)
+        q = gated_queries(rng, rows, H, dh)
+        check(cache.attend(q, tables, [T], starts), q, k, v)
+
+
+@pytest.mark.parametrize("H,kv,dh", [(6, 2, 32), (16, 1, 128), (4, 4, 64)])
+@pytest.mark.parametrize("rows", [1, 20])
+@pytest.mark.parametrize("size,nats", [(4e5, 18), (4e5, 20.5), (300, 15), (600, 20), (30, 12), (17, 0.5), (200, 3)])
+def test_a_large_row_of_little_weight(H, kv, dh, rows, size, nats):
+    """Its score lies `nats` below that of a key of zeros."""
+    rng = np.random.default_rng(int(size + nats) + dh + rows)
+    T = 340
+    for row in (5, 150, 310):
+        sizes = np.full((T, kv, dh), 0.05)
+        sizes[row] = size
+        cache, tables, starts, k, v = sequence(rng, T, rows, kv, dh, LIVE, sizes)
+        slot = [tables[0, row // PAGE] * PAGE + row % PAGE]
+        k[row] = 0.0
+        k[row, :, 0] = -nats * np.sqrt(dh) / 2.0
+        cache.append(k[row:row + 1], v[row:row + 1], slot)
+        k[row:row + 1], v[row:row + 1] = cache.rows(slot)
+        q = gated_queries(rng, rows, H, dh)
+        check(cache.attend(q, tables, [T], starts), q, k, v)
+
+
+@pytest.mark.parametrize("H,kv,dh", [(2, 2, 32), (8, 1, 64), (4, 2, 128)])
+@pytest.mark.parametrize("rows", [1, 20])
+@pytest.mark.parametrize("factors", [(1e-5, 1, 1e3), (1e3, 1e-3, 1), (1e-4, 1e4, 1e-4), (1, 1e5, 1e-2)])
+def test_sizes_page_by_page(H, kv, dh, rows, factors):
+    rng = np.random.default_rng(dh * rows)
+    T = 40 * PAGE + 30
+    live = list(range(7, T, 211))
+    sizes = np.array(factors)[np.arange(T) // PAGE * len(factors) // (T // PAGE + 1)][:, None, None] * np.ones((1, kv, dh))
+    cache, tables, starts, k, v = sequence(rng, T, rows, kv, dh, live, sizes)
+    q = gated_queries(rng, rows, H, dh)
+    check(cache.attend(q, tables, [T], starts), q, k, v)
