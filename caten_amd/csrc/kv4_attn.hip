@@ -335,7 +335,7 @@ __global__ __launch_bounds__(256, DH == 128 ? 3 : 4) void k_kv4_attn(Kv4Attn a) 
       for (int k = 0; k < 8; k++) {
         // the order in which a dword's nibbles come apart: channels 0 2 4 6 1 3 5 7
         const int ch = k < 4 ? (k & 1) * 2 + (k >> 1) * 4 : 1 + (k & 1) * 2 + ((k - 4) >> 1) * 4;
-        const float y = bad ? 0.0f : mine8[ch] * up;
+        const float y = bad ? NAN : mine8[ch] * up;  // (every score of the row a NaN, and those that are masked minus infinity: without a key it is zero)
         hi[k] = (_Float16)y;
         lo[k] = (_Float16)(y - (float)hi[k]);
       }
@@ -343,7 +343,7 @@ __global__ __launch_bounds__(256, DH == 128 ? 3 : 4) void k_kv4_attn(Kv4Attn a) 
       *(half8 *)(smem + L::Q + wv * 2048 + 1024 + lane * 16) = lo;
     }
     // scores as powers of two: log2(e) / sqrt(DH), and the power of two taken off again
-    weight = bad ? NAN : (DH == 32 ? 0.25503487f : DH == 64 ? 0.18033688f : 0.12751743f) * down;
+    weight = (DH == 32 ? 0.25503487f : DH == 64 ? 0.18033688f : 0.12751743f) * down;
   }
 
   f32x4 o[NB][2];

@@ -149,3 +149,23 @@ def test_sizes_page_by_page(H, kv, dh, rows, factors):
     cache, tables, starts, k, v = sequence(rng, T, rows, kv, dh, live, sizes)
     q = gated_queries(rng, rows, H, dh)
     check(cache.attend(q, tables, [T], starts), q, k, v)
+
+
+@pytest.mark.parametrize("H,kv,dh", [(2, 2, 64), (16, 2, 32), (4, 1, 128)])
+@pytest.mark.parametrize("what", [np.nan, np.inf, -np.inf])
+def test_a_query_that_is_not_finite_and_sees_no_key(H, kv, dh, what):
+    """Its row is zero like any other without keys, next to rows that see some; one that sees a key is NaN."""
+    rng = np.random.default_rng(H + dh)
+    lens, rows = [3, 100, 70], [8, 1, 1]
+    cache, tables, starts, held = batch(rng, lens, rows, kv, dh)
+    q = rng.normal(0, 1, (10, H, dh)).astype(np.float32)
+    clean = cache.attend(q, tables, lens, starts)
+    q[1, :, 5], q[4, 0, 0], q[8, :, dh - 1] = what, what, what
+    tables[1] = -1, cache.n_pages  # (all of the second sequence's pages are outside the pool)
+    got = cache.attend(q, tables, lens, starts)
+    assert not got[:5].any() and not got[8].any()
+    assert np.array_equal(got[5:8], clean[5:8]) and np.array_equal(got[9], clean[9])
+    q[6, 0, 1] = what
+    got = cache.attend(q, tables, lens, starts)
+    assert np.isnan(got[6, 0]).all() and np.array_equal(got[6, 1:], clean[6, 1:]) and not got[:5].any()
+    assert np.array_equal(got[[5, 7, 9]], clean[[5, 7, 9]])
