@@ -276,7 +276,8 @@ __global__ __launch_bounds__(kSelectThreads) void k_beam_merge(BeamArgs a) {
   // which the lists of a beam's slices have among themselves.
   auto head = [&](int i, int at) { return held ? list[i * K + at] : ((const BeamPair *)(recs + (int64_t)i * record_bytes + 24))[at]; };
   auto value = [&](int beam, BeamPair p) {
-    return p.x == -INFINITY ? -INFINITY : s_base[beam] + (p.x == s_top[beam] ? 0.0 : (double)p.x - (double)s_top[beam]);
+    const double z = s_base[beam] + (p.x == s_top[beam] ? 0.0 : (double)p.x - (double)s_top[beam]);
+    return p.x > -INFINITY && z == z ? z : -INFINITY;  // (a score of infinity less a logit of infinity is no number)
   };
   auto before = [](double y1, int b1, BeamPair p1, double y2, int b2, BeamPair p2) {
     return y1 > y2 || (y1 == y2 && (b1 < b2 || (b1 == b2 && beam_before(p1.x, p1.token, p2.x, p2.token))));

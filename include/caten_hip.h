@@ -412,8 +412,8 @@ int cthip_sdpa_paged_q4(float *out, const float *q, int64_t q_stride, const void
                         const int *lens, const int *starts, int n_seqs, int n_rows, int H, int Hkv, int Dh, void *workspace);
 /* The n_beams best continuations of each request: candidates (beam, token) score scores[beam] + log softmax(logits[beam])[token];
  * a finished beam (finished may be NULL) has one, its eos with its score as it is.  Highest score first; ties go to the lower
- * beam, then to the higher logit, then to the lower token.  NaN logits and scores count as minus infinity, and a
- * candidate of minus infinity is taken only where nothing else is left.  logits rows (n_batch * n_beams, vocab), logits_stride
+ * beam, then to the higher logit, then to the lower token.  NaN logits and scores count as minus infinity
+ * (infinity less infinity among them), and a candidate of minus infinity is taken only where nothing else is left.  logits rows (n_batch * n_beams, vocab), logits_stride
  * floats apart; scores, finished and the outputs (n_batch, n_beams); parents count within the request; finished_out (may be
  * NULL) = the parent's, or token == eos; eos -1 = none.  n_beams 1 .. 32, vocab >= n_beams, at most 2^18 beams of all requests.  Not in place.
  * workspace: cthip_beam_select_workspace(...) = 256 + 4 n_batch + 32 n_batch n_beams (24 + 8 n_beams) bytes, 16-byte aligned, whatever
