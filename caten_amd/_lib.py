@@ -108,6 +108,7 @@ PROTOTYPES = {
     "cthip_sdpa_cached_paged": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _i]),
     "cthip_kv_page_bytes_q4": (_i64, [_i, _i]),
     "cthip_kv_plan_paged": (_i, [_vp, _vp, _vp, _vp, _i, _vp, _vp, _vp, _vp, _vp, _i, _vp, _vp, _i]),
+    "cthip_kv_free_paged": (_i, [_vp, _vp, _vp, _i, _vp, _i, _i]),
     "cthip_kv_append_paged_q4": (_i, [_vp, _vp, _vp, _vp, _i64, _i64, _vp, _i, _i, _i, _i]),
     "cthip_kv_rows_paged_q4": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i]),
     "cthip_sdpa_paged_q4_workspace": (_i64, [_i]),

@@ -3,6 +3,8 @@
 // (external/llm/layers.lisp:19-33) and one sequence; a server holds many sequences of different lengths, so here all of them
 // take pages from one pool, and everything a step needs to know about who owns what is worked out on the device: a step's
 // launches can be captured once and replayed.  Layout of a page: kv4.h.
+#include <algorithm>
+
 #include "kv4.h"
 
 namespace cthip {
@@ -122,6 +124,43 @@ __global__ __launch_bounds__(kPlanThreads) void k_kv_plan(int *__restrict__ slot
     slots[r] = slot;
     if (positions) positions[r] = at;
   }
+}
+
+// ---- pages back to the free stack ----
+// The stack's own array is the set of pages: filled with all ids, those in use struck out (by any number of threads, with the same value), and
+// what is left moved to the front, one workgroup, 8192 at a time: a chunk has been read by all threads before what is left of it is
+// written, in front of the next one's place.  Three launches: 9.5 us for 144 beams and a pool of 3000 pages; 100000 pages, 71 us, wait for that one
+// workgroup's round trips.
+constexpr int kFreeEach = 8;
+__global__ __launch_bounds__(256) void k_kv_free_all(int *free_pages, int n_pages) {
+  for (int64_t i = blockIdx.x * 256 + threadIdx.x; i < n_pages; i += (int64_t)gridDim.x * 256) free_pages[i] = (int)i;
+}
+__global__ __launch_bounds__(256) void k_kv_free_strike(int *free_pages, const int *__restrict__ tables, int table_stride, const int *__restrict__ lens, int n_pages) {
+  const int len = max(lens[blockIdx.x], 0), pages = min(len / kKvPageRows + (len % kKvPageRows != 0), table_stride);
+  for (int c = threadIdx.x; c < pages; c += 256) {
+    const int id = tables[(int64_t)blockIdx.x * table_stride + c];
+    if (id >= 0 && id < n_pages) free_pages[id] = -1;
+  }
+}
+__global__ __launch_bounds__(kPlanThreads) void k_kv_free_pack(int *free_pages, int *n_free, int n_pages) {
+  __shared__ int64_t part[2][kPlanThreads / 64];
+  int kept = 0;
+  for (int i0 = 0, round = 0; i0 < n_pages; i0 += kFreeEach * kPlanThreads, round++) {
+    int id[kFreeEach], mine = 0;
+#pragma unroll
+    for (int k = 0; k < kFreeEach; k++) {
+      const int i = i0 + kFreeEach * (int)threadIdx.x + k;
+      id[k] = i < n_pages ? free_pages[i] : -1;
+      mine += id[k] >= 0;
+    }
+    int64_t all;
+    int at = kept + (int)block_scan(mine, part[round & 1], all);
+#pragma unroll
+    for (int k = 0; k < kFreeEach; k++)
+      if (id[k] >= 0) free_pages[at++] = id[k];
+    kept += (int)all;
+  }
+  if (threadIdx.x == 0) n_free[0] = kept;
 }
 
 // ---- rows into the cache ----
@@ -494,6 +533,24 @@ int cthip_kv_plan_paged(int *slots, int *positions, int *starts, int *tables, in
                        new_lens, n_seqs, free_pages, n_free, max_rows, false, true);
     CTHIP_LAUNCH_CHECK();
   }
+  return 0;
+}
+
+int cthip_kv_free_paged(int *free_pages, int *n_free, const int *tables, int table_stride, const int *lens, int n_seqs, int n_pages) {
+  CTHIP_REQUIRE_INIT();
+  CTHIP_ARG(n_seqs >= 0 && n_pages >= 0 && n_pages <= INT_MAX / kKvPageRows && table_stride > 0);
+  if (n_seqs > 65535) return fail(CTHIP_E_UNSUPPORTED, "cthip_kv_free_paged: %d sequences in one call (at most 65535)", n_seqs);
+  CTHIP_ARG(n_free && (n_pages == 0 || free_pages) && (n_seqs == 0 || (tables && lens)));
+  if (n_pages > 0) {
+    hipLaunchKernelGGL(k_kv_free_all, dim3((unsigned)std::min(1024, (n_pages + 255) / 256)), dim3(256), 0, state().stream, free_pages, n_pages);
+    CTHIP_LAUNCH_CHECK();
+  }
+  if (n_pages > 0 && n_seqs > 0) {
+    hipLaunchKernelGGL(k_kv_free_strike, dim3((unsigned)n_seqs), dim3(256), 0, state().stream, free_pages, tables, table_stride, lens, n_pages);
+    CTHIP_LAUNCH_CHECK();
+  }
+  hipLaunchKernelGGL(k_kv_free_pack, dim3(1), dim3(kPlanThreads), 0, state().stream, free_pages, n_free, n_pages);
+  CTHIP_LAUNCH_CHECK();
   return 0;
 }
 

@@ -272,6 +272,17 @@ def kv_plan(lens, new_lens, tables, free_pages, max_rows: int, n_free: Optional[
                 refused=int(refused.numpy()[0]))
 
 
+def kv_free_pages(tables, lens, n_pages: int) -> np.ndarray:
+    """The pages of a pool that no sequence's rows are in (cthip_kv_free_paged), as a stack for `kv_plan`."""
+    tables, lens = (np.ascontiguousarray(a, np.int32) for a in (tables, lens))
+    if tables.ndim != 2 or tables.shape[0] != lens.size:
+        raise ValueError(f"kv_free_pages: {lens.size} lengths and a table of shape {tables.shape}")
+    d_tables, d_lens = DeviceArray.from_numpy(tables), DeviceArray.from_numpy(lens)
+    d_free, d_n = DeviceArray((max(n_pages, 1),), np.int32), DeviceArray((1,), np.int32)
+    _lib.check(_lib.init().cthip_kv_free_paged(d_free.ptr, d_n.ptr, d_tables.ptr, tables.shape[1], d_lens.ptr, lens.size, n_pages))
+    return d_free.numpy()[:int(d_n.numpy()[0])]
+
+
 class PagedCacheQ4:
     """The keys and values of a batch of sequences in 4 bits, in pages of 64 rows (one layer, or `layers` of them)."""
 

@@ -388,6 +388,13 @@ int64_t cthip_kv_page_bytes_q4(int kv_heads, int head_dim); /* of one page of ke
  * max_rows 2^30. */
 int cthip_kv_plan_paged(int *slots, int *positions, int *starts, int *tables, int table_stride, int *lens_out, int *n_free_out, int *refused,
                         const int *lens, const int *new_lens, int n_seqs, const int *free_pages, const int *n_free, int max_rows);
+/* The free stack anew: all pages of the pool but those that the first ceil(lens[i] / rows of a page) entries of a sequence's table name, ids
+ * rising, and their number; free_pages has room for n_pages, what lies behind the number is undefined.  The plan only takes pages.  Those of a
+ * sequence that has left (length 0), and those that a beam search's reordering leaves behind -- a beam without children has full pages
+ * that no table names any more, up to n_beams - 1 for every page's rows of a request -- come back by this call alone: it belongs in front of a
+ * step's plan, whenever pages run low or in every step.  tables and lens are all there are of this pool; entries outside it are passed over.
+ * At most 65535 sequences. */
+int cthip_kv_free_paged(int *free_pages, int *n_free, const int *tables, int table_stride, const int *lens, int n_seqs, int n_pages);
 /* Key and value rows (n_rows, kv_heads * head_dim), k_stride / v_stride floats apart (they may be slices of a fused product),
  * into the cache rows their slots name; a slot outside the pool (-1) is skipped, two rows with one slot are undefined.  Per block
  * of 32: m = the value of largest magnitude (the positive one of two), d = fp16(m / -8) held within +-65504, number =
@@ -427,7 +434,7 @@ int cthip_beam_select(int *tokens, int *parents, float *scores_out, int *finishe
  * for its first child, and for further ones the page of a beam without children, into which the parent's is copied in
  * all n_layers pools ((n_layers, n_pages, page bytes) each); behind it row j of tables.  history_out (n_batch * n_beams, cols; may be NULL):
  * the parent's row of history with tokens[j] in column step[0].  tables_out and history_out are not in place.  At most 32 beams,
- * 65535 beams of all requests. */
+ * 65535 beams of all requests.  Full pages of beams without children are in no table afterwards: cthip_kv_free_paged. */
 int cthip_beam_reorder_paged_q4(int *tables_out, int *history_out, void *k_pages, void *v_pages, int n_layers, int n_pages, const int *tables, int table_stride,
                                 const int *lens, const int *parents, int n_batch, int n_beams, int kv_heads, int head_dim, const int *history, int cols,
                                 const int *tokens, const int *step);
