@@ -384,8 +384,10 @@ int64_t cthip_kv_page_bytes_q4(int kv_heads, int head_dim); /* of one page of ke
  * free_pages is a stack of n_free[0] page ids: pages are taken from its end, in the order of the sequences, and the array
  * itself is not changed.  A sequence is refused whole -- length kept, slots and positions -1, no pages -- where a count is
  * negative, its table row or max_rows is too short, or too few pages are left; once pages have run out, every later
- * sequence that needs one is refused too.  refused[0] is their number: such a sequence's rows must not be attended.  At most 4096 sequences,
- * max_rows 2^30. */
+ * sequence that needs one is refused too.  refused[0] is their number.  A captured step goes on with the others: of a refused sequence nothing
+ * is appended (slots -1) and nothing changes, so a later step can take the same rows again; cthip_sdpa_paged_q4 takes its rows for the last ones of
+ * the lens[i] keys it holds, and what it makes of them is to be thrown away, as is all that is made of that.  The host looks at refused[0]
+ * behind a step, and where it is not 0 at positions[starts[i]] of the sequences with new rows (-1: refused).  At most 4096 sequences, max_rows 2^30. */
 int cthip_kv_plan_paged(int *slots, int *positions, int *starts, int *tables, int table_stride, int *lens_out, int *n_free_out, int *refused,
                         const int *lens, const int *new_lens, int n_seqs, const int *free_pages, const int *n_free, int max_rows);
 /* The free stack anew: all pages of the pool but those that the first ceil(lens[i] / rows of a page) entries of a sequence's table name, ids
