@@ -30,7 +30,7 @@ def gated_queries(rng, rows, H, dh):
 
 def channels(q, k, v, p_of=None, q_of=None):
     """(out, tolerance) of the last rows of a sequence, channel by channel; p_of / q_of: what a poorer kernel would make of
-    weights relative to the largest, and of queries.
+    weights (of the largest) times scales and of queries.
 
     Of one live key, per unit of its weighted value:
       q     two fp16 terms of the row's largest: off by 2^-23 of it; times the key's channels: q_err
@@ -53,9 +53,11 @@ def channels(q, k, v, p_of=None, q_of=None):
             s = kk @ used[r, h] / np.sqrt(dh)
             live = s > s.max() - 100
             p = np.exp(s - s.max())
-            if p_of is not None:
-                p = p_of(p)
-            out[r, h] = p[live] @ vv[live] / p[live].sum()
+            if p_of is None:
+                out[r, h] = p[live] @ vv[live] / p[live].sum()
+            else:  # a block's scale is its largest value's size / 8, within a rounding: of values that are whole multiples of it
+                d = np.repeat(np.abs(vv[live]).reshape(-1, NB, 32).max(-1) / 8, 32, 1)
+                out[r, h] = (p_of(p[live][:, None], d) * (vv[live] / np.where(d > 0, d, 1))).sum(0) / p[live].sum()
             size = (np.abs(kk[live]) @ np.abs(q[r, h])).max() / np.sqrt(dh)
             q_err = np.abs(kk[live]).sum(1).max() * np.abs(q[r, h]).max() * 2.0 ** -23 / np.sqrt(dh)
             one = q_err + size * (6 * NB + 2) * 2.0 ** -23 + 2.0 ** -20 + 2.0 ** -22 + 2.0 ** -21
@@ -84,6 +86,34 @@ def sequence(rng, T, rows, kv, dh, live, sizes):
 
 
 LIVE = [3, 40, 70, 100, 130, 200, 260, 290]
+
+
+def half(x):
+    return np.float16(x).astype(np.float64)
+
+
+POORER = dict(
+    one_term_of_p=dict(p_of=lambda p, d: half(p * 2.0 ** 14) * d / 2.0 ** 14),
+    one_term_of_p_d=dict(p_of=lambda p, d: half(p * d * 2.0 ** 14) / 2.0 ** 14),
+    no_second_term_times_d=dict(p_of=lambda p, d: (half(half(p * 2.0 ** 14) * d) + half(half(p * 2.0 ** 14) * d - half(half(p * 2.0 ** 14) * d))) / 2.0 ** 14),
+    one_term_of_q=dict(q_of=lambda q: half(q * 256) / 256),
+    bfloat16_of_q=dict(q_of=lambda q: (np.float32(q).view(np.uint32) + 0x8000 & 0xFFFF0000).view(np.float32).astype(np.float64)))
+
+
+@pytest.mark.parametrize("H,kv,dh", [(4, 2, 64), (16, 1, 128), (3, 3, 32), (12, 12, 64), (32, 4, 128), (17, 1, 64)])
+@pytest.mark.parametrize("rows", [1, 20])
+@pytest.mark.parametrize("T,live", [(340, LIVE), (64, [0, 1, 20, 35]), (3000, list(range(7, 2960, 301)))])
+def test_every_term_counts(H, kv, dh, rows, T, live):
+    """Within the bound, which a kernel that lost the second term of a product would not be: that is asked of the definition
+    with the term left out."""
+    rng = np.random.default_rng(H * rows + T)
+    cache, tables, starts, k, v = sequence(rng, T, rows, kv, dh, live, np.ones((T, kv, dh)))
+    q = gated_queries(rng, rows, H, dh)
+    want, tol = check(cache.attend(q, tables, [T], starts), q, k, v)
+    for name, poorer in POORER.items():
+        lost = np.abs(channels(q, k, v, **poorer)[0] - want) / tol
+        print(name, float(lost.max()), flush=True)
+        assert lost.max() > 4, name
 
 
 @pytest.mark.parametrize("H,kv,dh", [(4, 2, 64), (16, 1, 128), (3, 3, 64), (32, 4, 128)])
