@@ -9,7 +9,9 @@
 // bound from below on the n_beams best, found lane by lane, and the candidates' way through LDS: 384 rows of 32000 (49 MB) 17.4 us + 8.4
 // for the merge.  Smaller chunks with the next one on its way while one is worked on (29 - 37 us) do that more often; a looser
 // bound by fewer steps (28.4) has more candidates.
-// Everything behind the exponentials is in 64 bits: between beams, candidates are compared by sums that a rounding could turn round.
+// Exponentials, and the sums of a thread's 16 or 32, are in 32 bits (off by 2^-21 of a row's sum at most: that much of a score, alike for all of a
+// beam's candidates); sums over threads and slices, logarithms and what candidates are compared by in 64: within a beam no rounding turns two
+// round, between beams scores that are closer than 2^-21 may be.
 #include <algorithm>
 
 #include "common.h"
@@ -388,6 +390,7 @@ extern "C" {
 
 int64_t cthip_beam_select_workspace(int n_batch, int n_beams) {
   if (n_batch < 0 || n_beams < 1 || n_beams > kMaxSelectBeams) return fail(CTHIP_E_BAD_ARG, "cthip_beam_select_workspace: %d x %d beams (at most %d)", n_batch, n_beams, kMaxSelectBeams);
+  // (the records take what n_batch * n_beams gives; what is asked for besides is not used, and kept since callers work the size out themselves)
   return 256 + 4ll * n_batch + (int64_t)n_batch * n_beams * kMaxSlices * (24 + 8 * n_beams);
 }
 

@@ -135,7 +135,7 @@ __device__ __forceinline__ void look(const Kv4Attn &a, const Read &read, Batch &
   s.rows = s.row0 == reach && end > s.row0 ? end - s.row0 : 0;
   s.tiles = (s.rows * a.group + kTileRows - 1) / kTileRows;
   const int pages = a.n_pages > 0 && s.len > 0 ? (int)min(((unsigned)s.len + kKvPageRows - 1) / kKvPageRows, (unsigned)a.table_stride) : 0;
-  s.cost = max(1, pages + (1 << a.piece_log2) - 1 >> a.piece_log2) + kJobPieces;  // (without keys there is still a row to write)
+  s.cost = max(1, (pages + (1 << a.piece_log2) - 1) >> a.piece_log2) + kJobPieces;  // (without keys there is still a row to write)
   s.upto = s.before + wave_scan_int(s.tiles * a.Hkv * s.cost);
 }
 struct Job {
@@ -250,7 +250,7 @@ __global__ __launch_bounds__(256, DH == 128 ? 3 : 4) void k_kv4_attn(Kv4Attn a) 
   const int last = (int)min((int64_t)w.len - w.rows + j1, all - 1), least = (int)min((int64_t)w.len - w.rows + j0, all - 1);
   const int pages = a.n_pages > 0 && last >= 0 ? last / kKvPageRows + 1 : 0;
   // its pieces lie on the line behind those that stand for the rest (a job without pages is one piece of none)
-  const int pieces = max(1, pages + (1 << a.piece_log2) - 1 >> a.piece_log2), line = w.at + kJobPieces;
+  const int pieces = max(1, (pages + (1 << a.piece_log2) - 1) >> a.piece_log2), line = w.at + kJobPieces;
   const int owner = uniform_fast_div(line, per), shares = uniform_fast_div(line + pieces - 1, per) - owner + 1, share = me - owner;
   const int from_piece = max(x0 - line, 0), to_piece = min(x1 - line, pieces);
   if (from_piece >= to_piece) continue;
@@ -707,7 +707,7 @@ extern "C" {
 
 int64_t cthip_sdpa_paged_q4_workspace(int head_dim) {
   if (!kv4_shape_ok(1, head_dim)) return fail(CTHIP_E_BAD_ARG, "cthip_sdpa_paged_q4_workspace: head size %d (32, 64, 128)", head_dim);
-  return 4 * (2048ll + 2048ll * 16 * (head_dim + 2));
+  return 4ll * kSplitSlots * (1 + kTileRows * (head_dim + 2));  // a ticket and a record each
 }
 
 int cthip_sdpa_paged_q4(float *out, const float *q, int64_t q_stride, const void *k_pages, const void *v_pages, int n_pages, const int *tables, int table_stride,
