@@ -8,11 +8,11 @@
 // What bounds it is the vector unit, not memory: taking the nibbles apart (9 instructions for 8 numbers of a key, 20 for 16 of
 // values), the scales (one a number of the 16 x 64 scores, two terms of p d), exponentials.  Per page and 16 rows 450 instructions at
 // Dh = 64 and some 650 at 128, of 4 cycles each, against 512 and 1024 cycles of matrix instructions and, at Dh = 128, 9 KB.
-//   700-row prompts of 5 sequences, 32 heads over 4 of 64 (25 GFLOP): 109 us, the vector units busy 67 % of it, the matrix units 17 %.
-//   32 sequences of 150 .. 20000, 64 heads over 8 of 128 (159 MB): 48 us = 3.3 TB/s; vector units 47 %, matrix units 14 %; some 12 us are what a
+//   700-row prompts of 5 sequences, 32 heads over 4 of 64 (25 GFLOP): 109 - 111 us, the vector units busy 67 % of it, the matrix units 17 %.
+//   32 sequences of 150 .. 20000, 64 heads over 8 of 128 (159 MB): 45.3 us = 3.5 TB/s; vector units 48 %, matrix units 14 %; some 12 us are what a
 //   workgroup does before its first page and after its last.
-//   8 sequences of 1500 .. 5000, 32 heads of 128 (93 MB): 30 us = 3.1 TB/s, 15 of a tile's 16 rows empty.
-//   One sequence of 701, 12 heads of 64: 8.7 us, a chain of round trips: lengths, table, page, record, ticket, records.
+//   8 sequences of 1500 .. 5000, 32 heads of 128 (93 MB): 28.6 us = 3.25 TB/s, 15 of a tile's 16 rows empty.
+//   One sequence of 701, 12 heads of 64: 8.4 us, a chain of round trips: lengths, table, page, record, ticket, records.
 #include <algorithm>
 #include <type_traits>
 
@@ -725,8 +725,8 @@ int cthip_sdpa_paged_q4(float *out, const float *q, int64_t q_stride, const void
   const int64_t tiles = (int64_t)n_rows * (H / Hkv) / kTileRows + (n_seqs < n_rows ? n_seqs : n_rows), jobs = tiles * Hkv;
   if (jobs > (1 << 21) || n_rows > (1 << 20))
     return fail(CTHIP_E_UNSUPPORTED, "cthip_sdpa_paged_q4: %d rows of %d heads in one call (at most 2^20 rows, and 2^21 tiles of 16 heads of them)", n_rows, H);
-  // as many workgroups as run at once (three or four a compute unit for their registers and pages; with two or three and no spilled register
-  // prompts take 119 us instead of 112, the batches 50 and 32 instead of 48 and 30), a multiple of the XCDs
+  // as many workgroups as run at once (three or four a compute unit for their registers and pages; with two or three prompts took 119 us
+  // where these took 112, the batches 50 and 32 where these took 48 and 30), a multiple of the XCDs
   const int at_once = std::min(kSplitSlots / 2, state().compute_units * (Dh == 128 ? 3 : 4) / 8 * 8);
   int piece = 2;  // (the line is shorter than 2^30, and a workgroup's part of it below what fast_div holds for)
   while (jobs * ((table_stride >> piece) + 1 + kJobPieces) > std::min((int64_t)INT_MAX / 2, (int64_t)at_once << 20)) piece++;

@@ -368,8 +368,10 @@ int cthip_sdpa_cached_paged(float *out, const float *q, const void *const *k_pag
 /* ---- many sequences over one pool of pages, rows in 4 bits; beam search ----
  * The reference decodes one sequence over a dense fp32 cache (layers.lisp:19-33, apps/gpt2/gpt2.lisp:97-113).  A step of a
  * batch is cthip_kv_plan_paged, then per layer cthip_kv_append_paged_q4 and cthip_sdpa_paged_q4, then cthip_argmax or
- * cthip_beam_select and cthip_beam_reorder_paged_q4; lengths, tables and page ids stay on the device, so a step can be
- * captured into a graph and replayed.  All arrays are device memory, indices int32, arrays of different arguments
+ * cthip_beam_select and cthip_beam_reorder_paged_q4; lengths, tables and page ids stay on the device, so plan, append and attention of a
+ * decode step can be captured into a graph whose replay is the next step.  A beam search's reordering takes lengths a request (the plan keeps
+ * them a sequence) and the step's column from the caller, and its tables go to and fro between two arrays: captured, two steps a graph, the caller
+ * writing these in front of a replay.  All arrays are device memory, indices int32, arrays of different arguments
  * do not overlap unless an entry says so.
  * Pages: cthip_kv_page_rows() rows of every key / value head; a pool is (n_pages, cthip_kv_page_bytes_q4) bytes for the keys
  * and the same for the values, 16-byte aligned.  A row's block of 32 channels is an fp16 scale and 32 numbers -8 .. 7 (4.5
