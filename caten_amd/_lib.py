@@ -16,6 +16,7 @@ LIB_PATH = os.path.join(_HERE, "libcaten_hip.so")
 F32, F16, Q4_0, Q8_0 = 0, 1, 2, 8
 GGML_TYPE = {"f32": F32, "f16": F16, "q4_0": Q4_0, "q8_0": Q8_0}
 PRO_NONE, PRO_LAYERNORM, PRO_RMSNORM, PRO_SWIGLU = 0, 1, 2, 3
+ROPE_PAIRS, ROPE_HALVES = 0, 1
 ACT_NONE, ACT_RELU, ACT_GELU, ACT_SILU, ACT_SIGMOID, ACT_TANH = 0, 1, 2, 3, 4, 5
 ARCH_GPT2, ARCH_LLAMA = 0, 1
 
@@ -116,6 +117,15 @@ PROTOTYPES = {
     "cthip_beam_select_workspace": (_i64, [_i, _i]),
     "cthip_beam_select": (_i, [_vp, _vp, _vp, _vp, _vp, _i64, _vp, _vp, _i, _i, _i, _i, _vp]),
     "cthip_beam_reorder_paged_q4": (_i, [_vp, _vp, _vp, _vp, _i, _i, _vp, _i, _vp, _vp, _i, _i, _i, _i, _vp, _i, _vp, _vp]),
+    "cthip_rope_rows": (_i, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i, _i, _i, _i, _i, _i, _vp, _f]),
+    "cthip_rope_frequencies": (_i, [_vp, _i, C.c_double, C.c_double, _i, C.c_double, C.c_double]),
+    "cthip_kv_fork_paged_q4": (_i, [_vp, _i, _vp, _i, _vp, _vp, _vp, _vp, _i, _i, _vp, _vp, _vp, _i, _vp, _vp, _i, _i]),
+    "cthip_kv_compact_paged_q4_workspace": (_i64, [_i]),
+    "cthip_kv_compact_paged_q4": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _vp, _i, _vp, _i, _i, _i, _vp]),
+    "cthip_sdpa_shared_paged_q4_workspace": (_i64, [_i, _i, _i]),
+    "cthip_sdpa_shared_paged_q4": (_i, [_vp, _vp, _i64, _vp, _vp, _i, _vp, _i, _vp, _vp, _i, _i, _vp, _vp, _i, _i, _i, _i, _vp]),
+    "cthip_draft_verify_workspace": (_i64, [_i]),
+    "cthip_draft_verify": (_i, [_vp, _vp, _vp, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _vp]),
     "cthip_decoder_create": (_i, [_vpp, C.POINTER(DecoderConfig)]),
     "cthip_decoder_destroy": (_i, [_vp]),
     "cthip_decoder_load": (_i, [_vp, C.c_char_p, _i, _vp, _i64, _i64]),

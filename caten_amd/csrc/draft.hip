@@ -1,0 +1,214 @@
+// Verification of drafted tokens against the target's probabilities, from random numbers that are given.  The reference takes the most
+// probable token (apps/gpt2/gpt2.lisp:97-113: cthip_argmax); with no drafts this is sampling by the target's probabilities.
+//
+// Draft x of a row, drawn from q, stays where u q(x) < p(x); the first that does not is replaced by a token drawn from max(p - q, 0), and behind
+// the last that stays one more is drawn from p: what comes out is distributed as the target's own samples are.  Drawn is the lowest token at which the running sum of
+// the weights is above u times their sum.  u q is exact in 64 bits, differences and sums are taken in 64: near a border between two
+// tokens 32 bits would settle for a neighbour once in some thousand draws from a large vocabulary.
+//
+// Two launches.  A row is cut into slices; a workgroup finds its sequence's first rejected draft for itself (one load of two
+// numbers a draft) and leaves its slice's sums, the replacement's and, in case that one is nothing, the target's own.  Then a wavefront
+// finds the slice and a workgroup the token in it.  Bound by the two rows of the vocabulary that a sequence needs.
+#include <algorithm>
+
+#include "common.h"
+
+namespace cthip {
+
+constexpr int kDraftThreads = 256, kDraftSlices = 64;
+constexpr int kDraftWorkspace = 2048;  // bytes a sequence
+static_assert(16 * kDraftSlices <= kDraftWorkspace, "the sums of a sequence's slices");
+
+struct DraftArgs {
+  int *tokens_out, *accepted, *lens_out;
+  const float *target, *draft;
+  int64_t target_stride, draft_stride;
+  const int *tokens;
+  const float *uniforms;
+  const int *starts, *positions, *lens;
+  int n_rows, vocab, slices, slice;
+  double *sums;  // (sequence, 128): of each slice the weights', of each slice the target's
+};
+
+__device__ __forceinline__ double draft_wave_sum(double v) {
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
+
+// The rows of a sequence, those of drafts that stay, and the token row that the last one is drawn from
+struct Verified {
+  int row0, rows, stay;
+  bool there;
+  __device__ __forceinline__ Verified(const DraftArgs &a, int seq) {
+    const int lane = threadIdx.x & 63;
+    row0 = a.starts[seq];
+    const int end = a.starts[seq + 1];
+    rows = end - row0;
+    there = row0 >= 0 && rows > 0 && end <= a.n_rows;
+    stay = 0;
+    if (!there) return;
+    there = !a.positions || a.positions[row0] >= 0;
+    if (!there) return;
+    for (int j0 = 0; j0 < rows - 1; j0 += 64) {  // (every wavefront for itself)
+      const int j = j0 + lane;
+      bool good = true;
+      if (j < rows - 1) {
+        const int x = a.tokens[row0 + j + 1];
+        good = x >= 0 && x < a.vocab;
+        if (good) {
+          const float p = a.target[(int64_t)(row0 + j) * a.target_stride + x], q = a.draft ? a.draft[(int64_t)(row0 + j) * a.draft_stride + x] : 1.0f;
+          good = (double)a.uniforms[row0 + j] * (double)q < (double)p;
+        }
+      }
+      const unsigned long long bad = __ballot(!good);
+      if (bad) {
+        stay = j0 + (int)__builtin_ctzll(bad);
+        return;
+      }
+    }
+    stay = rows - 1;
+  }
+};
+
+// What a token weighs: NaN and what is below nothing, as nothing
+struct DraftRow {
+  const float *p, *q;
+  int taken;  // the rejected draft, where there are no probabilities of the draft's: the whole of them was its
+  __device__ __forceinline__ DraftRow(const DraftArgs &a, const Verified &v) {
+    p = a.target + (int64_t)(v.row0 + v.stay) * a.target_stride;
+    const bool rejected = v.stay < v.rows - 1;
+    q = rejected && a.draft ? a.draft + (int64_t)(v.row0 + v.stay) * a.draft_stride : nullptr;
+    taken = rejected && !a.draft ? a.tokens[v.row0 + v.stay + 1] : -1;
+  }
+  __device__ __forceinline__ void at(int t, double &w, double &own) const {
+    const float x = p[t];
+    own = x > 0.0f ? (double)x : 0.0;
+    const double left = (double)x - (q ? (double)q[t] : 0.0);
+    w = t == taken ? 0.0 : left > 0.0 ? left : 0.0;
+  }
+};
+
+__global__ __launch_bounds__(kDraftThreads) void k_draft_slice(DraftArgs a) {
+  __shared__ double part[2][kDraftThreads / 64];
+  const int seq = blockIdx.y, tid = threadIdx.x;
+  const Verified v(a, seq);
+  if (!v.there) return;
+  const DraftRow row(a, v);
+  double w = 0.0, own = 0.0;
+  const int t1 = min(a.vocab, ((int)blockIdx.x + 1) * a.slice);
+  for (int t = blockIdx.x * a.slice + tid; t < t1; t += kDraftThreads) {
+    double x, y;
+    row.at(t, x, y);
+    w += x, own += y;
+  }
+  w = draft_wave_sum(w), own = draft_wave_sum(own);
+  if ((tid & 63) == 0) part[0][tid >> 6] = w, part[1][tid >> 6] = own;
+  __syncthreads();
+  if (tid < 2) a.sums[(int64_t)seq * (2 * kDraftSlices) + kDraftSlices * tid + blockIdx.x] = (part[tid][0] + part[tid][1]) + (part[tid][2] + part[tid][3]);
+}
+
+// inclusive, over a wavefront
+__device__ __forceinline__ double draft_wave_scan(double v) {
+  const int lane = threadIdx.x & 63;
+  for (int o = 1; o < 64; o <<= 1) {
+    const double y = __shfl_up(v, o, 64);
+    if (lane >= o) v += y;
+  }
+  return v;
+}
+
+__global__ __launch_bounds__(kDraftThreads) void k_draft_token(DraftArgs a) {
+  __shared__ double part[2][kDraftThreads / 64];
+  __shared__ int s_found[2], s_last[2];
+  const int seq = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+  const Verified v(a, seq);
+  int token = -1;
+  if (v.there) {
+    const DraftRow row(a, v);
+    const double *sums = a.sums + (int64_t)seq * (2 * kDraftSlices);
+    double mine = lane < a.slices ? sums[lane] : 0.0;
+    double upto = draft_wave_scan(mine), total = __shfl(upto, 63, 64);
+    const bool own = !(total > 0.0);  // nothing is left of the target behind the draft's: by roundings alone, then its own
+    if (own) {
+      mine = lane < a.slices ? sums[kDraftSlices + lane] : 0.0;
+      upto = draft_wave_scan(mine), total = __shfl(upto, 63, 64);
+    }
+    if (total > 0.0) {
+      const double goal = (double)a.uniforms[v.row0 + v.rows - 1] * total;
+      // the first slice that reaches past the goal, or the last that weighs anything
+      const unsigned long long past = __ballot(upto > goal && mine > 0.0), any = __ballot(mine > 0.0);
+      const int s = past ? (int)__builtin_ctzll(past) : 63 - (int)__builtin_clzll(any);
+      double before = s > 0 ? __shfl(upto, s - 1, 64) : 0.0;
+      const int t1 = min(a.vocab, (s + 1) * a.slice);
+      if (tid < 2) s_last[tid] = -1;
+      int last = -1;
+      for (int t0 = s * a.slice, round = 0; t0 < t1; t0 += kDraftThreads, round ^= 1) {
+        const int t = t0 + tid;
+        double w = 0.0, o = 0.0;
+        if (t < t1) row.at(t, w, o);
+        if (own) w = o;
+        const double sum = draft_wave_scan(w);
+        if (lane == 63) part[round][wv] = sum;
+        if (tid == 0) s_found[round] = INT_MAX;
+        __syncthreads();
+        double front = before;
+        for (int k = 0; k < kDraftThreads / 64; k++) {
+          if (k < wv) front += part[round][k];
+          before += part[round][k];
+        }
+        if (w > 0.0) {
+          last = t;
+          if (front + sum > goal) atomicMin(&s_found[round], t);
+        }
+        __syncthreads();
+        if (s_found[round] != INT_MAX) {
+          token = s_found[round];
+          break;
+        }
+      }
+      if (token < 0) {  // (sums of other orders, or a number that is not below one)
+        if (last >= 0) atomicMax(&s_last[0], last);
+        __syncthreads();
+        token = s_last[0];
+      }
+    }
+    for (int j = tid; j < v.rows; j += kDraftThreads) a.tokens_out[v.row0 + j] = j < v.stay ? a.tokens[v.row0 + j + 1] : j == v.stay ? token : -1;
+  } else if (v.row0 >= 0 && v.rows > 0 && v.row0 + v.rows <= a.n_rows) {
+    for (int j = tid; j < v.rows; j += kDraftThreads) a.tokens_out[v.row0 + j] = -1;
+  }
+  if (tid == 0) {
+    a.accepted[seq] = v.there ? v.stay : 0;
+    if (a.lens_out) a.lens_out[seq] = a.lens[seq] - (v.there ? v.rows - 1 - v.stay : 0);
+  }
+}
+
+}  // namespace cthip
+
+using namespace cthip;
+
+extern "C" {
+
+int64_t cthip_draft_verify_workspace(int n_seqs) {
+  if (n_seqs < 0) return fail(CTHIP_E_BAD_ARG, "cthip_draft_verify_workspace: %d sequences", n_seqs);
+  return (int64_t)n_seqs * kDraftWorkspace;
+}
+
+int cthip_draft_verify(int *tokens_out, int *accepted, int *lens_out, const float *target, int64_t target_stride, const float *draft, int64_t draft_stride, const int *tokens,
+                       const float *uniforms, const int *starts, const int *positions, const int *lens, int n_seqs, int n_rows, int vocab, void *workspace) {
+  CTHIP_REQUIRE_INIT();
+  CTHIP_ARG(n_seqs >= 0 && n_rows >= 0 && vocab >= 1 && vocab <= (1 << 30) && target_stride >= vocab && (!draft || draft_stride >= vocab));
+  if (n_seqs > 65535) return fail(CTHIP_E_UNSUPPORTED, "cthip_draft_verify: %d sequences in one call (at most 65535)", n_seqs);
+  if (n_seqs == 0) return 0;
+  CTHIP_ARG(accepted && starts && workspace && ((uintptr_t)workspace & 15) == 0 && (!lens_out || lens));
+  CTHIP_ARG(n_rows == 0 || (tokens_out && target && tokens && uniforms && tokens_out != tokens));
+  const int slices = std::min(kDraftSlices, (vocab + 1023) / 1024), slice = (vocab + slices - 1) / slices;
+  const DraftArgs a = {tokens_out, accepted, lens_out, target, draft, target_stride, draft_stride, tokens, uniforms, starts, positions, lens, n_rows, vocab, (vocab + slice - 1) / slice, slice,
+                       (double *)workspace};
+  hipLaunchKernelGGL(k_draft_slice, dim3((unsigned)a.slices, (unsigned)n_seqs), dim3(kDraftThreads), 0, state().stream, a);
+  CTHIP_LAUNCH_CHECK();
+  hipLaunchKernelGGL(k_draft_token, dim3((unsigned)n_seqs), dim3(kDraftThreads), 0, state().stream, a);
+  CTHIP_LAUNCH_CHECK();
+  return 0;
+}
+
+}  // extern "C"

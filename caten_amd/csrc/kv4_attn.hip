@@ -32,7 +32,13 @@ struct Kv4Attn {
   int piece_log2;  // pages are shared out in pieces of this many
   int *tickets;    // workspace: a counter per job that is shared, zero between calls
   float *parts;    // and the shares' records: 16 rows of unnormalised outputs, their maxima, their sums
+  // sequences that share their first pages
+  const int *groups, *shared;
+  int n_groups;
+  float *stats;    // of a (row, head): maximum and sum over the shared pages; the outputs over them lie in `out`, unnormalised
 };
+// What a launch is: a batch by itself; the pages that a group's sequences share, for all of its rows; what the sequences have behind those
+enum { kAttnWhole = 0, kAttnShared = 1, kAttnBehind = 2 };
 
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef _Float16 half4 __attribute__((ext_vector_type(4)));
@@ -44,6 +50,8 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kTileRows = 16;       // rows (query row, query head of the group) of a tile
 constexpr int kSplitSlots = 2048;   // records of shares in the workspace, two a workgroup
+constexpr int kSharedTickets = 4096, kSharedRecordRows = 131072;  // tickets, and rows of records, in the workspace of a batch with shared pages
+static_assert(kSharedTickets >= kSplitSlots && kSharedRecordRows >= kSplitSlots * kTileRows, "those of k_kv4_attn");
 constexpr int kJobPieces = 1;       // what a job costs besides its pages, in pieces of them (2: 52 us instead of 50, 34 instead of 31, for the batches above)
 
 // floor(x / d) where that is below 2^21, x below 2^30: the quotient by a reciprocal is off by one at most, which what it leaves shows.  (A division
@@ -105,51 +113,90 @@ __device__ __forceinline__ float max32(float v) {
 // shared by many workgroups and many short ones go to one.  The lengths are on the device only: every wavefront works
 // the division out for itself, 64 sequences at a time (0.4 us each: 33 us for 4096 sequences of which one has a row; 57 where each
 // 64 waited for their lengths and were gone through again for a job).
+template <int MODE>
 struct Batch {
+  static constexpr int FIELDS = MODE == kAttnWhole ? 6 : 7;
   int first = 0, before = 0;  // of the 64 sequences in the lanes: the first, and the cost in front of it
   int reach = 0;              // the largest start up to the last of them
   int len, row0, rows, tiles, cost, upto;  // this lane's; cost: of one job; upto: of all up to the end of this sequence
+  int aside;  // kAttnShared: the group's first sequence; kAttnBehind: pages of the sequence that are shared
   // A wavefront keeps them in LDS while it works on a job: they are needed again for the next one only.
   __device__ __forceinline__ void put(int (*to)[64]) const {
     const int l = lane_now();
     to[0][l] = len, to[1][l] = row0, to[2][l] = rows, to[3][l] = tiles, to[4][l] = cost, to[5][l] = upto;
+    if constexpr (MODE != kAttnWhole) to[6][l] = aside;
   }
   __device__ __forceinline__ void get(const int (*from)[64]) {
     const int l = lane_now();
     len = from[0][l], row0 = from[1][l], rows = from[2][l], tiles = from[3][l], cost = from[4][l], upto = from[5][l];
+    if constexpr (MODE != kAttnWhole) aside = from[6][l];
   }
 };
-struct Read {  // of a sequence
-  int len = 0, row0 = 0, end = 0;
+// The pages that group g's sequences share, 0 where there is one of them only (it reads its pages by itself), and the first and the end of them
+__device__ __forceinline__ int shared_pages(const Kv4Attn &a, int g, int &first, int &end) {
+  first = min(max(a.groups[g], 0), a.n_seqs), end = min(max(a.groups[g + 1], 0), a.n_seqs);
+  return end - first > 1 && a.n_pages > 0 ? min(max(a.shared[g], 0) / kKvPageRows, a.table_stride) : 0;
+}
+template <int MODE>
+struct Read {  // of a sequence, or of a group
+  int len = 0, row0 = 0, end = 0, aside = 0;
   __device__ __forceinline__ Read(const Kv4Attn &a, int first) {
     const int i = first + lane_now();
-    if (i < a.n_seqs) len = a.lens[i], row0 = a.starts[i], end = a.starts[i + 1];
+    if constexpr (MODE == kAttnShared) {
+      if (i < a.n_groups) {
+        int last;
+        const int pages = shared_pages(a, i, aside, last);
+        len = pages * kKvPageRows;
+        if (pages) row0 = a.starts[aside], end = a.starts[last];
+      }
+    } else {
+      if (i < a.n_seqs) len = a.lens[i], row0 = a.starts[i], end = a.starts[i + 1];
+      if constexpr (MODE == kAttnBehind) {
+        if (i < a.n_seqs && a.n_groups > 0) {
+          int lo = 0, hi = a.n_groups;  // groups[lo] <= i where there is such a group
+          while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (a.groups[mid] <= i) lo = mid;
+            else hi = mid;
+          }
+          int g0, g1;
+          const int pages = shared_pages(a, lo, g0, g1);
+          if (i >= g0 && i < g1) aside = pages;
+        }
+      }
+    }
   }
 };
-__device__ __forceinline__ void look(const Kv4Attn &a, const Read &read, Batch &s) {
+template <int MODE>
+__device__ __forceinline__ int in_all(const Kv4Attn &a) { return MODE == kAttnShared ? a.n_groups : a.n_seqs; }
+template <int MODE>
+__device__ __forceinline__ void look(const Kv4Attn &a, const Read<MODE> &read, Batch<MODE> &s) {
   s.len = max(read.len, 0), s.row0 = read.row0;
+  if constexpr (MODE != kAttnWhole) s.aside = read.aside;
   const int end = min(read.end, a.n_rows);
   // (rows in front of an earlier sequence's are nobody's: no row is two sequences', and the costs of all stay within their bound)
   const int reach = max(s.reach, wave_scan_max(s.row0));
   s.reach = __builtin_amdgcn_readlane(reach, 63);
   s.rows = s.row0 == reach && end > s.row0 ? end - s.row0 : 0;
   s.tiles = (s.rows * a.group + kTileRows - 1) / kTileRows;
-  const int pages = a.n_pages > 0 && s.len > 0 ? (int)min(((unsigned)s.len + kKvPageRows - 1) / kKvPageRows, (unsigned)a.table_stride) : 0;
+  const int pages = a.n_pages > 0 && s.len > 0 ? (int)min(((unsigned)s.len + kKvPageRows - 1) / kKvPageRows, (unsigned)a.table_stride) - (MODE == kAttnBehind ? s.aside : 0) : 0;
   s.cost = max(1, (pages + (1 << a.piece_log2) - 1) >> a.piece_log2) + kJobPieces;  // (without keys there is still a row to write)
   s.upto = s.before + wave_scan_int(s.tiles * a.Hkv * s.cost);
 }
 struct Job {
   int seq, head, tile;
+  int skip;             // pages of the sequence in front of the job's
   int len, rows, row0;  // of the sequence: keys, rows of this step and the first of them
   int at, cost;         // its place on the line of all costs
 };
 // the job at a place on the line, which lies in front of its end; fronts: what 64 sequences at a time have in front of them, cost and largest start
-__device__ __forceinline__ bool find_job(const Kv4Attn &a, Batch &s, int (*kept)[64], const int (*fronts)[64], int place, Job &j) {
+template <int MODE>
+__device__ __forceinline__ bool find_job(const Kv4Attn &a, Batch<MODE> &s, int (*kept)[64], const int (*fronts)[64], int place, Job &j) {
   if (place < s.before || place >= __builtin_amdgcn_readlane(s.upto, 63)) {
     const int lane = lane_now();
-    const int block = __popcll(__ballot(lane * 64 < a.n_seqs && fronts[0][lane] <= place)) - 1;
+    const int block = __popcll(__ballot(lane * 64 < in_all<MODE>(a) && fronts[0][lane] <= place)) - 1;
     s.first = 64 * block, s.before = __builtin_amdgcn_readfirstlane(fronts[0][block]), s.reach = __builtin_amdgcn_readfirstlane(fronts[1][block]);
-    look(a, Read(a, s.first), s);
+    look(a, Read<MODE>(a, s.first), s);
     s.put(kept);
   }
   const unsigned long long past = __ballot(s.upto > place);
@@ -159,7 +206,8 @@ __device__ __forceinline__ bool find_job(const Kv4Attn &a, Batch &s, int (*kept)
   j.cost = __builtin_amdgcn_readlane(s.cost, l);
   const int start = __builtin_amdgcn_readlane(s.upto, l) - all * j.cost, job = uniform_fast_div(place - start, j.cost);
   j.at = start + job * j.cost;
-  j.seq = s.first + l;
+  j.seq = MODE == kAttnShared ? __builtin_amdgcn_readlane(s.aside, l) : s.first + l;
+  j.skip = MODE == kAttnBehind ? __builtin_amdgcn_readlane(s.aside, l) : 0;
   j.head = tiles == 1 ? job : uniform_fast_div(job, tiles);
   // tiles from both ends in turn: in a prompt's own pages late rows see more than early ones, and a workgroup gets some of each
   const int t = job - j.head * tiles;
@@ -173,9 +221,9 @@ __device__ __forceinline__ bool find_job(const Kv4Attn &a, Batch &s, int (*kept)
 // The pages come straight into LDS, into a wavefront's own place: the keys and the values of a head as they lie in memory.  A page's
 // key quants are taken to registers when their turn comes, and the next page's are asked for at once; the rest follows when the scores, or the
 // outputs, are there.
-template <int DH>
+template <int DH, int FIELDS>
 struct Kv4Lds {
-  static constexpr int HEAD = 36 * DH, WAVE = 2 * HEAD, STATS = 4 * WAVE, SEQS = STATS + 14 * kTileRows * 4, FRONTS = SEQS + 4 * 6 * 64 * 4, Q = FRONTS + 2 * 64 * 4,
+  static constexpr int HEAD = 36 * DH, WAVE = 2 * HEAD, STATS = 4 * WAVE, SEQS = STATS + 14 * kTileRows * 4, FRONTS = SEQS + 4 * FIELDS * 64 * 4, Q = FRONTS + 2 * 64 * 4,
                        BYTES = Q + DH / 32 * 2048;
   static constexpr int REQUESTS = DH / 32 + (DH / 32 + 1) / 2;  // of a head's part of a page: 16 bytes a lane, then 4
   static constexpr int SHARES = DH == 32 ? 128 : 256;  // of one tile, at most: their records are added up by one workgroup
@@ -193,25 +241,26 @@ struct Kv4Lds {
 //           2^f p, f >= -4, from a scale of 2 on (on d it would put the page's other scales on fp16's subnormal grid: off by 5 % beside a
 //           value of 4e5 that has no weight).  Pages with a scale of 32 or more take the fp32 matrix instructions, p d as one fp32 number, at an
 //           eighth of the rate (where all pages have one the batches above take 85 and 57 us, the prompts 239).
-template <int DH>
+template <int DH, int MODE>
 __global__ __launch_bounds__(256, DH == 128 ? 3 : 4) void k_kv4_attn(Kv4Attn a) {
-  using L = Kv4Lds<DH>;
+  constexpr int FIELDS = Batch<MODE>::FIELDS;
+  using L = Kv4Lds<DH, FIELDS>;
   constexpr int NB = DH / 32;
   extern __shared__ __align__(16) unsigned char smem[];
   float (*s_m)[kTileRows] = (float (*)[kTileRows])(smem + L::STATS), (*s_l)[kTileRows] = s_m + 4, (*s_w)[kTileRows] = s_m + 8, *s_sum = s_m[12];
   int *s_ticket = (int *)s_m[13];
-  int (*s_seqs)[6][64] = (int (*)[6][64])(smem + L::SEQS);
+  int (*s_seqs)[FIELDS][64] = (int (*)[FIELDS][64])(smem + L::SEQS);
   int (*s_fronts)[64] = (int (*)[64])(smem + L::FRONTS);  // (every wavefront writes all of it, the same)
   // a wavefront's results lie where its own pages did
   auto s_o = [&](int wave, int row) { return (float *)(smem + wave * L::WAVE) + row * (DH + 4); };
   const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int G = a.group;
   int total = 0, longest = 0;
-  Batch s;
-  for (Read read(a, 0);;) {
-    const bool more = s.first + 64 < a.n_seqs;
+  Batch<MODE> s;
+  for (Read<MODE> read(a, 0);;) {
+    const bool more = s.first + 64 < in_all<MODE>(a);
     if (lane_now() == 0) s_fronts[0][s.first >> 6] = s.before, s_fronts[1][s.first >> 6] = s.reach;
-    const Read next(a, more ? s.first + 64 : a.n_seqs);  // (on its way while these are looked at)
+    const Read<MODE> next(a, more ? s.first + 64 : in_all<MODE>(a));  // (on its way while these are looked at)
     look(a, read, s);
     longest = max(longest, s.tiles ? s.cost : 0);
     total = __builtin_amdgcn_readlane(s.upto, 63);
@@ -244,11 +293,13 @@ __global__ __launch_bounds__(256, DH == 128 ? 3 : 4) void k_kv4_attn(Kv4Attn a) 
   const bool active = j < w.rows;
   const int head = w.head * G + rho - j * G;
   const int64_t all = (int64_t)a.table_stride * kKvPageRows;
-  const int limit = active ? (int)min((int64_t)w.len - w.rows + j, all - 1) : -1;  // the last key it sees
+  // the last key it sees; of shared pages all
+  const int limit = !active ? -1 : MODE == kAttnShared ? w.len - 1 : (int)min((int64_t)w.len - w.rows + j, all - 1);
   // pages that any row / every row of the tile sees (rows rise with n)
   const int j1 = min(w.rows - 1, uniform_fast_div(w.tile * kTileRows + kTileRows - 1, G)), j0 = uniform_fast_div(w.tile * kTileRows, G);
-  const int last = (int)min((int64_t)w.len - w.rows + j1, all - 1), least = (int)min((int64_t)w.len - w.rows + j0, all - 1);
-  const int pages = a.n_pages > 0 && last >= 0 ? last / kKvPageRows + 1 : 0;
+  const int last = MODE == kAttnShared ? w.len - 1 : (int)min((int64_t)w.len - w.rows + j1, all - 1);
+  const int least = MODE == kAttnShared ? w.len - 1 : (int)min((int64_t)w.len - w.rows + j0, all - 1);
+  const int pages = a.n_pages > 0 && last >= 0 ? max(last / kKvPageRows + 1 - w.skip, 0) : 0;
   // its pieces lie on the line behind those that stand for the rest (a job without pages is one piece of none)
   const int pieces = max(1, (pages + (1 << a.piece_log2) - 1) >> a.piece_log2), line = w.at + kJobPieces;
   const int owner = uniform_fast_div(line, per), shares = uniform_fast_div(line + pieces - 1, per) - owner + 1, share = me - owner;
@@ -257,7 +308,7 @@ __global__ __launch_bounds__(256, DH == 128 ? 3 : 4) void k_kv4_attn(Kv4Attn a) 
   const int p0 = from_piece << a.piece_log2, p1 = (int)min((int64_t)pages, (int64_t)to_piece << a.piece_log2);
 
   // page ids of the next 64 pages of this wavefront, one a lane
-  const int *table = a.tables + (int64_t)w.seq * a.table_stride;
+  const int *table = a.tables + (int64_t)w.seq * a.table_stride + w.skip;
   int ids, ids_from;
   auto page_id = [&](int k) {  // k: this wavefront's k-th page (the same in every lane)
     if (k >= ids_from + 64) {
@@ -377,7 +428,7 @@ __global__ __launch_bounds__(256, DH == 128 ? 3 : 4) void k_kv4_attn(Kv4Attn a) 
       else if (left > per) __builtin_amdgcn_s_setprio(1);
       else __builtin_amdgcn_s_setprio(0);
     }
-    const int page = p0 + wv + 4 * k;
+    const int page = w.skip + p0 + wv + 4 * k;
     const int from = valid(id) ? page * kKvPageRows : INT_MAX - (kKvPageRows - 1);  // (absent: behind every limit)
     const bool whole = from + kKvPageRows - 1 <= least;                            // every row of the tile sees every row of the page (uniform)
     // the scales of block b, rows 16 t + 4 g ..
@@ -578,16 +629,32 @@ __global__ __launch_bounds__(256, DH == 128 ? 3 : 4) void k_kv4_attn(Kv4Attn a) 
       sum = fmaf(e, s_l[x][tid], sum);
     }
     s_sum[tid] = sum;
+    if constexpr (MODE != kAttnWhole) s_l[0][tid] = M;  // (its own sums have been read)
     if (shares > 1) {
       float *to = record_of(share) + kTileRows * DH + 2 * tid;
       __hip_atomic_store((unsigned long long *)to, __builtin_bit_cast(unsigned long long, (f32x2){M, sum}), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
   }
   __syncthreads();
-  // where a pair of channels of a tile's row goes
-  auto out_at = [&](int r, int c) {
+  // a pair of channels of a tile's row: where it goes, as what it is
+  auto finish = [&](int r, int c, f32x2 x, float top, float sum) {
     const int rr = w.tile * kTileRows + r, jj = fast_div(rr, G);
-    return a.out + ((int64_t)(w.row0 + jj) * a.H + w.head * G + rr - jj * G) * DH + c;
+    const int64_t at = (int64_t)(w.row0 + jj) * a.H + w.head * G + rr - jj * G;
+    f2_any *to = (f2_any *)(a.out + at * DH + c);
+    if constexpr (MODE == kAttnShared) {
+      *to = f2_any{x[0], x[1]};
+      if (c == 0) *(f2_any *)(a.stats + 2 * at) = f2_any{top, sum};
+      return;
+    }
+    if constexpr (MODE == kAttnBehind) {
+      if (w.skip) {  // what the launch in front of this one has left of the row
+        const f2_any y = *to, its = *(const f2_any *)(a.stats + 2 * at);
+        const float high = fmaxf(top, its[0]), f = weight_of(top, sum, high), g = weight_of(its[0], its[1], high);
+        sum = fmaf(f, sum, g * its[1]);
+        x[0] = fmaf(f, x[0], g * y[0]), x[1] = fmaf(f, x[1], g * y[1]);
+      }
+    }
+    *to = sum != 0.0f ? f2_any{x[0] / sum, x[1] / sum} : f2_any{0.0f, 0.0f};
   };
   for (int e = tid; e < nr * DH / 2; e += 256) {
     const int r = e / (DH / 2), c = e % (DH / 2) * 2;
@@ -600,8 +667,7 @@ __global__ __launch_bounds__(256, DH == 128 ? 3 : 4) void k_kv4_attn(Kv4Attn a) 
     if (shares > 1) {
       __hip_atomic_store((unsigned long long *)(record_of(share) + 2 * e), __builtin_bit_cast(unsigned long long, x), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     } else {
-      const float sum = s_sum[r];
-      *(f2_any *)out_at(r, c) = sum != 0.0f ? f2_any{x[0] / sum, x[1] / sum} : f2_any{0.0f, 0.0f};
+      finish(r, c, x, MODE != kAttnWhole ? s_l[0][r] : 0.0f, s_sum[r]);
     }
   }
   if (shares > 1) {
@@ -640,7 +706,7 @@ __global__ __launch_bounds__(256, DH == 128 ? 3 : 4) void k_kv4_attn(Kv4Attn a) 
               }
             }
           }
-          *(f2_any *)out_at(r, c) = sum != 0.0f ? f2_any{x[0] / sum, x[1] / sum} : f2_any{0.0f, 0.0f};
+          finish(r, c, x, M, sum);
         }
       } else {
         float (*weights)[kTileRows] = (float (*)[kTileRows])smem;
@@ -690,7 +756,7 @@ __global__ __launch_bounds__(256, DH == 128 ? 3 : 4) void k_kv4_attn(Kv4Attn a) 
               }
             }
           }
-          *(f2_any *)out_at(r, c) = sum != 0.0f ? f2_any{x[0] / sum, x[1] / sum} : f2_any{0.0f, 0.0f};
+          finish(r, c, x, MODE != kAttnWhole ? fmaxf(fmaxf(s_m[0][r], s_m[1][r]), fmaxf(s_m[2][r], s_m[3][r])) : 0.0f, sum);
         }
       }
     }
@@ -702,6 +768,36 @@ __global__ __launch_bounds__(256, DH == 128 ? 3 : 4) void k_kv4_attn(Kv4Attn a) 
 }  // namespace cthip
 
 using namespace cthip;
+
+// What both entries have in common behind their arguments' checks
+static int attn_unsupported(const char *who, int n_seqs, int n_rows, int H, int Hkv, int Dh) {
+  if (!kv4_shape_ok(Hkv, Dh) || H > 65535) return fail(CTHIP_E_UNSUPPORTED, "%s: %d heads over %d of %d (at most 65535 heads, head sizes 32, 64, 128)", who, H, Hkv, Dh);
+  if (n_seqs > kKv4MaxSeqs) return fail(CTHIP_E_UNSUPPORTED, "%s: %d sequences in one call (at most %d)", who, n_seqs, kKv4MaxSeqs);
+  return 0;
+}
+template <int MODE>
+static int launch_kv4_attn(const char *who, Kv4Attn a, int Dh) {
+  // rows of a tile share a key / value head: at most this many tiles of all sequences, and as many jobs a head
+  const int64_t tiles = (int64_t)a.n_rows * (a.H / a.Hkv) / kTileRows + (a.n_seqs < a.n_rows ? a.n_seqs : a.n_rows), jobs = tiles * a.Hkv;
+  if (jobs > (1 << 21) || a.n_rows > (1 << 20))
+    return fail(CTHIP_E_UNSUPPORTED, "%s: %d rows of %d heads in one call (at most 2^20 rows, and 2^21 tiles of 16 heads of them)", who, a.n_rows, a.H);
+  // as many workgroups as run at once (three or four a compute unit for their registers and pages; with two or three prompts took 119 us
+  // where these took 112, the batches 50 and 32 where these took 48 and 30), a multiple of the XCDs
+  const int at_once = std::min(kSplitSlots / 2, state().compute_units * (Dh == 128 ? 3 : 4) / 8 * 8);
+  a.group = a.H / a.Hkv;
+  a.piece_log2 = 2;  // (the line is shorter than 2^30, and a workgroup's part of it below what fast_div holds for)
+  while (jobs * ((a.table_stride >> a.piece_log2) + 1 + kJobPieces) > std::min((int64_t)INT_MAX / 2, (int64_t)at_once << 20)) a.piece_log2++;
+  const dim3 grid((unsigned)at_once), block(256);
+#define ATT(DH_) hipLaunchKernelGGL((k_kv4_attn<DH_, MODE>), grid, block, (Kv4Lds<DH_, Batch<MODE>::FIELDS>::BYTES), state().stream, a)
+  switch (Dh) {
+    case 32: ATT(32); break;
+    case 64: ATT(64); break;
+    default: ATT(128); break;
+  }
+#undef ATT
+  CTHIP_LAUNCH_CHECK();
+  return 0;
+}
 
 extern "C" {
 
@@ -715,33 +811,39 @@ int cthip_sdpa_paged_q4(float *out, const float *q, int64_t q_stride, const void
   CTHIP_REQUIRE_INIT();
   CTHIP_ARG(n_seqs >= 0 && n_rows >= 0 && n_pages >= 0 && n_pages <= INT_MAX / kKvPageRows && table_stride > 0 && table_stride <= INT_MAX / kKvPageRows);
   CTHIP_ARG(H > 0 && Hkv > 0 && H % Hkv == 0);
-  if (!kv4_shape_ok(Hkv, Dh) || H > 65535) return fail(CTHIP_E_UNSUPPORTED, "cthip_sdpa_paged_q4: %d heads over %d of %d (at most 65535 heads, head sizes 32, 64, 128)", H, Hkv, Dh);
-  if (n_seqs > kKv4MaxSeqs) return fail(CTHIP_E_UNSUPPORTED, "cthip_sdpa_paged_q4: %d sequences in one call (at most %d)", n_seqs, kKv4MaxSeqs);
+  if (const int rc = attn_unsupported(__func__, n_seqs, n_rows, H, Hkv, Dh)) return rc;
   if (n_seqs == 0 || n_rows == 0) return 0;
   CTHIP_ARG(out && q && out != q && tables && lens && starts && workspace && q_stride >= (int64_t)H * Dh);
   CTHIP_ARG(n_pages == 0 || (k_pages && v_pages));
   CTHIP_ARG((((uintptr_t)k_pages | (uintptr_t)v_pages | (uintptr_t)workspace) & 15) == 0);
-  // rows of a tile share a key / value head: at most this many tiles of all sequences, and as many jobs a head
-  const int64_t tiles = (int64_t)n_rows * (H / Hkv) / kTileRows + (n_seqs < n_rows ? n_seqs : n_rows), jobs = tiles * Hkv;
-  if (jobs > (1 << 21) || n_rows > (1 << 20))
-    return fail(CTHIP_E_UNSUPPORTED, "cthip_sdpa_paged_q4: %d rows of %d heads in one call (at most 2^20 rows, and 2^21 tiles of 16 heads of them)", n_rows, H);
-  // as many workgroups as run at once (three or four a compute unit for their registers and pages; with two or three prompts took 119 us
-  // where these took 112, the batches 50 and 32 where these took 48 and 30), a multiple of the XCDs
-  const int at_once = std::min(kSplitSlots / 2, state().compute_units * (Dh == 128 ? 3 : 4) / 8 * 8);
-  int piece = 2;  // (the line is shorter than 2^30, and a workgroup's part of it below what fast_div holds for)
-  while (jobs * ((table_stride >> piece) + 1 + kJobPieces) > std::min((int64_t)INT_MAX / 2, (int64_t)at_once << 20)) piece++;
-  const Kv4Attn a = {out,     q,     (const unsigned char *)k_pages, (const unsigned char *)v_pages, tables, lens, starts, q_stride, n_pages, table_stride, n_seqs, n_rows, H, Hkv,
-                     H / Hkv, piece, (int *)workspace, (float *)workspace + kSplitSlots};
-  const dim3 grid((unsigned)at_once), block(256);
-#define ATT(DH_) hipLaunchKernelGGL(k_kv4_attn<DH_>, grid, block, Kv4Lds<DH_>::BYTES, state().stream, a)
-  switch (Dh) {
-    case 32: ATT(32); break;
-    case 64: ATT(64); break;
-    default: ATT(128); break;
-  }
-#undef ATT
-  CTHIP_LAUNCH_CHECK();
-  return 0;
+  Kv4Attn a = {out, q, (const unsigned char *)k_pages, (const unsigned char *)v_pages, tables, lens, starts, q_stride, n_pages, table_stride, n_seqs, n_rows, H, Hkv};
+  a.tickets = (int *)workspace, a.parts = (float *)workspace + kSplitSlots;
+  return launch_kv4_attn<kAttnWhole>(__func__, a, Dh);
+}
+
+int64_t cthip_sdpa_shared_paged_q4_workspace(int n_rows, int H, int head_dim) {
+  if (!kv4_shape_ok(1, head_dim) || n_rows < 0 || H < 0) return fail(CTHIP_E_BAD_ARG, "cthip_sdpa_shared_paged_q4_workspace: %d rows of %d heads of %d (head sizes 32, 64, 128)", n_rows, H, head_dim);
+  return 4ll * (kSharedTickets + (int64_t)kSharedRecordRows * (head_dim + 2) + 2ll * n_rows * H);
+}
+
+int cthip_sdpa_shared_paged_q4(float *out, const float *q, int64_t q_stride, const void *k_pages, const void *v_pages, int n_pages, const int *tables, int table_stride,
+                               const int *lens, const int *starts, int n_seqs, int n_rows, const int *groups, const int *shared, int n_groups, int H, int Hkv, int Dh,
+                               void *workspace) {
+  CTHIP_REQUIRE_INIT();
+  CTHIP_ARG(n_seqs >= 0 && n_rows >= 0 && n_pages >= 0 && n_pages <= INT_MAX / kKvPageRows && table_stride > 0 && table_stride <= INT_MAX / kKvPageRows);
+  CTHIP_ARG(H > 0 && Hkv > 0 && H % Hkv == 0 && n_groups >= 0 && n_groups <= n_seqs);
+  if (const int rc = attn_unsupported(__func__, n_seqs, n_rows, H, Hkv, Dh)) return rc;
+  if (n_seqs == 0 || n_rows == 0) return 0;
+  CTHIP_ARG(out && q && out != q && tables && lens && starts && workspace && q_stride >= (int64_t)H * Dh && (n_groups == 0 || (groups && shared)));
+  CTHIP_ARG(n_pages == 0 || (k_pages && v_pages));
+  CTHIP_ARG((((uintptr_t)k_pages | (uintptr_t)v_pages | (uintptr_t)workspace) & 15) == 0);
+  Kv4Attn a = {out, q, (const unsigned char *)k_pages, (const unsigned char *)v_pages, tables, lens, starts, q_stride, n_pages, table_stride, n_seqs, n_rows, H, Hkv};
+  a.tickets = (int *)workspace, a.parts = (float *)workspace + kSharedTickets;
+  a.groups = groups, a.shared = shared, a.n_groups = n_groups;
+  a.stats = a.parts + (int64_t)kSharedRecordRows * (Dh + 2);
+  if (n_groups > 0)
+    if (const int rc = launch_kv4_attn<kAttnShared>(__func__, a, Dh)) return rc;
+  return launch_kv4_attn<kAttnBehind>(__func__, a, Dh);
 }
 
 }  // extern "C"

@@ -243,6 +243,31 @@ def rope(x, base=10000.0, start_pos=0):
     return out.numpy()
 
 
+_ROPE = {"pairs": _lib.ROPE_PAIRS, "halves": _lib.ROPE_HALVES}
+
+
+def rope_frequencies(rotary_dim: int, base: float = 10000.0, factor: float = 1.0, trained: int = 0, slow: float = 1.0, fast: float = 4.0) -> np.ndarray:
+    """The angles a position of each pair of channels (cthip_rope_frequencies), scaled by `factor`: all of them, or by parts where `trained` is given."""
+    out = np.empty(rotary_dim // 2, np.float64)
+    _lib.check(_lib.load().cthip_rope_frequencies(out.ctypes.data, rotary_dim, base, factor, trained, slow, fast))
+    return out
+
+
+def rope_rows(q, k, positions, frequencies, layout: str = "pairs", magnitude: float = 1.0):
+    """Query rows (n, heads, head_dim) and key rows (n, kv_heads, head_dim) turned by their own positions (cthip_rope_rows); rows at a
+    position below 0 come back as they are.  k may be None."""
+    q = np.ascontiguousarray(q, np.float32)
+    k = np.zeros((q.shape[0], 0, q.shape[-1]), np.float32) if k is None else np.ascontiguousarray(k, np.float32)
+    positions, frequencies = np.ascontiguousarray(positions, np.int32), np.ascontiguousarray(frequencies, np.float64)
+    if q.ndim != 3 or k.ndim != 3 or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2] or positions.shape != q.shape[:1] or frequencies.ndim != 1:
+        raise ValueError(f"rope_rows: queries {q.shape}, keys {k.shape}, positions {positions.shape}, frequencies {frequencies.shape}")
+    (n, heads, dh), code = q.shape, _ROPE[layout]
+    dq, dk, dp, df = (DeviceArray.from_numpy(a) for a in (q, k, positions, frequencies))
+    _lib.check(_lib.init().cthip_rope_rows(dq.ptr, heads * dh, dk.ptr, k.shape[1] * dh, dq.ptr, heads * dh, dk.ptr, k.shape[1] * dh, dp.ptr, n, heads, k.shape[1], dh, 2 * frequencies.size,
+                                           code, df.ptr, magnitude))
+    return dq.numpy(), dk.numpy()
+
+
 def sdpa_cached(q, k_cache, v_cache, start_pos: int):
     """q (S,H,Dh) at positions start_pos.., caches (max_len,Hkv,Dh) -> (S,H,Dh), causal."""
     q = np.ascontiguousarray(q, np.float32)
@@ -337,6 +362,55 @@ class PagedCacheQ4:
                                                    self.kv_heads, dh, self.workspace.ptr))
         return out.numpy()
 
+    def attend_shared(self, q, tables, lens, starts, groups, shared, layer: int = 0) -> np.ndarray:
+        """`attend` where sequences groups[g] .. groups[g + 1] have their first shared[g] rows, in whole pages, in common (cthip_sdpa_shared_paged_q4)."""
+        q = np.ascontiguousarray(q, np.float32)
+        n_rows, heads, dh = q.shape
+        if dh != self.head_dim:
+            raise ValueError(f"PagedCacheQ4.attend_shared: heads of {dh}, the cache's have {self.head_dim}")
+        tables, lens, starts, groups, shared = (np.ascontiguousarray(a, np.int32) for a in (tables, lens, starts, groups, shared))
+        if tables.ndim != 2 or tables.shape[0] != lens.size or starts.size != lens.size + 1 or groups.size != shared.size + 1:
+            raise ValueError(f"PagedCacheQ4.attend_shared: a table of shape {tables.shape}, {lens.size} lengths, {starts.size} starts, {groups.size} borders of {shared.size} groups")
+        lib = _lib.load()
+        size = int(lib.cthip_sdpa_shared_paged_q4_workspace(n_rows, heads, dh))
+        if size < 0:
+            _lib.check(size)
+        dq, dt, dl, ds, dg, dsh = (DeviceArray.from_numpy(a) for a in (q, tables, lens, starts, groups, shared))
+        out, ws = DeviceArray(q.shape, np.float32), DeviceArray((size,), np.uint8)
+        kp, vp = self._pools(layer)
+        _lib.check(lib.cthip_sdpa_shared_paged_q4(out.ptr, dq.ptr, heads * dh, kp, vp, self.n_pages, dt.ptr, tables.shape[1], dl.ptr, ds.ptr, lens.size, n_rows, dg.ptr, dsh.ptr, shared.size,
+                                                  heads, self.kv_heads, dh, ws.ptr))
+        return out.numpy()
+
+    def fork(self, tables, lens, parents, children, at, free_pages, n_free: Optional[int] = None) -> dict:
+        """Sequences children[f] become the first at[f] rows of sequences parents[f], in all layers (cthip_kv_fork_paged_q4)."""
+        tables, lens, parents, children, at, free_pages = (np.ascontiguousarray(a, np.int32) for a in (tables, lens, parents, children, at, free_pages))
+        if tables.ndim != 2 or tables.shape[0] != lens.size or parents.size != children.size or parents.size != at.size:
+            raise ValueError(f"PagedCacheQ4.fork: a table of shape {tables.shape}, {lens.size} lengths, {parents.size} parents, {children.size} children at {at.size} rows")
+        n_free = free_pages.size if n_free is None else int(n_free)
+        if not 0 <= n_free <= free_pages.size:
+            raise ValueError(f"PagedCacheQ4.fork: {n_free} free pages of a stack of {free_pages.size}")
+        dt, dl, dp, dc, da, df, dn = (DeviceArray.from_numpy(a) for a in (tables, lens, parents, children, at, free_pages, np.array([n_free], np.int32)))
+        refused = DeviceArray((parents.size,), np.int32)
+        _lib.check(_lib.load().cthip_kv_fork_paged_q4(dt.ptr, tables.shape[1], dl.ptr, lens.size, dn.ptr, refused.ptr, self.k.ptr, self.v.ptr, self.layers, self.n_pages, dp.ptr, dc.ptr, da.ptr,
+                                                      parents.size, df.ptr, dn.ptr, self.kv_heads, self.head_dim))
+        return dict(tables=dt.numpy(), lens=dl.numpy(), n_free=int(dn.numpy()[0]), refused=refused.numpy())
+
+    def compact(self, tables, lens) -> dict:
+        """The pages in use to the front of the pool, in all layers (cthip_kv_compact_paged_q4): the new tables, and the free stack."""
+        tables, lens = (np.ascontiguousarray(a, np.int32) for a in (tables, lens))
+        if tables.ndim != 2 or tables.shape[0] != lens.size:
+            raise ValueError(f"PagedCacheQ4.compact: {lens.size} lengths and a table of shape {tables.shape}")
+        lib = _lib.load()
+        size = int(lib.cthip_kv_compact_paged_q4_workspace(self.n_pages))
+        if size < 0:
+            _lib.check(size)
+        dt, dl, ws = DeviceArray.from_numpy(tables), DeviceArray.from_numpy(lens), DeviceArray((size,), np.uint8)
+        free, n = DeviceArray((self.n_pages,), np.int32), DeviceArray((1,), np.int32)
+        _lib.check(lib.cthip_kv_compact_paged_q4(dt.ptr, free.ptr, n.ptr, self.k.ptr, self.v.ptr, self.layers, self.n_pages, dt.ptr, tables.shape[1], dl.ptr, lens.size, self.kv_heads,
+                                                 self.head_dim, ws.ptr))
+        return dict(tables=dt.numpy(), free_pages=free.numpy()[:int(n.numpy()[0])])
+
     def reorder(self, tables, lens, parents, history=None, tokens=None, step: int = 0):
         """A beam search's reordering (cthip_beam_reorder_paged_q4) in all layers: `parents` (requests, beams), `lens` per
         request, `tables` (requests * beams, stride).  Returns the new tables, and the new history where one is given."""
@@ -375,3 +449,22 @@ def beam_select(logits, scores, finished=None, eos: int = -1) -> dict:
     best = DeviceArray((n, k), np.float32)
     _lib.check(_lib.load().cthip_beam_select(tokens.ptr, parents.ptr, best.ptr, done.ptr, dl.ptr, vocab, dsc.ptr, _p(df), n, k, vocab, eos, ws.ptr))
     return dict(tokens=tokens.numpy(), parents=parents.numpy(), scores=best.numpy(), finished=done.numpy())
+
+
+def draft_verify(target, draft, tokens, uniforms, starts, lens=None, positions=None) -> dict:
+    """Drafted tokens against the target's probabilities (cthip_draft_verify): target and draft (rows, vocab), tokens and uniforms (rows), the rows
+    of sequence i from starts[i] on.  draft may be None."""
+    target = np.ascontiguousarray(target, np.float32)
+    draft = None if draft is None else np.ascontiguousarray(draft, np.float32)
+    tokens, uniforms, starts = np.ascontiguousarray(tokens, np.int32), np.ascontiguousarray(uniforms, np.float32), np.ascontiguousarray(starts, np.int32)
+    if target.ndim != 2 or (draft is not None and draft.shape != target.shape) or tokens.shape != target.shape[:1] or uniforms.shape != tokens.shape or starts.size < 1:
+        raise ValueError(f"draft_verify: target {target.shape}, draft {None if draft is None else draft.shape}, tokens {tokens.shape}, uniforms {uniforms.shape}, {starts.size} starts")
+    n, (rows, vocab) = starts.size - 1, target.shape
+    if (lens is not None and np.size(lens) != n) or (positions is not None and np.size(positions) != rows):
+        raise ValueError(f"draft_verify: {n} sequences of {rows} rows, {np.size(lens)} lengths, {np.size(positions)} positions")
+    size = int(_lib.init().cthip_draft_verify_workspace(n))
+    dt, dk, du, ds, ws = (*(DeviceArray.from_numpy(a) for a in (target, tokens, uniforms, starts)), DeviceArray((size,), np.uint8))
+    dd, dl, dp = _dev(draft), _dev(lens, np.int32), _dev(positions, np.int32)
+    out, accepted = DeviceArray.from_numpy(np.full(rows, -1, np.int32)), DeviceArray((n,), np.int32)
+    _lib.check(_lib.load().cthip_draft_verify(out.ptr, accepted.ptr, _p(dl), dt.ptr, vocab, _p(dd), vocab, dk.ptr, du.ptr, ds.ptr, _p(dp), _p(dl), n, rows, vocab, ws.ptr))
+    return dict(tokens=out.numpy(), accepted=accepted.numpy(), lens=None if dl is None else dl.numpy())

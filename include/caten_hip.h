@@ -443,6 +443,69 @@ int cthip_beam_reorder_paged_q4(int *tables_out, int *history_out, void *k_pages
                                 const int *lens, const int *parents, int n_batch, int n_beams, int kv_heads, int head_dim, const int *history, int cols,
                                 const int *tokens, const int *step);
 
+/* ---- many answers to one prompt, drafted tokens ----
+ * What a server needs besides, over the same pool and the arrays of cthip_kv_plan_paged: rows turned by their positions between a layer's
+ * Linears and its append, sequences that go on from others, attention that reads what they share once, drafted tokens verified behind the last
+ * Linear, and the pool packed.  The reference has one sequence, decoded greedily (apps/gpt2/gpt2.lisp:97-113). */
+#define CTHIP_ROPE_PAIRS 0  /* channels 2i and 2i + 1 turn together (cthip_rope's layout) */
+#define CTHIP_ROPE_HALVES 1 /* channels i and i + rotary_dim / 2 */
+/* Rotary positions (nn/positional-encoding.lisp:3-64) of a step's rows: queries (n_rows, H, Dh) and keys (n_rows, Hkv, Dh), rows the strides apart
+ * in floats (slices of a fused product; outputs may be the inputs themselves, with the same stride, and may not overlap them otherwise).  Row r is
+ * at positions[r]; one below 0 is left as it was (the plan gives -1 to rows behind the last and to those of refused sequences).  The first rotary_dim
+ * channels of a head turn, pair i by position * frequencies[i], times magnitude; the others are copied.  H or Hkv may be 0.  frequencies: rotary_dim / 2 doubles on
+ * the device.  Angles are taken in 64 bits: sines and cosines are off by 2^-23 at any position.  At most 2^23 rows, 65535 heads of
+ * either kind and channels of a head; in the layout of pairs Dh is even. */
+int cthip_rope_rows(float *q_out, int64_t q_out_stride, float *k_out, int64_t k_out_stride, const float *q, int64_t q_stride, const float *k, int64_t k_stride,
+                    const int *positions, int n_rows, int H, int Hkv, int Dh, int rotary_dim, int layout, const double *frequencies, float magnitude);
+/* The table for it, in HOST memory: base^(-2i / rotary_dim), scaled for contexts longer than the trained one.  trained 0: all divided by `factor` (1 =
+ * none).  Otherwise by parts: a pair that makes at most `slow` turns over `trained` positions is divided by factor, one that makes `fast` or more is kept, those
+ * between are mixed in proportion to their turns.  (A larger base is the third way.)  Needs no device. */
+int cthip_rope_frequencies(double *frequencies, int rotary_dim, double base, double factor, int trained, double slow, double fast);
+/* Sequences that go on from others.  Fork f makes sequence children[f] the first at[f] rows of sequence parents[f]: its table row names the parent's full
+ * pages, a partly filled one is copied in all n_layers pools ((n_layers, n_pages, page bytes) each) into a page from the free stack (the plan's, taken
+ * from its end in the order of the forks; the array is not changed), lens[child] = at[f].  Entries of the child's row behind those, and tables and
+ * lengths of all others, stay.  Refused, with refused[f] = 1 (0 otherwise) and nothing changed: an index outside 0 .. n_seqs - 1, at[f] below 0 or above the parent's
+ * length or a table row, a child that an earlier fork names or that is anybody's parent in this call, too few pages (then every later fork that
+ * needs one as well).  n_free_out = what is left; may be n_free (one more launch).  What the child's row named before comes back by cthip_kv_free_paged.
+ * Rows below at[f] / 64 * 64 are both sequences' from now on: neither may be shortened below that and written again.  At most 4096 sequences and forks. */
+int cthip_kv_fork_paged_q4(int *tables, int table_stride, int *lens, int n_seqs, int *n_free_out, int *refused, void *k_pages, void *v_pages, int n_layers, int n_pages,
+                           const int *parents, const int *children, const int *at, int n_forks, const int *free_pages, const int *n_free, int kv_heads, int head_dim);
+/* The pages in use -- those that the first ceil(lens[i] / rows of a page) entries of a sequence's table name, all there are of this pool -- to the front of it: of u
+ * pages, those with ids from u on go, ids rising, to the free places below u, in all n_layers pools.  tables_out (may be tables): the new ids; entries
+ * outside the pool and behind a sequence's pages as they were.  free_pages (n_pages) = n_pages - 1 .. u falling, so that the plan takes the lowest first, then -1; n_free
+ * their number.  Pages from u on hold nothing any more: a pool can be cut there.  workspace: cthip_kv_compact_paged_q4_workspace(n_pages) = 64 + 8 n_pages bytes, 16-byte
+ * aligned, whatever they hold; calls that may overlap need one each.  At most 65535 sequences, 65534 layers. */
+int64_t cthip_kv_compact_paged_q4_workspace(int n_pages);
+int cthip_kv_compact_paged_q4(int *tables_out, int *free_pages, int *n_free, void *k_pages, void *v_pages, int n_layers, int n_pages, const int *tables, int table_stride,
+                              const int *lens, int n_seqs, int kv_heads, int head_dim, void *workspace);
+/* cthip_sdpa_paged_q4 where sequences have their first pages in common.  Group g is sequences groups[g] .. groups[g + 1] - 1; the first shared[g] / 64 (whole) pages of the
+ * table of its first sequence are all of its sequences', and are read once for all of their rows.  A row sees all of them, and of its own sequence's
+ * rows behind them those up to its own position; so with equal table entries, and no row's position in front of them, the result is that of
+ * cthip_sdpa_paged_q4 up to rounding.  lens count the shared rows.  groups (n_groups + 1) and starts rise; sequences in no group share nothing; groups and starts that
+ * fall, or leave their range, give undefined rows.  At most as many groups as sequences; otherwise arguments, precision, limits and what is left as it was are as
+ * there.  workspace: cthip_sdpa_shared_paged_q4_workspace(n_rows, H, Dh) = 4 * (4096 + 131072 * (Dh + 2) + 2 * n_rows * H) bytes, 16-byte aligned, its first 16384 zeroed
+ * once (cthip_alloc does); every call leaves it ready for the next, of any shape.  Calls that may overlap need one each. */
+int64_t cthip_sdpa_shared_paged_q4_workspace(int n_rows, int H, int Dh);
+int cthip_sdpa_shared_paged_q4(float *out, const float *q, int64_t q_stride, const void *k_pages, const void *v_pages, int n_pages, const int *tables, int table_stride,
+                               const int *lens, const int *starts, int n_seqs, int n_rows, const int *groups, const int *shared, int n_groups, int H, int Hkv, int Dh,
+                               void *workspace);
+/* Drafted tokens against the target's probabilities.  Rows starts[i] .. starts[i + 1] - 1 are sequence i's in this step: tokens[row] went in, of the first row the
+ * last token there was, of the others drafted ones.  Row r of target (n_rows, vocab; target_stride floats apart) holds the probabilities of the token behind r, row r
+ * of draft those that tokens[r + 1] was drawn from (NULL: that token was certain).  In order, the draft tokens[r + 1] stays where uniforms[r] * draft[r][it] <
+ * target[r][it].  Behind the last that stays one token is drawn: from max(target - draft, 0) of the row whose draft was rejected (from its target where that is nothing), or,
+ * where all stay, from the last row's target: the lowest token at which the running sum is above uniforms[last row] times the whole.  Products, differences and
+ * sums are taken in 64 bits; what is NaN or negative counts as 0, and a draft outside the vocabulary is rejected.  Random numbers lie in [0, 1); one that does not
+ * draws the last token with a weight.  Rows need not sum to 1 to be drawn from, but the comparison takes them as they are.
+ *   tokens_out (n_rows)  a sequence's drafts that stay, the drawn token (-1 where no token has a probability), -1 in its further rows
+ *   accepted (n_seqs)    drafts that stay
+ *   lens_out (n_seqs)    lens less the rejected drafts: what the cache holds then; may be lens, or NULL
+ * A sequence without rows, with rows outside 0 .. n_rows - 1 or, where positions (may be NULL) is given, refused by the plan (its first row's -1) keeps its length
+ * and accepts nothing; its rows, if they are inside, are -1.  Without drafts this draws a token a sequence.  At most 65535 sequences.
+ * workspace: cthip_draft_verify_workspace(n_seqs) = 2048 n_seqs bytes, 16-byte aligned, whatever they hold; calls that may overlap need one each. */
+int64_t cthip_draft_verify_workspace(int n_seqs);
+int cthip_draft_verify(int *tokens_out, int *accepted, int *lens_out, const float *target, int64_t target_stride, const float *draft, int64_t draft_stride, const int *tokens,
+                       const float *uniforms, const int *starts, const int *positions, const int *lens, int n_seqs, int n_rows, int vocab, void *workspace);
+
 /* ================================================================== */
 /* Decoder session: Transformer (external/llm/layers.lisp:73-90) and   */
 /* the gpt2-generate loop (apps/gpt2/gpt2.lisp:97-113)                 */

@@ -1,0 +1,266 @@
+"""Attention of a batch whose sequences share their first pages: against its definition in 64 bits, with the tolerance of attention over the 4-bit cache
+(derived in test_gpu_paged_q4.close; maxima and sums joined once more are two fp32 roundings, within what is left there)."""
+import numpy as np
+import pytest
+
+from tests.test_gpu_paged_q4 import PAGE, _fill, attention, close
+
+pytestmark = pytest.mark.gpu
+
+
+def answers(rng, groups, kv, dh, spare=3):
+    """groups: (rows shared, [(rows held in all, query rows)]); pages in any order, what no row was written to is NaN.
+    (cache, tables, lens, starts, borders, shared, [(k, v)])"""
+    from caten_amd import ops
+    seqs = [s for _, m in groups for s in m]
+    stride = max(1, max(-(-t // PAGE) for t, _ in seqs))
+    pages = list(rng.permutation(sum(p // PAGE + sum(-(-t // PAGE) for t, _ in m) for p, m in groups) + spare))
+    cache = ops.PagedCacheQ4(len(pages), kv, dh)
+    _fill(cache, 0xff)
+    tables, held, i = np.full((len(seqs), stride), -1, np.int32), [], 0
+
+    def rows(mine, first, n):
+        if n <= 0:
+            return np.zeros((0, kv, dh), np.float32), np.zeros((0, kv, dh), np.float32)
+        k = (rng.normal(0, 1, (n, kv, dh)) * np.exp(0.5 * rng.normal(0, 1, (1, kv, dh)))).astype(np.float32)
+        v = (rng.normal(0, 1, (n, kv, dh)) * np.exp(0.5 * rng.normal(0, 1, (1, kv, dh)))).astype(np.float32)
+        slots = np.array([mine[t // PAGE] * PAGE + t % PAGE for t in range(first, first + n)], np.int32)
+        cache.append(k, v, slots)
+        return cache.rows(slots)
+    for p, m in groups:
+        common = [pages.pop() for _ in range(p // PAGE)]
+        first = rows(common, 0, p // PAGE * PAGE)
+        for t, _ in m:
+            mine = common + [pages.pop() for _ in range(-(-t // PAGE) - p // PAGE)]
+            tables[i, :len(mine)] = mine
+            own = rows(mine, p // PAGE * PAGE, t - p // PAGE * PAGE)
+            held.append([np.concatenate([a, b]) for a, b in zip(first, own)])
+            i += 1
+    return (cache, tables, np.array([t for t, _ in seqs]), np.concatenate([[0], np.cumsum([r for _, r in seqs])]), np.concatenate([[0], np.cumsum([len(m) for _, m in groups])]),
+            np.array([p for p, _ in groups]), held)
+
+
+def seen(q, k, v, whole):
+    """`attention` of the last rows of a sequence whose first `whole` keys every row sees."""
+    n, at = len(q), len(k) - len(q)
+    if at + 1 >= whole:
+        return attention(q, k, v)
+    parts = [attention(q[r:r + 1], k[:max(at + r + 1, whole)], v[:max(at + r + 1, whole)]) for r in range(n)]
+    return tuple(np.concatenate(x) for x in zip(*parts))
+
+
+def compare(rng, H, kv, dh, groups, scale=1.0):
+    cache, tables, lens, starts, borders, shared, held = answers(rng, groups, kv, dh)
+    q = (scale * rng.normal(0, 1, (starts[-1], H, dh))).astype(np.float32)
+    got = cache.attend_shared(q, tables, lens, starts, borders, shared)
+    whole = np.concatenate([[p // PAGE * PAGE * (len(m) > 1)] * len(m) for p, m in groups]).astype(int)
+    for i, (k, v) in enumerate(held):
+        if starts[i + 1] > starts[i]:
+            close(got[starts[i]:starts[i + 1]], *seen(q[starts[i]:starts[i + 1]], k, v, whole[i]))
+    assert np.array_equal(got, cache.attend_shared(q, tables, lens, starts, borders, shared))  # two runs, the same bits
+    return cache, tables, lens, starts, borders, shared, held, q, got
+
+
+SHAPES = [(12, 12, 64), (32, 4, 64), (8, 1, 128), (4, 4, 128), (6, 2, 32), (16, 1, 32), (21, 3, 128), (17, 1, 64)]
+
+
+@pytest.mark.parametrize("H,kv,dh", SHAPES)
+@pytest.mark.parametrize("groups", [
+    [(64, [(65, 1), (66, 1)])],
+    [(200, [(201, 1), (264, 1), (330, 1), (193, 1), (500, 1)])],
+    [(128, [(140, 5), (129, 1), (300, 0), (200, 17)]), (63, [(70, 3), (64, 1)]), (64, [(90, 2)]), (320, [(321, 1)] * 9)],
+    [(1000, [(1001, 1)] * 20)]])
+def test_groups(H, kv, dh, groups):
+    print(f"case: {H} heads over {kv} of {dh}, groups {groups}", flush=True)
+    compare(np.random.default_rng(H + dh + len(groups)), H, kv, dh, groups)
+
+
+@pytest.mark.parametrize("H,kv,dh,groups", [
+    (32, 32, 128, [(1000, [(1001 + 3 * i, 1) for i in range(64)])]),
+    (64, 8, 128, [(700, [(800 + i, 5) for i in range(14)]), (320, [(330 + 60 * i, 4) for i in range(9)])]),
+    (64, 1, 128, [(192, [(193 + i, 3) for i in range(7)])]),
+    (8, 8, 64, [(450, [(460 + i, 1 + i % 40) for i in range(41)])]),
+    (4, 2, 32, [(256, [(300 + i, 33) for i in range(9)])]),
+    (6, 3, 128, [(128, [(128 + 200, 200), (128 + 150, 150)])])])
+def test_many_rows(H, kv, dh, groups):
+    print(f"case: many rows, {H} heads over {kv} of {dh}, {len(groups)} groups", flush=True)
+    compare(np.random.default_rng(H + dh), H, kv, dh, groups)
+
+
+@pytest.mark.parametrize("H,kv,dh,members", [(4, 1, 64, 3), (8, 8, 128, 40), (16, 1, 128, 9)])
+def test_a_long_prefix(H, kv, dh, members):
+    compare(np.random.default_rng(members), H, kv, dh, [(20000, [(20001 + i, 1) for i in range(members)])])
+
+
+def test_many_groups():
+    rng = np.random.default_rng(12)
+    compare(rng, 4, 2, 64, [(64 * (i % 3), [(64 * (i % 3) + 1 + (i * 37 + j) % 100, (i + j) % 3) for j in range(i % 4 + 1)]) for i in range(150)])
+
+
+def test_the_same_as_without_sharing():
+    """Against the attention that reads every sequence's pages by itself: both are within the tolerance of the same numbers.  A batch without groups, or with groups that share
+    nothing or have one sequence, is the same bits."""
+    rng = np.random.default_rng(13)
+    cache, tables, lens, starts, borders, shared, held, q, got = compare(rng, 12, 4, 64, [(300, [(310, 2), (305, 1), (400, 7)]), (90, [(95, 1)])])
+    plain = cache.attend(q, tables, lens, starts)
+    for i, (k, v) in enumerate(held):
+        _, size, big = attention(q[starts[i]:starts[i + 1]], k, v)
+        close(got[starts[i]:starts[i + 1]], plain[starts[i]:starts[i + 1]], 2 * size, 2 * big)
+    for b, s in (([0], []), ([0, 3, 4], [0, 0]), ([0, 3, 4], [63, 64]), ([0, 0, 0, 1, 1], [640] * 4), ([2, 3], [300]), ([0, 3], [-5])):
+        assert np.array_equal(cache.attend_shared(q, tables, lens, starts, b, s), plain), (b, s)
+    # some sequences in front of the groups and behind them
+    for b, s in (([1, 3], [300]), ([0, 2], [300]), ([0, 1, 3, 4], [300, 256, 90])):
+        part = cache.attend_shared(q, tables, lens, starts, b, s)
+        for i, (k, v) in enumerate(held):
+            close(part[starts[i]:starts[i + 1]], *attention(q[starts[i]:starts[i + 1]], k, v))
+
+
+def test_rows_in_front_of_what_is_shared():
+    """A row sees all of its group's shared pages, whatever its position, and of what is behind them what its own position reaches."""
+    rng = np.random.default_rng(14)
+    H, kv, dh = 6, 2, 64
+    cache, tables, lens, starts, borders, shared, held = answers(rng, [(128, [(200, 1), (150, 1), (140, 3)])], kv, dh)
+    q = rng.normal(0, 1, (5, H, dh)).astype(np.float32)
+    short = np.array([200, 100, 130])  # the second ends inside the shared pages, the third's first rows lie in them
+    got = cache.attend_shared(q, tables, short, starts, borders, shared)
+    for row, (i, t) in enumerate([(0, 200), (1, 128), (2, 128), (2, 129), (2, 130)]):
+        k, v = (x[:t] for x in held[i])
+        close(got[row:row + 1], *attention(q[row:row + 1], k, v))
+
+
+def test_pages_outside_the_pool():
+    """Shared pages that are nowhere hold no key; where a sequence has none besides either, its rows are zero; a table's end."""
+    rng = np.random.default_rng(15)
+    H, kv, dh = 8, 2, 64
+    cache, tables, lens, starts, borders, shared, held = answers(rng, [(192, [(193, 1), (200, 2), (192, 1)])], kv, dh)
+    q = rng.normal(0, 1, (4, H, dh)).astype(np.float32)
+    gone = tables.copy()
+    gone[0, 1] = -1
+    got = cache.attend_shared(q, gone, lens, starts, borders, shared)
+    for row, (i, t) in enumerate([(0, 193), (1, 199), (1, 200), (2, 192)]):
+        k, v = (np.concatenate([x[:64], x[128:t]]) for x in held[i])
+        close(got[row:row + 1], *attention(q[row:row + 1], k, v))
+    gone[0, :3] = cache.n_pages, -1, 2 ** 31 - 1
+    got = cache.attend_shared(q, gone, lens, starts, borders, shared)
+    for row, (i, t) in enumerate([(0, 193), (1, 199), (1, 200)]):
+        k, v = (x[192:t] for x in held[i])
+        close(got[row:row + 1], *attention(q[row:row + 1], k, v))
+    assert not got[3].any()
+    got = cache.attend_shared(q, tables[:, :2], lens, starts, borders, [10 ** 6])  # a table of two pages
+    for row, i in enumerate([0, 1, 1, 2]):
+        k, v = (x[:128] for x in held[i])
+        close(got[row:row + 1], *attention(q[row:row + 1], k, v))
+
+
+@pytest.mark.parametrize("rows", [1, 20])
+@pytest.mark.parametrize("factors", [(1e-6, 1), (1, 1e-6), (30, 1), (1e5, 1), (1, 1e5), (1e3, 1e-3), (0, 1), (1, 0)])
+def test_sizes_of_values(rows, factors):
+    """Values of the shared pages and of the others of different sizes (a power of two goes with each part's sums)."""
+    rng = np.random.default_rng(rows)
+    H, kv, dh = 8, 2, 64
+    cache, tables, lens, starts, borders, shared, held = answers(rng, [(192, [(220, rows), (300, rows), (193, 1)])], kv, dh)
+    for i in range(3):
+        for first, n, factor in ((0, 192, factors[0]), (192, lens[i] - 192, factors[1])):
+            slots = np.array([tables[i, t // PAGE] * PAGE + t % PAGE for t in range(first, first + n)], np.int32)
+            k, v = (x[first:first + n] for x in held[i])
+            if first or i == 0:
+                cache.append(k, np.float32(factor) * v, slots)
+            got = cache.rows(slots)
+            held[i][0][first:first + n], held[i][1][first:first + n] = got
+    q = rng.normal(0, 1, (starts[-1], H, dh)).astype(np.float32)
+    got = cache.attend_shared(q, tables, lens, starts, borders, shared)
+    for i, (k, v) in enumerate(held):
+        close(got[starts[i]:starts[i + 1]], *attention(q[starts[i]:starts[i + 1]], k, v))
+
+
+@pytest.mark.parametrize("scale", [1e-30, 30.0, 3e3, 1e6])
+def test_sizes_of_queries(scale):
+    compare(np.random.default_rng(16), 8, 2, 64, [(256, [(270, 1), (300, 3), (257, 1)])], scale)
+
+
+def test_infinities_and_nan():
+    """A query row that is not finite is NaN and its neighbours are not; a key that is not, in the shared pages, is everybody's; behind them, its sequence's."""
+    rng = np.random.default_rng(17)
+    H, kv, dh = 4, 2, 64
+    cache, tables, lens, starts, borders, shared, held, q, want = compare(rng, H, kv, dh, [(128, [(140, 1), (150, 2), (129, 1)])])
+    for bad in (np.nan, np.inf, -np.inf):
+        x = q.copy()
+        x[1, 2, 5] = bad
+        got = cache.attend_shared(x, tables, lens, starts, borders, shared)
+        assert np.isnan(got[1, 2]).all()
+        keep = np.ones((4, H), bool)
+        keep[1, 2] = False
+        assert np.array_equal(got[keep], want[keep])
+    one = np.zeros((1, kv, dh), np.float32)
+    one[0, 0, 3] = np.nan
+    cache.append(one, one, np.array([tables[2, 2] * PAGE], np.int32))  # the last sequence's own row
+    got = cache.attend_shared(q, tables, lens, starts, borders, shared)
+    assert np.array_equal(got[:3], want[:3]) and np.isnan(got[3, :2]).any() and np.isfinite(got[3, 2:]).all()
+    cache.append(one, one, np.array([tables[0, 0] * PAGE + 9], np.int32))
+    got = cache.attend_shared(q, tables, lens, starts, borders, shared)
+    assert np.isnan(got[:, :2]).any(-1).all() and np.isfinite(got[:, 2:]).all()
+
+
+def test_rows_behind_the_last_and_a_workspace_of_other_shapes():
+    """Rows behind the last sequence's stay; one workspace goes from shape to shape."""
+    from caten_amd import _lib, ops
+    lib, rng = _lib.init(), np.random.default_rng(18)
+    ws = ops.DeviceArray((int(lib.cthip_sdpa_shared_paged_q4_workspace(200, 64, 128)),), np.uint8)
+    for H, kv, dh, groups in ((64, 8, 128, [(400, [(500 + i, 3) for i in range(20)])]), (12, 12, 64, [(900, [(901 + i, 1) for i in range(8)])]), (6, 2, 32, [(64, [(65, 1), (700, 30)])]),
+                              (64, 8, 128, [(5000, [(5001 + i, 1) for i in range(3)])]), (16, 1, 64, [(128, [(129, 2)] * 60)])):
+        cache, tables, lens, starts, borders, shared, held = answers(rng, groups, kv, dh)
+        n = int(starts[-1])
+        q = rng.normal(0, 1, (n + 5, H, dh)).astype(np.float32)
+        dq, dt, dl, ds, dg, dsh = (ops.DeviceArray.from_numpy(np.ascontiguousarray(a, t)) for a, t in ((q, np.float32), (tables, np.int32), (lens, np.int32), (starts, np.int32), (borders, np.int32),
+                                                                                                        (shared, np.int32)))
+        out = ops.DeviceArray.from_numpy(np.full(q.shape, 7.0, np.float32))
+        for _ in range(2):
+            _lib.check(lib.cthip_sdpa_shared_paged_q4(out.ptr, dq.ptr, H * dh, cache.k.ptr, cache.v.ptr, cache.n_pages, dt.ptr, tables.shape[1], dl.ptr, ds.ptr, len(lens), n + 5, dg.ptr, dsh.ptr,
+                                                      len(shared), H, kv, dh, ws.ptr))
+            got = out.numpy()
+            assert (got[n:] == 7.0).all()
+            for i, (k, v) in enumerate(held):
+                close(got[starts[i]:starts[i + 1]], *attention(q[starts[i]:starts[i + 1]], k, v))
+        assert not ws.numpy()[:16384].any()
+
+
+def test_places_past_32_bits():
+    """Shared pages at the end of a pool of more than 2^32 bytes."""
+    from caten_amd import ops
+    rng = np.random.default_rng(19)
+    kv, dh, n_pages, H = 32, 128, 30000, 32
+    cache = ops.PagedCacheQ4(n_pages, kv, dh)
+    tables = np.array([[n_pages - 1, n_pages - 2, 3], [n_pages - 1, n_pages - 2, n_pages - 3], [n_pages - 1, n_pages - 2, n_pages - 4]], np.int32)
+    lens, held = [130, 150, 192], []
+    for i, t in enumerate(lens):
+        slots = np.array([tables[i, j // PAGE] * PAGE + j % PAGE for j in range(t)], np.int32)
+        new = slots if i == 0 else slots[128:]
+        cache.append(*(rng.normal(0, 1, (len(new), kv, dh)).astype(np.float32) for _ in range(2)), new)
+        held.append(cache.rows(slots))
+    q = rng.normal(0, 1, (3, H, dh)).astype(np.float32)
+    got = cache.attend_shared(q, tables, lens, [0, 1, 2, 3], [0, 3], [128])
+    for i, (k, v) in enumerate(held):
+        close(got[i:i + 1], *attention(q[i:i + 1], k, v))
+
+
+def test_refusals():
+    from caten_amd import _lib, ops
+    lib, d = _lib.init(), ops.DeviceArray((1 << 16,), np.uint8)
+    p = d.ptr
+
+    def call(**k):
+        a = dict(out=p, q=p + 4096, qs=128, kp=p + 8192, vp=p + 8192 + 2304, pages=1, t=p + 16384, stride=4, lens=p + 17408, starts=p + 18432, n=2, rows=2, groups=p + 19456, shared=p + 20480, g=1, H=2,
+                 kv=1, dh=64, ws=p + 32768)
+        a.update(k)
+        return lib.cthip_sdpa_shared_paged_q4(*a.values())
+
+    for bad in (dict(n=-1), dict(rows=-1), dict(pages=-1), dict(stride=0), dict(H=0), dict(kv=0), dict(H=3, kv=2, qs=300), dict(g=-1), dict(g=3), dict(groups=None), dict(shared=None), dict(out=None),
+                dict(q=None), dict(q=p), dict(t=None), dict(lens=None), dict(starts=None), dict(ws=None), dict(ws=p + 32772), dict(kp=None), dict(vp=p + 8200), dict(qs=127)):
+        assert call(**bad) == _lib.E_BAD_ARG, bad
+    for bad in (dict(dh=48), dict(H=65536, qs=1 << 30), dict(n=4097), dict(rows=(1 << 20) + 1)):
+        assert call(**bad) == _lib.E_UNSUPPORTED, bad
+    assert call(n=0, g=0, q=None) == 0 and call(rows=0, q=None) == 0
+    cache = ops.PagedCacheQ4(2, 1, 64)
+    for groups, shared, dh in (([0, 1], [64, 64], 64), ([0, 1], [64], 32)):
+        with pytest.raises(ValueError):
+            cache.attend_shared(np.zeros((1, 2, dh)), np.zeros((1, 1)), [1], [0, 1], groups, shared)
