@@ -17,7 +17,8 @@ namespace cthip {
 
 constexpr int kDraftThreads = 256, kDraftSlices = 64;
 constexpr int kDraftWorkspace = 2048;  // bytes a sequence
-static_assert(16 * kDraftSlices <= kDraftWorkspace, "the sums of a sequence's slices");
+constexpr int kDraftEach = 8;          // tokens that a thread looks at side by side, at most
+static_assert(16 * kDraftSlices + 4 <= kDraftWorkspace, "the sums of a sequence's slices");
 
 struct DraftArgs {
   int *tokens_out, *accepted, *lens_out;
@@ -27,7 +28,10 @@ struct DraftArgs {
   const float *uniforms;
   const int *starts, *positions, *lens;
   int n_rows, vocab, slices, slice;
-  double *sums;  // (sequence, 128): of each slice the weights', of each slice the target's
+  unsigned char *workspace;
+  // of a sequence: of each slice the weights' sum, of each slice the target's; and its drafts that stay, -1 where it sits out
+  __device__ __forceinline__ double *sums(int seq) const { return (double *)(workspace + (int64_t)seq * kDraftWorkspace); }
+  __device__ __forceinline__ int *stays(int seq) const { return (int *)(sums(seq) + 2 * kDraftSlices); }
 };
 
 __device__ __forceinline__ double draft_wave_sum(double v) {
@@ -74,11 +78,11 @@ struct Verified {
 struct DraftRow {
   const float *p, *q;
   int taken;  // the rejected draft, where there are no probabilities of the draft's: the whole of them was its
-  __device__ __forceinline__ DraftRow(const DraftArgs &a, const Verified &v) {
-    p = a.target + (int64_t)(v.row0 + v.stay) * a.target_stride;
-    const bool rejected = v.stay < v.rows - 1;
-    q = rejected && a.draft ? a.draft + (int64_t)(v.row0 + v.stay) * a.draft_stride : nullptr;
-    taken = rejected && !a.draft ? a.tokens[v.row0 + v.stay + 1] : -1;
+  __device__ __forceinline__ DraftRow(const DraftArgs &a, int row0, int rows, int stay) {
+    p = a.target + (int64_t)(row0 + stay) * a.target_stride;
+    const bool rejected = stay < rows - 1;
+    q = rejected && a.draft ? a.draft + (int64_t)(row0 + stay) * a.draft_stride : nullptr;
+    taken = rejected && !a.draft ? a.tokens[row0 + stay + 1] : -1;
   }
   __device__ __forceinline__ void at(int t, double &w, double &own) const {
     const float x = p[t];
@@ -92,8 +96,9 @@ __global__ __launch_bounds__(kDraftThreads) void k_draft_slice(DraftArgs a) {
   __shared__ double part[2][kDraftThreads / 64];
   const int seq = blockIdx.y, tid = threadIdx.x;
   const Verified v(a, seq);
+  if (blockIdx.x == 0 && tid == 0) a.stays(seq)[0] = v.there ? v.stay : -1;
   if (!v.there) return;
-  const DraftRow row(a, v);
+  const DraftRow row(a, v.row0, v.rows, v.stay);
   double w = 0.0, own = 0.0;
   const int t1 = min(a.vocab, ((int)blockIdx.x + 1) * a.slice);
   for (int t = blockIdx.x * a.slice + tid; t < t1; t += kDraftThreads) {
@@ -104,12 +109,13 @@ __global__ __launch_bounds__(kDraftThreads) void k_draft_slice(DraftArgs a) {
   w = draft_wave_sum(w), own = draft_wave_sum(own);
   if ((tid & 63) == 0) part[0][tid >> 6] = w, part[1][tid >> 6] = own;
   __syncthreads();
-  if (tid < 2) a.sums[(int64_t)seq * (2 * kDraftSlices) + kDraftSlices * tid + blockIdx.x] = (part[tid][0] + part[tid][1]) + (part[tid][2] + part[tid][3]);
+  if (tid < 2) a.sums(seq)[kDraftSlices * tid + blockIdx.x] = (part[tid][0] + part[tid][1]) + (part[tid][2] + part[tid][3]);
 }
 
 // inclusive, over a wavefront
 __device__ __forceinline__ double draft_wave_scan(double v) {
   const int lane = threadIdx.x & 63;
+#pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
     const double y = __shfl_up(v, o, 64);
     if (lane >= o) v += y;
@@ -119,67 +125,84 @@ __device__ __forceinline__ double draft_wave_scan(double v) {
 
 __global__ __launch_bounds__(kDraftThreads) void k_draft_token(DraftArgs a) {
   __shared__ double part[2][kDraftThreads / 64];
-  __shared__ int s_found[2], s_last[2];
+  __shared__ int s_found[2], s_last;
   const int seq = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
-  const Verified v(a, seq);
-  int token = -1;
-  if (v.there) {
-    const DraftRow row(a, v);
-    const double *sums = a.sums + (int64_t)seq * (2 * kDraftSlices);
-    double mine = lane < a.slices ? sums[lane] : 0.0;
-    double upto = draft_wave_scan(mine), total = __shfl(upto, 63, 64);
-    const bool own = !(total > 0.0);  // nothing is left of the target behind the draft's: by roundings alone, then its own
-    if (own) {
-      mine = lane < a.slices ? sums[kDraftSlices + lane] : 0.0;
-      upto = draft_wave_scan(mine), total = __shfl(upto, 63, 64);
-    }
-    if (total > 0.0) {
-      const double goal = (double)a.uniforms[v.row0 + v.rows - 1] * total;
-      // the first slice that reaches past the goal, or the last that weighs anything
-      const unsigned long long past = __ballot(upto > goal && mine > 0.0), any = __ballot(mine > 0.0);
-      const int s = past ? (int)__builtin_ctzll(past) : 63 - (int)__builtin_clzll(any);
-      double before = s > 0 ? __shfl(upto, s - 1, 64) : 0.0;
-      const int t1 = min(a.vocab, (s + 1) * a.slice);
-      if (tid < 2) s_last[tid] = -1;
-      int last = -1;
-      for (int t0 = s * a.slice, round = 0; t0 < t1; t0 += kDraftThreads, round ^= 1) {
-        const int t = t0 + tid;
-        double w = 0.0, o = 0.0;
-        if (t < t1) row.at(t, w, o);
-        if (own) w = o;
-        const double sum = draft_wave_scan(w);
-        if (lane == 63) part[round][wv] = sum;
-        if (tid == 0) s_found[round] = INT_MAX;
-        __syncthreads();
-        double front = before;
-        for (int k = 0; k < kDraftThreads / 64; k++) {
-          if (k < wv) front += part[round][k];
-          before += part[round][k];
-        }
-        if (w > 0.0) {
-          last = t;
-          if (front + sum > goal) atomicMin(&s_found[round], t);
-        }
-        __syncthreads();
-        if (s_found[round] != INT_MAX) {
-          token = s_found[round];
-          break;
-        }
-      }
-      if (token < 0) {  // (sums of other orders, or a number that is not below one)
-        if (last >= 0) atomicMax(&s_last[0], last);
-        __syncthreads();
-        token = s_last[0];
-      }
-    }
-    for (int j = tid; j < v.rows; j += kDraftThreads) a.tokens_out[v.row0 + j] = j < v.stay ? a.tokens[v.row0 + j + 1] : j == v.stay ? token : -1;
-  } else if (v.row0 >= 0 && v.rows > 0 && v.row0 + v.rows <= a.n_rows) {
-    for (int j = tid; j < v.rows; j += kDraftThreads) a.tokens_out[v.row0 + j] = -1;
-  }
+  // (all of these at once)
+  const int row0 = a.starts[seq], rows = a.starts[seq + 1] - row0, stay = a.stays(seq)[0];
+  const double *sums = a.sums(seq);
+  const double left = lane < a.slices ? sums[lane] : 0.0, all = lane < a.slices ? sums[kDraftSlices + lane] : 0.0;
   if (tid == 0) {
-    a.accepted[seq] = v.there ? v.stay : 0;
-    if (a.lens_out) a.lens_out[seq] = a.lens[seq] - (v.there ? v.rows - 1 - v.stay : 0);
+    a.accepted[seq] = max(stay, 0);
+    if (a.lens_out) a.lens_out[seq] = a.lens[seq] - (stay >= 0 ? rows - 1 - stay : 0);
   }
+  if (stay < 0) {
+    if (row0 >= 0 && rows > 0 && row0 + rows <= a.n_rows)
+      for (int j = tid; j < rows; j += kDraftThreads) a.tokens_out[row0 + j] = -1;
+    return;
+  }
+  const float u = a.uniforms[row0 + rows - 1];
+  const DraftRow row(a, row0, rows, stay);
+  int token = -1;
+  double mine = left, upto = draft_wave_scan(left), total = __shfl(upto, 63, 64);
+  const bool own = !(total > 0.0);  // nothing is left of the target behind the draft's: by roundings alone, then its own
+  if (own) mine = all, upto = draft_wave_scan(all), total = __shfl(upto, 63, 64);
+  if (total > 0.0) {
+    const double goal = (double)u * total;
+    // the first slice that reaches past the goal, or the last that weighs anything
+    const unsigned long long past = __ballot(upto > goal && mine > 0.0), any = __ballot(mine > 0.0);
+    const int s = past ? (int)__builtin_ctzll(past) : 63 - (int)__builtin_clzll(any);
+    double before = s > 0 ? __shfl(upto, s - 1, 64) : 0.0;
+    const int t1 = min(a.vocab, (s + 1) * a.slice);
+    if (tid == 0) s_last = -1;
+    int last = -1;
+    // a thread's tokens lie side by side: their sums, over the workgroup, and then the one among them
+    for (int t0 = s * a.slice, round = 0; t0 < t1; t0 += kDraftEach * kDraftThreads, round ^= 1) {
+      const int each = min(kDraftEach, (t1 - t0 + kDraftThreads - 1) / kDraftThreads), t = t0 + tid * each, end = min(t + each, t1);
+      double w[kDraftEach], sum = 0.0;
+#pragma unroll
+      for (int e = 0; e < kDraftEach; e++) {
+        double o = 0.0;
+        w[e] = 0.0;
+        if (t + e < end) row.at(t + e, w[e], o);
+        if (own) w[e] = o;
+      }
+#pragma unroll
+      for (int e = 0; e < kDraftEach; e++) sum += w[e];
+      const double scan = draft_wave_scan(sum);
+      if (lane == 63) part[round][wv] = scan;
+      if (tid == 0) s_found[round] = INT_MAX;
+      __syncthreads();
+      double front = before + scan - sum;
+#pragma unroll
+      for (int k = 0; k < kDraftThreads / 64; k++) {
+        if (k < wv) front += part[round][k];
+        before += part[round][k];
+      }
+      if (sum > 0.0) {
+        int found = INT_MAX;
+#pragma unroll
+        for (int e = 0; e < kDraftEach; e++) {
+          front += w[e];
+          if (w[e] > 0.0) {
+            last = t + e;
+            if (found == INT_MAX && front > goal) found = t + e;
+          }
+        }
+        if (found != INT_MAX) atomicMin(&s_found[round], found);
+      }
+      __syncthreads();
+      if (s_found[round] != INT_MAX) {
+        token = s_found[round];
+        break;
+      }
+    }
+    if (token < 0) {  // (sums of other orders, or a number that is not below one)
+      if (last >= 0) atomicMax(&s_last, last);
+      __syncthreads();
+      token = s_last;
+    }
+  }
+  for (int j = tid; j < rows; j += kDraftThreads) a.tokens_out[row0 + j] = j < stay ? a.tokens[row0 + j + 1] : j == stay ? token : -1;
 }
 
 }  // namespace cthip
@@ -203,7 +226,7 @@ int cthip_draft_verify(int *tokens_out, int *accepted, int *lens_out, const floa
   CTHIP_ARG(n_rows == 0 || (tokens_out && target && tokens && uniforms && tokens_out != tokens));
   const int slices = std::min(kDraftSlices, (vocab + 1023) / 1024), slice = (vocab + slices - 1) / slices;
   const DraftArgs a = {tokens_out, accepted, lens_out, target, draft, target_stride, draft_stride, tokens, uniforms, starts, positions, lens, n_rows, vocab, (vocab + slice - 1) / slice, slice,
-                       (double *)workspace};
+                       (unsigned char *)workspace};
   hipLaunchKernelGGL(k_draft_slice, dim3((unsigned)a.slices, (unsigned)n_seqs), dim3(kDraftThreads), 0, state().stream, a);
   CTHIP_LAUNCH_CHECK();
   hipLaunchKernelGGL(k_draft_token, dim3((unsigned)n_seqs), dim3(kDraftThreads), 0, state().stream, a);

@@ -99,6 +99,7 @@ __global__ __launch_bounds__(256) void k_kv_fork(ForkArgs a) {
 // read is not what is written, and a call repeated on the same tables writes the same bytes.  map: in use (1) or not, then where each page
 // goes; moves: (from, to).
 constexpr int kPackThreads = 1024;
+constexpr int kBitPages = 1 << 17;  // pages that there are bits for in LDS
 __global__ __launch_bounds__(256) void k_kv_compact_clear(int *map, int n_pages) {
   for (int64_t i = blockIdx.x * 256 + threadIdx.x; i < n_pages; i += (int64_t)gridDim.x * 256) map[i] = 0;
 }
@@ -130,17 +131,38 @@ __device__ __forceinline__ int2 pack_scan(int2 v, int2 (*part)[kPackThreads / 64
   }
   return {before.x + s.x - v.x, before.y + s.y - v.y};
 }
-__global__ __launch_bounds__(kPackThreads) void k_kv_compact_plan(int *map, int2 *moves, int *n_moves, int *free_pages, int *n_free, int n_pages) {
+// MARK: the pages in use are found here too, as bits in LDS.  Otherwise another launch has marked them in map, where a bit for each would not fit.
+template <bool MARK>
+__global__ __launch_bounds__(kPackThreads) void k_kv_compact_plan(int *map, int2 *moves, int *n_moves, int *free_pages, int *n_free, int n_pages, const int *__restrict__ tables,
+                                                                  int table_stride, const int *__restrict__ lens, int n_seqs) {
   __shared__ int2 part[kPackThreads / 64];
+  __shared__ unsigned s_bits[MARK ? kBitPages / 32 : 1];
   const int tid = threadIdx.x;
+  if (MARK) {
+    for (int i = tid; i < (n_pages + 31) / 32; i += kPackThreads) s_bits[i] = 0;
+    __syncthreads();
+    // a wavefront a sequence
+    for (int i = tid >> 6; n_pages > 0 && i < n_seqs; i += kPackThreads / 64) {
+      const int pages = pages_of(lens[i], table_stride);
+      for (int c = tid & 63; c < pages; c += 64) {
+        const int id = tables[(int64_t)i * table_stride + c];
+        if (id >= 0 && id < n_pages) atomicOr(&s_bits[id >> 5], 1u << (id & 31));
+      }
+    }
+    __syncthreads();
+  }
+  auto in_use = [&](int i) { return MARK ? (int)(s_bits[i >> 5] >> (i & 31) & 1u) : map[i]; };
   int used = 0;
-  for (int i = tid; i < n_pages; i += kPackThreads) used += map[i];
+  if (MARK)
+    for (int i = tid; i < (n_pages + 31) / 32; i += kPackThreads) used += __popc(s_bits[i]);
+  else
+    for (int i = tid; i < n_pages; i += kPackThreads) used += map[i];
   int2 total;
   pack_scan({used, 0}, &part, total);
   used = total.x;
   int2 done = {0, 0};
   for (int i0 = 0; i0 < n_pages; i0 += kPackThreads) {
-    const int i = i0 + tid, there = i < n_pages ? map[i] : 0;
+    const int i = i0 + tid, there = i < n_pages ? in_use(i) : 0;
     const int2 mine = {i >= used && there, i < used && !there};
     const int2 at = pack_scan(mine, &part, total);
     if (mine.x) moves[done.x + at.x].x = i;
@@ -233,15 +255,17 @@ int cthip_kv_compact_paged_q4(int *tables_out, int *free_pages, int *n_free, voi
   CTHIP_ARG(n_layers == 0 || n_pages == 0 || (k_pages && v_pages && pools_ok(k_pages, v_pages)));
   int *n_moves = (int *)workspace, *map = n_moves + 16;
   int2 *moves = (int2 *)(map + n_pages + (n_pages & 1));  // (half of the pages at most)
-  if (n_pages > 0) {
+  // Up to 2^17 pages, and as many table entries as one workgroup reads in the time of the two launches that it saves
+  const bool mark = n_pages == 0 || (n_pages <= kBitPages && (int64_t)n_seqs * table_stride <= (1 << 14));
+  if (mark) {
+    hipLaunchKernelGGL(k_kv_compact_plan<true>, dim3(1), dim3(kPackThreads), 0, state().stream, map, moves, n_moves, free_pages, n_free, n_pages, tables, table_stride, lens, n_seqs);
+  } else {
     hipLaunchKernelGGL(k_kv_compact_clear, dim3((unsigned)std::min(1024, (n_pages + 255) / 256)), dim3(256), 0, state().stream, map, n_pages);
     CTHIP_LAUNCH_CHECK();
-  }
-  if (n_pages > 0 && n_seqs > 0) {
-    hipLaunchKernelGGL(k_kv_compact_mark, dim3((unsigned)n_seqs), dim3(256), 0, state().stream, map, tables, table_stride, lens, n_pages);
+    if (n_seqs > 0) hipLaunchKernelGGL(k_kv_compact_mark, dim3((unsigned)n_seqs), dim3(256), 0, state().stream, map, tables, table_stride, lens, n_pages);
     CTHIP_LAUNCH_CHECK();
+    hipLaunchKernelGGL(k_kv_compact_plan<false>, dim3(1), dim3(kPackThreads), 0, state().stream, map, moves, n_moves, free_pages, n_free, n_pages, nullptr, 0, nullptr, 0);
   }
-  hipLaunchKernelGGL(k_kv_compact_plan, dim3(1), dim3(kPackThreads), 0, state().stream, map, moves, n_moves, free_pages, n_free, n_pages);
   CTHIP_LAUNCH_CHECK();
   const MoveArgs a = {tables_out, (unsigned char *)k_pages, (unsigned char *)v_pages, tables, lens, map, n_moves, moves, table_stride, n_seqs, n_layers, n_pages,
                       kv_heads * kv4_head_bytes(head_dim)};
