@@ -35,10 +35,13 @@ struct Kv4Attn {
   // sequences that share their first pages
   const int *groups, *shared;
   int n_groups;
-  float *stats;    // of a (row, head): maximum and sum over the shared pages; the outputs over them lie in `out`, unnormalised
+  float *stats;    // of a (row, head), what the launch over the shared pages has left: maximum and sum, the outputs lying in `out` unnormalised; or whose shares they are
+  float *slots;    // of the shares of shared pages
 };
-// What a launch is: a batch by itself; the pages that a group's sequences share, for all of its rows; what the sequences have behind those
-enum { kAttnWhole = 0, kAttnShared = 1, kAttnBehind = 2 };
+// What a launch is: a batch by itself; the pages that a group's sequences share, for all of its rows; what the sequences have behind those, a
+// job taken by workgroups as in the others, or by wavefronts, each with parts of its own
+enum { kAttnWhole = 0, kAttnShared = 1, kAttnBehind = 2, kAttnBehindWaves = 3 };
+constexpr bool attn_behind(int mode) { return mode >= kAttnBehind; }
 
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef _Float16 half4 __attribute__((ext_vector_type(4)));
@@ -50,9 +53,19 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kTileRows = 16;       // rows (query row, query head of the group) of a tile
 constexpr int kSplitSlots = 2048;   // records of shares in the workspace, two a workgroup
-constexpr int kSharedTickets = 4096, kSharedRecordRows = 131072;  // tickets, and rows of records, in the workspace of a batch with shared pages
-static_assert(kSharedTickets >= kSplitSlots && kSharedRecordRows >= kSplitSlots * kTileRows, "those of k_kv4_attn");
+// in the workspace of a batch with shared pages: tickets, and floats for Dh + 2 of them a row -- records, two a wavefront that has parts of its own, then
+// slots, one a workgroup
+constexpr int kSharedTickets = 4096, kSharedRows = 131072, kMaxWorkers = 3072;
+static_assert(kMaxWorkers <= kSharedTickets && kSplitSlots <= kSharedTickets && kMaxWorkers >= kSplitSlots / 2 &&
+                  17 * (kSharedRows - 2 * kMaxWorkers * kTileRows) >= 18 * (kSplitSlots / 2) * kTileRows, "a slot has Dh + 4 floats a row: at Dh = 32 18 / 17 of Dh + 2");
 constexpr int kJobPieces = 1;       // what a job costs besides its pages, in pieces of them (2: 52 us instead of 50, 34 instead of 31, for the batches above)
+constexpr int kJobPages = 3;        // what a job costs a wavefront of its own besides its pages, in pages
+
+// Where several workgroups have shares of a row's shared pages, its stats are a NaN that holds the first one's number, and row of the tile + 256 * shares.
+// Outputs of the first lie in `out`; each workgroup has a slot: outputs of the share that goes on from the workgroup before (it has one of these at most), their
+// maxima and sums, and maxima and sums of the share that goes on in the next.
+constexpr unsigned kInShares = 0x7FC00000u;
+__device__ __forceinline__ float *share_slot(float *base, int workgroup, int dh) { return base + (int64_t)workgroup * kTileRows * (dh + 4); }
 
 // floor(x / d) where that is below 2^21, x below 2^30: the quotient by a reciprocal is off by one at most, which what it leaves shows.  (A division
 // of integers is forty instructions that nothing runs beside.)
@@ -151,7 +164,7 @@ struct Read {  // of a sequence, or of a group
       }
     } else {
       if (i < a.n_seqs) len = a.lens[i], row0 = a.starts[i], end = a.starts[i + 1];
-      if constexpr (MODE == kAttnBehind) {
+      if constexpr (attn_behind(MODE)) {
         if (i < a.n_seqs && a.n_groups > 0) {
           int lo = 0, hi = a.n_groups;  // groups[lo] <= i where there is such a group
           while (hi - lo > 1) {
@@ -179,8 +192,8 @@ __device__ __forceinline__ void look(const Kv4Attn &a, const Read<MODE> &read, B
   s.reach = __builtin_amdgcn_readlane(reach, 63);
   s.rows = s.row0 == reach && end > s.row0 ? end - s.row0 : 0;
   s.tiles = (s.rows * a.group + kTileRows - 1) / kTileRows;
-  const int pages = a.n_pages > 0 && s.len > 0 ? (int)min(((unsigned)s.len + kKvPageRows - 1) / kKvPageRows, (unsigned)a.table_stride) - (MODE == kAttnBehind ? s.aside : 0) : 0;
-  s.cost = max(1, (pages + (1 << a.piece_log2) - 1) >> a.piece_log2) + kJobPieces;  // (without keys there is still a row to write)
+  const int pages = a.n_pages > 0 && s.len > 0 ? (int)min(((unsigned)s.len + kKvPageRows - 1) / kKvPageRows, (unsigned)a.table_stride) - (attn_behind(MODE) ? s.aside : 0) : 0;
+  s.cost = max(1, (pages + (1 << a.piece_log2) - 1) >> a.piece_log2) + (MODE == kAttnBehindWaves ? kJobPages : kJobPieces);  // (without keys there is still a row to write)
   s.upto = s.before + wave_scan_int(s.tiles * a.Hkv * s.cost);
 }
 struct Job {
@@ -207,7 +220,7 @@ __device__ __forceinline__ bool find_job(const Kv4Attn &a, Batch<MODE> &s, int (
   const int start = __builtin_amdgcn_readlane(s.upto, l) - all * j.cost, job = uniform_fast_div(place - start, j.cost);
   j.at = start + job * j.cost;
   j.seq = MODE == kAttnShared ? __builtin_amdgcn_readlane(s.aside, l) : s.first + l;
-  j.skip = MODE == kAttnBehind ? __builtin_amdgcn_readlane(s.aside, l) : 0;
+  j.skip = attn_behind(MODE) ? __builtin_amdgcn_readlane(s.aside, l) : 0;
   j.head = tiles == 1 ? job : uniform_fast_div(job, tiles);
   // tiles from both ends in turn: in a prompt's own pages late rows see more than early ones, and a workgroup gets some of each
   const int t = job - j.head * tiles;
@@ -221,10 +234,10 @@ __device__ __forceinline__ bool find_job(const Kv4Attn &a, Batch<MODE> &s, int (
 // The pages come straight into LDS, into a wavefront's own place: the keys and the values of a head as they lie in memory.  A page's
 // key quants are taken to registers when their turn comes, and the next page's are asked for at once; the rest follows when the scores, or the
 // outputs, are there.
-template <int DH, int FIELDS>
+template <int DH, int MODE>
 struct Kv4Lds {
-  static constexpr int HEAD = 36 * DH, WAVE = 2 * HEAD, STATS = 4 * WAVE, SEQS = STATS + 14 * kTileRows * 4, FRONTS = SEQS + 4 * FIELDS * 64 * 4, Q = FRONTS + 2 * 64 * 4,
-                       BYTES = Q + DH / 32 * 2048;
+  static constexpr int HEAD = 36 * DH, WAVE = 2 * HEAD, STATS = 4 * WAVE, SEQS = STATS + 14 * kTileRows * 4, FRONTS = SEQS + 4 * Batch<MODE>::FIELDS * 64 * 4, Q = FRONTS + 2 * 64 * 4,
+                       QUERIES = DH / 32 * 2048, BYTES = Q + (MODE == kAttnBehindWaves ? 4 : 1) * QUERIES;
   static constexpr int REQUESTS = DH / 32 + (DH / 32 + 1) / 2;  // of a head's part of a page: 16 bytes a lane, then 4
   static constexpr int SHARES = DH == 32 ? 128 : 256;  // of one tile, at most: their records are added up by one workgroup
   static_assert(WAVE >= kTileRows * (DH + 4) * 4 && 4 * WAVE >= 4 * SHARES * kTileRows, "results, and weights of shares, in the pages' place");
@@ -242,9 +255,10 @@ struct Kv4Lds {
 //           value of 4e5 that has no weight).  Pages with a scale of 32 or more take the fp32 matrix instructions, p d as one fp32 number, at an
 //           eighth of the rate (where all pages have one the batches above take 85 and 57 us, the prompts 239).
 template <int DH, int MODE>
-__global__ __launch_bounds__(256, DH == 128 ? 3 : 4) void k_kv4_attn(Kv4Attn a) {
+__global__ __launch_bounds__(256, MODE == kAttnBehindWaves ? (DH == 128 ? 2 : 3) : DH == 128 ? 3 : 4) void k_kv4_attn(Kv4Attn a) {
   constexpr int FIELDS = Batch<MODE>::FIELDS;
-  using L = Kv4Lds<DH, FIELDS>;
+  constexpr bool ALONE = MODE == kAttnBehindWaves;  // a wavefront has parts of its own
+  using L = Kv4Lds<DH, MODE>;
   constexpr int NB = DH / 32;
   extern __shared__ __align__(16) unsigned char smem[];
   float (*s_m)[kTileRows] = (float (*)[kTileRows])(smem + L::STATS), (*s_l)[kTileRows] = s_m + 4, (*s_w)[kTileRows] = s_m + 8, *s_sum = s_m[12];
@@ -273,12 +287,12 @@ __global__ __launch_bounds__(256, DH == 128 ? 3 : 4) void k_kv4_attn(Kv4Attn a) 
   s.put(s_seqs[wv]);
   // A part's length: of the whole, or what keeps a tile's shares below their number, or, since its last workgroup reads all of a tile's
   // records, as many pieces as come out about even with that (sqrt(longest / 20): 32768 keys of one head of 128 27.3 -> 22.5 us, 131072 38.0 -> 34.1).
-  const int even = __builtin_amdgcn_readfirstlane((int)__builtin_sqrtf(0.05f * (float)longest));
-  const int per = max(max(uniform_fast_div(total + (int)gridDim.x - 1, (int)gridDim.x), (longest + L::SHARES - 2) / (L::SHARES - 1)), even);
+  const int even = __builtin_amdgcn_readfirstlane((int)__builtin_sqrtf((ALONE ? 0.1f : 0.05f) * (float)longest)), workers = (int)gridDim.x * (ALONE ? 4 : 1);
+  const int per = max(max(uniform_fast_div(total + workers - 1, workers), (longest + L::SHARES - 2) / (L::SHARES - 1)), even);
   // Workgroups are dealt to the eight XCDs in turn.  Neighbours on the line, which may read the same pages and join their shares, on one of
   // them, and all XCDs alike where there are fewer parts than workgroups (one sequence of 2048, 8 heads of 128, 72 parts: 15.3 us on one XCD,
   // 10.8 on eight).
-  const int parts = uniform_fast_div(total + per - 1, per), of_xcd = (parts + 7) >> 3, nth = blockIdx.x >> 3;
+  const int parts = uniform_fast_div(total + per - 1, per), of_xcd = (parts + 7) >> 3, nth = ALONE ? 4 * (int)(blockIdx.x >> 3) + wv : blockIdx.x >> 3;
   const int me = nth < of_xcd ? (int)(blockIdx.x & 7) * of_xcd + nth : parts;
   const int x0 = (int)min((int64_t)me * per, (int64_t)total), x1 = min(total - x0, per) + x0;
   for (int x = x0; x < x1;) {
@@ -301,7 +315,7 @@ __global__ __launch_bounds__(256, DH == 128 ? 3 : 4) void k_kv4_attn(Kv4Attn a) 
   const int least = MODE == kAttnShared ? w.len - 1 : (int)min((int64_t)w.len - w.rows + j0, all - 1);
   const int pages = a.n_pages > 0 && last >= 0 ? max(last / kKvPageRows + 1 - w.skip, 0) : 0;
   // its pieces lie on the line behind those that stand for the rest (a job without pages is one piece of none)
-  const int pieces = max(1, (pages + (1 << a.piece_log2) - 1) >> a.piece_log2), line = w.at + kJobPieces;
+  const int pieces = max(1, (pages + (1 << a.piece_log2) - 1) >> a.piece_log2), line = w.at + (ALONE ? kJobPages : kJobPieces);
   const int owner = uniform_fast_div(line, per), shares = uniform_fast_div(line + pieces - 1, per) - owner + 1, share = me - owner;
   const int from_piece = max(x0 - line, 0), to_piece = min(x1 - line, pieces);
   if (from_piece >= to_piece) continue;
@@ -313,15 +327,15 @@ __global__ __launch_bounds__(256, DH == 128 ? 3 : 4) void k_kv4_attn(Kv4Attn a) 
   auto page_id = [&](int k) {  // k: this wavefront's k-th page (the same in every lane)
     if (k >= ids_from + 64) {
       ids_from = k;
-      const int p = p0 + wv + 4 * (k + lane);
+      const int p = ALONE ? p0 + k + lane : p0 + wv + 4 * (k + lane);
       ids = p < p1 ? table[p] : -1;
       asm volatile("" : "+v"(ids));  // (waited for here: behind the branch it would be waited for with all pages on their way, page after page)
     }
     return __builtin_amdgcn_readlane(ids, k - ids_from);
   };
-  const int mine = p0 + wv < p1 ? (p1 - p0 - wv + 3) / 4 : 0;  // pages of this wavefront
+  const int mine = ALONE ? max(p1 - p0, 0) : p0 + wv < p1 ? (p1 - p0 - wv + 3) / 4 : 0;  // pages of this wavefront
   {
-    const int p = p0 + wv + 4 * lane;
+    const int p = ALONE ? p0 + lane : p0 + wv + 4 * lane;
     ids_from = 0;
     ids = p < p1 ? table[p] : -1;
   }
@@ -354,6 +368,7 @@ __global__ __launch_bounds__(256, DH == 128 ? 3 : 4) void k_kv4_attn(Kv4Attn a) 
 
   // The row's query as two fp16 terms, in LDS as the matrix instructions take them: [block][term][lane][8].  (Held in registers they are a
   // quarter of what a wavefront has.)  Every wavefront looks at the whole row, block b is wavefront b's to convert.
+  unsigned char *const queries = smem + L::Q + (ALONE ? wv * L::QUERIES : 0);
   float weight;
   {
     float x[NB][8], mine8[8];
@@ -380,18 +395,24 @@ __global__ __launch_bounds__(256, DH == 128 ? 3 : 4) void k_kv4_attn(Kv4Attn a) 
     // 2^(9 - e), e the exponent of the row's largest, brings that into [2^9, 2^10): fp16's own 11 bits, and 11 below them
     const int e = min(max((int)(__float_as_uint(top) >> 23) - 127, -100), 127);
     const float up = __uint_as_float((unsigned)(127 + 9 - e) << 23), down = __uint_as_float((unsigned)(127 - 9 + e) << 23);
-    if (wv < NB) {
+    auto convert = [&](const float *from, int b) {
       half8 hi, lo;
 #pragma unroll
       for (int k = 0; k < 8; k++) {
         // the order in which a dword's nibbles come apart: channels 0 2 4 6 1 3 5 7
         const int ch = k < 4 ? (k & 1) * 2 + (k >> 1) * 4 : 1 + (k & 1) * 2 + ((k - 4) >> 1) * 4;
-        const float y = bad ? NAN : mine8[ch] * up;  // (every score of the row a NaN, and those that are masked minus infinity: without a key it is zero)
+        const float y = bad ? NAN : from[ch] * up;  // (every score of the row a NaN, and those that are masked minus infinity: without a key it is zero)
         hi[k] = (_Float16)y;
         lo[k] = (_Float16)(y - (float)hi[k]);
       }
-      *(half8 *)(smem + L::Q + wv * 2048 + lane * 16) = hi;
-      *(half8 *)(smem + L::Q + wv * 2048 + 1024 + lane * 16) = lo;
+      *(half8 *)(queries + b * 2048 + lane * 16) = hi;
+      *(half8 *)(queries + b * 2048 + 1024 + lane * 16) = lo;
+    };
+    if constexpr (ALONE) {
+#pragma unroll
+      for (int b = 0; b < NB; b++) convert(x[b], b);
+    } else if (wv < NB) {
+      convert(mine8, wv);
     }
     // scores as powers of two: log2(e) / sqrt(DH), and the power of two taken off again
     weight = (DH == 32 ? 0.25503487f : DH == 64 ? 0.18033688f : 0.12751743f) * down;
@@ -416,19 +437,20 @@ __global__ __launch_bounds__(256, DH == 128 ? 3 : 4) void k_kv4_attn(Kv4Attn a) 
   asm volatile("" : "+s"(lower), "+s"(upper), "+v"(e_lower), "+v"(e_upper));
   auto lower_of = [&](uint32_t u) { return __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2v, (u & lower) ^ e_lower) - (_Float16)1032.0f); };
   auto upper_of = [&](uint32_t u) { return __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2v, (u & upper) ^ e_upper) - (_Float16)72.0f); };
-  __syncthreads();
+  if constexpr (ALONE) wait_lds();
+  else __syncthreads();
   for (int k = 0; k < mine; k++) {
     {
       // Of the wavefronts on a SIMD the oldest goes first, and what it gains the others lose: the last workgroup of a compute unit ended at
       // twice the first one's time, the SIMDs to itself.  So who has more left goes first, by quarters of a part (prompts 122 -> 112 us, the
       // batches 52 -> 48 and 34 -> 30).
-      const int left = 4 * (x1 - line - from_piece - (k << 2 >> a.piece_log2));
+      const int left = 4 * (x1 - line - from_piece - ((ALONE ? k : k << 2) >> a.piece_log2));
       if (left > 3 * per) __builtin_amdgcn_s_setprio(3);
       else if (left > 2 * per) __builtin_amdgcn_s_setprio(2);
       else if (left > per) __builtin_amdgcn_s_setprio(1);
       else __builtin_amdgcn_s_setprio(0);
     }
-    const int page = w.skip + p0 + wv + 4 * k;
+    const int page = w.skip + p0 + (ALONE ? k : wv + 4 * k);
     const int from = valid(id) ? page * kKvPageRows : INT_MAX - (kKvPageRows - 1);  // (absent: behind every limit)
     const bool whole = from + kKvPageRows - 1 <= least;                            // every row of the tile sees every row of the page (uniform)
     // the scales of block b, rows 16 t + 4 g ..
@@ -449,7 +471,7 @@ __global__ __launch_bounds__(256, DH == 128 ? 3 : 4) void k_kv4_attn(Kv4Attn a) 
     if (more) ask_quants(a.k_pages, next, k_at);
 #pragma unroll
     for (int b = 0; b < NB; b++) {
-      const half8 q_hi = *(const half8 *)(smem + L::Q + b * 2048 + lane * 16), q_lo = *(const half8 *)(smem + L::Q + b * 2048 + 1024 + lane * 16);
+      const half8 q_hi = *(const half8 *)(queries + b * 2048 + lane * 16), q_lo = *(const half8 *)(queries + b * 2048 + 1024 + lane * 16);
 #pragma unroll
       for (int t = 0; t < 4; t++) {
         const uint32_t u = kq[t][b], v = u >> 8;
@@ -603,11 +625,121 @@ __global__ __launch_bounds__(256, DH == 128 ? 3 : 4) void k_kv4_attn(Kv4Attn a) 
   l += __shfl_xor(l, 16, 64);
   l += __shfl_xor(l, 32, 64);
 
+  const int nr = min(kTileRows, w.rows * G - w.tile * kTileRows);  // rows of the tile that there are
+  const float back = ldexpf(1.0f, f == 100 ? 0 : -f);
+  // a share that goes on from the workgroup before, and one that goes on in the next: a workgroup has one of each at most
+  auto record_of = [&](int k) { return a.parts + (int64_t)(2 * (owner + k) + (k == 0)) * kTileRows * (DH + 2); };
+  auto weight_of = [](float mk, float lk, float M) { return mk > -INFINITY ? __builtin_amdgcn_exp2f(mk - M) : lk == lk ? 0.0f : 1.0f; };  // (a NaN stays one)
+  // up to eight parts of a row's outputs, their maxima and sums, added to what there is
+  auto add_up = [&](f32x2 &x, float &top, float &sum, int n, auto ml, auto y) {
+    float high = top;
+#pragma unroll
+    for (int k = 0; k < 8; k++)
+      if (k < n) high = fmaxf(high, ml(k)[0]);
+    const float f = weight_of(top, sum, high);
+    top = high, sum *= f, x[0] *= f, x[1] *= f;
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+      if (k < n) {
+        const float g = weight_of(ml(k)[0], ml(k)[1], high);
+        sum = fmaf(g, ml(k)[1], sum);
+        x[0] = fmaf(g, y(k)[0], x[0]), x[1] = fmaf(g, y(k)[1], x[1]);
+      }
+    }
+  };
+  // where a row of the tile goes, of all rows and heads
+  auto row_at = [&](int r) {
+    const int rr = w.tile * kTileRows + r, jj = fast_div(rr, G);
+    return (int64_t)(w.row0 + jj) * a.H + w.head * G + rr - jj * G;
+  };
+  // a pair of channels of a tile's row: where it goes, as what it is
+  auto finish = [&](int r, int c, f32x2 x, float top, float sum) {
+    const int64_t at = row_at(r);
+    f2_any *to = (f2_any *)(a.out + at * DH + c);
+    if constexpr (MODE == kAttnShared) {
+      *to = f2_any{x[0], x[1]};
+      if (c == 0) *(f2_any *)(a.stats + 2 * at) = f2_any{top, sum};
+      return;
+    }
+    if constexpr (attn_behind(MODE)) {
+      if (w.skip) {  // what the launch in front of this one has left of the row
+        const f2_any whole = *to, its = *(const f2_any *)(a.stats + 2 * at);
+        if (its[0] == its[0]) {
+          add_up(x, top, sum, 1, [&](int) { return f32x2{its[0], its[1]}; }, [&](int) { return f32x2{whole[0], whole[1]}; });
+        } else {
+          const unsigned code = __float_as_uint(its[1]);
+          const int first = (int)(__float_as_uint(its[0]) & ~kInShares), n = (int)(code >> 8), row = (int)(code & 255u);
+          for (int k0 = 0; k0 < n; k0 += 8) {
+            f2_any y[8], ml[8];
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+              const int share = min(k0 + k, n - 1);
+              const float *slot = share_slot(a.slots, first + share, DH);
+              ml[k] = *(const f2_any *)(slot + kTileRows * DH + 2 * row + (share == 0 ? 2 * kTileRows : 0));
+              y[k] = *(const f2_any *)(share == 0 ? (const float *)to : slot + row * DH + c);
+            }
+            add_up(x, top, sum, min(8, n - k0), [&](int k) { return f32x2{ml[k][0], ml[k][1]}; }, [&](int k) { return f32x2{y[k][0], y[k][1]}; });
+          }
+        }
+      }
+    }
+    *to = sum != 0.0f ? f2_any{x[0] / sum, x[1] / sum} : f2_any{0.0f, 0.0f};
+  };
+  // the records of all shares, in their order, eight at a time
+  auto join = [&](int first, int step) {
+    for (int e = first; e < nr * DH / 2; e += step) {
+      const int r = e / (DH / 2), c = e % (DH / 2) * 2;
+      f32x2 x = {0.0f, 0.0f};
+      float top = -INFINITY, sum = 0.0f;
+      for (int k0 = 0; k0 < shares; k0 += 8) {
+        unsigned long long y[8], ml[8];
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+          const float *from = record_of(min(k0 + k, shares - 1));
+          ml[k] = __hip_atomic_load((const unsigned long long *)(from + kTileRows * DH + 2 * r), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+          y[k] = __hip_atomic_load((const unsigned long long *)(from + 2 * e), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+        add_up(x, top, sum, min(8, shares - k0), [&](int k) { return __builtin_bit_cast(f32x2, ml[k]); }, [&](int k) { return __builtin_bit_cast(f32x2, y[k]); });
+      }
+      finish(r, c, x, top, sum);
+    }
+  };
+  if constexpr (ALONE) {
+    const int lane = lane_now(), n = lane & 15, g = lane >> 4;
+    if (n < nr) {
+#pragma unroll
+      for (int b = 0; b < NB; b++)
+#pragma unroll
+        for (int half = 0; half < 2; half++) *(f32x4 *)(s_o(wv, n) + b * 32 + half * 16 + 4 * g) = o[b][half] * back;
+    }
+    if (g == 0) s_m[wv][n] = m > -INFINITY ? base_of(m) : -INFINITY, s_l[wv][n] = l;
+    wait_lds();
+    if (shares == 1) {
+      for (int e = lane; e < nr * DH / 2; e += 64) {
+        const int r = e / (DH / 2), c = e % (DH / 2) * 2;
+        finish(r, c, *(const f32x2 *)(s_o(wv, r) + c), s_m[wv][r], s_l[wv][r]);
+      }
+    } else {
+      float *rec = record_of(share);
+      for (int e = lane; e < nr * DH / 2; e += 64)
+        __hip_atomic_store((unsigned long long *)(rec + 2 * e), __builtin_bit_cast(unsigned long long, *(const f32x2 *)(s_o(wv, e / (DH / 2)) + e % (DH / 2) * 2)), __ATOMIC_RELAXED,
+                           __HIP_MEMORY_SCOPE_AGENT);
+      if (lane < nr)
+        __hip_atomic_store((unsigned long long *)(rec + kTileRows * DH + 2 * lane), __builtin_bit_cast(unsigned long long, (f32x2){s_m[wv][lane], s_l[wv][lane]}), __ATOMIC_RELAXED,
+                           __HIP_MEMORY_SCOPE_AGENT);
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wavefront's device-scope stores have reached memory
+      int drawn = 0;
+      if (lane == 0) drawn = __hip_atomic_fetch_add(a.tickets + owner, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      if (__builtin_amdgcn_readfirstlane(drawn) == shares - 1) {  // the last of the job's wavefronts adds the shares up, in their order
+        if (lane == 0) __hip_atomic_store(a.tickets + owner, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);  // the next call counts again
+        join(lane, 64);
+      }
+    }
+    wait_lds();  // (the next job's pages come to the same place)
+  } else {
   // the four wavefronts' results meet
   const int tid = wv * 64 + lane_now(), n_out = tid & 15, g_out = (tid >> 4) & 3;
-  const int nr = min(kTileRows, w.rows * G - w.tile * kTileRows);  // rows of the tile that there are
   if (g_out == 0) s_m[wv][n_out] = m > -INFINITY ? base_of(m) : -INFINITY, s_l[wv][n_out] = l;
-  const float back = ldexpf(1.0f, f == 100 ? 0 : -f);
   if (n_out < nr) {
 #pragma unroll
     for (int b = 0; b < NB; b++)
@@ -615,9 +747,6 @@ __global__ __launch_bounds__(256, DH == 128 ? 3 : 4) void k_kv4_attn(Kv4Attn a) 
       for (int half = 0; half < 2; half++) *(f32x4 *)(s_o(wv, n_out) + b * 32 + half * 16 + 4 * g_out) = o[b][half] * back;
   }
   __syncthreads();
-  // a share that goes on from the workgroup before, and one that goes on in the next: a workgroup has one of each at most
-  auto record_of = [&](int k) { return a.parts + (int64_t)(2 * (owner + k) + (k == 0)) * kTileRows * (DH + 2); };
-  auto weight_of = [](float mk, float lk, float M) { return mk > -INFINITY ? __builtin_amdgcn_exp2f(mk - M) : lk == lk ? 0.0f : 1.0f; };  // (a NaN stays one)
   if (tid < nr) {
     float M = -INFINITY, sum = 0.0f;
 #pragma unroll
@@ -630,32 +759,14 @@ __global__ __launch_bounds__(256, DH == 128 ? 3 : 4) void k_kv4_attn(Kv4Attn a) 
     }
     s_sum[tid] = sum;
     if constexpr (MODE != kAttnWhole) s_l[0][tid] = M;  // (its own sums have been read)
-    if (shares > 1) {
+    if (MODE == kAttnShared && shares > 1) {
+      *(f2_any *)(share_slot(a.slots, me, DH) + kTileRows * DH + 2 * tid + (share == 0 ? 2 * kTileRows : 0)) = f2_any{M, sum};
+    } else if (shares > 1) {
       float *to = record_of(share) + kTileRows * DH + 2 * tid;
       __hip_atomic_store((unsigned long long *)to, __builtin_bit_cast(unsigned long long, (f32x2){M, sum}), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
   }
   __syncthreads();
-  // a pair of channels of a tile's row: where it goes, as what it is
-  auto finish = [&](int r, int c, f32x2 x, float top, float sum) {
-    const int rr = w.tile * kTileRows + r, jj = fast_div(rr, G);
-    const int64_t at = (int64_t)(w.row0 + jj) * a.H + w.head * G + rr - jj * G;
-    f2_any *to = (f2_any *)(a.out + at * DH + c);
-    if constexpr (MODE == kAttnShared) {
-      *to = f2_any{x[0], x[1]};
-      if (c == 0) *(f2_any *)(a.stats + 2 * at) = f2_any{top, sum};
-      return;
-    }
-    if constexpr (MODE == kAttnBehind) {
-      if (w.skip) {  // what the launch in front of this one has left of the row
-        const f2_any y = *to, its = *(const f2_any *)(a.stats + 2 * at);
-        const float high = fmaxf(top, its[0]), f = weight_of(top, sum, high), g = weight_of(its[0], its[1], high);
-        sum = fmaf(f, sum, g * its[1]);
-        x[0] = fmaf(f, x[0], g * y[0]), x[1] = fmaf(f, x[1], g * y[1]);
-      }
-    }
-    *to = sum != 0.0f ? f2_any{x[0] / sum, x[1] / sum} : f2_any{0.0f, 0.0f};
-  };
   for (int e = tid; e < nr * DH / 2; e += 256) {
     const int r = e / (DH / 2), c = e % (DH / 2) * 2;
     f32x2 x = {0.0f, 0.0f};
@@ -664,13 +775,17 @@ __global__ __launch_bounds__(256, DH == 128 ? 3 : 4) void k_kv4_attn(Kv4Attn a) 
       const f32x2 y = *(const f32x2 *)(s_o(k, r) + c);
       x[0] = fmaf(s_w[k][r], y[0], x[0]), x[1] = fmaf(s_w[k][r], y[1], x[1]);
     }
-    if (shares > 1) {
+    if (MODE == kAttnShared && shares > 1) {
+      *(f2_any *)(share == 0 ? a.out + row_at(r) * DH + c : share_slot(a.slots, me, DH) + 2 * e) = f2_any{x[0], x[1]};
+    } else if (shares > 1) {
       __hip_atomic_store((unsigned long long *)(record_of(share) + 2 * e), __builtin_bit_cast(unsigned long long, x), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     } else {
       finish(r, c, x, MODE != kAttnWhole ? s_l[0][r] : 0.0f, s_sum[r]);
     }
   }
-  if (shares > 1) {
+  if (MODE == kAttnShared && shares > 1) {  // the launch behind this one adds the shares up
+    if (share == 0 && tid < nr) *(f2_any *)(a.stats + 2 * row_at(tid)) = f2_any{__uint_as_float(kInShares | (unsigned)me), __uint_as_float((unsigned)(tid + (shares << 8)))};
+  } else if (shares > 1) {
     int *tickets = a.tickets + 2 * owner;
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this thread's device-scope stores have reached memory
     __syncthreads();
@@ -681,7 +796,9 @@ __global__ __launch_bounds__(256, DH == 128 ? 3 : 4) void k_kv4_attn(Kv4Attn a) 
       // Maxima and sums of all shares, asked for at once, then the outputs, eight or sixteen shares at a time: a load after the other would be a
       // round trip to memory for each share.  Up to 16 shares every thread works the weights out for itself (9.3 us for one sequence of 701, 12
       // heads of 64, against 10.4; with all parts on one XCD), else once for all (8192: 14.4 against 15.9).
-      if (shares <= 16) {
+      if constexpr (MODE != kAttnWhole) {
+        join(tid, 256);
+      } else if (shares <= 16) {
         f32x2 (*ml)[kTileRows] = (f32x2 (*)[kTileRows])smem;
         if ((tid >> 4) < shares && (tid & 15) < nr)
           ml[tid >> 4][tid & 15] =
@@ -756,12 +873,13 @@ __global__ __launch_bounds__(256, DH == 128 ? 3 : 4) void k_kv4_attn(Kv4Attn a) 
               }
             }
           }
-          finish(r, c, x, MODE != kAttnWhole ? fmaxf(fmaxf(s_m[0][r], s_m[1][r]), fmaxf(s_m[2][r], s_m[3][r])) : 0.0f, sum);
+          finish(r, c, x, 0.0f, sum);
         }
       }
     }
   }
   __syncthreads();  // the next job's results go through the same LDS
+  }
   }
 }
 
@@ -783,12 +901,13 @@ static int launch_kv4_attn(const char *who, Kv4Attn a, int Dh) {
     return fail(CTHIP_E_UNSUPPORTED, "%s: %d rows of %d heads in one call (at most 2^20 rows, and 2^21 tiles of 16 heads of them)", who, a.n_rows, a.H);
   // as many workgroups as run at once (three or four a compute unit for their registers and pages; with two or three prompts took 119 us
   // where these took 112, the batches 50 and 32 where these took 48 and 30), a multiple of the XCDs
-  const int at_once = std::min(kSplitSlots / 2, state().compute_units * (Dh == 128 ? 3 : 4) / 8 * 8);
+  // (a wavefront for itself: two or three, for its queries in LDS)
+  const int at_once = MODE == kAttnBehindWaves ? std::min(kMaxWorkers / 4, state().compute_units * (Dh == 128 ? 2 : 3) / 8 * 8) : std::min(kSplitSlots / 2, state().compute_units * (Dh == 128 ? 3 : 4) / 8 * 8);
   a.group = a.H / a.Hkv;
-  a.piece_log2 = 2;  // (the line is shorter than 2^30, and a workgroup's part of it below what fast_div holds for)
-  while (jobs * ((a.table_stride >> a.piece_log2) + 1 + kJobPieces) > std::min((int64_t)INT_MAX / 2, (int64_t)at_once << 20)) a.piece_log2++;
+  a.piece_log2 = MODE == kAttnBehindWaves ? 0 : 2;  // (the line is shorter than 2^30, and a workgroup's part of it below what fast_div holds for)
+  while (jobs * ((a.table_stride >> a.piece_log2) + 1 + (MODE == kAttnBehindWaves ? kJobPages : kJobPieces)) > std::min((int64_t)INT_MAX / 2, (int64_t)at_once << 20)) a.piece_log2++;
   const dim3 grid((unsigned)at_once), block(256);
-#define ATT(DH_) hipLaunchKernelGGL((k_kv4_attn<DH_, MODE>), grid, block, (Kv4Lds<DH_, Batch<MODE>::FIELDS>::BYTES), state().stream, a)
+#define ATT(DH_) hipLaunchKernelGGL((k_kv4_attn<DH_, MODE>), grid, block, (Kv4Lds<DH_, MODE>::BYTES), state().stream, a)
   switch (Dh) {
     case 32: ATT(32); break;
     case 64: ATT(64); break;
@@ -823,7 +942,7 @@ int cthip_sdpa_paged_q4(float *out, const float *q, int64_t q_stride, const void
 
 int64_t cthip_sdpa_shared_paged_q4_workspace(int n_rows, int H, int head_dim) {
   if (!kv4_shape_ok(1, head_dim) || n_rows < 0 || H < 0) return fail(CTHIP_E_BAD_ARG, "cthip_sdpa_shared_paged_q4_workspace: %d rows of %d heads of %d (head sizes 32, 64, 128)", n_rows, H, head_dim);
-  return 4ll * (kSharedTickets + (int64_t)kSharedRecordRows * (head_dim + 2) + 2ll * n_rows * H);
+  return 4ll * (kSharedTickets + (int64_t)kSharedRows * (head_dim + 2) + 2ll * n_rows * H);
 }
 
 int cthip_sdpa_shared_paged_q4(float *out, const float *q, int64_t q_stride, const void *k_pages, const void *v_pages, int n_pages, const int *tables, int table_stride,
@@ -840,10 +959,15 @@ int cthip_sdpa_shared_paged_q4(float *out, const float *q, int64_t q_stride, con
   Kv4Attn a = {out, q, (const unsigned char *)k_pages, (const unsigned char *)v_pages, tables, lens, starts, q_stride, n_pages, table_stride, n_seqs, n_rows, H, Hkv};
   a.tickets = (int *)workspace, a.parts = (float *)workspace + kSharedTickets;
   a.groups = groups, a.shared = shared, a.n_groups = n_groups;
-  a.stats = a.parts + (int64_t)kSharedRecordRows * (Dh + 2);
-  if (n_groups > 0)
-    if (const int rc = launch_kv4_attn<kAttnShared>(__func__, a, Dh)) return rc;
-  return launch_kv4_attn<kAttnBehind>(__func__, a, Dh);
+  a.slots = a.parts + (int64_t)2 * kMaxWorkers * kTileRows * (Dh + 2), a.stats = a.parts + (int64_t)kSharedRows * (Dh + 2);
+  if (n_groups == 0) return launch_kv4_attn<kAttnWhole>(__func__, a, Dh);
+  // What a sequence has behind its group's pages is a job a head, often of a page or two.  Where there are more jobs than workgroups, each of a few rows, a job is a
+  // wavefront's own: its chain of round trips, not its pages, is what it takes, and four times as many run at once.  32 heads of 128 over 1024 shared rows, 70 rows behind them at
+  // most, both launches: 24 sequences 24.4 us by workgroups, 25.3 by wavefronts; 32: 33.7 and 25.7; 64: 45.2 and 29.3 (600 rows: 50.0 and 43.2); four rows each
+  // 55.4 and 44.6; with eight rows of a head, whose results are joined by fewer lanes then, 512 jobs 34 and 46.
+  const bool few = (int64_t)n_rows * (H / Hkv) <= 4ll * n_seqs && (int64_t)n_seqs * Hkv > state().compute_units * (Dh == 128 ? 3 : 4);
+  if (const int rc = launch_kv4_attn<kAttnShared>(__func__, a, Dh)) return rc;
+  return few ? launch_kv4_attn<kAttnBehindWaves>(__func__, a, Dh) : launch_kv4_attn<kAttnBehind>(__func__, a, Dh);
 }
 
 }  // extern "C"
