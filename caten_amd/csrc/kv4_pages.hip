@@ -41,19 +41,27 @@ __global__ __launch_bounds__(256) void k_kv_fork(ForkArgs a) {
   __shared__ unsigned s_parent[kKv4MaxSeqs / 32];      // whether it is a parent
   __shared__ int s_count[2][4];
   const int tid = threadIdx.x, mine = blockIdx.y;
+  // This workgroup's own fork and a fork a thread are asked for first, and so is what lies behind them wherever that is in range: round trips beside those of the checks
+  // (one after the other 6.0 us for 8 forks of one sequence in 12 layers, so 5.2)
+  const bool own = mine < a.n_forks, some = tid < a.n_forks;
+  const int my_parent = own ? a.parents[mine] : -1, my_child = own ? a.children[mine] : -1, my_at = own ? a.at[mine] : 0;
+  const int tid_parent = some ? a.parents[tid] : -1, tid_child = some ? a.children[tid] : -1, tid_at = some ? a.at[tid] : 0;
+  const int have = max(a.n_free[0], 0);
+  const bool my_parent_ok = my_parent >= 0 && my_parent < a.n_seqs, reads = my_parent_ok && my_at >= 0 && my_at / kKvPageRows < a.table_stride;
+  const int *from = a.tables + (int64_t)(my_parent_ok ? my_parent : 0) * a.table_stride;
+  const int src = reads ? from[my_at / kKvPageRows] : -1, tid_len = tid_parent >= 0 && tid_parent < a.n_seqs ? a.lens[tid_parent] : -1;
   for (int i = tid; i < a.n_seqs; i += 256) s_first[i] = INT_MAX;
   for (int i = tid; i < (a.n_seqs + 31) / 32; i += 256) s_parent[i] = 0;
   __syncthreads();
   for (int f = tid; f < a.n_forks; f += 256) {
-    const int p = a.parents[f], c = a.children[f];
+    const int p = f == tid ? tid_parent : a.parents[f], c = f == tid ? tid_child : a.children[f];
     if (c >= 0 && c < a.n_seqs) atomicMin(&s_first[c], f);
     if (p >= 0 && p < a.n_seqs) atomicOr(&s_parent[p >> 5], 1u << (p & 31));
   }
   __syncthreads();
   // whether a fork can be made but for its page, and whether it needs one
-  auto fine = [&](int f, bool &need) {
-    const int p = a.parents[f], c = a.children[f], at = a.at[f];
-    const bool ok = p >= 0 && p < a.n_seqs && c >= 0 && c < a.n_seqs && at >= 0 && s_first[c] == f && !((s_parent[c >> 5] >> (c & 31)) & 1u) && at <= a.lens[p] &&
+  auto fine = [&](int f, int p, int c, int at, int len, bool &need) {
+    const bool ok = p >= 0 && p < a.n_seqs && c >= 0 && c < a.n_seqs && at >= 0 && s_first[c] == f && !((s_parent[c >> 5] >> (c & 31)) & 1u) && at <= len &&
                     at <= a.table_stride * kKvPageRows;
     need = ok && at % kKvPageRows != 0;
     return ok;
@@ -61,7 +69,9 @@ __global__ __launch_bounds__(256) void k_kv_fork(ForkArgs a) {
   int before = 0, all = 0;  // forks that need a page
   for (int f = tid; f < a.n_forks; f += 256) {
     bool need;
-    fine(f, need);
+    const int p = f == tid ? tid_parent : a.parents[f];
+    const int c = f == tid ? tid_child : a.children[f], at = f == tid ? tid_at : a.at[f], len = f == tid ? tid_len : p >= 0 && p < a.n_seqs ? a.lens[p] : -1;
+    fine(f, p, c, at, len, need);
     all += need;
     before += need && f < mine;
   }
@@ -70,25 +80,20 @@ __global__ __launch_bounds__(256) void k_kv_fork(ForkArgs a) {
   __syncthreads();
   before = (s_count[0][0] + s_count[0][1]) + (s_count[0][2] + s_count[0][3]);
   all = (s_count[1][0] + s_count[1][1]) + (s_count[1][2] + s_count[1][3]);
-  const int have = max(a.n_free[0], 0);
   if (a.free_too && blockIdx.x == 0 && mine == 0 && tid == 0) a.n_free_out[0] = a.n_free[0] - min(all, have);
   if (!a.rows_too) return;
-  bool need, ok = fine(mine, need);
+  bool need, ok = fine(mine, my_parent, my_child, my_at, my_parent_ok ? a.lens[my_parent] : -1, need);
   ok = ok && (!need || before < have);
   if (blockIdx.x == 0 && tid == 0) a.refused[mine] = ok ? 0 : 1;
   if (!ok) return;
-  const int at = a.at[mine], full = at / kKvPageRows;
-  const int *from = a.tables + (int64_t)a.parents[mine] * a.table_stride;
-  const int page = need ? a.free_pages[have - 1 - before] : -1;
+  const int full = my_at / kKvPageRows, page = need ? a.free_pages[have - 1 - before] : -1;
   if (blockIdx.x == 0) {
-    int *to = a.tables + (int64_t)a.children[mine] * a.table_stride;
+    int *to = a.tables + (int64_t)my_child * a.table_stride;
     for (int c = tid; c < full + need; c += 256) to[c] = c < full ? from[c] : page;
-    if (tid == 0) a.lens[a.children[mine]] = at;
+    if (tid == 0) a.lens[my_child] = my_at;
     return;
   }
-  if (!need) return;
-  const int src = from[full];
-  if (src < 0 || src >= a.n_pages || page < 0 || page >= a.n_pages) return;
+  if (!need || src < 0 || src >= a.n_pages || page < 0 || page >= a.n_pages) return;
   const int64_t layer = (int64_t)(blockIdx.x - 1) * a.n_pages * a.page_bytes;
   copy_page(a.k_pages + layer, src, page, a.page_bytes);
   copy_page(a.v_pages + layer, src, page, a.page_bytes);
@@ -131,50 +136,67 @@ __device__ __forceinline__ int2 pack_scan(int2 v, int2 (*part)[kPackThreads / 64
   }
   return {before.x + s.x - v.x, before.y + s.y - v.y};
 }
-// MARK: the pages in use are found here too, as bits in LDS.  Otherwise another launch has marked them in map, where a bit for each would not fit.
+// MARK: the pages in use are found here too, as bits in LDS; a thread then has the 32 pages of a word.  Otherwise another launch has marked them in map, where a bit
+// for each would not fit, and a thread has eight.
 template <bool MARK>
 __global__ __launch_bounds__(kPackThreads) void k_kv_compact_plan(int *map, int2 *moves, int *n_moves, int *free_pages, int *n_free, int n_pages, const int *__restrict__ tables,
                                                                   int table_stride, const int *__restrict__ lens, int n_seqs) {
+  constexpr int EACH = MARK ? 32 : 8;
   __shared__ int2 part[kPackThreads / 64];
   __shared__ unsigned s_bits[MARK ? kBitPages / 32 : 1];
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, groups = (n_pages + EACH - 1) / EACH;
   if (MARK) {
-    for (int i = tid; i < (n_pages + 31) / 32; i += kPackThreads) s_bits[i] = 0;
+    for (int i = tid; i < groups; i += kPackThreads) s_bits[i] = 0;
     __syncthreads();
-    // a wavefront a sequence
-    for (int i = tid >> 6; n_pages > 0 && i < n_seqs; i += kPackThreads / 64) {
-      const int pages = pages_of(lens[i], table_stride);
-      for (int c = tid & 63; c < pages; c += 64) {
-        const int id = tables[(int64_t)i * table_stride + c];
-        if (id >= 0 && id < n_pages) atomicOr(&s_bits[id >> 5], 1u << (id & 31));
+    const int entries = n_pages > 0 ? n_seqs * table_stride : 0;
+    for (int e0 = tid; e0 < entries; e0 += 4 * kPackThreads) {  // (lengths and entries of four at once)
+      int id[4], len[4];
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        const int e = e0 + k * kPackThreads;
+        if (e < entries) id[k] = tables[e], len[k] = lens[e / table_stride];
+      }
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        const int e = e0 + k * kPackThreads;
+        if (e < entries && e % table_stride < pages_of(len[k], table_stride) && id[k] >= 0 && id[k] < n_pages) atomicOr(&s_bits[id[k] >> 5], 1u << (id[k] & 31));
       }
     }
     __syncthreads();
   }
-  auto in_use = [&](int i) { return MARK ? (int)(s_bits[i >> 5] >> (i & 31) & 1u) : map[i]; };
+  auto in_use = [&](int i) {  // of pages EACH i and on, as bits
+    if (MARK) return s_bits[i];
+    unsigned w = 0;
+    for (int k = 0; k < EACH; k++)
+      if (EACH * i + k < n_pages && map[EACH * i + k]) w |= 1u << k;
+    return w;
+  };
   int used = 0;
-  if (MARK)
-    for (int i = tid; i < (n_pages + 31) / 32; i += kPackThreads) used += __popc(s_bits[i]);
-  else
-    for (int i = tid; i < n_pages; i += kPackThreads) used += map[i];
+  for (int i = tid; i < groups; i += kPackThreads) used += __popc(in_use(i));
   int2 total;
   pack_scan({used, 0}, &part, total);
   used = total.x;
   int2 done = {0, 0};
-  for (int i0 = 0; i0 < n_pages; i0 += kPackThreads) {
-    const int i = i0 + tid, there = i < n_pages ? in_use(i) : 0;
-    const int2 mine = {i >= used && there, i < used && !there};
-    const int2 at = pack_scan(mine, &part, total);
-    if (mine.x) moves[done.x + at.x].x = i;
-    if (mine.y) moves[done.y + at.y].y = i;
-    done.x += total.x, done.y += total.y;
-    if (i < n_pages) {
-      map[i] = i;
-      free_pages[i] = i < n_pages - used ? n_pages - 1 - i : -1;
+  for (int i0 = 0; i0 < groups; i0 += kPackThreads) {
+    const int i = i0 + tid, first = EACH * i;
+    unsigned go = 0, hole = 0;
+    if (i < groups) {
+      const unsigned w = in_use(i), all = EACH == 32 && n_pages - first >= 32 ? ~0u : (1u << min(EACH, n_pages - first)) - 1u;
+      const unsigned front = used <= first ? 0u : used - first >= 32 ? ~0u : (1u << (used - first)) - 1u;  // those whose id is below the number in use
+      go = w & ~front, hole = ~w & front & all;
     }
+    int2 at = pack_scan({(int)__popc(go), (int)__popc(hole)}, &part, total);
+    at.x += done.x, at.y += done.y;
+    for (; go; go &= go - 1) moves[at.x++].x = first + __builtin_ctz(go);
+    for (; hole; hole &= hole - 1) moves[at.y++].y = first + __builtin_ctz(hole);
+    done.x += total.x, done.y += total.y;
+  }
+  for (int i = tid; i < n_pages; i += kPackThreads) {
+    free_pages[i] = i < n_pages - used ? n_pages - 1 - i : -1;
+    if (i < used) map[i] = i;
   }
   __syncthreads();
-  for (int k = tid; k < done.x; k += kPackThreads) map[moves[k].x] = moves[k].y;
+  for (int k = tid; k < done.x; k += kPackThreads) map[moves[k].x] = moves[k].y;  // (no other page from `used` on is in use)
   if (tid == 0) n_free[0] = n_pages - used, n_moves[0] = done.x;
 }
 struct MoveArgs {
@@ -255,8 +277,9 @@ int cthip_kv_compact_paged_q4(int *tables_out, int *free_pages, int *n_free, voi
   CTHIP_ARG(n_layers == 0 || n_pages == 0 || (k_pages && v_pages && pools_ok(k_pages, v_pages)));
   int *n_moves = (int *)workspace, *map = n_moves + 16;
   int2 *moves = (int2 *)(map + n_pages + (n_pages & 1));  // (half of the pages at most)
-  // Up to 2^17 pages, and as many table entries as one workgroup reads in the time of the two launches that it saves
-  const bool mark = n_pages == 0 || (n_pages <= kBitPages && (int64_t)n_seqs * table_stride <= (1 << 14));
+  // One launch that reads whole tables, or three of which one reads what is in use of them: full tables of 30 x 32 entries 7.4 us and 11.1, 128 x 128 16.7 and 33.9,
+  // 512 x 128 49 and 110.  An entry costs one workgroup 0.45 ns, the other way a page 1.2 and the launches 3 us.
+  const bool mark = n_pages == 0 || (n_pages <= kBitPages && (int64_t)n_seqs * table_stride <= 2ll * n_pages + (1 << 14));
   if (mark) {
     hipLaunchKernelGGL(k_kv_compact_plan<true>, dim3(1), dim3(kPackThreads), 0, state().stream, map, moves, n_moves, free_pages, n_free, n_pages, tables, table_stride, lens, n_seqs);
   } else {
