@@ -59,7 +59,6 @@ constexpr int kSharedTickets = 4096, kSharedRows = 131072, kMaxWorkers = 3072;
 static_assert(kMaxWorkers <= kSharedTickets && kSplitSlots <= kSharedTickets && kMaxWorkers >= kSplitSlots / 2 &&
                   17 * (kSharedRows - 2 * kMaxWorkers * kTileRows) >= 18 * (kSplitSlots / 2) * kTileRows, "a slot has Dh + 4 floats a row: at Dh = 32 18 / 17 of Dh + 2");
 constexpr int kJobPieces = 1;       // what a job costs besides its pages, in pieces of them (2: 52 us instead of 50, 34 instead of 31, for the batches above)
-constexpr int kJobPages = 3;        // what a job costs a wavefront of its own besides its pages, in pages
 
 // Where several workgroups have shares of a row's shared pages, its stats are a NaN that holds the first one's number, and row of the tile + 256 * shares.
 // Outputs of the first lie in `out`; each workgroup has a slot: outputs of the share that goes on from the workgroup before (it has one of these at most), their
@@ -193,7 +192,7 @@ __device__ __forceinline__ void look(const Kv4Attn &a, const Read<MODE> &read, B
   s.rows = s.row0 == reach && end > s.row0 ? end - s.row0 : 0;
   s.tiles = (s.rows * a.group + kTileRows - 1) / kTileRows;
   const int pages = a.n_pages > 0 && s.len > 0 ? (int)min(((unsigned)s.len + kKvPageRows - 1) / kKvPageRows, (unsigned)a.table_stride) - (attn_behind(MODE) ? s.aside : 0) : 0;
-  s.cost = max(1, (pages + (1 << a.piece_log2) - 1) >> a.piece_log2) + (MODE == kAttnBehindWaves ? kJobPages : kJobPieces);  // (without keys there is still a row to write)
+  s.cost = max(1, (pages + (1 << a.piece_log2) - 1) >> a.piece_log2) + kJobPieces;  // (without keys there is still a row to write)
   s.upto = s.before + wave_scan_int(s.tiles * a.Hkv * s.cost);
 }
 struct Job {
@@ -315,7 +314,7 @@ __global__ __launch_bounds__(256, MODE == kAttnBehindWaves ? (DH == 128 ? 2 : 3)
   const int least = MODE == kAttnShared ? w.len - 1 : (int)min((int64_t)w.len - w.rows + j0, all - 1);
   const int pages = a.n_pages > 0 && last >= 0 ? max(last / kKvPageRows + 1 - w.skip, 0) : 0;
   // its pieces lie on the line behind those that stand for the rest (a job without pages is one piece of none)
-  const int pieces = max(1, (pages + (1 << a.piece_log2) - 1) >> a.piece_log2), line = w.at + (ALONE ? kJobPages : kJobPieces);
+  const int pieces = max(1, (pages + (1 << a.piece_log2) - 1) >> a.piece_log2), line = w.at + kJobPieces;
   const int owner = uniform_fast_div(line, per), shares = uniform_fast_div(line + pieces - 1, per) - owner + 1, share = me - owner;
   const int from_piece = max(x0 - line, 0), to_piece = min(x1 - line, pieces);
   if (from_piece >= to_piece) continue;
@@ -905,7 +904,7 @@ static int launch_kv4_attn(const char *who, Kv4Attn a, int Dh) {
   const int at_once = MODE == kAttnBehindWaves ? std::min(kMaxWorkers / 4, state().compute_units * (Dh == 128 ? 2 : 3) / 8 * 8) : std::min(kSplitSlots / 2, state().compute_units * (Dh == 128 ? 3 : 4) / 8 * 8);
   a.group = a.H / a.Hkv;
   a.piece_log2 = MODE == kAttnBehindWaves ? 0 : 2;  // (the line is shorter than 2^30, and a workgroup's part of it below what fast_div holds for)
-  while (jobs * ((a.table_stride >> a.piece_log2) + 1 + (MODE == kAttnBehindWaves ? kJobPages : kJobPieces)) > std::min((int64_t)INT_MAX / 2, (int64_t)at_once << 20)) a.piece_log2++;
+  while (jobs * ((a.table_stride >> a.piece_log2) + 1 + kJobPieces) > std::min((int64_t)INT_MAX / 2, (int64_t)at_once << 20)) a.piece_log2++;
   const dim3 grid((unsigned)at_once), block(256);
 #define ATT(DH_) hipLaunchKernelGGL((k_kv4_attn<DH_, MODE>), grid, block, (Kv4Lds<DH_, MODE>::BYTES), state().stream, a)
   switch (Dh) {
@@ -963,8 +962,8 @@ int cthip_sdpa_shared_paged_q4(float *out, const float *q, int64_t q_stride, con
   if (n_groups == 0) return launch_kv4_attn<kAttnWhole>(__func__, a, Dh);
   // What a sequence has behind its group's pages is a job a head, often of a page or two.  Where there are more jobs than workgroups, each of a few rows, a job is a
   // wavefront's own: its chain of round trips, not its pages, is what it takes, and four times as many run at once.  32 heads of 128 over 1024 shared rows, 70 rows behind them at
-  // most, both launches: 24 sequences 24.4 us by workgroups, 25.3 by wavefronts; 32: 33.7 and 25.7; 64: 45.2 and 29.3 (600 rows: 50.0 and 43.2); four rows each
-  // 55.4 and 44.6; with eight rows of a head, whose results are joined by fewer lanes then, 512 jobs 34 and 46.
+  // most, both launches: 24 sequences 24.2 us by workgroups, 24.8 by wavefronts; 32: 33.6 and 25.2; 64: 44.7 and 28.9 (600 rows: 49.7 and 40.8); four rows each
+  // 55.3 and 44.5; with eight rows of a head, whose results are joined by fewer lanes then, 512 jobs 34 and 46.
   const bool few = (int64_t)n_rows * (H / Hkv) <= 4ll * n_seqs && (int64_t)n_seqs * Hkv > state().compute_units * (Dh == 128 ? 3 : 4);
   if (const int rc = launch_kv4_attn<kAttnShared>(__func__, a, Dh)) return rc;
   return few ? launch_kv4_attn<kAttnBehindWaves>(__func__, a, Dh) : launch_kv4_attn<kAttnBehind>(__func__, a, Dh);
