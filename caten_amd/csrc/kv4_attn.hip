@@ -667,13 +667,14 @@ __global__ __launch_bounds__(256, MODE == kAttnBehindWaves ? (DH == 128 ? 2 : 3)
           add_up(x, top, sum, 1, [&](int) { return f32x2{its[0], its[1]}; }, [&](int) { return f32x2{whole[0], whole[1]}; });
         } else {
           const unsigned code = __float_as_uint(its[1]);
-          const int first = (int)(__float_as_uint(its[0]) & ~kInShares), n = (int)(code >> 8), row = (int)(code & 255u);
+          // (kept within their ranges: groups or starts that fall leave stats of another call)
+          const int first = (int)(__float_as_uint(its[0]) & ~kInShares), n = min((int)(code >> 8), L::SHARES), row = (int)(code & (kTileRows - 1));
           for (int k0 = 0; k0 < n; k0 += 8) {
             f2_any y[8], ml[8];
 #pragma unroll
             for (int k = 0; k < 8; k++) {
               const int share = min(k0 + k, n - 1);
-              const float *slot = share_slot(a.slots, first + share, DH);
+              const float *slot = share_slot(a.slots, min(first + share, kSplitSlots / 2 - 1), DH);
               ml[k] = *(const f2_any *)(slot + kTileRows * DH + 2 * row + (share == 0 ? 2 * kTileRows : 0));
               y[k] = *(const f2_any *)(share == 0 ? (const float *)to : slot + row * DH + c);
             }
