@@ -47,8 +47,8 @@ struct Verified {
     const int lane = threadIdx.x & 63;
     row0 = a.starts[seq];
     const int end = a.starts[seq + 1];
-    rows = end - row0;
-    there = row0 >= 0 && rows > 0 && end <= a.n_rows;
+    there = row0 >= 0 && end > row0 && end <= a.n_rows;
+    rows = there ? end - row0 : 0;
     stay = 0;
     if (!there) return;
     there = !a.positions || a.positions[row0] >= 0;
@@ -128,7 +128,8 @@ __global__ __launch_bounds__(kDraftThreads) void k_draft_token(DraftArgs a) {
   __shared__ int s_found[2], s_last;
   const int seq = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
   // (all of these at once)
-  const int row0 = a.starts[seq], rows = a.starts[seq + 1] - row0, stay = a.stays(seq)[0];
+  const int row0 = a.starts[seq], end = a.starts[seq + 1], stay = a.stays(seq)[0];
+  const int rows = row0 >= 0 && end > row0 && end <= a.n_rows ? end - row0 : 0;
   const double *sums = a.sums(seq);
   const double left = lane < a.slices ? sums[lane] : 0.0, all = lane < a.slices ? sums[kDraftSlices + lane] : 0.0;
   if (tid == 0) {
@@ -136,8 +137,7 @@ __global__ __launch_bounds__(kDraftThreads) void k_draft_token(DraftArgs a) {
     if (a.lens_out) a.lens_out[seq] = a.lens[seq] - (stay >= 0 ? rows - 1 - stay : 0);
   }
   if (stay < 0) {
-    if (row0 >= 0 && rows > 0 && row0 + rows <= a.n_rows)
-      for (int j = tid; j < rows; j += kDraftThreads) a.tokens_out[row0 + j] = -1;
+    for (int j = tid; j < rows; j += kDraftThreads) a.tokens_out[row0 + j] = -1;
     return;
   }
   const float u = a.uniforms[row0 + rows - 1];

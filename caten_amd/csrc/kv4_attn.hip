@@ -55,7 +55,7 @@ constexpr int kTileRows = 16;       // rows (query row, query head of the group)
 constexpr int kSplitSlots = 2048;   // records of shares in the workspace, two a workgroup
 // in the workspace of a batch with shared pages: tickets, and floats for Dh + 2 of them a row -- records, two a wavefront that has parts of its own, then
 // slots, one a workgroup
-constexpr int kSharedTickets = 4096, kSharedRows = 131072, kMaxWorkers = 3072;
+constexpr int kSharedTickets = 4096, kSharedRows = 131072, kMaxWorkers = 3 * 1024;
 static_assert(kMaxWorkers <= kSharedTickets && kSplitSlots <= kSharedTickets && kMaxWorkers >= kSplitSlots / 2 &&
                   17 * (kSharedRows - 2 * kMaxWorkers * kTileRows) >= 18 * (kSplitSlots / 2) * kTileRows, "a slot has Dh + 4 floats a row: at Dh = 32 18 / 17 of Dh + 2");
 constexpr int kJobPieces = 1;       // what a job costs besides its pages, in pieces of them (2: 52 us instead of 50, 34 instead of 31, for the batches above)
@@ -159,7 +159,7 @@ struct Read {  // of a sequence, or of a group
         int last;
         const int pages = shared_pages(a, i, aside, last);
         len = pages * kKvPageRows;
-        if (pages) row0 = a.starts[aside], end = a.starts[last];
+        row0 = a.starts[aside], end = pages ? a.starts[last] : row0;  // (with every group's first row known none has rows of one in front of it, see `reach`)
       }
     } else {
       if (i < a.n_seqs) len = a.lens[i], row0 = a.starts[i], end = a.starts[i + 1];
@@ -668,7 +668,7 @@ __global__ __launch_bounds__(256, MODE == kAttnBehindWaves ? (DH == 128 ? 2 : 3)
         } else {
           const unsigned code = __float_as_uint(its[1]);
           // (kept within their ranges: groups or starts that fall leave stats of another call)
-          const int first = (int)(__float_as_uint(its[0]) & ~kInShares), n = min((int)(code >> 8), L::SHARES), row = (int)(code & (kTileRows - 1));
+          const int first = (int)(__float_as_uint(its[0]) & 0x3FFFFFu), n = min((int)(code >> 8), L::SHARES), row = (int)(code & (kTileRows - 1));
           for (int k0 = 0; k0 < n; k0 += 8) {
             f2_any y[8], ml[8];
 #pragma unroll

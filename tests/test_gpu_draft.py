@@ -169,6 +169,15 @@ def test_sequences_that_sit_out():
         assert np.array_equal(accepted.numpy(), want["accepted"]) and np.array_equal(to.numpy(), want["lens"])
 
 
+@pytest.mark.parametrize("starts", [[1, -2 ** 31], [5, -2 ** 31 + 3, 4], [-2 ** 31, 2 ** 31 - 1, -1], [-1, 3, 2 ** 31 - 1, 0], [2 ** 31 - 1, -2 ** 31, 2 ** 31 - 1]])
+def test_starts_far_outside(starts):
+    """Differences of starts that 32 bits do not hold are no rows."""
+    from caten_amd import ops
+    target, draft, tokens, uniforms, _, _ = some(np.random.default_rng(12), [3, 2], 100)
+    got = ops.draft_verify(target, draft, tokens, uniforms, starts, np.arange(len(starts) - 1) + 10)
+    same(got, verified(target, draft, tokens, uniforms, starts, np.arange(len(starts) - 1) + 10))
+
+
 def test_strides():
     from caten_amd import _lib, ops
     lib, rng = _lib.init(), np.random.default_rng(10)

@@ -225,13 +225,13 @@ def test_refusals():
     p = d.ptr
 
     def fork(**k):
-        a = dict(t=p, stride=4, lens=p + 1024, n=2, nfo=p + 2048, ref=p + 3072, kp=p + 8192, vp=p + 8192 + 1152 * 4, layers=1, pages=4, par=p + 4096, ch=p + 4352, at=p + 4608, f=0, free=p + 5120,
+        a = dict(t=p, stride=4, lens=p + 1024, n=2, nfo=p + 2048, ref=p + 3000, kp=p + 8192, vp=p + 8192 + 1152 * 4, layers=1, pages=4, par=p + 4096, ch=p + 4352, at=p + 4608, f=0, free=p + 5120,
                  nf=p + 6144, kv=1, dh=32)
         a.update(k)
         return lib.cthip_kv_fork_paged_q4(*a.values())
 
     def compact(**k):
-        a = dict(to=p, free=p + 1024, nf=p + 2048, kp=p + 8192, vp=p + 8192 + 1152 * 4, layers=1, pages=4, t=p + 3072, stride=4, lens=p + 4096, n=0, kv=1, dh=32, ws=p + 5120)
+        a = dict(to=p, free=p + 1024, nf=p + 2048, kp=p + 8192, vp=p + 8192 + 1152 * 4, layers=1, pages=4, t=p + 3000, stride=4, lens=p + 4096, n=0, kv=1, dh=32, ws=p + 5120)
         a.update(k)
         return lib.cthip_kv_compact_paged_q4(*a.values())
 

@@ -225,6 +225,49 @@ def test_rows_behind_the_last_and_a_workspace_of_other_shapes():
         assert not ws.numpy()[:16384].any()
 
 
+@pytest.mark.parametrize("fill", [0x7f, 0xff])
+def test_whatever_the_workspace_holds(fill):
+    """Behind its tickets: large numbers, NaN; the groups are one of many jobs, some of shares, and a batch by wavefronts."""
+    from caten_amd import _lib, ops
+    lib, rng = _lib.init(), np.random.default_rng(20)
+    for H, kv, dh, groups in ((64, 8, 128, [(900, [(1000 + i, 3) for i in range(20)])]), (32, 32, 128, [(300, [(301 + i, 1) for i in range(40)])]), (6, 2, 64, [(640, [(650, 1), (700, 30)])])):
+        cache, tables, lens, starts, borders, shared, held = answers(rng, groups, kv, dh)
+        q = rng.normal(0, 1, (starts[-1], H, dh)).astype(np.float32)
+        raw = np.full(int(lib.cthip_sdpa_shared_paged_q4_workspace(len(q), H, dh)), fill, np.uint8)
+        raw[:16384] = 0
+        ws, dq, dt, dl, ds, dg, dsh = (ops.DeviceArray.from_numpy(np.ascontiguousarray(a, t)) for a, t in ((raw, np.uint8), (q, np.float32), (tables, np.int32), (lens, np.int32),
+                                                                                                            (starts, np.int32), (borders, np.int32), (shared, np.int32)))
+        out = ops.DeviceArray(q.shape, np.float32)
+        _lib.check(lib.cthip_sdpa_shared_paged_q4(out.ptr, dq.ptr, H * dh, cache.k.ptr, cache.v.ptr, cache.n_pages, dt.ptr, tables.shape[1], dl.ptr, ds.ptr, len(lens), len(q), dg.ptr, dsh.ptr,
+                                                  len(shared), H, kv, dh, ws.ptr))
+        got = out.numpy()
+        for i, (k, v) in enumerate(held):
+            close(got[starts[i]:starts[i + 1]], *attention(q[starts[i]:starts[i + 1]], k, v))
+        assert np.array_equal(got, cache.attend_shared(q, tables, lens, starts, borders, shared))
+
+
+@pytest.mark.parametrize("borders", [[1, 3, 2, 3], [-4, 0, 9, 2, 4], [2 ** 31 - 1, -2 ** 31], [1, 3, 1, 3, 1, 3]])
+def test_groups_out_of_order(borders):
+    """Rows of groups that fall or leave the batch are anybody's guess; those of sequences in front of all groups and behind them are right."""
+    from caten_amd import _lib, ops
+    rng = np.random.default_rng(21)
+    H, kv, dh = 8, 2, 64
+    cache, tables, lens, starts, _, _, held = answers(rng, [(200, [(210, 1), (300, 3), (260, 2), (201, 1)]), (0, [(77, 2)])], kv, dh)
+    q = rng.normal(0, 1, (starts[-1], H, dh)).astype(np.float32)
+    lib = _lib.init()
+    raw = np.full(int(lib.cthip_sdpa_shared_paged_q4_workspace(len(q), H, dh)), 0xff, np.uint8)  # (what rows left out find there)
+    raw[:16384] = 0
+    ws, dq, dt, dl, ds, dg, dsh = (ops.DeviceArray.from_numpy(np.ascontiguousarray(a, t)) for a, t in ((raw, np.uint8), (q, np.float32), (tables, np.int32), (lens, np.int32), (starts, np.int32),
+                                                                                                        (borders, np.int32), ([192] * (len(borders) - 1), np.int32)))
+    out = ops.DeviceArray(q.shape, np.float32)
+    _lib.check(lib.cthip_sdpa_shared_paged_q4(out.ptr, dq.ptr, H * dh, cache.k.ptr, cache.v.ptr, cache.n_pages, dt.ptr, tables.shape[1], dl.ptr, ds.ptr, len(lens), len(q), dg.ptr, dsh.ptr,
+                                              len(borders) - 1, H, kv, dh, ws.ptr))
+    got = out.numpy()
+    for i, (k, v) in enumerate(held):
+        if i < min(max(min(borders), 0), 5) or i >= min(max(borders), 5) or borders[0] > 5:
+            close(got[starts[i]:starts[i + 1]], *attention(q[starts[i]:starts[i + 1]], k, v))
+
+
 def test_places_past_32_bits():
     """Shared pages at the end of a pool of more than 2^32 bytes."""
     from caten_amd import ops
