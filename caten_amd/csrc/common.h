@@ -47,6 +47,9 @@ struct State {
   // option "kv_cache": how sessions created afterwards keep their KV cache: 1 = as Q8_0 rows (kvq.hip), 2 = fp32 rows in
   // pages opened as the position reaches them (kvp.hip)
   int kv_cache = 0;
+  // option "shared_prefix": whether cthip_sdpa_shared_paged_q4 takes shared pages once for a group, in a launch of their own: 0 = never, 1 = where
+  // that is faster, 2 = always
+  int shared_prefix = 1;
 };
 State &state();
 // cthip_alloc without the zero fill, for temporaries that are fully written before they are read

@@ -13,6 +13,20 @@
 //   workgroup does before its first page and after its last.
 //   8 sequences of 1500 .. 5000, 32 heads of 128 (93 MB): 28.6 us = 3.25 TB/s, 15 of a tile's 16 rows empty.
 //   One sequence of 701, 12 heads of 64: 8.4 us, a chain of round trips: lengths, table, page, record, ticket, records.
+//
+// Where sequences have their first pages in common, softmax over (shared keys, own keys) is that over each of them, with their maxima and sums, joined.  Two
+// launches of the same loop.  The first takes a group's shared pages for the rows of all its sequences, sixteen of them (a key / value head's) in a tile: every
+// page is read and taken apart once for sixteen rows, not once a sequence, and no row is masked.  The second takes what lies behind
+// them for each sequence and, as it stores a row, joins to it what the first one has left: its outputs, unnormalised, in `out`, its maximum and sum in the
+// workspace, or, where several workgroups had shares of them, all shares (joined by the first launch itself, by ticket, they cost it 4 to 6 us and save
+// the second 3).  Bound by the vector unit, as above: at 128 channels 667 vector instructions a page and 16 rows beside 64 matrix ones; where the own
+// parts are short, by the two launches' chains of round trips.
+//   64 samples, 4100 shared rows and up to 400 own, 32 heads of 128 (44.8 MB): 26 + 23 us; each sequence by itself 490 MB.
+//   3 groups of up to 14 sequences of 5 rows, 9000 shared rows, 64 heads over 8 of 128 (22.8 GFLOP): 76 + 32 us; vector units 70 - 75 % busy, matrix units 24 %.
+//   8 answers, 900 shared rows, 12 heads of 64: 7.2 + 8.7 us.
+// Longer tiles would take a page apart once for more rows, and gain nothing: 256 rows over 32768 shared keys of 8 heads of 128, 115 us, takes 107 - 119 with
+// tiles of 32 rows (half as many wavefronts hide a page's latencies), 124 - 150 with a page taken apart in LDS for four or eight wavefronts (two barriers a page).
+// At 128 channels three workgroups share a compute unit's LDS only up to 53760 bytes each (granules of 1280): the launches over shared pages use 53632.
 #include <algorithm>
 #include <type_traits>
 
@@ -37,6 +51,8 @@ struct Kv4Attn {
   int n_groups;
   float *stats;    // of a (row, head), what the launch over the shared pages has left: maximum and sum, the outputs lying in `out` unnormalised; or whose shares they are
   float *slots;    // of the shares of shared pages
+  int *apart;      // whether a launch over the shared pages is in front, which says so there (null: none is, they are every sequence's own)
+  int always;      // whatever it gains
 };
 // What a launch is: a batch by itself; the pages that a group's sequences share, for all of its rows; what the sequences have behind those, a
 // job taken by workgroups as in the others, or by wavefronts, each with parts of its own
@@ -57,7 +73,7 @@ constexpr int kSplitSlots = 2048;   // records of shares in the workspace, two a
 // slots, one a workgroup
 constexpr int kSharedTickets = 4096, kSharedRows = 131072, kMaxWorkers = 3 * 1024;
 static_assert(kMaxWorkers <= kSharedTickets && kSplitSlots <= kSharedTickets && kMaxWorkers >= kSplitSlots / 2 &&
-                  17 * (kSharedRows - 2 * kMaxWorkers * kTileRows) >= 18 * (kSplitSlots / 2) * kTileRows, "a slot has Dh + 4 floats a row: at Dh = 32 18 / 17 of Dh + 2");
+                  17 * (kSharedRows - 2 * kMaxWorkers * kTileRows - 1) >= 18 * (kSplitSlots / 2) * kTileRows, "a slot has Dh + 4 floats a row: at Dh = 32 18 / 17 of Dh + 2");
 constexpr int kJobPieces = 1;       // what a job costs besides its pages, in pieces of them (2: 52 us instead of 50, 34 instead of 31, for the batches above)
 
 // Where several workgroups have shares of a row's shared pages, its stats are a NaN that holds the first one's number, and row of the tile + 256 * shares.
@@ -131,19 +147,30 @@ struct Batch {
   int first = 0, before = 0;  // of the 64 sequences in the lanes: the first, and the cost in front of it
   int reach = 0;              // the largest start up to the last of them
   int len, row0, rows, tiles, cost, upto;  // this lane's; cost: of one job; upto: of all up to the end of this sequence
-  int aside;  // kAttnShared: the group's first sequence; kAttnBehind: pages of the sequence that are shared
+  int leader;  // the first sequence of the group
+  int aside;   // pages of the sequence that are shared
   // A wavefront keeps them in LDS while it works on a job: they are needed again for the next one only.
   __device__ __forceinline__ void put(int (*to)[64]) const {
     const int l = lane_now();
-    to[0][l] = len, to[1][l] = row0, to[2][l] = rows, to[3][l] = tiles, to[4][l] = cost, to[5][l] = upto;
-    if constexpr (MODE != kAttnWhole) to[6][l] = aside;
+    to[0][l] = len, to[1][l] = row0, to[2][l] = rows, to[3][l] = attn_behind(MODE) ? aside : tiles, to[4][l] = cost, to[5][l] = upto;
+    if constexpr (MODE != kAttnWhole) to[6][l] = leader;
   }
-  __device__ __forceinline__ void get(const int (*from)[64]) {
+  __device__ __forceinline__ void get(const int (*from)[64], int group) {
     const int l = lane_now();
-    len = from[0][l], row0 = from[1][l], rows = from[2][l], tiles = from[3][l], cost = from[4][l], upto = from[5][l];
-    if constexpr (MODE != kAttnWhole) aside = from[6][l];
+    len = from[0][l], row0 = from[1][l], rows = from[2][l], cost = from[4][l], upto = from[5][l];
+    if constexpr (MODE != kAttnWhole) leader = from[6][l];
+    if constexpr (attn_behind(MODE)) aside = from[3][l], tiles = (rows * group + kTileRows - 1) / kTileRows;
+    else tiles = from[3][l];
   }
 };
+// What a launch over shared pages saves less what joining its rows costs, as channels of pages that a tile takes apart, of a group of `members` sequences with
+// `rows` rows in `tiles` tiles a head; by themselves they have one each, or on average half a one more than their rows fill.
+__host__ __device__ __forceinline__ float sharing_gains(int rows, int members, int tiles, int pages, int group, int H, int dh) {
+  const float each = fminf((float)members, (float)rows), fill = (float)rows * (float)group / kTileRows;
+  const float own = rows <= members ? (float)rows * (float)((group + kTileRows - 1) / kTileRows) : fmaxf(each, fill + 0.5f * each);
+  return fmaxf(own - (float)tiles, 0.0f) * (float)pages * (float)(H / group * dh) - 128.0f * (float)rows * (float)H;
+}
+constexpr float kSharingCosts = 500000.0f;  // the launch, in the same
 // The pages that group g's sequences share, 0 where there is one of them only (it reads its pages by itself), and the first and the end of them
 __device__ __forceinline__ int shared_pages(const Kv4Attn &a, int g, int &first, int &end) {
   first = min(max(a.groups[g], 0), a.n_seqs), end = min(max(a.groups[g + 1], 0), a.n_seqs);
@@ -151,15 +178,15 @@ __device__ __forceinline__ int shared_pages(const Kv4Attn &a, int g, int &first,
 }
 template <int MODE>
 struct Read {  // of a sequence, or of a group
-  int len = 0, row0 = 0, end = 0, aside = 0;
+  int len = 0, row0 = 0, end = 0, leader = 0, aside = 0;  // aside: kAttnShared: the group's sequences
   __device__ __forceinline__ Read(const Kv4Attn &a, int first) {
     const int i = first + lane_now();
     if constexpr (MODE == kAttnShared) {
       if (i < a.n_groups) {
         int last;
-        const int pages = shared_pages(a, i, aside, last);
-        len = pages * kKvPageRows;
-        row0 = a.starts[aside], end = pages ? a.starts[last] : row0;  // (with every group's first row known none has rows of one in front of it, see `reach`)
+        const int pages = shared_pages(a, i, leader, last);
+        len = pages * kKvPageRows, aside = last - leader;
+        row0 = a.starts[leader], end = pages ? a.starts[last] : row0;  // (with every group's first row known none has rows of one in front of it, see `reach`)
       }
     } else {
       if (i < a.n_seqs) len = a.lens[i], row0 = a.starts[i], end = a.starts[i + 1];
@@ -173,7 +200,7 @@ struct Read {  // of a sequence, or of a group
           }
           int g0, g1;
           const int pages = shared_pages(a, lo, g0, g1);
-          if (i >= g0 && i < g1) aside = pages;
+          if (i >= g0 && i < g1) aside = pages, leader = g0;
         }
       }
     }
@@ -182,33 +209,35 @@ struct Read {  // of a sequence, or of a group
 template <int MODE>
 __device__ __forceinline__ int in_all(const Kv4Attn &a) { return MODE == kAttnShared ? a.n_groups : a.n_seqs; }
 template <int MODE>
-__device__ __forceinline__ void look(const Kv4Attn &a, const Read<MODE> &read, Batch<MODE> &s) {
+__device__ __forceinline__ void look(const Kv4Attn &a, const Read<MODE> &read, Batch<MODE> &s, bool apart) {
   s.len = max(read.len, 0), s.row0 = read.row0;
-  if constexpr (MODE != kAttnWhole) s.aside = read.aside;
+  if constexpr (MODE != kAttnWhole) s.leader = read.leader, s.aside = read.aside;
   const int end = min(read.end, a.n_rows);
   // (rows in front of an earlier sequence's are nobody's: no row is two sequences', and the costs of all stay within their bound)
   const int reach = max(s.reach, wave_scan_max(s.row0));
   s.reach = __builtin_amdgcn_readlane(reach, 63);
   s.rows = s.row0 == reach && end > s.row0 ? end - s.row0 : 0;
   s.tiles = (s.rows * a.group + kTileRows - 1) / kTileRows;
-  const int pages = a.n_pages > 0 && s.len > 0 ? (int)min(((unsigned)s.len + kKvPageRows - 1) / kKvPageRows, (unsigned)a.table_stride) - (attn_behind(MODE) ? s.aside : 0) : 0;
+  int pages = a.n_pages > 0 && s.len > 0 ? (int)min(((unsigned)s.len + kKvPageRows - 1) / kKvPageRows, (unsigned)a.table_stride) : 0;
+  if constexpr (attn_behind(MODE)) pages = apart ? pages - s.aside : max(pages, s.aside);
   s.cost = max(1, (pages + (1 << a.piece_log2) - 1) >> a.piece_log2) + kJobPieces;  // (without keys there is still a row to write)
   s.upto = s.before + wave_scan_int(s.tiles * a.Hkv * s.cost);
 }
 struct Job {
   int seq, head, tile;
   int skip;             // pages of the sequence in front of the job's
+  int common, leader;   // pages of it that are its group's, and the sequence that has them
   int len, rows, row0;  // of the sequence: keys, rows of this step and the first of them
   int at, cost;         // its place on the line of all costs
 };
 // the job at a place on the line, which lies in front of its end; fronts: what 64 sequences at a time have in front of them, cost and largest start
 template <int MODE>
-__device__ __forceinline__ bool find_job(const Kv4Attn &a, Batch<MODE> &s, int (*kept)[64], const int (*fronts)[64], int place, Job &j) {
+__device__ __forceinline__ bool find_job(const Kv4Attn &a, Batch<MODE> &s, int (*kept)[64], const int (*fronts)[64], int place, bool apart, Job &j) {
   if (place < s.before || place >= __builtin_amdgcn_readlane(s.upto, 63)) {
     const int lane = lane_now();
     const int block = __popcll(__ballot(lane * 64 < in_all<MODE>(a) && fronts[0][lane] <= place)) - 1;
     s.first = 64 * block, s.before = __builtin_amdgcn_readfirstlane(fronts[0][block]), s.reach = __builtin_amdgcn_readfirstlane(fronts[1][block]);
-    look(a, Read<MODE>(a, s.first), s);
+    look(a, Read<MODE>(a, s.first), s, apart);
     s.put(kept);
   }
   const unsigned long long past = __ballot(s.upto > place);
@@ -218,8 +247,10 @@ __device__ __forceinline__ bool find_job(const Kv4Attn &a, Batch<MODE> &s, int (
   j.cost = __builtin_amdgcn_readlane(s.cost, l);
   const int start = __builtin_amdgcn_readlane(s.upto, l) - all * j.cost, job = uniform_fast_div(place - start, j.cost);
   j.at = start + job * j.cost;
-  j.seq = MODE == kAttnShared ? __builtin_amdgcn_readlane(s.aside, l) : s.first + l;
-  j.skip = attn_behind(MODE) ? __builtin_amdgcn_readlane(s.aside, l) : 0;
+  if constexpr (MODE != kAttnWhole) j.leader = __builtin_amdgcn_readlane(s.leader, l);
+  j.seq = MODE == kAttnShared ? j.leader : s.first + l;
+  const int aside = attn_behind(MODE) ? __builtin_amdgcn_readlane(s.aside, l) : 0;
+  j.skip = apart ? aside : 0, j.common = apart ? 0 : aside;
   j.head = tiles == 1 ? job : uniform_fast_div(job, tiles);
   // tiles from both ends in turn: in a prompt's own pages late rows see more than early ones, and a workgroup gets some of each
   const int t = job - j.head * tiles;
@@ -241,6 +272,13 @@ struct Kv4Lds {
   static constexpr int SHARES = DH == 32 ? 128 : 256;  // of one tile, at most: their records are added up by one workgroup
   static_assert(WAVE >= kTileRows * (DH + 4) * 4 && 4 * WAVE >= 4 * SHARES * kTileRows, "results, and weights of shares, in the pages' place");
 };
+
+// the other lane's; with its number, as above, asked for anew
+template <int MODE, class T>
+__device__ __forceinline__ T across(T v, int lanes) {
+  if constexpr (attn_behind(MODE)) return __builtin_bit_cast(T, __builtin_amdgcn_ds_bpermute((lane_now() ^ lanes) << 2, __builtin_bit_cast(int, v)));
+  else return __shfl_xor(v, lanes, 64);
+}
 
 // One page for one wavefront and 16 rows.  S^T = K Q^T and O^T = V^T P^T: the row is the lane's number modulo 16 throughout (scores,
 // maxima, sums and outputs), lane group g = lane / 16 holds keys 16 s + 4 g + i of the page and channels 4 g + i of a result tile.
@@ -267,14 +305,19 @@ __global__ __launch_bounds__(256, MODE == kAttnBehindWaves ? (DH == 128 ? 2 : 3)
   // a wavefront's results lie where its own pages did
   auto s_o = [&](int wave, int row) { return (float *)(smem + wave * L::WAVE) + row * (DH + 4); };
   const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int G = a.group;
+  int G = a.group;
   int total = 0, longest = 0;
+  float gain = 0.0f;
   Batch<MODE> s;
+  const bool apart = attn_behind(MODE) && a.apart && __builtin_amdgcn_readfirstlane(*a.apart);
   for (Read<MODE> read(a, 0);;) {
     const bool more = s.first + 64 < in_all<MODE>(a);
     if (lane_now() == 0) s_fronts[0][s.first >> 6] = s.before, s_fronts[1][s.first >> 6] = s.reach;
     const Read<MODE> next(a, more ? s.first + 64 : in_all<MODE>(a));  // (on its way while these are looked at)
-    look(a, read, s);
+    look(a, read, s, apart);
+    if constexpr (MODE == kAttnShared) {
+      if (s.tiles && s.len) gain += sharing_gains(s.rows, s.aside, s.tiles, s.len / kKvPageRows, G, a.H, DH);
+    }
     longest = max(longest, s.tiles ? s.cost : 0);
     total = __builtin_amdgcn_readlane(s.upto, 63);
     if (!more) break;
@@ -283,11 +326,18 @@ __global__ __launch_bounds__(256, MODE == kAttnBehindWaves ? (DH == 128 ? 2 : 3)
     read = next;
   }
   longest = __builtin_amdgcn_readlane(wave_scan_max(longest), 63);
+  if constexpr (MODE == kAttnShared) {  // (every wavefront finds the same)
+    for (int o = 32; o > 0; o >>= 1) gain += __shfl_xor(gain, o, 64);
+    const int pays = __builtin_amdgcn_readfirstlane(a.always || gain > kSharingCosts);
+    if (blockIdx.x == 0 && threadIdx.x == 0) *a.apart = pays;
+    if (!pays) return;
+  }
   s.put(s_seqs[wv]);
   // A part's length: of the whole, or what keeps a tile's shares below their number, or, since its last workgroup reads all of a tile's
   // records, as many pieces as come out about even with that (sqrt(longest / 20): 32768 keys of one head of 128 27.3 -> 22.5 us, 131072 38.0 -> 34.1).
   const int even = __builtin_amdgcn_readfirstlane((int)__builtin_sqrtf((ALONE ? 0.1f : 0.05f) * (float)longest)), workers = (int)gridDim.x * (ALONE ? 4 : 1);
-  const int per = max(max(uniform_fast_div(total + workers - 1, workers), (longest + L::SHARES - 2) / (L::SHARES - 1)), even);
+  int per = max(max(uniform_fast_div(total + workers - 1, workers), (longest + L::SHARES - 2) / (L::SHARES - 1)), even);
+  if constexpr (attn_behind(MODE)) per = __builtin_amdgcn_readfirstlane(per);
   // Workgroups are dealt to the eight XCDs in turn.  Neighbours on the line, which may read the same pages and join their shares, on one of
   // them, and all XCDs alike where there are fewer parts than workgroups (one sequence of 2048, 8 heads of 128, 72 parts: 15.3 us on one XCD,
   // 10.8 on eight).
@@ -296,9 +346,10 @@ __global__ __launch_bounds__(256, MODE == kAttnBehindWaves ? (DH == 128 ? 2 : 3)
   const int x0 = (int)min((int64_t)me * per, (int64_t)total), x1 = min(total - x0, per) + x0;
   for (int x = x0; x < x1;) {
   Job w;
-  if (x != x0) s.get(s_seqs[wv]);
-  if (!find_job(a, s, s_seqs[wv], s_fronts, x, w)) break;
+  if (x != x0) s.get(s_seqs[wv], G);
+  if (!find_job(a, s, s_seqs[wv], s_fronts, x, apart, w)) break;
   x = w.at + w.cost;
+  if constexpr (attn_behind(MODE)) asm volatile("" : "+s"(G), "+s"(per));  // (their reciprocals are not held over the loop)
   const int lane = lane_now();
   const int n = lane & 15, g = lane >> 4;
   // this lane's row
@@ -306,12 +357,12 @@ __global__ __launch_bounds__(256, MODE == kAttnBehindWaves ? (DH == 128 ? 2 : 3)
   const bool active = j < w.rows;
   const int head = w.head * G + rho - j * G;
   const int64_t all = (int64_t)a.table_stride * kKvPageRows;
-  // the last key it sees; of shared pages all
-  const int limit = !active ? -1 : MODE == kAttnShared ? w.len - 1 : (int)min((int64_t)w.len - w.rows + j, all - 1);
+  // the last key that row j of the sequence sees; of shared pages all
+  auto reaches = [&](int j) { return MODE == kAttnShared ? w.len - 1 : max((int)min((int64_t)w.len - w.rows + j, all - 1), attn_behind(MODE) ? w.common * kKvPageRows - 1 : INT_MIN); };
+  const int limit = !active ? -1 : reaches(j);
   // pages that any row / every row of the tile sees (rows rise with n)
   const int j1 = min(w.rows - 1, uniform_fast_div(w.tile * kTileRows + kTileRows - 1, G)), j0 = uniform_fast_div(w.tile * kTileRows, G);
-  const int last = MODE == kAttnShared ? w.len - 1 : (int)min((int64_t)w.len - w.rows + j1, all - 1);
-  const int least = MODE == kAttnShared ? w.len - 1 : (int)min((int64_t)w.len - w.rows + j0, all - 1);
+  const int last = __builtin_amdgcn_readfirstlane(reaches(j1)), least = __builtin_amdgcn_readfirstlane(reaches(j0));  // (uniform)
   const int pages = a.n_pages > 0 && last >= 0 ? max(last / kKvPageRows + 1 - w.skip, 0) : 0;
   // its pieces lie on the line behind those that stand for the rest (a job without pages is one piece of none)
   const int pieces = max(1, (pages + (1 << a.piece_log2) - 1) >> a.piece_log2), line = w.at + kJobPieces;
@@ -322,12 +373,16 @@ __global__ __launch_bounds__(256, MODE == kAttnBehindWaves ? (DH == 128 ? 2 : 3)
 
   // page ids of the next 64 pages of this wavefront, one a lane
   const int *table = a.tables + (int64_t)w.seq * a.table_stride + w.skip;
+  // (what is needed once in 64 pages is kept in LDS, not in registers)
+  volatile int *const lot = s_ticket + 4 + 2 * wv;
+  if constexpr (attn_behind(MODE)) lot[0] = w.common, lot[1] = w.leader - w.seq;
+  auto entry = [&](int p) { return table[attn_behind(MODE) && p < lot[0] ? p + (int64_t)lot[1] * a.table_stride : p]; };
   int ids, ids_from;
   auto page_id = [&](int k) {  // k: this wavefront's k-th page (the same in every lane)
     if (k >= ids_from + 64) {
       ids_from = k;
       const int p = ALONE ? p0 + k + lane : p0 + wv + 4 * (k + lane);
-      ids = p < p1 ? table[p] : -1;
+      ids = p < p1 ? entry(p) : -1;
       asm volatile("" : "+v"(ids));  // (waited for here: behind the branch it would be waited for with all pages on their way, page after page)
     }
     return __builtin_amdgcn_readlane(ids, k - ids_from);
@@ -336,7 +391,7 @@ __global__ __launch_bounds__(256, MODE == kAttnBehindWaves ? (DH == 128 ? 2 : 3)
   {
     const int p = ALONE ? p0 + lane : p0 + wv + 4 * lane;
     ids_from = 0;
-    ids = p < p1 ? table[p] : -1;
+    ids = p < p1 ? entry(p) : -1;
   }
   auto valid = [&](int id) { return id >= 0 && id < a.n_pages; };
   const unsigned char *ring = smem + wv * L::WAVE;
@@ -386,11 +441,11 @@ __global__ __launch_bounds__(256, MODE == kAttnBehindWaves ? (DH == 128 ? 2 : 3)
 #pragma unroll
       for (int e = 0; e < 8; e++) mine8[e] = b == 0 || wv == b ? x[b][e] : mine8[e];
     }
-    top = fmaxf(top, __shfl_xor(top, 16, 64));
-    top = fmaxf(top, __shfl_xor(top, 32, 64));
+    top = fmaxf(top, across<MODE>(top, 16));
+    top = fmaxf(top, across<MODE>(top, 32));
     int bad = odd;
-    bad |= __shfl_xor(bad, 16, 64);
-    bad |= __shfl_xor(bad, 32, 64);
+    bad |= across<MODE>(bad, 16);
+    bad |= across<MODE>(bad, 32);
     // 2^(9 - e), e the exponent of the row's largest, brings that into [2^9, 2^10): fp16's own 11 bits, and 11 below them
     const int e = min(max((int)(__float_as_uint(top) >> 23) - 127, -100), 127);
     const float up = __uint_as_float((unsigned)(127 + 9 - e) << 23), down = __uint_as_float((unsigned)(127 - 9 + e) << 23);
@@ -961,6 +1016,11 @@ int cthip_sdpa_shared_paged_q4(float *out, const float *q, int64_t q_stride, con
   a.groups = groups, a.shared = shared, a.n_groups = n_groups;
   a.slots = a.parts + (int64_t)2 * kMaxWorkers * kTileRows * (Dh + 2), a.stats = a.parts + (int64_t)kSharedRows * (Dh + 2);
   if (n_groups == 0) return launch_kv4_attn<kAttnWhole>(__func__, a, Dh);
+  const int G = H / Hkv, tiles = (int)std::min(((int64_t)n_rows * G + kTileRows - 1) / kTileRows, (int64_t)INT_MAX);
+  a.always = state().shared_prefix == 2;
+  if (state().shared_prefix == 0 || (state().shared_prefix == 1 && sharing_gains(n_rows, n_seqs, tiles, table_stride, G, H, Dh) <= kSharingCosts))
+    return launch_kv4_attn<kAttnBehind>(__func__, a, Dh);
+  a.apart = (int *)(a.slots + (int64_t)kSplitSlots / 2 * kTileRows * (Dh + 4));
   // What a sequence has behind its group's pages is a job a head, often of a page or two.  Where there are more jobs than workgroups, each of a few rows, a job is a
   // wavefront's own: its chain of round trips, not its pages, is what it takes, and four times as many run at once.  32 heads of 128 over 1024 shared rows, 70 rows behind them at
   // most, both launches: 24 sequences 24.2 us by workgroups, 24.8 by wavefronts; 32: 33.6 and 25.2; 64: 44.7 and 28.9 (600 rows: 49.7 and 40.8); four rows each

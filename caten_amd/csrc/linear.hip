@@ -888,6 +888,11 @@ int cthip_set_option(const char *name, int value) {
     state().kv_cache = value;
     return 0;
   }
+  if (!strcmp(name, "shared_prefix")) {
+    if (value < 0 || value > 2) return fail(CTHIP_E_BAD_ARG, "cthip_set_option: shared_prefix is 0 (never), 1 (where that is faster) or 2 (always)");
+    state().shared_prefix = value;
+    return 0;
+  }
   if (!strcmp(name, "weight_planes")) {
     if (value < 0) return fail(CTHIP_E_BAD_ARG, "cthip_set_option: weight_planes is a limit in MiB");
     weight_planes_limit((int64_t)value << 20);

@@ -8,6 +8,15 @@ from tests.test_gpu_paged_q4 import PAGE, _fill, attention, close
 pytestmark = pytest.mark.gpu
 
 
+@pytest.fixture(autouse=True, params=[2, 0], ids=["apart", "together"])
+def way(request):
+    """Shared pages in a launch of their own, or as every sequence's own: option "shared_prefix"."""
+    from caten_amd import _lib
+    _lib.check(_lib.init().cthip_set_option(b"shared_prefix", request.param))
+    yield request.param
+    _lib.check(_lib.load().cthip_set_option(b"shared_prefix", 1))
+
+
 def answers(rng, groups, kv, dh, spare=3):
     """groups: (rows shared, [(rows held in all, query rows)]); pages in any order, what no row was written to is NaN.
     (cache, tables, lens, starts, borders, shared, [(k, v)])"""
@@ -308,3 +317,27 @@ def test_refusals():
     for groups, shared, dh in (([0, 1], [64, 64], 64), ([0, 1], [64], 32)):
         with pytest.raises(ValueError):
             cache.attend_shared(np.zeros((1, 2, dh)), np.zeros((1, 1)), [1], [0, 1], groups, shared)
+
+
+@pytest.mark.parametrize("H,kv,dh,groups,stride,want", [
+    (12, 12, 64, [(600, [(601, 1)] * 4)], None, 0),          # nothing to gain, known from the sizes
+    (12, 12, 64, [(600, [(601, 1)] * 4)], 4096, 0),          # from the groups only
+    (32, 32, 128, [(1300, [(1301, 1)] * 40)], None, 2),
+    (64, 8, 128, [(1300, [(1301, 6)] * 30)], None, 0),       # tiles as full without sharing
+    (32, 32, 128, [(640, [(650, 1)] * 20), (1300, [(1301, 1)] * 12)], 100, 2)])
+def test_the_rule(H, kv, dh, groups, stride, want, way):
+    """By default the way is taken that is faster; either has its own roundings."""
+    from caten_amd import _lib
+    rng = np.random.default_rng(22)
+    cache, tables, lens, starts, borders, shared, held = answers(rng, groups, kv, dh)
+    if stride:
+        tables = np.concatenate([tables, np.full((len(tables), stride - tables.shape[1]), -1, np.int32)], 1)
+    q = rng.normal(0, 1, (starts[-1], H, dh)).astype(np.float32)
+    forced = cache.attend_shared(q, tables, lens, starts, borders, shared)
+    _lib.check(_lib.load().cthip_set_option(b"shared_prefix", 1))
+    got = cache.attend_shared(q, tables, lens, starts, borders, shared)
+    assert np.array_equal(got, forced) == (way == want)
+    for i, (k, v) in enumerate(held):
+        close(got[starts[i]:starts[i + 1]], *attention(q[starts[i]:starts[i + 1]], k, v))
+    for bad in (-1, 3):
+        assert _lib.load().cthip_set_option(b"shared_prefix", bad) == _lib.E_BAD_ARG
