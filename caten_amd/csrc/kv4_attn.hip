@@ -51,13 +51,15 @@ struct Kv4Attn {
   int n_groups;
   float *stats;    // of a (row, head), what the launch over the shared pages has left: maximum and sum, the outputs lying in `out` unnormalised; or whose shares they are
   float *slots;    // of the shares of shared pages
-  int *apart;      // whether a launch over the shared pages is in front, which says so there (null: none is, they are every sequence's own)
-  int always;      // whatever it gains
+  int *apart;      // whether the launch over the shared pages has taken them or left them to the one behind, which it says there
+  int always;      // it takes them whatever it gains
 };
-// What a launch is: a batch by itself; the pages that a group's sequences share, for all of its rows; what the sequences have behind those, a
-// job taken by workgroups as in the others, or by wavefronts, each with parts of its own
-enum { kAttnWhole = 0, kAttnShared = 1, kAttnBehind = 2, kAttnBehindWaves = 3 };
-constexpr bool attn_behind(int mode) { return mode >= kAttnBehind; }
+// What a launch is: a batch by itself; the pages that a group's sequences share, for all of its rows; what the sequences have behind those (or all, where the launch over
+// the shared pages has left them), a job taken by workgroups as in the others, or by wavefronts, each with parts of its own; all, the shared pages as everyone's
+enum { kAttnWhole = 0, kAttnShared = 1, kAttnBehind = 2, kAttnBehindWaves = 3, kAttnTogether = 4 };
+constexpr bool attn_grouped(int mode) { return mode >= kAttnBehind; }  // of sequences in groups
+constexpr bool attn_behind(int mode) { return mode == kAttnBehind || mode == kAttnBehindWaves; }
+constexpr bool attn_one(int mode) { return mode == kAttnWhole || mode == kAttnTogether; }  // nothing of another launch is joined
 
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef _Float16 half4 __attribute__((ext_vector_type(4)));
@@ -152,14 +154,14 @@ struct Batch {
   // A wavefront keeps them in LDS while it works on a job: they are needed again for the next one only.
   __device__ __forceinline__ void put(int (*to)[64]) const {
     const int l = lane_now();
-    to[0][l] = len, to[1][l] = row0, to[2][l] = rows, to[3][l] = attn_behind(MODE) ? aside : tiles, to[4][l] = cost, to[5][l] = upto;
+    to[0][l] = len, to[1][l] = row0, to[2][l] = rows, to[3][l] = attn_grouped(MODE) ? aside : tiles, to[4][l] = cost, to[5][l] = upto;
     if constexpr (MODE != kAttnWhole) to[6][l] = leader;
   }
   __device__ __forceinline__ void get(const int (*from)[64], int group) {
     const int l = lane_now();
     len = from[0][l], row0 = from[1][l], rows = from[2][l], cost = from[4][l], upto = from[5][l];
     if constexpr (MODE != kAttnWhole) leader = from[6][l];
-    if constexpr (attn_behind(MODE)) aside = from[3][l], tiles = (rows * group + kTileRows - 1) / kTileRows;
+    if constexpr (attn_grouped(MODE)) aside = from[3][l], tiles = (rows * group + kTileRows - 1) / kTileRows;
     else tiles = from[3][l];
   }
 };
@@ -170,7 +172,7 @@ __host__ __device__ __forceinline__ float sharing_gains(int rows, int members, i
   const float own = rows <= members ? (float)rows * (float)((group + kTileRows - 1) / kTileRows) : fmaxf(each, fill + 0.5f * each);
   return fmaxf(own - (float)tiles, 0.0f) * (float)pages * (float)(H / group * dh) - 128.0f * (float)rows * (float)H;
 }
-constexpr float kSharingCosts = 500000.0f;  // the launch, in the same
+constexpr float kSharingCosts = 500000.0f;  // the launch, in the same; once it is there it shares what gains anything
 // The pages that group g's sequences share, 0 where there is one of them only (it reads its pages by itself), and the first and the end of them
 __device__ __forceinline__ int shared_pages(const Kv4Attn &a, int g, int &first, int &end) {
   first = min(max(a.groups[g], 0), a.n_seqs), end = min(max(a.groups[g + 1], 0), a.n_seqs);
@@ -190,7 +192,7 @@ struct Read {  // of a sequence, or of a group
       }
     } else {
       if (i < a.n_seqs) len = a.lens[i], row0 = a.starts[i], end = a.starts[i + 1];
-      if constexpr (attn_behind(MODE)) {
+      if constexpr (attn_grouped(MODE)) {
         if (i < a.n_seqs && a.n_groups > 0) {
           int lo = 0, hi = a.n_groups;  // groups[lo] <= i where there is such a group
           while (hi - lo > 1) {
@@ -219,7 +221,7 @@ __device__ __forceinline__ void look(const Kv4Attn &a, const Read<MODE> &read, B
   s.rows = s.row0 == reach && end > s.row0 ? end - s.row0 : 0;
   s.tiles = (s.rows * a.group + kTileRows - 1) / kTileRows;
   int pages = a.n_pages > 0 && s.len > 0 ? (int)min(((unsigned)s.len + kKvPageRows - 1) / kKvPageRows, (unsigned)a.table_stride) : 0;
-  if constexpr (attn_behind(MODE)) pages = apart ? pages - s.aside : max(pages, s.aside);
+  if constexpr (attn_grouped(MODE)) pages = apart ? pages - s.aside : max(pages, s.aside);
   s.cost = max(1, (pages + (1 << a.piece_log2) - 1) >> a.piece_log2) + kJobPieces;  // (without keys there is still a row to write)
   s.upto = s.before + wave_scan_int(s.tiles * a.Hkv * s.cost);
 }
@@ -249,7 +251,7 @@ __device__ __forceinline__ bool find_job(const Kv4Attn &a, Batch<MODE> &s, int (
   j.at = start + job * j.cost;
   if constexpr (MODE != kAttnWhole) j.leader = __builtin_amdgcn_readlane(s.leader, l);
   j.seq = MODE == kAttnShared ? j.leader : s.first + l;
-  const int aside = attn_behind(MODE) ? __builtin_amdgcn_readlane(s.aside, l) : 0;
+  const int aside = attn_grouped(MODE) ? __builtin_amdgcn_readlane(s.aside, l) : 0;
   j.skip = apart ? aside : 0, j.common = apart ? 0 : aside;
   j.head = tiles == 1 ? job : uniform_fast_div(job, tiles);
   // tiles from both ends in turn: in a prompt's own pages late rows see more than early ones, and a workgroup gets some of each
@@ -276,7 +278,7 @@ struct Kv4Lds {
 // the other lane's; with its number, as above, asked for anew
 template <int MODE, class T>
 __device__ __forceinline__ T across(T v, int lanes) {
-  if constexpr (attn_behind(MODE)) return __builtin_bit_cast(T, __builtin_amdgcn_ds_bpermute((lane_now() ^ lanes) << 2, __builtin_bit_cast(int, v)));
+  if constexpr (attn_grouped(MODE)) return __builtin_bit_cast(T, __builtin_amdgcn_ds_bpermute((lane_now() ^ lanes) << 2, __builtin_bit_cast(int, v)));
   else return __shfl_xor(v, lanes, 64);
 }
 
@@ -309,7 +311,7 @@ __global__ __launch_bounds__(256, MODE == kAttnBehindWaves ? (DH == 128 ? 2 : 3)
   int total = 0, longest = 0;
   float gain = 0.0f;
   Batch<MODE> s;
-  const bool apart = attn_behind(MODE) && a.apart && __builtin_amdgcn_readfirstlane(*a.apart);
+  const bool apart = attn_behind(MODE) && __builtin_amdgcn_readfirstlane(*a.apart);
   for (Read<MODE> read(a, 0);;) {
     const bool more = s.first + 64 < in_all<MODE>(a);
     if (lane_now() == 0) s_fronts[0][s.first >> 6] = s.before, s_fronts[1][s.first >> 6] = s.reach;
@@ -328,7 +330,7 @@ __global__ __launch_bounds__(256, MODE == kAttnBehindWaves ? (DH == 128 ? 2 : 3)
   longest = __builtin_amdgcn_readlane(wave_scan_max(longest), 63);
   if constexpr (MODE == kAttnShared) {  // (every wavefront finds the same)
     for (int o = 32; o > 0; o >>= 1) gain += __shfl_xor(gain, o, 64);
-    const int pays = __builtin_amdgcn_readfirstlane(a.always || gain > kSharingCosts);
+    const int pays = __builtin_amdgcn_readfirstlane(a.always || gain > 0.0f);
     if (blockIdx.x == 0 && threadIdx.x == 0) *a.apart = pays;
     if (!pays) return;
   }
@@ -337,7 +339,7 @@ __global__ __launch_bounds__(256, MODE == kAttnBehindWaves ? (DH == 128 ? 2 : 3)
   // records, as many pieces as come out about even with that (sqrt(longest / 20): 32768 keys of one head of 128 27.3 -> 22.5 us, 131072 38.0 -> 34.1).
   const int even = __builtin_amdgcn_readfirstlane((int)__builtin_sqrtf((ALONE ? 0.1f : 0.05f) * (float)longest)), workers = (int)gridDim.x * (ALONE ? 4 : 1);
   int per = max(max(uniform_fast_div(total + workers - 1, workers), (longest + L::SHARES - 2) / (L::SHARES - 1)), even);
-  if constexpr (attn_behind(MODE)) per = __builtin_amdgcn_readfirstlane(per);
+  if constexpr (attn_grouped(MODE)) per = __builtin_amdgcn_readfirstlane(per);
   // Workgroups are dealt to the eight XCDs in turn.  Neighbours on the line, which may read the same pages and join their shares, on one of
   // them, and all XCDs alike where there are fewer parts than workgroups (one sequence of 2048, 8 heads of 128, 72 parts: 15.3 us on one XCD,
   // 10.8 on eight).
@@ -349,7 +351,7 @@ __global__ __launch_bounds__(256, MODE == kAttnBehindWaves ? (DH == 128 ? 2 : 3)
   if (x != x0) s.get(s_seqs[wv], G);
   if (!find_job(a, s, s_seqs[wv], s_fronts, x, apart, w)) break;
   x = w.at + w.cost;
-  if constexpr (attn_behind(MODE)) asm volatile("" : "+s"(G), "+s"(per));  // (their reciprocals are not held over the loop)
+  if constexpr (attn_grouped(MODE)) asm volatile("" : "+s"(G), "+s"(per));  // (their reciprocals are not held over the loop)
   const int lane = lane_now();
   const int n = lane & 15, g = lane >> 4;
   // this lane's row
@@ -358,7 +360,7 @@ __global__ __launch_bounds__(256, MODE == kAttnBehindWaves ? (DH == 128 ? 2 : 3)
   const int head = w.head * G + rho - j * G;
   const int64_t all = (int64_t)a.table_stride * kKvPageRows;
   // the last key that row j of the sequence sees; of shared pages all
-  auto reaches = [&](int j) { return MODE == kAttnShared ? w.len - 1 : max((int)min((int64_t)w.len - w.rows + j, all - 1), attn_behind(MODE) ? w.common * kKvPageRows - 1 : INT_MIN); };
+  auto reaches = [&](int j) { return MODE == kAttnShared ? w.len - 1 : max((int)min((int64_t)w.len - w.rows + j, all - 1), attn_grouped(MODE) ? w.common * kKvPageRows - 1 : INT_MIN); };
   const int limit = !active ? -1 : reaches(j);
   // pages that any row / every row of the tile sees (rows rise with n)
   const int j1 = min(w.rows - 1, uniform_fast_div(w.tile * kTileRows + kTileRows - 1, G)), j0 = uniform_fast_div(w.tile * kTileRows, G);
@@ -375,8 +377,8 @@ __global__ __launch_bounds__(256, MODE == kAttnBehindWaves ? (DH == 128 ? 2 : 3)
   const int *table = a.tables + (int64_t)w.seq * a.table_stride + w.skip;
   // (what is needed once in 64 pages is kept in LDS, not in registers)
   volatile int *const lot = s_ticket + 4 + 2 * wv;
-  if constexpr (attn_behind(MODE)) lot[0] = w.common, lot[1] = w.leader - w.seq;
-  auto entry = [&](int p) { return table[attn_behind(MODE) && p < lot[0] ? p + (int64_t)lot[1] * a.table_stride : p]; };
+  if constexpr (attn_grouped(MODE)) lot[0] = w.common, lot[1] = w.leader - w.seq;
+  auto entry = [&](int p) { return table[attn_grouped(MODE) && p < lot[0] ? p + (int64_t)lot[1] * a.table_stride : p]; };
   int ids, ids_from;
   auto page_id = [&](int k) {  // k: this wavefront's k-th page (the same in every lane)
     if (k >= ids_from + 64) {
@@ -813,7 +815,7 @@ __global__ __launch_bounds__(256, MODE == kAttnBehindWaves ? (DH == 128 ? 2 : 3)
       sum = fmaf(e, s_l[x][tid], sum);
     }
     s_sum[tid] = sum;
-    if constexpr (MODE != kAttnWhole) s_l[0][tid] = M;  // (its own sums have been read)
+    if constexpr (!attn_one(MODE)) s_l[0][tid] = M;  // (its own sums have been read)
     if (MODE == kAttnShared && shares > 1) {
       *(f2_any *)(share_slot(a.slots, me, DH) + kTileRows * DH + 2 * tid + (share == 0 ? 2 * kTileRows : 0)) = f2_any{M, sum};
     } else if (shares > 1) {
@@ -835,7 +837,7 @@ __global__ __launch_bounds__(256, MODE == kAttnBehindWaves ? (DH == 128 ? 2 : 3)
     } else if (shares > 1) {
       __hip_atomic_store((unsigned long long *)(record_of(share) + 2 * e), __builtin_bit_cast(unsigned long long, x), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     } else {
-      finish(r, c, x, MODE != kAttnWhole ? s_l[0][r] : 0.0f, s_sum[r]);
+      finish(r, c, x, !attn_one(MODE) ? s_l[0][r] : 0.0f, s_sum[r]);
     }
   }
   if (MODE == kAttnShared && shares > 1) {  // the launch behind this one adds the shares up
@@ -851,7 +853,7 @@ __global__ __launch_bounds__(256, MODE == kAttnBehindWaves ? (DH == 128 ? 2 : 3)
       // Maxima and sums of all shares, asked for at once, then the outputs, eight or sixteen shares at a time: a load after the other would be a
       // round trip to memory for each share.  Up to 16 shares every thread works the weights out for itself (9.3 us for one sequence of 701, 12
       // heads of 64, against 10.4; with all parts on one XCD), else once for all (8192: 14.4 against 15.9).
-      if constexpr (MODE != kAttnWhole) {
+      if constexpr (!attn_one(MODE)) {
         join(tid, 256);
       } else if (shares <= 16) {
         f32x2 (*ml)[kTileRows] = (f32x2 (*)[kTileRows])smem;
@@ -1019,7 +1021,7 @@ int cthip_sdpa_shared_paged_q4(float *out, const float *q, int64_t q_stride, con
   const int G = H / Hkv, tiles = (int)std::min(((int64_t)n_rows * G + kTileRows - 1) / kTileRows, (int64_t)INT_MAX);
   a.always = state().shared_prefix == 2;
   if (state().shared_prefix == 0 || (state().shared_prefix == 1 && sharing_gains(n_rows, n_seqs, tiles, table_stride, G, H, Dh) <= kSharingCosts))
-    return launch_kv4_attn<kAttnBehind>(__func__, a, Dh);
+    return launch_kv4_attn<kAttnTogether>(__func__, a, Dh);
   a.apart = (int *)(a.slots + (int64_t)kSplitSlots / 2 * kTileRows * (Dh + 4));
   // What a sequence has behind its group's pages is a job a head, often of a page or two.  Where there are more jobs than workgroups, each of a few rows, a job is a
   // wavefront's own: its chain of round trips, not its pages, is what it takes, and four times as many run at once.  32 heads of 128 over 1024 shared rows, 70 rows behind them at
