@@ -15,18 +15,21 @@
 //   One sequence of 701, 12 heads of 64: 8.4 us, a chain of round trips: lengths, table, page, record, ticket, records.
 //
 // Where sequences have their first pages in common, softmax over (shared keys, own keys) is that over each of them, with their maxima and sums, joined.  Two
-// launches of the same loop.  The first takes a group's shared pages for the rows of all its sequences, sixteen of them (a key / value head's) in a tile: every
+// launches of the same loop.  The first takes a group's shared pages for the rows of all its sequences, sixteen of them (a key / value head's) in a tile: a
 // page is read and taken apart once for sixteen rows, not once a sequence, and no row is masked.  The second takes what lies behind
 // them for each sequence and, as it stores a row, joins to it what the first one has left: its outputs, unnormalised, in `out`, its maximum and sum in the
 // workspace, or, where several workgroups had shares of them, all shares (joined by the first launch itself, by ticket, they cost it 4 to 6 us and save
 // the second 3).  Bound by the vector unit, as above: at 128 channels 667 vector instructions a page and 16 rows beside 64 matrix ones; where the own
 // parts are short, by the two launches' chains of round trips.
-//   64 samples, 4100 shared rows and up to 400 own, 32 heads of 128 (44.8 MB): 26 + 23 us; each sequence by itself 490 MB.
-//   3 groups of up to 14 sequences of 5 rows, 9000 shared rows, 64 heads over 8 of 128 (22.8 GFLOP): 76 + 32 us; vector units 70 - 75 % busy, matrix units 24 %.
-//   8 answers, 900 shared rows, 12 heads of 64: 7.2 + 8.7 us.
+//   64 samples, 4100 shared rows and up to 400 own, 32 heads of 128 (44.8 MB): 26 + 23 us; each by itself 215.
+//   3 groups of up to 14 sequences of 5 rows, 9000 shared rows, 64 heads over 8 of 128 (22.8 GFLOP): 76 + 32 us; of the first the vector units 64 %, the matrix units 21 %.
+// Sharing saves tiles that are not full.  Rows that fill theirs by themselves, as those 3 groups' nearly do (each by itself 103 us), and short prefixes pay for the second
+// launch and the joining: then one launch takes every sequence's pages, its group's among them.  8 answers, 900 shared rows, 12 heads of 64: 11.6 us, two launches
+// 7.2 + 8.7.  Over 207 batches of 2 .. 1500 sequences, prefixes of 300 .. 30000 rows, one row a sequence or up to five, the way taken is within 0.6 % of the
+// faster (geometric mean; at worst 19 %); sharing always would take 28 % longer and up to twice as long, never sharing 19 % and up to ten times.
 // Longer tiles would take a page apart once for more rows, and gain nothing: 256 rows over 32768 shared keys of 8 heads of 128, 115 us, takes 107 - 119 with
 // tiles of 32 rows (half as many wavefronts hide a page's latencies), 124 - 150 with a page taken apart in LDS for four or eight wavefronts (two barriers a page).
-// At 128 channels three workgroups share a compute unit's LDS only up to 53760 bytes each (granules of 1280): the launches over shared pages use 53632.
+// At 128 channels three workgroups share a compute unit's LDS only up to 53760 bytes each (granules of 1280): these launches use 53632.
 #include <algorithm>
 #include <type_traits>
 
@@ -165,14 +168,15 @@ struct Batch {
     else tiles = from[3][l];
   }
 };
-// What a launch over shared pages saves less what joining its rows costs, as channels of pages that a tile takes apart, of a group of `members` sequences with
-// `rows` rows in `tiles` tiles a head; by themselves they have one each, or on average half a one more than their rows fill.
+// What a launch over shared pages saves less what joining its rows costs, as channels of pages that a tile takes apart (some 14 ps each), of a group of `members` sequences
+// with `rows` rows in `tiles` tiles a head; by themselves they have one each, or on average half a one more than their rows fill.  A row of a head costs as much as 128,
+// the launch as 500000 (7 us).
 __host__ __device__ __forceinline__ float sharing_gains(int rows, int members, int tiles, int pages, int group, int H, int dh) {
   const float each = fminf((float)members, (float)rows), fill = (float)rows * (float)group / kTileRows;
   const float own = rows <= members ? (float)rows * (float)((group + kTileRows - 1) / kTileRows) : fmaxf(each, fill + 0.5f * each);
   return fmaxf(own - (float)tiles, 0.0f) * (float)pages * (float)(H / group * dh) - 128.0f * (float)rows * (float)H;
 }
-constexpr float kSharingCosts = 500000.0f;  // the launch, in the same; once it is there it shares what gains anything
+constexpr float kSharingCosts = 500000.0f;
 // The pages that group g's sequences share, 0 where there is one of them only (it reads its pages by itself), and the first and the end of them
 __device__ __forceinline__ int shared_pages(const Kv4Attn &a, int g, int &first, int &end) {
   first = min(max(a.groups[g], 0), a.n_seqs), end = min(max(a.groups[g + 1], 0), a.n_seqs);
@@ -330,7 +334,7 @@ __global__ __launch_bounds__(256, MODE == kAttnBehindWaves ? (DH == 128 ? 2 : 3)
   longest = __builtin_amdgcn_readlane(wave_scan_max(longest), 63);
   if constexpr (MODE == kAttnShared) {  // (every wavefront finds the same)
     for (int o = 32; o > 0; o >>= 1) gain += __shfl_xor(gain, o, 64);
-    const int pays = __builtin_amdgcn_readfirstlane(a.always || gain > 0.0f);
+    const int pays = __builtin_amdgcn_readfirstlane(a.always || gain > 0.0f);  // (this launch is paid for)
     if (blockIdx.x == 0 && threadIdx.x == 0) *a.apart = pays;
     if (!pays) return;
   }
@@ -1018,6 +1022,8 @@ int cthip_sdpa_shared_paged_q4(float *out, const float *q, int64_t q_stride, con
   a.groups = groups, a.shared = shared, a.n_groups = n_groups;
   a.slots = a.parts + (int64_t)2 * kMaxWorkers * kTileRows * (Dh + 2), a.stats = a.parts + (int64_t)kSharedRows * (Dh + 2);
   if (n_groups == 0) return launch_kv4_attn<kAttnWhole>(__func__, a, Dh);
+  // What the groups share is on the device only.  If it does not pay where one group shared all that its tables hold, there is one launch; otherwise the first of
+  // two knows what they share, and leaves it to the second where that gains nothing.
   const int G = H / Hkv, tiles = (int)std::min(((int64_t)n_rows * G + kTileRows - 1) / kTileRows, (int64_t)INT_MAX);
   a.always = state().shared_prefix == 2;
   if (state().shared_prefix == 0 || (state().shared_prefix == 1 && sharing_gains(n_rows, n_seqs, tiles, table_stride, G, H, Dh) <= kSharingCosts))

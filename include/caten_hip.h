@@ -286,6 +286,9 @@ int cthip_linear(float *y, const void *wmat, const float *x, int m, const float 
  *   They are given back when a matrix is destroyed, by cthip_cache_trim, by an allocation here that finds no memory,
  *   and by a lower limit; 0 = none are kept.  Results do not depend on it where the same launch is chosen; past the
  *   limit the terms are made by every call that still pays with them.
+ * "shared_prefix": whether cthip_sdpa_shared_paged_q4 takes the pages that a group shares once for all of its rows, in a launch in
+ *   front of that over the rest: 1 (default) = where that is faster (prefixes of some hundred rows and more, sequences whose rows do not fill a tile of
+ *   16 by themselves: rows times query heads of a key / value head), 0 = never (one launch), 2 = always.  Results differ in summation order only.
  * "decode_skip": knock-out timing of the three-launch decode step -- a mask of launches a session created
  *   afterwards leaves out (1 qkv, 2 attention + projection, 4 MLP, 8 the sum in front of lm_head,
  *   16 lm_head + argmax).  Tokens and logits of such a session are meaningless; 0 (default) = none.
@@ -479,7 +482,7 @@ int64_t cthip_kv_compact_paged_q4_workspace(int n_pages);
 int cthip_kv_compact_paged_q4(int *tables_out, int *free_pages, int *n_free, void *k_pages, void *v_pages, int n_layers, int n_pages, const int *tables, int table_stride,
                               const int *lens, int n_seqs, int kv_heads, int head_dim, void *workspace);
 /* cthip_sdpa_paged_q4 where sequences have their first pages in common.  Group g is sequences groups[g] .. groups[g + 1] - 1; the first shared[g] / 64 (whole) pages of the
- * table of its first sequence are all of its sequences', and are read once for all of their rows.  A row sees all of them, and of its own sequence's
+ * table of its first sequence are all of its sequences', and are read once for all of their rows where that is faster (option "shared_prefix").  A row sees all of them, and of its own sequence's
  * rows behind them those up to its own position; so with equal table entries, and no row's position in front of them, the result is that of
  * cthip_sdpa_paged_q4 up to rounding.  lens count the shared rows.  groups (n_groups + 1) and starts rise; sequences in no group share nothing; groups and starts that
  * fall, or leave their range, give undefined rows.  At most as many groups as sequences; otherwise arguments, precision, limits and what is left as it was are as
@@ -498,7 +501,8 @@ int cthip_sdpa_shared_paged_q4(float *out, const float *q, int64_t q_stride, con
  * draws the last token with a weight.  Rows need not sum to 1 to be drawn from, but the comparison takes them as they are.
  *   tokens_out (n_rows)  a sequence's drafts that stay, the drawn token (-1 where no token has a probability), -1 in its further rows
  *   accepted (n_seqs)    drafts that stay
- *   lens_out (n_seqs)    lens less the rejected drafts: what the cache holds then; may be lens, or NULL
+ *   lens_out (n_seqs)    lens less the rejected drafts: what the cache holds then; may be lens, or NULL (a page that held rejected rows only
+ *                        comes back by cthip_kv_free_paged)
  * A sequence without rows, with rows outside 0 .. n_rows - 1 or, where positions (may be NULL) is given, refused by the plan (its first row's -1) keeps its length
  * and accepts nothing; its rows, if they are inside, are -1.  Without drafts this draws a token a sequence.  At most 65535 sequences.
  * workspace: cthip_draft_verify_workspace(n_seqs) = 2048 n_seqs bytes, 16-byte aligned, whatever they hold; calls that may overlap need one each. */
