@@ -364,11 +364,17 @@ __global__ __launch_bounds__(256, MODE == kAttnBehindWaves ? (DH == 128 ? 2 : 3)
   const int head = w.head * G + rho - j * G;
   const int64_t all = (int64_t)a.table_stride * kKvPageRows;
   // the last key that row j of the sequence sees; of shared pages all
-  auto reaches = [&](int j) { return MODE == kAttnShared ? w.len - 1 : max((int)min((int64_t)w.len - w.rows + j, all - 1), attn_grouped(MODE) ? w.common * kKvPageRows - 1 : INT_MIN); };
+  auto reaches = [&](int j) {
+    if constexpr (MODE == kAttnShared) return w.len - 1;
+    const int own = (int)min((int64_t)w.len - w.rows + j, all - 1);
+    if constexpr (attn_grouped(MODE)) return max(own, w.common * kKvPageRows - 1);
+    else return own;
+  };
   const int limit = !active ? -1 : reaches(j);
   // pages that any row / every row of the tile sees (rows rise with n)
   const int j1 = min(w.rows - 1, uniform_fast_div(w.tile * kTileRows + kTileRows - 1, G)), j0 = uniform_fast_div(w.tile * kTileRows, G);
-  const int last = __builtin_amdgcn_readfirstlane(reaches(j1)), least = __builtin_amdgcn_readfirstlane(reaches(j0));  // (uniform)
+  int last = reaches(j1), least = reaches(j0);
+  if constexpr (attn_grouped(MODE)) last = __builtin_amdgcn_readfirstlane(last), least = __builtin_amdgcn_readfirstlane(least);  // (uniform)
   const int pages = a.n_pages > 0 && last >= 0 ? max(last / kKvPageRows + 1 - w.skip, 0) : 0;
   // its pieces lie on the line behind those that stand for the rest (a job without pages is one piece of none)
   const int pieces = max(1, (pages + (1 << a.piece_log2) - 1) >> a.piece_log2), line = w.at + kJobPieces;
