@@ -14,7 +14,16 @@ from tests.test_gpu_shared_prefix import close, seen
 pytestmark = pytest.mark.gpu
 
 
-def test_answers_to_a_prompt():
+@pytest.fixture(params=[1, 2], ids=["as it pays", "apart"])
+def way(request):
+    """Shared pages in a launch of their own where that pays (nowhere here), and always."""
+    from caten_amd import _lib
+    _lib.check(_lib.init().cthip_set_option(b"shared_prefix", request.param))
+    yield
+    _lib.check(_lib.load().cthip_set_option(b"shared_prefix", 1))
+
+
+def test_answers_to_a_prompt(way):
     from caten_amd import ops
     rng = np.random.default_rng(41)
     H, kv, dh, vocab, n, layers, table, n_pages = 8, 2, 64, 301, 6, 2, 12, 60
@@ -98,7 +107,7 @@ def test_answers_to_a_prompt():
                 assert np.array_equal(k, held[i][layer][0]) and np.array_equal(v, held[i][layer][1])
 
 
-def test_a_captured_step():
+def test_a_captured_step(way):
     """Rotary rows, append, shared attention, probabilities and verification of a step, recorded: replays give the next steps.  Two graphs with workspaces of their own,
     eager work between the replays."""
     from caten_amd import _lib, ops
@@ -175,3 +184,65 @@ def test_a_captured_step():
     for graph, run in runs:
         lib.hipGraphExecDestroy(run)
         lib.hipGraphDestroy(graph)
+
+
+def test_captured_forks_and_packing():
+    """Forks (the number of free pages in place) and a packed pool behind them, recorded once, replayed over other tables and pages: as eager calls."""
+    from caten_amd import _lib, ops
+    lib = _lib.init()
+    stream = C.c_void_p(lib.cthip_stream())
+    n, table, n_pages, layers, kv, dh, forks = 9, 6, 60, 3, 2, 64, 4
+    page = int(lib.cthip_kv_page_bytes_q4(kv, dh))
+    r = np.random.default_rng(45)
+
+    def some():
+        lens = r.integers(0, table * PAGE + 1, n)
+        ids, tables = r.permutation(n_pages), np.full((n, table), -1)
+        used = 0
+        for i in range(n):
+            c = -(-int(lens[i]) // PAGE)
+            tables[i, :c] = ids[used:used + c]
+            used += c
+        who = r.permutation(n)
+        parents, children = r.choice(who[:n - forks], forks), who[n - forks:]
+        return dict(tables=tables, lens=lens, free=np.concatenate([ids[used:], np.full(used, -1)]), n=[n_pages - used], parents=parents, children=children, at=[r.integers(0, lens[p] + 1) for p in parents],
+                    pools=r.integers(0, 256, (2, layers, n_pages, page), np.uint8))
+
+    def fresh():
+        d = {k: ops.DeviceArray((m,), np.int32) for k, m in dict(tables=n * table, lens=n, free=n_pages, n=1, parents=forks, children=forks, at=forks, refused=forks).items()}
+        d["pools"], d["ws"] = ops.DeviceArray((2 * layers * n_pages * page,), np.uint8), ops.DeviceArray((64 + 8 * n_pages,), np.uint8)
+
+        def feed(case):
+            for k, v in case.items():
+                a = np.ascontiguousarray(v, np.uint8 if k == "pools" else np.int32)
+                _lib.check(lib.cthip_h2d(d[k].ptr, a.ctypes.data, a.nbytes))
+
+        def step():
+            kp, vp = d["pools"].ptr, d["pools"].ptr + layers * n_pages * page
+            _lib.check(lib.cthip_kv_fork_paged_q4(d["tables"].ptr, table, d["lens"].ptr, n, d["n"].ptr, d["refused"].ptr, kp, vp, layers, n_pages, d["parents"].ptr, d["children"].ptr, d["at"].ptr, forks,
+                                                  d["free"].ptr, d["n"].ptr, kv, dh))
+            _lib.check(lib.cthip_kv_compact_paged_q4(d["tables"].ptr, d["free"].ptr, d["n"].ptr, kp, vp, layers, n_pages, d["tables"].ptr, table, d["lens"].ptr, n, kv, dh, d["ws"].ptr))
+        return d, feed, step
+
+    eager, graphed = fresh(), fresh()
+    graph, run = C.c_void_p(), C.c_void_p()
+    assert lib.hipStreamBeginCapture(stream, 1) == 0
+    graphed[2]()
+    assert lib.hipStreamEndCapture(stream, C.byref(graph)) == 0
+    assert lib.hipGraphInstantiate(C.byref(run), graph, None, None, C.c_size_t(0)) == 0
+    moved = 0
+    for _ in range(5):
+        case = some()
+        eager[1](case)
+        eager[2]()
+        graphed[1](case)
+        assert lib.hipGraphLaunch(run, stream) == 0
+        for k in ("tables", "lens", "free", "n", "refused"):
+            assert np.array_equal(graphed[0][k].numpy(), eager[0][k].numpy()), k
+        used = n_pages - int(eager[0]["n"].numpy()[0])
+        a, b = (x[0]["pools"].numpy().reshape(2, layers, n_pages, page) for x in (eager, graphed))
+        assert np.array_equal(a, b) and used < n_pages
+        moved += (a[:, :, :used] != case["pools"][:, :, :used]).any(-1).sum()
+    assert moved > 0
+    lib.hipGraphExecDestroy(run)
+    lib.hipGraphDestroy(graph)
