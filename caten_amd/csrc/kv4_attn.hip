@@ -386,7 +386,7 @@ __global__ __launch_bounds__(256, MODE == kAttnBehindWaves ? (DH == 128 ? 2 : 3)
   // page ids of the next 64 pages of this wavefront, one a lane
   const int *table = a.tables + (int64_t)w.seq * a.table_stride + w.skip;
   // (what is needed once in 64 pages is kept in LDS, not in registers)
-  volatile int *const lot = s_ticket + 4 + 2 * wv;
+  volatile __attribute__((address_space(3))) int *const lot = (volatile __attribute__((address_space(3))) int *)(s_ticket + 4 + 2 * wv);
   if constexpr (attn_grouped(MODE)) lot[0] = w.common, lot[1] = w.leader - w.seq;
   auto entry = [&](int p) { return table[attn_grouped(MODE) && p < lot[0] ? p + (int64_t)lot[1] * a.table_stride : p]; };
   int ids, ids_from;
