@@ -106,6 +106,16 @@ def test_many_groups():
     compare(rng, 4, 2, 64, [(64 * (i % 3), [(64 * (i % 3) + 1 + (i * 37 + j) % 100, (i + j) % 3) for j in range(i % 4 + 1)]) for i in range(150)])
 
 
+def test_as_many_sequences_as_there_may_be():
+    rng = np.random.default_rng(23)
+    groups, left = [], 4096
+    while left:
+        m = min(left, 1 + len(groups) % 8)
+        left -= m
+        groups.append((64 * (len(groups) % 3), [(64 * (len(groups) % 3) + 1 + j, (j + len(groups)) % 4 != 0) for j in range(m)]))
+    compare(rng, 2, 1, 32, groups)
+
+
 def test_the_same_as_without_sharing():
     """Against the attention that reads every sequence's pages by itself: both are within the tolerance of the same numbers, with groups that share nothing or have one
     sequence too.  A batch without groups is the same bits."""
