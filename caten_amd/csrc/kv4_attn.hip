@@ -25,8 +25,8 @@
 //   3 groups of up to 14 sequences of 5 rows, 9000 shared rows, 64 heads over 8 of 128 (22.8 GFLOP): 76 + 32 us; of the first the vector units 64 %, the matrix units 21 %.
 // Sharing saves tiles that are not full.  Rows that fill theirs by themselves, as those 3 groups' nearly do (each by itself 103 us), and short prefixes pay for the second
 // launch and the joining: then one launch takes every sequence's pages, its group's among them.  8 answers, 900 shared rows, 12 heads of 64: 11.6 us, two launches
-// 7.2 + 8.7.  Over 207 batches of 2 .. 1500 sequences, prefixes of 300 .. 30000 rows, one row a sequence or up to five, the way taken is within 0.6 % of the
-// faster (geometric mean; at worst 19 %); sharing always would take 28 % longer and up to twice as long, never sharing 19 % and up to ten times.
+// 7.2 + 8.7.  Over 207 batches of 2 .. 1500 sequences, prefixes of 300 .. 30000 rows, one row a sequence or up to five, the way taken is within 0.8 % of the
+// faster (geometric mean; at worst 17 %); sharing always would take 28 % longer and up to twice as long, never sharing 20 % and up to ten times.
 // Longer tiles would take a page apart once for more rows, and gain nothing: 256 rows over 32768 shared keys of 8 heads of 128, 115 us, takes 107 - 119 with
 // tiles of 32 rows (half as many wavefronts hide a page's latencies), 124 - 150 with a page taken apart in LDS for four or eight wavefronts (two barriers a page).
 // At 128 channels three workgroups share a compute unit's LDS only up to 53760 bytes each (granules of 1280): these launches use 53632.
@@ -178,36 +178,56 @@ __host__ __device__ __forceinline__ float sharing_gains(int rows, int members, i
 }
 constexpr float kSharingCosts = 500000.0f;
 // The pages that group g's sequences share, 0 where there is one of them only (it reads its pages by itself), and the first and the end of them
-__device__ __forceinline__ int shared_pages(const Kv4Attn &a, int g, int &first, int &end) {
-  first = min(max(a.groups[g], 0), a.n_seqs), end = min(max(a.groups[g + 1], 0), a.n_seqs);
-  return end - first > 1 && a.n_pages > 0 ? min(max(a.shared[g], 0) / kKvPageRows, a.table_stride) : 0;
+__device__ __forceinline__ int shared_pages(const Kv4Attn &a, int border, int next, int rows, int &first, int &end) {
+  first = min(max(border, 0), a.n_seqs), end = min(max(next, 0), a.n_seqs);
+  return end - first > 1 && a.n_pages > 0 ? min(max(rows, 0) / kKvPageRows, a.table_stride) : 0;
+}
+// The groups that 64 sequences from `first` on are in, if they are in any, one a lane: among the borders of `from` and the next 63, which the wavefront asks for at once, the
+// last that is not past the lane's.  (A search of each lane's own, through memory, took 427 sequences in 200 groups, 32 heads of 64, 38 us where this takes 34, 2752 in 600 142 and 108.)
+__device__ __forceinline__ int borders_of(const Kv4Attn &a, int from, int apart) {
+  const int g = from + lane_now() * apart;
+  return g < a.n_groups ? a.groups[g] : INT_MAX;
+}
+__device__ __forceinline__ int group_of(const Kv4Attn &a, int first, int from) {
+  const int i = first + lane_now(), border = borders_of(a, from, 1);
+  int k = 0;
+#pragma unroll
+  for (int s = 32; s > 0; s >>= 1)
+    if (__builtin_amdgcn_ds_bpermute((k + s) << 2, border) <= i) k += s;
+  int lo = min(from + k, a.n_groups - 1);
+  if (k == 63)  // there may be more: groups without sequences are among them
+    for (int hi = a.n_groups; hi - lo > 1;) {
+      const int mid = (lo + hi) >> 1;
+      if (a.groups[mid] <= i) lo = mid;
+      else hi = mid;
+    }
+  return lo;
+}
+// where to begin
+__device__ __forceinline__ int first_group(const Kv4Attn &a, int first) {
+  auto passed = [&](int border) { return max((int)__popcll(__ballot(border <= first)) - 1, 0); };
+  const int each = (a.n_groups + 63) >> 6, from = passed(borders_of(a, 0, each)) * each;
+  return min(each > 1 ? from + passed(borders_of(a, from, 1)) : from, a.n_groups - 1);
 }
 template <int MODE>
 struct Read {  // of a sequence, or of a group
   int len = 0, row0 = 0, end = 0, leader = 0, aside = 0;  // aside: kAttnShared: the group's sequences
-  __device__ __forceinline__ Read(const Kv4Attn &a, int first) {
+  int from = 0, border, next, shared;                     // of sequences in groups: the last one's group; what there is of each's
+  __device__ __forceinline__ Read(const Kv4Attn &a, int first, int from_ = 0) {
     const int i = first + lane_now();
     if constexpr (MODE == kAttnShared) {
       if (i < a.n_groups) {
         int last;
-        const int pages = shared_pages(a, i, leader, last);
+        const int pages = shared_pages(a, a.groups[i], a.groups[i + 1], a.shared[i], leader, last);
         len = pages * kKvPageRows, aside = last - leader;
         row0 = a.starts[leader], end = pages ? a.starts[last] : row0;  // (with every group's first row known none has rows of one in front of it, see `reach`)
       }
     } else {
       if (i < a.n_seqs) len = a.lens[i], row0 = a.starts[i], end = a.starts[i + 1];
       if constexpr (attn_grouped(MODE)) {
-        if (i < a.n_seqs && a.n_groups > 0) {
-          int lo = 0, hi = a.n_groups;  // groups[lo] <= i where there is such a group
-          while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (a.groups[mid] <= i) lo = mid;
-            else hi = mid;
-          }
-          int g0, g1;
-          const int pages = shared_pages(a, lo, g0, g1);
-          if (i >= g0 && i < g1) aside = pages, leader = g0;
-        }
+        int lo = 0;
+        if (a.n_groups > 1 && first < a.n_seqs) lo = group_of(a, first, from_), from = __builtin_amdgcn_readlane(lo, 63);
+        border = a.groups[lo], next = a.groups[lo + 1], shared = a.shared[lo];  // (looked at with the rest)
       }
     }
   }
@@ -217,7 +237,13 @@ __device__ __forceinline__ int in_all(const Kv4Attn &a) { return MODE == kAttnSh
 template <int MODE>
 __device__ __forceinline__ void look(const Kv4Attn &a, const Read<MODE> &read, Batch<MODE> &s, bool apart) {
   s.len = max(read.len, 0), s.row0 = read.row0;
-  if constexpr (MODE != kAttnWhole) s.leader = read.leader, s.aside = read.aside;
+  if constexpr (MODE == kAttnShared) s.leader = read.leader, s.aside = read.aside;
+  if constexpr (attn_grouped(MODE)) {
+    int g0, g1;
+    const int i = s.first + lane_now(), common = shared_pages(a, read.border, read.next, read.shared, g0, g1);
+    const bool in = i >= g0 && i < g1;
+    s.leader = in ? g0 : 0, s.aside = in ? common : 0;
+  }
   const int end = min(read.end, a.n_rows);
   // (rows in front of an earlier sequence's are nobody's: no row is two sequences', and the costs of all stay within their bound)
   const int reach = max(s.reach, wave_scan_max(s.row0));
@@ -243,7 +269,7 @@ __device__ __forceinline__ bool find_job(const Kv4Attn &a, Batch<MODE> &s, int (
     const int lane = lane_now();
     const int block = __popcll(__ballot(lane * 64 < in_all<MODE>(a) && fronts[0][lane] <= place)) - 1;
     s.first = 64 * block, s.before = __builtin_amdgcn_readfirstlane(fronts[0][block]), s.reach = __builtin_amdgcn_readfirstlane(fronts[1][block]);
-    look(a, Read<MODE>(a, s.first), s, apart);
+    look(a, Read<MODE>(a, s.first, attn_grouped(MODE) && a.n_groups > 1 ? first_group(a, s.first) : 0), s, apart);
     s.put(kept);
   }
   const unsigned long long past = __ballot(s.upto > place);
@@ -319,7 +345,7 @@ __global__ __launch_bounds__(256, MODE == kAttnBehindWaves ? (DH == 128 ? 2 : 3)
   for (Read<MODE> read(a, 0);;) {
     const bool more = s.first + 64 < in_all<MODE>(a);
     if (lane_now() == 0) s_fronts[0][s.first >> 6] = s.before, s_fronts[1][s.first >> 6] = s.reach;
-    const Read<MODE> next(a, more ? s.first + 64 : in_all<MODE>(a));  // (on its way while these are looked at)
+    const Read<MODE> next(a, more ? s.first + 64 : in_all<MODE>(a), read.from);  // (on its way while these are looked at)
     look(a, read, s, apart);
     if constexpr (MODE == kAttnShared) {
       if (s.tiles && s.len) gain += sharing_gains(s.rows, s.aside, s.tiles, s.len / kKvPageRows, G, a.H, DH);
