@@ -25,7 +25,7 @@
 //   3 groups of up to 14 sequences of 5 rows, 9000 shared rows, 64 heads over 8 of 128 (22.8 GFLOP): 76 + 32 us; of the first the vector units 64 %, the matrix units 21 %.
 // Sharing saves tiles that are not full.  Rows that fill theirs by themselves, as those 3 groups' nearly do (each by itself 103 us), and short prefixes pay for the second
 // launch and the joining: then one launch takes every sequence's pages, its group's among them.  8 answers, 900 shared rows, 12 heads of 64: 11.6 us, two launches
-// 7.2 + 8.7.  Over 207 batches of 2 .. 1500 sequences, prefixes of 300 .. 30000 rows, one row a sequence or up to five, the way taken is within 0.8 % of the
+// 7.2 + 8.7.  Over 207 batches of 2 .. 1500 sequences, prefixes of 300 .. 30000 rows, one row a sequence or up to five, the way taken is within 1.1 % of the
 // faster (geometric mean; at worst 17 %); sharing always would take 28 % longer and up to twice as long, never sharing 20 % and up to ten times.
 // Longer tiles would take a page apart once for more rows, and gain nothing: 256 rows over 32768 shared keys of 8 heads of 128, 115 us, takes 107 - 119 with
 // tiles of 32 rows (half as many wavefronts hide a page's latencies), 124 - 150 with a page taken apart in LDS for four or eight wavefronts (two barriers a page).
@@ -77,7 +77,7 @@ constexpr int kSplitSlots = 2048;   // records of shares in the workspace, two a
 // in the workspace of a batch with shared pages: tickets, and floats for Dh + 2 of them a row -- records, two a wavefront that has parts of its own, then
 // slots, one a workgroup
 constexpr int kSharedTickets = 4096, kSharedRows = 131072, kMaxWorkers = 3 * 1024;
-static_assert(kMaxWorkers <= kSharedTickets && kSplitSlots <= kSharedTickets && kMaxWorkers >= kSplitSlots / 2 &&
+static_assert(kMaxWorkers < kSharedTickets && kSplitSlots < kSharedTickets && kMaxWorkers >= kSplitSlots / 2 &&
                   17 * (kSharedRows - 2 * kMaxWorkers * kTileRows - 1) >= 18 * (kSplitSlots / 2) * kTileRows, "a slot has Dh + 4 floats a row: at Dh = 32 18 / 17 of Dh + 2");
 constexpr int kJobPieces = 1;       // what a job costs besides its pages, in pieces of them (2: 52 us instead of 50, 34 instead of 31, for the batches above)
 
@@ -1054,18 +1054,24 @@ int cthip_sdpa_shared_paged_q4(float *out, const float *q, int64_t q_stride, con
   a.groups = groups, a.shared = shared, a.n_groups = n_groups;
   a.slots = a.parts + (int64_t)2 * kMaxWorkers * kTileRows * (Dh + 2), a.stats = a.parts + (int64_t)kSharedRows * (Dh + 2);
   if (n_groups == 0) return launch_kv4_attn<kAttnWhole>(__func__, a, Dh);
-  // What the groups share is on the device only.  If it does not pay where one group shared all that its tables hold, there is one launch; otherwise the first of
-  // two knows what they share, and leaves it to the second where that gains nothing.
-  const int G = H / Hkv, tiles = (int)std::min(((int64_t)n_rows * G + kTileRows - 1) / kTileRows, (int64_t)INT_MAX);
-  a.always = state().shared_prefix == 2;
-  if (state().shared_prefix == 0 || (state().shared_prefix == 1 && sharing_gains(n_rows, n_seqs, tiles, table_stride, G, H, Dh) <= kSharingCosts))
-    return launch_kv4_attn<kAttnTogether>(__func__, a, Dh);
-  a.apart = (int *)(a.slots + (int64_t)kSplitSlots / 2 * kTileRows * (Dh + 4));
   // What a sequence has behind its group's pages is a job a head, often of a page or two.  Where there are more jobs than workgroups, each of a few rows, a job is a
   // wavefront's own: its chain of round trips, not its pages, is what it takes, and four times as many run at once.  32 heads of 128 over 1024 shared rows, 70 rows behind them at
   // most, both launches: 24 sequences 24.2 us by workgroups, 24.8 by wavefronts; 32: 33.6 and 25.2; 64: 44.7 and 28.9 (600 rows: 49.7 and 40.8); four rows each
   // 55.3 and 44.5; with eight rows of a head, whose results are joined by fewer lanes then, 512 jobs 34 and 46.
   const bool few = (int64_t)n_rows * (H / Hkv) <= 4ll * n_seqs && (int64_t)n_seqs * Hkv > state().compute_units * (Dh == 128 ? 3 : 4);
+  // What the groups share is on the device only.  If it would not pay even if they shared all that their tables hold, there is one launch; otherwise the first of
+  // two knows what they share, and leaves it to the second where that gains nothing.
+  const int G = H / Hkv, tiles = (int)std::min(std::max(((int64_t)n_rows * G + kTileRows - 1) / kTileRows, (int64_t)std::min(n_groups, n_rows)), (int64_t)INT_MAX);
+  a.always = state().shared_prefix == 2;
+  if (state().shared_prefix == 0 || (state().shared_prefix == 1 && sharing_gains(n_rows, n_seqs, tiles, table_stride, G, H, Dh) <= kSharingCosts)) {
+    // By wavefronts too, but for 128 channels, where two and not three workgroups of them share a compute unit: 12 heads of 64, 522 sequences in 300 groups of 300 shared rows
+    // and up to 300 more 83 us by workgroups, 65 by wavefronts, up to 1000 more 119 and 101; 2752 sequences, 4 heads of 32, 111 and 70; 49 sequences, 32 heads of 128, 45 and 43, with up to
+    // 3000 rows 118 and 128.
+    if (!few || Dh == 128) return launch_kv4_attn<kAttnTogether>(__func__, a, Dh);
+    a.apart = a.tickets + kSharedTickets - 1;  // nobody's ticket: zero, there is no launch in front
+    return launch_kv4_attn<kAttnBehindWaves>(__func__, a, Dh);
+  }
+  a.apart = (int *)(a.slots + (int64_t)kSplitSlots / 2 * kTileRows * (Dh + 4));
   if (const int rc = launch_kv4_attn<kAttnShared>(__func__, a, Dh)) return rc;
   return few ? launch_kv4_attn<kAttnBehindWaves>(__func__, a, Dh) : launch_kv4_attn<kAttnBehind>(__func__, a, Dh);
 }
