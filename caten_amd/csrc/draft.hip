@@ -10,8 +10,8 @@
 // numbers a draft) and leaves its slice's sums, the replacement's and, in case that one is nothing, the target's own.  Then a wavefront
 // finds the slice and a workgroup the token in it, eight side by side a thread.  Bound by the two rows of the vocabulary that a sequence needs, and
 // by two launches of four to six round trips each where those are short.  (One launch of a workgroup a sequence would read 64 rows with 64 of 256 compute units.)
-//   64 sequences of 1 .. 6 rows, 128256 tokens (65.7 MB needed): 14.5 + 6.5 us; the sums at 4.5 TB/s.
-//   48 sequences of up to 7 rows, 32000 tokens: 5.5 + 6.4 us.  One sequence of 4 rows, 50257 tokens: 3.9 + 5.4 us.
+//   64 sequences of 1 .. 5 rows, 128256 tokens (65.7 MB needed): 13.3 + 7 us; the sums at 5 TB/s.
+//   48 sequences of up to 8 rows, 32000 tokens: 5.7 + 6.1 us.  One sequence of 5 rows, 50257 tokens: 3.9 + 5.0 us.
 #include <algorithm>
 
 #include "common.h"
@@ -31,6 +31,7 @@ struct DraftArgs {
   const float *uniforms;
   const int *starts, *positions, *lens;
   int n_rows, vocab, slices, slice;
+  int each;  // slices that a workgroup sums up, one after the other
   unsigned char *workspace;
   // of a sequence: of each slice the weights' sum, of each slice the target's; and its drafts that stay, -1 where it sits out
   __device__ __forceinline__ double *sums(int seq) const { return (double *)(workspace + (int64_t)seq * kDraftWorkspace); }
@@ -96,23 +97,29 @@ struct DraftRow {
 };
 
 __global__ __launch_bounds__(kDraftThreads) void k_draft_slice(DraftArgs a) {
-  __shared__ double part[2][kDraftThreads / 64];
+  __shared__ double part[kDraftSlices][2][kDraftThreads / 64];  // of its slices
   const int seq = blockIdx.y, tid = threadIdx.x;
   const Verified v(a, seq);
   if (blockIdx.x == 0 && tid == 0) a.stays(seq)[0] = v.there ? v.stay : -1;
   if (!v.there) return;
   const DraftRow row(a, v.row0, v.rows, v.stay);
-  double w = 0.0, own = 0.0;
-  const int t1 = min(a.vocab, ((int)blockIdx.x + 1) * a.slice);
-  for (int t = blockIdx.x * a.slice + tid; t < t1; t += kDraftThreads) {
-    double x, y;
-    row.at(t, x, y);
-    w += x, own += y;
+  const int s0 = blockIdx.x * a.each, n = min(a.slices - s0, a.each);
+  for (int s = 0; s < n; s++) {
+    double w = 0.0, own = 0.0;
+    const int t1 = min(a.vocab, (s0 + s + 1) * a.slice);
+    for (int t = (s0 + s) * a.slice + tid; t < t1; t += kDraftThreads) {
+      double x, y;
+      row.at(t, x, y);
+      w += x, own += y;
+    }
+    w = draft_wave_sum(w), own = draft_wave_sum(own);
+    if ((tid & 63) == 0) part[s][0][tid >> 6] = w, part[s][1][tid >> 6] = own;
   }
-  w = draft_wave_sum(w), own = draft_wave_sum(own);
-  if ((tid & 63) == 0) part[0][tid >> 6] = w, part[1][tid >> 6] = own;
   __syncthreads();
-  if (tid < 2) a.sums(seq)[kDraftSlices * tid + blockIdx.x] = (part[tid][0] + part[tid][1]) + (part[tid][2] + part[tid][3]);
+  if (tid < 2 * n) {
+    const double *sums = part[tid >> 1][tid & 1];
+    a.sums(seq)[kDraftSlices * (tid & 1) + s0 + (tid >> 1)] = (sums[0] + sums[1]) + (sums[2] + sums[3]);
+  }
 }
 
 // inclusive, over a wavefront
@@ -228,9 +235,12 @@ int cthip_draft_verify(int *tokens_out, int *accepted, int *lens_out, const floa
   CTHIP_ARG(accepted && starts && workspace && ((uintptr_t)workspace & 15) == 0 && (!lens_out || lens));
   CTHIP_ARG(n_rows == 0 || (tokens_out && target && tokens && uniforms && tokens_out != tokens));
   const int slices = std::min(kDraftSlices, (vocab + 1023) / 1024), slice = (vocab + slices - 1) / slices;
-  const DraftArgs a = {tokens_out, accepted, lens_out, target, draft, target_stride, draft_stride, tokens, uniforms, starts, positions, lens, n_rows, vocab, (vocab + slice - 1) / slice, slice,
+  // As many workgroups as run at once, eight a compute unit: each has to find the row first (64 rows of 128256: a workgroup a slice 15.0 us, so 13.3; half as many
+  // slices 12.3, and the second launch 10.2 instead of 7).
+  const int at_once = 8 * state().compute_units, each = (int)std::min((int64_t)slices, ((int64_t)n_seqs * slices + at_once - 1) / at_once);
+  const DraftArgs a = {tokens_out, accepted, lens_out, target, draft, target_stride, draft_stride, tokens, uniforms, starts, positions, lens, n_rows, vocab, (vocab + slice - 1) / slice, slice, each,
                        (unsigned char *)workspace};
-  hipLaunchKernelGGL(k_draft_slice, dim3((unsigned)a.slices, (unsigned)n_seqs), dim3(kDraftThreads), 0, state().stream, a);
+  hipLaunchKernelGGL(k_draft_slice, dim3((unsigned)((a.slices + each - 1) / each), (unsigned)n_seqs), dim3(kDraftThreads), 0, state().stream, a);
   CTHIP_LAUNCH_CHECK();
   hipLaunchKernelGGL(k_draft_token, dim3((unsigned)n_seqs), dim3(kDraftThreads), 0, state().stream, a);
   CTHIP_LAUNCH_CHECK();

@@ -87,6 +87,14 @@ def test_a_large_vocabulary_and_many_sequences():
         same(ops.draft_verify(*args), verified(*args))
 
 
+@pytest.mark.parametrize("n,vocab,draft", [(150, 17003, False), (70, 16 * 1024 + 1, True), (450, 4099, False)])
+def test_workgroups_of_several_slices(n, vocab, draft):
+    from caten_amd import ops
+    rng = np.random.default_rng(n)
+    args = list(some(rng, [1 if draft else 0] * n, vocab))
+    same(ops.draft_verify(*args), verified(*args))
+
+
 def test_borders():
     """Weights that are whole steps of 1/256: sums and products are exact in any order, and a number on a border belongs to the token behind it."""
     from caten_amd import ops
