@@ -25,7 +25,8 @@ __device__ __forceinline__ void copy_page(unsigned char *pool, int src, int dst,
 }
 
 // ---- sequences that go on from others ----
-// Full pages are the same for parent and child and stay shared; a partly filled one is copied into a page from the free stack.  A child is nobody's parent
+// Full pages are the same for parent and child and stay shared; a partly filled one is copied into a page from the free stack.  One that lies outside the pool holds no
+// rows: the child's entry is then the parent's, since a page from the stack would show the child what its last owner left there.  A child is nobody's parent
 // in the same call and named once, so what is read (parents' tables and lengths) is not what is written (children's), and the forks need no
 // order among themselves but that of the pages they take: how many forks in front of it need one, every workgroup counts for itself.
 struct ForkArgs {
@@ -49,7 +50,9 @@ __global__ __launch_bounds__(256) void k_kv_fork(ForkArgs a) {
   const int have = max(a.n_free[0], 0);
   const bool my_parent_ok = my_parent >= 0 && my_parent < a.n_seqs, reads = my_parent_ok && my_at >= 0 && my_at / kKvPageRows < a.table_stride;
   const int *from = a.tables + (int64_t)(my_parent_ok ? my_parent : 0) * a.table_stride;
-  const int src = reads ? from[my_at / kKvPageRows] : -1, tid_len = tid_parent >= 0 && tid_parent < a.n_seqs ? a.lens[tid_parent] : -1;
+  // the parent's page that a fork ends in
+  auto ends_in = [&](int p, int at) { return p >= 0 && p < a.n_seqs && at >= 0 && at / kKvPageRows < a.table_stride ? a.tables[(int64_t)p * a.table_stride + at / kKvPageRows] : -1; };
+  const int src = reads ? from[my_at / kKvPageRows] : -1, tid_len = tid_parent >= 0 && tid_parent < a.n_seqs ? a.lens[tid_parent] : -1, tid_src = ends_in(tid_parent, tid_at);
   for (int i = tid; i < a.n_seqs; i += 256) s_first[i] = INT_MAX;
   for (int i = tid; i < (a.n_seqs + 31) / 32; i += 256) s_parent[i] = 0;
   __syncthreads();
@@ -60,10 +63,10 @@ __global__ __launch_bounds__(256) void k_kv_fork(ForkArgs a) {
   }
   __syncthreads();
   // whether a fork can be made but for its page, and whether it needs one
-  auto fine = [&](int f, int p, int c, int at, int len, bool &need) {
+  auto fine = [&](int f, int p, int c, int at, int len, int page, bool &need) {
     const bool ok = p >= 0 && p < a.n_seqs && c >= 0 && c < a.n_seqs && at >= 0 && s_first[c] == f && !((s_parent[c >> 5] >> (c & 31)) & 1u) && at <= len &&
                     at <= a.table_stride * kKvPageRows;
-    need = ok && at % kKvPageRows != 0;
+    need = ok && at % kKvPageRows != 0 && page >= 0 && page < a.n_pages;
     return ok;
   };
   int before = 0, all = 0;  // forks that need a page
@@ -71,7 +74,7 @@ __global__ __launch_bounds__(256) void k_kv_fork(ForkArgs a) {
     bool need;
     const int p = f == tid ? tid_parent : a.parents[f];
     const int c = f == tid ? tid_child : a.children[f], at = f == tid ? tid_at : a.at[f], len = f == tid ? tid_len : p >= 0 && p < a.n_seqs ? a.lens[p] : -1;
-    fine(f, p, c, at, len, need);
+    fine(f, p, c, at, len, f == tid ? tid_src : ends_in(p, at), need);
     all += need;
     before += need && f < mine;
   }
@@ -82,18 +85,18 @@ __global__ __launch_bounds__(256) void k_kv_fork(ForkArgs a) {
   all = (s_count[1][0] + s_count[1][1]) + (s_count[1][2] + s_count[1][3]);
   if (a.free_too && blockIdx.x == 0 && mine == 0 && tid == 0) a.n_free_out[0] = a.n_free[0] - min(all, have);
   if (!a.rows_too) return;
-  bool need, ok = fine(mine, my_parent, my_child, my_at, my_parent_ok ? a.lens[my_parent] : -1, need);
+  bool need, ok = fine(mine, my_parent, my_child, my_at, my_parent_ok ? a.lens[my_parent] : -1, src, need);
   ok = ok && (!need || before < have);
   if (blockIdx.x == 0 && tid == 0) a.refused[mine] = ok ? 0 : 1;
   if (!ok) return;
   const int full = my_at / kKvPageRows, page = need ? a.free_pages[have - 1 - before] : -1;
   if (blockIdx.x == 0) {
     int *to = a.tables + (int64_t)my_child * a.table_stride;
-    for (int c = tid; c < full + need; c += 256) to[c] = c < full ? from[c] : page;
+    for (int c = tid; c < full + (my_at % kKvPageRows != 0); c += 256) to[c] = c == full && need ? page : from[c];
     if (tid == 0) a.lens[my_child] = my_at;
     return;
   }
-  if (!need || src < 0 || src >= a.n_pages || page < 0 || page >= a.n_pages) return;
+  if (!need || page < 0 || page >= a.n_pages) return;
   const int64_t layer = (int64_t)(blockIdx.x - 1) * a.n_pages * a.page_bytes;
   copy_page(a.k_pages + layer, src, page, a.page_bytes);
   copy_page(a.v_pages + layer, src, page, a.page_bytes);

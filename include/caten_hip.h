@@ -466,7 +466,8 @@ int cthip_rope_rows(float *q_out, int64_t q_out_stride, float *k_out, int64_t k_
 int cthip_rope_frequencies(double *frequencies, int rotary_dim, double base, double factor, int trained, double slow, double fast);
 /* Sequences that go on from others.  Fork f makes sequence children[f] the first at[f] rows of sequence parents[f]: its table row names the parent's full
  * pages, a partly filled one is copied in all n_layers pools ((n_layers, n_pages, page bytes) each) into a page from the free stack (the plan's, taken
- * from its end in the order of the forks; the array is not changed), lens[child] = at[f].  Entries of the child's row behind those, and tables and
+ * from its end in the order of the forks; the array is not changed), lens[child] = at[f].  A partly filled page outside the pool holds no rows: the child's entry is the
+ * parent's, and no page is taken.  Entries of the child's row behind those, and tables and
  * lengths of all others, stay.  Refused, with refused[f] = 1 (0 otherwise) and nothing changed: an index outside 0 .. n_seqs - 1, at[f] below 0 or above the parent's
  * length or a table row, a child that an earlier fork names or that is anybody's parent in this call, too few pages (then every later fork that
  * needs one as well).  n_free_out = what is left; may be n_free (one more launch).  What the child's row named before comes back by cthip_kv_free_paged.

@@ -102,6 +102,48 @@ def test_forks_from_pages_outside_the_pool():
     fork_and_compare(rng, cache, tables, [130, 190, 0, 0, 0], [0, 0, 1], [2, 3, 4], [100, 130, 70], [7, 9, -3, 8])
 
 
+@pytest.mark.parametrize("spare", [0, 300])
+def test_forks_that_end_in_a_page_outside_the_pool(spare):
+    """It holds no key, so the child's entry is the parent's and no page is taken: one from the stack would show the child what its last owner left there.  spare: forks in
+    front of these, more than a workgroup's threads."""
+    from caten_amd import ops
+    rng = np.random.default_rng(11)
+    n_pages, n = 12 + spare, 9 + spare
+    cache = filled(rng, n_pages, 1, 32, 2)
+    k, v = cache.k.numpy(), cache.v.numpy()
+    tables = np.full((n, 3), -1, np.int32)
+    tables[0], tables[1], tables[2], tables[4] = [3, -1, n_pages], [2 ** 31 - 1, 4, 5], [6, 7, 1], [2, 2, 2]
+    lens = np.zeros(n, np.int32)
+    lens[:3] = 130, 190, 192
+    free = list(range(12, n_pages)) + [8, 9, 10, 11]
+    parents, children, at = [2] * spare + [0, 0, 1, 1, 0], list(range(9, n)) + [3, 4, 5, 6, 7], [1 + i % 63 for i in range(spare)] + [100, 130, 70, 20, 128]
+    for _ in range(2):  # (the same call again gives the same)
+        got = cache.fork(tables, lens, parents, children, at, free)
+        want = tables.copy()
+        want[9:, 0] = free[::-1][:spare]
+        page = free[::-1][spare]  # for the one fork of these that ends in a page of the pool
+        want[3, :2], want[4], want[5, :2], want[6, :1], want[7, :2] = [3, -1], [3, -1, n_pages], [2 ** 31 - 1, page], [2 ** 31 - 1], [3, -1]
+        assert np.array_equal(got["tables"], want) and not got["refused"].any() and got["n_free"] == len(free) - spare - 1
+        assert np.array_equal(got["lens"][children], at)
+        for pool, now in ((k, cache.k.numpy()), (v, cache.v.numpy())):
+            pool[:, page] = pool[:, 4]
+            pool[:, want[9:, 0]] = pool[:, 6][:, None]
+            assert np.array_equal(now, pool)
+    # the plan takes pages from where the forks have left the stack, and the two that need none are made without any
+    got = cache.fork(tables, lens, [0, 0], [3, 4], [100, 130], [])
+    assert not got["refused"].any() and got["n_free"] == 0
+    # attention: the parent's rows that there are
+    from tests.test_gpu_paged_q4 import _fill
+    cache = ops.PagedCacheQ4(n_pages, 1, 32)
+    _fill(cache, 0xff)
+    rows = rng.normal(0, 1, (64 * 2, 1, 32)).astype(np.float32)
+    cache.append(rows, rows, np.concatenate([np.arange(64) + 3 * 64, np.arange(64) + 11 * 64]))  # page 11: of a sequence that has left
+    got = cache.fork(tables, lens, [0], [3], [100], free)
+    q = rng.normal(0, 1, (1, 2, 32)).astype(np.float32)
+    one = lambda table, length: cache.attend(q, table, [length], [0, 1])
+    assert np.array_equal(one(got["tables"][3:4], 100), one(tables[:1], 100))
+
+
 def test_as_many_forks_as_there_can_be():
     rng = np.random.default_rng(3)
     n, forks, stride = 4096, 4000, 2
