@@ -23,6 +23,9 @@ constexpr int kDraftWorkspace = 2048;  // bytes a sequence
 constexpr int kDraftEach = 8;          // tokens that a thread looks at side by side, at most
 static_assert(16 * kDraftSlices + 4 <= kDraftWorkspace, "the sums of a sequence's slices");
 
+// A probability of the draft's: below nothing, nothing; NaN stays NaN (it rejects its draft, and what it is taken off weighs nothing)
+__device__ __forceinline__ float draft_part(float q) { return q < 0.0f ? 0.0f : q; }
+
 struct DraftArgs {
   int *tokens_out, *accepted, *lens_out;
   const float *target, *draft;
@@ -64,7 +67,7 @@ struct Verified {
         const int x = a.tokens[row0 + j + 1];
         good = x >= 0 && x < a.vocab;
         if (good) {
-          const float p = a.target[(int64_t)(row0 + j) * a.target_stride + x], q = a.draft ? a.draft[(int64_t)(row0 + j) * a.draft_stride + x] : 1.0f;
+          const float p = a.target[(int64_t)(row0 + j) * a.target_stride + x], q = a.draft ? draft_part(a.draft[(int64_t)(row0 + j) * a.draft_stride + x]) : 1.0f;
           good = (double)a.uniforms[row0 + j] * (double)q < (double)p;
         }
       }
@@ -78,7 +81,7 @@ struct Verified {
   }
 };
 
-// What a token weighs: NaN and what is below nothing, as nothing
+// What a token weighs: a difference that is NaN or below nothing, as nothing
 struct DraftRow {
   const float *p, *q;
   int taken;  // the rejected draft, where there are no probabilities of the draft's: the whole of them was its
@@ -91,7 +94,7 @@ struct DraftRow {
   __device__ __forceinline__ void at(int t, double &w, double &own) const {
     const float x = p[t];
     own = x > 0.0f ? (double)x : 0.0;
-    const double left = (double)x - (q ? (double)q[t] : 0.0);
+    const double left = (double)x - (q ? (double)draft_part(q[t]) : 0.0);
     w = t == taken ? 0.0 : left > 0.0 ? left : 0.0;
   }
 };

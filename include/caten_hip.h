@@ -498,8 +498,9 @@ int cthip_sdpa_shared_paged_q4(float *out, const float *q, int64_t q_stride, con
  * of draft those that tokens[r + 1] was drawn from (NULL: that token was certain).  In order, the draft tokens[r + 1] stays where uniforms[r] * draft[r][it] <
  * target[r][it].  Behind the last that stays one token is drawn: from max(target - draft, 0) of the row whose draft was rejected (from its target where that is nothing), or,
  * where all stay, from the last row's target: the lowest token at which the running sum is above uniforms[last row] times the whole.  Products, differences and
- * sums are taken in 64 bits; what is NaN or negative counts as 0, and a draft outside the vocabulary is rejected.  Random numbers lie in [0, 1); one that does not
- * draws the last token with a weight.  Rows need not sum to 1 to be drawn from, but the comparison takes them as they are.
+ * sums are taken in 64 bits.  A probability below 0 counts as 0, and so does one of the target that is NaN; one of the draft that is NaN rejects its draft, and its token is not
+ * drawn from the difference.  A draft outside the vocabulary is rejected.  Random numbers lie in [0, 1); of others one of 1 and more, or NaN, draws the last token
+ * with a weight, one below 0 the first; what they accept is not defined.  Rows need not sum to 1 to be drawn from, but the comparison takes them as they are.
  *   tokens_out (n_rows)  a sequence's drafts that stay, the drawn token (-1 where no token has a probability), -1 in its further rows
  *   accepted (n_seqs)    drafts that stay
  *   lens_out (n_seqs)    lens less the rejected drafts: what the cache holds then; may be lens, or NULL (a page that held rejected rows only

@@ -150,6 +150,30 @@ def test_numbers_that_are_none():
     assert got["tokens"][12] == -1 and got["tokens"][13] == -1 and got["tokens"][15] == -1 and got["accepted"][8] == 0
 
 
+def test_probabilities_below_nothing():
+    """They count as 0, the draft's too: its token is not accepted where the target excludes it, and the difference is not more than the target."""
+    from caten_amd import ops
+    target = np.zeros((8, 6), np.float32)
+    target[:, 2:] = [0.5, 0.25, 0.25, 0.0]
+    draft = np.zeros((8, 6), np.float32)
+    draft[:, 3] = 1.0
+    tokens, uniforms, starts = np.zeros(8, np.int64), np.full(8, 0.9, np.float32), np.array([0, 2, 4, 6, 8])
+    draft[0, 1], tokens[1] = -0.5, 1                           # the target has nothing for the draft: rejected
+    draft[2, 2], draft[2, 0], tokens[3] = -7.0, -1.0, 3        # rejected; left are 2 (0.5) and 4 (0.25)
+    target[4, 5], draft[4, 5], tokens[5] = -0.25, -1.0, 5      # both below nothing: rejected, and 5 has no weight
+    draft[6, 4], tokens[7] = -np.inf, 4                        # the target has something for it: accepted
+    uniforms[[1, 3, 5]] = 0.1, 0.6, 0.999
+    want = dict(tokens=[2, -1, 2, -1, 4, -1, 4, 4], accepted=[0, 0, 0, 1], lens=[9, 9, 9, 10])
+    same(ops.draft_verify(target, draft, tokens, uniforms, starts, [10] * 4), {k: np.array(v) for k, v in want.items()})
+    # over a vocabulary of several slices: the definition with such a draft's zeros
+    rng = np.random.default_rng(13)
+    target, draft, tokens, uniforms, starts, lens = some(rng, [3, 0, 5, 1, 1, 2], 4099)
+    clean = np.where(rng.random(draft.shape) < 0.3, 0.0, draft).astype(np.float32)
+    for below in (-1.0, -1e-30, -np.inf):
+        draft = np.where(clean == 0, np.float32(below), clean)
+        same(ops.draft_verify(target, draft, tokens, uniforms, starts, lens), verified(target, clean, tokens, uniforms, starts, lens))
+
+
 def test_sequences_that_sit_out():
     """No rows, rows refused by the plan, rows outside; lengths may be left out, in place or apart."""
     from caten_amd import _lib, ops
