@@ -177,6 +177,14 @@ __host__ __device__ __forceinline__ float sharing_gains(int rows, int members, i
   return fmaxf(own - (float)tiles, 0.0f) * (float)pages * (float)(H / group * dh) - 128.0f * (float)rows * (float)H;
 }
 constexpr float kSharingCosts = 500000.0f;
+// The most that can be, whichever of the sequences the groups have and whatever pages up to `pages` they share: rows of no group cost nothing and save nothing, so it is not
+// what the whole batch would save.  Of m sequences with r rows, r <= m, a row saves `most` of a tile at most; with more rows they save max(m - r group / 16, m / 2), no
+// more than m rows would.  Each row that saves something is joined, and a group has a tile at least (one without sequences is counted as one with a sequence).
+static float sharing_may_gain(int rows, int members, int groups, int pages, int group, int H, int dh) {
+  const float each = (float)((group + kTileRows - 1) / kTileRows), most = std::max(each - (float)group / kTileRows, 0.5f);
+  const float saved = std::min(most * (float)std::min(rows, members), std::min((float)rows * each - 1.0f, (float)members * each - (float)groups));
+  return std::max(saved, 0.0f) * ((float)pages * (float)(H / group * dh) - 128.0f * (float)H / most);
+}
 // The pages that group g's sequences share, 0 where there is one of them only (it reads its pages by itself), and the first and the end of them
 __device__ __forceinline__ int shared_pages(const Kv4Attn &a, int border, int next, int rows, int &first, int &end) {
   first = min(max(border, 0), a.n_seqs), end = min(max(next, 0), a.n_seqs);
@@ -1059,11 +1067,14 @@ int cthip_sdpa_shared_paged_q4(float *out, const float *q, int64_t q_stride, con
   // most, both launches: 24 sequences 24.2 us by workgroups, 24.8 by wavefronts; 32: 33.6 and 25.2; 64: 44.7 and 28.9 (600 rows: 49.7 and 40.8); four rows each
   // 55.3 and 44.5; with eight rows of a head, whose results are joined by fewer lanes then, 512 jobs 34 and 46.
   const bool few = (int64_t)n_rows * (H / Hkv) <= 4ll * n_seqs && (int64_t)n_seqs * Hkv > state().compute_units * (Dh == 128 ? 3 : 4);
-  // What the groups share is on the device only.  If it would not pay even if they shared all that their tables hold, there is one launch; otherwise the first of
-  // two knows what they share, and leaves it to the second where that gains nothing.
+  // What the groups share, and which rows are theirs, is on the device only.  Two launches where it would pay if tables were full of it and the rows were the groups', as many in
+  // each sequence, or where the most it could save, whosever the rows are, is four times a launch: the first of the two knows, and leaves shared pages to the second
+  // where that gains nothing, which costs 4 to 6 us.  64 samples of one row over 4100 shared ones, 32 heads of 128, beside a prompt of 2500 rows in no group 553 us in one launch
+  // and 390 so; below four launches either happens (beside 256 rows, 64 heads over 8: 88 and 82, or, where those see 3000 more, 153 and 173).
   const int G = H / Hkv, tiles = (int)std::min(std::max(((int64_t)n_rows * G + kTileRows - 1) / kTileRows, (int64_t)std::min(n_groups, n_rows)), (int64_t)INT_MAX);
+  const bool pays = sharing_gains(n_rows, n_seqs, tiles, table_stride, G, H, Dh) > kSharingCosts || sharing_may_gain(n_rows, n_seqs, n_groups, table_stride, G, H, Dh) > 4.0f * kSharingCosts;
   a.always = state().shared_prefix == 2;
-  if (state().shared_prefix == 0 || (state().shared_prefix == 1 && sharing_gains(n_rows, n_seqs, tiles, table_stride, G, H, Dh) <= kSharingCosts)) {
+  if (state().shared_prefix == 0 || (state().shared_prefix == 1 && !pays)) {
     // By wavefronts too, but for 128 channels, where two and not three workgroups of them share a compute unit: 12 heads of 64, 522 sequences in 300 groups of 300 shared rows
     // and up to 300 more 83 us by workgroups, 65 by wavefronts, up to 1000 more 119 and 101; 2752 sequences, 4 heads of 32, 111 and 70; 49 sequences, 32 heads of 128, 45 and 43, with up to
     // 3000 rows 118 and 128.

@@ -353,3 +353,20 @@ def test_the_rule(H, kv, dh, groups, stride, want, way):
         close(got[starts[i]:starts[i + 1]], *seen(q[starts[i]:starts[i + 1]], k, v, next(p // PAGE * PAGE for p, e in zip(shared, borders[1:]) if i < e)))
     for bad in (-1, 3):
         assert _lib.load().cthip_set_option(b"shared_prefix", bad) == _lib.E_BAD_ARG
+
+
+@pytest.mark.parametrize("H,kv,members,prefix,piece", [(32, 32, 40, 1300, 600), (16, 8, 64, 2500, 600)])
+def test_the_rule_beside_rows_of_no_group(H, kv, members, prefix, piece, way):
+    """A piece of another prompt in the same step takes nothing from what the samples of one save: their pages are taken apart as they are without it."""
+    from caten_amd import _lib
+    rng = np.random.default_rng(24)
+    print(f"case: {members} samples over {prefix} rows beside a piece of {piece}, {H} heads over {kv}", flush=True)
+    cache, tables, lens, starts, borders, shared, held = answers(rng, [(prefix, [(prefix + 1 + i % 3, 1) for i in range(members)]), (0, [(piece + 50, piece)])], kv, 128)
+    borders, shared = borders[:2], shared[:1]
+    q = rng.normal(0, 1, (starts[-1], H, 128)).astype(np.float32)
+    forced = cache.attend_shared(q, tables, lens, starts, borders, shared)
+    _lib.check(_lib.load().cthip_set_option(b"shared_prefix", 1))
+    got = cache.attend_shared(q, tables, lens, starts, borders, shared)
+    assert np.array_equal(got, forced) == (way == 2)
+    for i, (k, v) in enumerate(held):
+        close(got[starts[i]:starts[i + 1]], *attention(q[starts[i]:starts[i + 1]], k, v))
