@@ -319,6 +319,7 @@ class PagedCacheQ4:
             _lib.check(self.page_bytes)
         self.k, self.v = (DeviceArray((layers, n_pages, self.page_bytes), np.uint8) for _ in range(2))
         self.workspace = DeviceArray((int(lib.cthip_sdpa_paged_q4_workspace(head_dim)),), np.uint8)
+        self.shared_workspace: Optional[DeviceArray] = None  # of `attend_shared`, from its first call on; as large as the largest batch has asked for
 
     def _pools(self, layer):
         if not 0 <= layer < self.layers:
@@ -376,7 +377,9 @@ class PagedCacheQ4:
         if size < 0:
             _lib.check(size)
         dq, dt, dl, ds, dg, dsh = (DeviceArray.from_numpy(a) for a in (q, tables, lens, starts, groups, shared))
-        out, ws = DeviceArray(q.shape, np.float32), DeviceArray((size,), np.uint8)
+        if self.shared_workspace is None or self.shared_workspace.nbytes < size:
+            self.shared_workspace = DeviceArray((size,), np.uint8)
+        out, ws = DeviceArray(q.shape, np.float32), self.shared_workspace
         kp, vp = self._pools(layer)
         _lib.check(lib.cthip_sdpa_shared_paged_q4(out.ptr, dq.ptr, heads * dh, kp, vp, self.n_pages, dt.ptr, tables.shape[1], dl.ptr, ds.ptr, lens.size, n_rows, dg.ptr, dsh.ptr, shared.size,
                                                   heads, self.kv_heads, dh, ws.ptr))

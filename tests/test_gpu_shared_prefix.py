@@ -244,6 +244,22 @@ def test_rows_behind_the_last_and_a_workspace_of_other_shapes():
         assert not ws.numpy()[:16384].any()
 
 
+def test_a_caches_workspace_is_kept():
+    """One for all calls, as large as the largest has asked for: its size does not depend on the batch but for its rows, and it is left ready for any."""
+    rng = np.random.default_rng(25)
+    cache, tables, lens, starts, borders, shared, held = answers(rng, [(192, [(200, 1), (230, 9), (193, 1)])], 2, 64)
+    q = rng.normal(0, 1, (starts[-1], 8, 64)).astype(np.float32)
+    few = cache.attend_shared(q[:1, :2], tables, lens, [0, 1, 1, 1], borders, shared)
+    first = cache.shared_workspace
+    got = cache.attend_shared(q, tables, lens, starts, borders, shared)
+    larger = cache.shared_workspace
+    assert larger.nbytes > first.nbytes and not larger.numpy()[:16384].any()
+    assert np.array_equal(cache.attend_shared(q[:1, :2], tables, lens, [0, 1, 1, 1], borders, shared), few)
+    assert np.array_equal(cache.attend_shared(q, tables, lens, starts, borders, shared), got) and cache.shared_workspace is larger
+    for i, (k, v) in enumerate(held):
+        close(got[starts[i]:starts[i + 1]], *attention(q[starts[i]:starts[i + 1]], k, v))
+
+
 @pytest.mark.parametrize("fill", [0x7f, 0xff])
 def test_whatever_the_workspace_holds(fill):
     """Behind its tickets: large numbers, NaN; the groups are one of many jobs, some of shares, and a batch by wavefronts."""
