@@ -106,6 +106,46 @@ def test_many_groups():
     compare(rng, 4, 2, 64, [(64 * (i % 3), [(64 * (i % 3) + 1 + (i * 37 + j) % 100, (i + j) % 3) for j in range(i % 4 + 1)]) for i in range(150)])
 
 
+# More jobs than workgroups that run at once, each of four rows of a head at most: a wavefront takes a job by itself (at 64 channels and fewer in one launch as well).  One
+# sequence or two hold far more behind the shared pages, whose shares many wavefronts join.
+@pytest.mark.parametrize("H,kv,dh,groups", [
+    (12, 12, 64, [(300, [(301 + 9 * i, 1) for i in range(40)] + [(9000, 1)]), (330, [(331 + i % 70, 1) for i in range(50)]), (0, [(1 + 5 * i, 1) for i in range(30)])]),
+    (4, 4, 32, [(320, [(321 + i, 1) for i in range(150)] + [(20000, 1)]), (290, [(300 + i % 300, i % 3 != 1) for i in range(160)])]),
+    (8, 4, 64, [(260, [(270 + i % 40, 1 + i % 3) for i in range(270)] + [(6000, 2)])]),
+    (32, 32, 128, [(200, [(201 + 4 * i, 1) for i in range(35)] + [(5000, 1)]), (64, [(65, 1), (3000, 1), (70, 4)])]),
+    (16, 8, 128, [(450, [(451 + i % 100, 2) for i in range(110)] + [(4000, 1)])])])
+def test_jobs_of_single_wavefronts(H, kv, dh, groups):
+    print(f"case: jobs of single wavefronts, {H} heads over {kv} of {dh}, {len(groups)} groups", flush=True)
+    compare(np.random.default_rng(26 + dh + H), H, kv, dh, groups)
+
+
+def test_wavefronts_with_more_pages_than_lanes():
+    """Parts of some 80 pages: a wavefront asks for page ids 64 at a time, of the group's table in one launch."""
+    from caten_amd import ops
+    rng = np.random.default_rng(27)
+    n, kv, dh, pages = 520, 2, 32, 240
+    cache = ops.PagedCacheQ4(pages + n + 3, kv, dh)
+    _fill(cache, 0xff)
+    ids = rng.permutation(cache.n_pages)
+    tables = np.concatenate([np.full((n, pages), -1), ids[pages:pages + n, None]], 1).astype(np.int32)
+    tables[0, :pages] = ids[:pages]  # (of what is shared the first sequence's entries are read)
+    own = 1 + np.arange(n) % 60
+    lens, starts = pages * PAGE + own, np.arange(n + 1)
+
+    def rows(slots):
+        k, v = (rng.normal(0, 1, (len(slots), kv, dh)).astype(np.float32) for _ in range(2))
+        cache.append(k, v, slots)
+        return cache.rows(slots)
+    first = rows((tables[0, :pages, None] * PAGE + np.arange(PAGE)).ravel())
+    behind = rows(np.concatenate([t * PAGE + np.arange(m) for t, m in zip(tables[:, -1], own)]))
+    q = rng.normal(0, 1, (n, kv, dh)).astype(np.float32)
+    got = cache.attend_shared(q, tables, lens, starts, [0, n], [pages * PAGE])
+    at = np.concatenate([[0], np.cumsum(own)])
+    for i in range(n):
+        close(got[i:i + 1], *attention(q[i:i + 1], *(np.concatenate([a, b[at[i]:at[i + 1]]]) for a, b in zip(first, behind))))
+    assert np.array_equal(got, cache.attend_shared(q, tables, lens, starts, [0, n], [pages * PAGE]))
+
+
 def test_as_many_sequences_as_there_may_be():
     rng = np.random.default_rng(23)
     groups, left = [], 4096
