@@ -9,7 +9,8 @@
 // Two launches.  A row is cut into slices; a workgroup finds its sequence's first rejected draft for itself (one load of two
 // numbers a draft) and leaves its slice's sums, the replacement's and, in case that one is nothing, the target's own.  Then a wavefront
 // finds the slice and a workgroup the token in it, eight side by side a thread.  Bound by the two rows of the vocabulary that a sequence needs, and
-// by two launches of four to six round trips each where those are short.  (One launch of a workgroup a sequence would read 64 rows with 64 of 256 compute units.)
+// by two launches of four to six round trips each where those are short.  (One launch of a workgroup a sequence would read 64 rows with 64 of 256 compute units; one in which the last of a sequence's workgroups, by ticket, finds the token has not
+// been built.)
 //   64 sequences of 1 .. 5 rows, 128256 tokens (65.7 MB needed): 13.3 + 7 us; the sums at 5 TB/s.
 //   48 sequences of up to 8 rows, 32000 tokens: 5.7 + 6.1 us.  One sequence of 5 rows, 50257 tokens: 3.9 + 5.0 us.
 #include <algorithm>

@@ -19,14 +19,16 @@
 // page is read and taken apart once for sixteen rows, not once a sequence, and no row is masked.  The second takes what lies behind
 // them for each sequence and, as it stores a row, joins to it what the first one has left: its outputs, unnormalised, in `out`, its maximum and sum in the
 // workspace, or, where several workgroups had shares of them, all shares (joined by the first launch itself, by ticket, they cost it 4 to 6 us and save
-// the second 3).  Bound by the vector unit, as above: at 128 channels 667 vector instructions a page and 16 rows beside 64 matrix ones; where the own
-// parts are short, by the two launches' chains of round trips.
-//   64 samples, 4100 shared rows and up to 400 own, 32 heads of 128 (44.8 MB): 26 + 23 us; each by itself 215.
-//   3 groups of up to 14 sequences of 5 rows, 9000 shared rows, 64 heads over 8 of 128 (22.8 GFLOP): 76 + 32 us; of the first the vector units 64 %, the matrix units 21 %.
-// Sharing saves tiles that are not full.  Rows that fill theirs by themselves, as those 3 groups' nearly do (each by itself 103 us), and short prefixes pay for the second
-// launch and the joining: then one launch takes every sequence's pages, its group's among them.  8 answers, 900 shared rows, 12 heads of 64: 11.6 us, two launches
-// 7.2 + 8.7.  Over 207 batches of 2 .. 1500 sequences, prefixes of 300 .. 30000 rows, one row a sequence or up to five, the way taken is within 1.1 % of the
-// faster (geometric mean; at worst 17 %); sharing always would take 28 % longer and up to twice as long, never sharing 20 % and up to ten times.
+// the second 3).  Many rows over long prefixes are bound by the vector unit, as above: at 128 channels 667 vector instructions a page and 16 rows beside 64 matrix ones.  Fewer, and short
+// own parts, are bound by no unit but by each launch's chain of round trips before its first page and after its last.
+//   64 samples, 4100 shared rows and up to 400 own, 32 heads of 128 (44.8 MB): 26 + 23 us, the vector units busy 43 and 30 % of it; each by itself 215.
+//   3 groups of up to 14 sequences of 5 rows, 9000 shared rows, 64 heads over 8 of 128 (22.8 GFLOP): 76 + 32 us; the vector units 64 and 25 %, the matrix units 21 and 3 %.
+// Sharing saves tiles that are not full.  Rows that fill theirs by themselves, and short prefixes, pay for the second
+// launch and the joining: then one launch takes every sequence's pages, its group's among them.  8 answers, 900 shared rows, 12 heads of 64: 10 us, two launches
+// 7.2 + 8.7.  Those 3 groups' rows nearly fill theirs, and one launch takes 103 us where the rule (below) takes two.
+// The rule estimates, from lengths of tables and numbers of rows where a step has room for more than there is.  206 batches of 1 .. 78 sequences, prefixes of 50 .. 20000 rows, 1 .. 60 rows a
+// sequence, geometric mean over the faster way (worst): tables as long as the longest sequence 1.010 (1.16), of 128 entries 1.059 (1.67), of 2048 1.216 (1.86: 9 us where one launch is enough, and two are 17);
+// one launch always 1.08 (6), two always 1.41 (2.1).
 // Longer tiles would take a page apart once for more rows, and gain nothing: 256 rows over 32768 shared keys of 8 heads of 128, 115 us, takes 107 - 119 with
 // tiles of 32 rows (half as many wavefronts hide a page's latencies), 124 - 150 with a page taken apart in LDS for four or eight wavefronts (two barriers a page).
 // At 128 channels three workgroups share a compute unit's LDS only up to 53760 bytes each (granules of 1280): these launches use 53632.
@@ -1066,6 +1068,7 @@ int cthip_sdpa_shared_paged_q4(float *out, const float *q, int64_t q_stride, con
   // wavefront's own: its chain of round trips, not its pages, is what it takes, and four times as many run at once.  32 heads of 128 over 1024 shared rows, 70 rows behind them at
   // most, both launches: 24 sequences 24.2 us by workgroups, 24.8 by wavefronts; 32: 33.6 and 25.2; 64: 44.7 and 28.9 (600 rows: 49.7 and 40.8); four rows each
   // 55.3 and 44.5; with eight rows of a head, whose results are joined by fewer lanes then, 512 jobs 34 and 46.
+  // (n_rows is what there is room for: 64 samples in a step for five times as many rows take 60.3 us, with room for four times as many 47.9)
   const bool few = (int64_t)n_rows * (H / Hkv) <= 4ll * n_seqs && (int64_t)n_seqs * Hkv > state().compute_units * (Dh == 128 ? 3 : 4);
   // What the groups share, and which rows are theirs, is on the device only.  Two launches where it would pay if tables were full of it and the rows were the groups', as many in
   // each sequence, or where the most it could save, whosever the rows are, is four times a launch: the first of the two knows, and leaves shared pages to the second

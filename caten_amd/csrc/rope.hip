@@ -3,9 +3,10 @@
 // positions (nn/positional-encoding.lisp:3-64: cthip_rope).
 //
 // A pair (a, b) at angle t = position * frequency becomes m (a cos t - b sin t, a sin t + b cos t).  t is a 64-bit product, and a whole number of quarter
-// turns is taken off it in 64 bits, so that sine and cosine are as exact at position 10^6 as at 1 (in 32 bits t alone would be off by 0.03 there).  A thread
-// works out the angles of its channels once and turns them in every head it takes, four channels (halves: eight) in one access of 16 bytes each, four
-// heads' loads on their way together.  Bound by the rows: read and written once.
+// turns is taken off it in 64 bits, so that sine and cosine are as exact at position 10^6 as at 1 (in 32 bits t alone would be off by 0.03 there; in 64 its rounding, 2^-53 of it, comes
+// to theirs, 2^-23, at 2^30 radians).  A thread
+// works out the angles of its channels once and turns them in every head it takes, four channels (halves: eight) in one access of 16 bytes each, one head
+// after the other (outputs may be the inputs, so a head's loads stay behind the stores of the one before; the other wavefronts run meanwhile).  Bound by the rows: read and written once.
 //   6001 rows of 64 + 8 heads of 128, halves (442 MB): 84 us = 5.2 TB/s, where a copy of 4 GiB reaches 4.7.
 //   48 rows of 32 + 4 heads of 64, pairs: 2.9 us, a launch and three round trips (position, frequencies, the rows).
 #include <algorithm>

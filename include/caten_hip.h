@@ -287,8 +287,10 @@ int cthip_linear(float *y, const void *wmat, const float *x, int m, const float 
  *   and by a lower limit; 0 = none are kept.  Results do not depend on it where the same launch is chosen; past the
  *   limit the terms are made by every call that still pays with them.
  * "shared_prefix": whether cthip_sdpa_shared_paged_q4 takes the pages that a group shares once for all of its rows, in a launch in
- *   front of that over the rest: 1 (default) = where that is faster (prefixes of some hundred rows and more, sequences whose rows do not fill a tile of
- *   16 by themselves: rows times query heads of a key / value head), 0 = never (one launch), 2 = always.  Results differ in summation order only.
+ *   front of that over the rest: 1 (default) = where an estimate says that this is faster (prefixes of some hundred rows and more, sequences whose rows do not fill a tile of
+ *   16 by themselves: rows times query heads of a key / value head), 0 = never (one launch), 2 = always.  The launch that knows what is shared is the first of the two; whether
+ *   there is one is estimated from n_seqs, n_rows, n_groups (groups without sequences count too) and table_stride, as if tables were full.  A few short answers under tables of some hundred entries take two launches,
+ *   3 to 8 us longer, where one would do: 0 suits them better.  Results differ in summation order only.
  * "decode_skip": knock-out timing of the three-launch decode step -- a mask of launches a session created
  *   afterwards leaves out (1 qkv, 2 attention + projection, 4 MLP, 8 the sum in front of lm_head,
  *   16 lm_head + argmax).  Tokens and logits of such a session are meaningless; 0 (default) = none.
@@ -456,7 +458,8 @@ int cthip_beam_reorder_paged_q4(int *tables_out, int *history_out, void *k_pages
  * in floats (slices of a fused product; outputs may be the inputs themselves, with the same stride, and may not overlap them otherwise).  Row r is
  * at positions[r]; one below 0 is left as it was (the plan gives -1 to rows behind the last and to those of refused sequences).  The first rotary_dim
  * channels of a head turn, pair i by position * frequencies[i], times magnitude; the others are copied.  H or Hkv may be 0.  frequencies: rotary_dim / 2 doubles on
- * the device.  Angles are taken in 64 bits: sines and cosines are off by 2^-23 at any position.  At most 2^23 rows, 65535 heads of
+ * the device.  Angles are products rounded to 64 bits, and
+ * sines and cosines of those are off by 2^-23 (at 2^30 radians the product itself by as much).  At most 2^23 rows, 65535 heads of
  * either kind and channels of a head; in the layout of pairs Dh is even. */
 int cthip_rope_rows(float *q_out, int64_t q_out_stride, float *k_out, int64_t k_out_stride, const float *q, int64_t q_stride, const float *k, int64_t k_stride,
                     const int *positions, int n_rows, int H, int Hkv, int Dh, int rotary_dim, int layout, const double *frequencies, float magnitude);
@@ -485,7 +488,7 @@ int cthip_kv_compact_paged_q4(int *tables_out, int *free_pages, int *n_free, voi
 /* cthip_sdpa_paged_q4 where sequences have their first pages in common.  Group g is sequences groups[g] .. groups[g + 1] - 1; the first shared[g] / 64 (whole) pages of the
  * table of its first sequence are all of its sequences', and are read once for all of their rows where that is faster (option "shared_prefix").  A row sees all of them, and of its own sequence's
  * rows behind them those up to its own position; so with equal table entries, and no row's position in front of them, the result is that of
- * cthip_sdpa_paged_q4 up to rounding.  lens count the shared rows.  groups (n_groups + 1) and starts rise; sequences in no group share nothing; groups and starts that
+ * cthip_sdpa_paged_q4 up to rounding.  lens count the shared rows.  A group of one sequence shares nothing; without groups it is that call.  groups (n_groups + 1) and starts rise; sequences in no group share nothing; groups and starts that
  * fall, or leave their range, give undefined rows.  At most as many groups as sequences; otherwise arguments, precision, limits and what is left as it was are as
  * there.  workspace: cthip_sdpa_shared_paged_q4_workspace(n_rows, H, Dh) = 4 * (4096 + 131072 * (Dh + 2) + 2 * n_rows * H) bytes, 16-byte aligned, its first 16384 zeroed
  * once (cthip_alloc does); every call leaves it ready for the next, of any shape.  Calls that may overlap need one each. */
